@@ -191,6 +191,133 @@ NEON_API int neon_cuda_matvec_q4_0_noalloc(neon_tensor_t W, const float* dX, siz
                                            size_t y_stride, size_t seq, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Long contexts: rotary positions, a KV cache in 8 bits, eviction          */
+/* ------------------------------------------------------------------------ */
+
+/* The operators of this section take device buffers of F32, F16 or BF16
+ * values (`type`, a NEON_GGML_* value; every buffer of one call has it),
+ * compute in fp32 and round once at the end. They run on the device that
+ * their buffers live on, allocate nothing, keep nothing between calls, and
+ * may be captured into a CUDA graph (after the first call on a device or
+ * neon_cuda_init): lengths and positions are read from device memory, so a
+ * replayed graph sees their current values. Calls on different buffers may
+ * run at the same time. None has a counterpart in the reference, whose RoPE
+ * (rope_apply, rawllm_forward.hpp:755-782) is the interleaved, linearly
+ * scaled case and whose KV cache is fp32. */
+
+/* How positions turn the pairs of a head: pair i of the first n_dims values
+ * by pos * f_i, f_i = base^(-2i / (freq_dim or n_dims)) / factors[i] / scale.
+ * With yarn > 0 a pair keeps its own frequency as far as it turns often in
+ * the first orig_ctx positions: with i(b) = n_dims * ln(orig_ctx / (2 pi b)) /
+ * (2 ln base), lo = max(0, floor(i(beta_fast))), hi = min(n_dims - 1,
+ * ceil(i(beta_slow))) and k_i = yarn * (1 - clamp((i - lo) / max(hi - lo,
+ * 0.001), 0, 1)), f_i is (1 - k_i) times the scaled frequency plus k_i times
+ * the unscaled one. Rotated values are multiplied by magnitude; values from
+ * n_dims on are copied. Angles are reduced in 64 bits, so far positions keep
+ * their accuracy. */
+#define NEON_ROPE_INTERLEAVED 0 /* pair i: values 2i and 2i + 1 (as the reference) */
+#define NEON_ROPE_HALF 1        /* pair i: values i and i + n_dims / 2 */
+typedef struct {
+    uint32_t n_dims;   /* rotated values of each head: even, 2 .. 256, at most head_dim */
+    uint32_t layout;   /* NEON_ROPE_* */
+    uint32_t freq_dim; /* the exponent's denominator; 0: n_dims */
+    uint32_t orig_ctx; /* with yarn > 0 */
+    double base, scale;
+    double yarn;       /* 0 (off) .. 1 */
+    double beta_fast, beta_slow;
+    double magnitude;
+    const float* factors; /* host array of n_dims / 2 divisors, or NULL */
+} neon_rope_t;
+
+/* One tensor of a rotation: n_heads heads of head_dim values per position,
+ * positions x_stride (y_stride) values apart. Y may be X (then y_stride is
+ * x_stride); otherwise they do not overlap. */
+typedef struct {
+    const void* X;
+    void* Y;
+    size_t x_stride, y_stride;
+    size_t n_heads;
+} neon_rope_target_t;
+
+/* Rotate 1 to 4 tensors (a step's queries and keys) of n positions in one
+ * launch: Y[t] = R(d_pos[t]) X[t], d_pos n int32 values on the device.
+ * backward != 0 rotates the other way, Y[t] = R(d_pos[t])^T X[t]: the
+ * gradient of the forward rotation with respect to X, X holding that of Y. */
+NEON_API int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* d_pos, size_t n, size_t head_dim,
+                            const neon_rope_target_t* targets, size_t n_targets, int backward, void* stream);
+
+/* A KV cache in 8 bits: for each KV head, int8 codes of K and V with one fp32
+ * scale for each block of 32 rows. A row's value is the fp32 number code *
+ * scale. The scale of a block is amax / 127 over the values of the rows that
+ * it holds, its codes are value / scale rounded to the nearest integer, ties
+ * to even; a block without a value of 127 * FLT_MIN or more has scale and
+ * codes 0; one with a value that is not finite has scale NaN, which every
+ * result that attends to it shows. The rows of the last two blocks that
+ * appends ended or began in are also held as they came (the tail), so a
+ * block's codes are those of its rows however they arrived, and an append
+ * may be repeated. All buffers are the caller's, on one device. */
+#define NEON_KV8_BLOCK 32
+typedef struct {
+    uint32_t n_kv_head;
+    uint32_t head_dim;  /* a multiple of 16, at most 256 */
+    uint32_t capacity;  /* rows, a multiple of 32 */
+    int8_t *k, *v;      /* codes [n_kv_head][capacity][head_dim], 16-byte aligned */
+    float *k_scale, *v_scale; /* [n_kv_head][capacity / 32] */
+    float* tail;        /* [2: K, V][2 slots][n_kv_head][32][head_dim], 16-byte aligned */
+    int32_t* tail_block; /* [2: K, V][n_kv_head][2 slots]: the block that a slot holds; -1, the start: none */
+    int32_t* past;      /* one value: the rows held before the tokens of the current step */
+} neon_kv8_t;
+
+/* Write the K and V rows of n new tokens at rows *past .. *past + n - 1
+ * (dK[t * k_stride + head * head_dim + d]). *past itself is left: the caller
+ * moves it on after the step (neon_cuda_kv8_attention reads it too), and may
+ * set it back to drop rows, not forward over rows that were not written.
+ * Rows from capacity on are dropped and reported by the next neon_cuda_sync
+ * on the device. */
+NEON_API int neon_cuda_kv8_append(const neon_kv8_t* cache, const void* dK, size_t k_stride, const void* dV,
+                                  size_t v_stride, size_t n, int type, void* stream);
+
+/* Rows [row0, row0 + n) as fp32 values: dK_out and dV_out [n][n_kv_head]
+ * [head_dim] (either may be NULL). */
+NEON_API int neon_cuda_kv8_read(const neon_kv8_t* cache, size_t row0, size_t n, float* dK_out, float* dV_out,
+                                void* stream);
+
+/* Causal attention of the n tokens at rows *past .. *past + n - 1, already
+ * appended, over the cache: query head h of token t (dQ[t * q_stride + h *
+ * head_dim + d]) attends to rows 0 .. *past + t of KV head h / (n_head /
+ * n_kv_head), with scores times `scale` (0: 1 / sqrt(head_dim)). Writes
+ * dO[t * o_stride + h * head_dim + d]; a token with no row to attend to
+ * (*past + t < 0) gets zeros. d_weight (or NULL): [n_kv_head][capacity] floats,
+ * the accumulated attention weight of each cached row: the probabilities that
+ * the queries of its group give a row are added for rows before *past and
+ * written for the new rows, which have no weight yet. `workspace`:
+ * neon_cuda_kv8_attention_workspace() bytes on the device, 16-byte aligned,
+ * not shared by calls that may run at the same time. Sums are taken in a
+ * fixed order: the same call gives the same bits. */
+NEON_API int neon_cuda_kv8_attention(const neon_kv8_t* cache, const void* dQ, size_t q_stride, void* dO,
+                                     size_t o_stride, size_t n, size_t n_head, float scale, int type,
+                                     float* d_weight, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace for calls of up to n tokens (host-only; needs no GPU). */
+NEON_API int neon_cuda_kv8_attention_workspace(const neon_kv8_t* cache, size_t n, size_t n_head, size_t* bytes);
+
+/* Eviction by accumulated attention weight, from `src` into the separate
+ * buffers of `dst` (same heads and head_dim, capacity at least `keep`): when
+ * src holds more than `keep` rows, each KV head keeps its first `sink` rows,
+ * its last `recent` rows, and of the rows between them the keep - sink -
+ * recent of the largest weight (among equals the lowest row first; a NaN
+ * counts as the largest); otherwise all rows stay. Kept rows move down in
+ * order, with their weights (d_weight_dst). A block whose rows all stay in
+ * place keeps its codes and scale; the others are quantised again from their
+ * rows' fp32 values. With `rope`, a K row that moves is first rotated by its
+ * new row minus its old (positions count cache rows, as kv_cache_shift leaves
+ * them, rawllm_forward.hpp:949-969; magnitude is not applied again). d_kept:
+ * [n_kv_head][keep] int32, the old row of each kept row (-1 behind the last).
+ * *dst->past becomes the rows kept, and dst's tail is empty. */
+NEON_API int neon_cuda_kv8_evict(const neon_kv8_t* src, const float* d_weight, const neon_kv8_t* dst,
+                                 float* d_weight_dst, size_t keep, size_t sink, size_t recent,
+                                 const neon_rope_t* rope, int32_t* d_kept, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Decode step on the device                                                */
 /* ------------------------------------------------------------------------ */
 

@@ -66,7 +66,8 @@ DeviceState g_dev[kMaxDevices];
 std::mutex g_init_mu;
 }  // namespace
 
-// Device-side error word: bit 0 = a bounded wait in a kernel timed out.
+// Device-side error word: bit 0 = a bounded wait in a kernel timed out, bit 1 =
+// rows beyond an 8-bit KV cache's capacity were dropped.
 static __device__ unsigned int g_neon_device_err;
 
 namespace {
@@ -701,6 +702,7 @@ int check_device_err(int device) {
     if (v) {
         const unsigned int zero = 0;
         cudaMemcpyToSymbol(g_neon_device_err, &zero, sizeof(zero));
+        if (v == 2u) return set_err(NEON_ERR_INVALID, "kv8: rows beyond the cache's capacity were dropped");
         return set_err(NEON_ERR_CUDA, "a device-side wait timed out (shared-memory copy never completed)");
     }
     return NEON_OK;
@@ -960,6 +962,7 @@ int device_sms(int device) {
     return rc ? -1 : g_dev[device].sms;
 }
 int check_device_error(int device) { return check_device_err(device); }
+unsigned* device_error_word(int device) { return init_device(device) ? nullptr : g_dev[device].err; }
 }  // namespace neon_internal
 
 extern "C" {

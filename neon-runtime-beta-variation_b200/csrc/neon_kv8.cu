@@ -1,0 +1,618 @@
+// neon_kv8.cu -- the KV cache in 8 bits: append, read and eviction
+// (neon_cuda_kv8_append / _read / _evict). The attention over it is in
+// neon_kv8_attn.cu.
+//
+// A block is 32 rows of one KV head: codes c = rint(x / s), s = amax / 127. A
+// code is the nearest integer to the exact quotient: the quotient is first
+// taken with the reciprocal of s, then the remainder e = x - r s, which one
+// FMA gives exactly (r is at most one off the nearest integer, so e is a
+// multiple of the smaller ulp and below s), moves r by one where |e| > s / 2
+// and to the even side where |e| = s / 2. So the codes do not depend on how a
+// quotient is rounded, and a block's codes are a function of its rows.
+#include "neon_longctx.cuh"
+#include "neon_kv8.h"
+
+#include <algorithm>
+
+namespace longctx {
+
+int kv8_check(const neon_kv8_t* c) {
+    using neon_internal::error;
+    if (!c) return error(NEON_ERR_INVALID, "null cache");
+    if (c->n_kv_head == 0 || c->n_kv_head > 16384) return error(NEON_ERR_INVALID, "kv8: n_kv_head must be 1 to 16384");
+    if (c->head_dim < 16 || c->head_dim % 16 || c->head_dim > 256)
+        return error(NEON_ERR_UNSUPPORTED, "kv8: head_dim must be a multiple of 16, from 16 to 256");
+    if (c->capacity == 0 || c->capacity % NEON_KV8_BLOCK || c->capacity > (1u << 30))
+        return error(NEON_ERR_INVALID, "kv8: capacity must be a multiple of 32, from 32 to 2^30");
+    return NEON_OK;
+}
+
+int kv8_check_buffers(const neon_kv8_t* c) {
+    using neon_internal::error;
+    int rc = kv8_check(c);
+    if (rc) return rc;
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->tail || !c->tail_block || !c->past)
+        return error(NEON_ERR_INVALID, "kv8: null buffer");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->tail, 16))
+        return error(NEON_ERR_INVALID, "kv8: codes and tail must be 16-byte aligned");
+    if (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) || !aligned(c->tail_block, 4) || !aligned(c->past, 4))
+        return error(NEON_ERR_INVALID, "kv8: buffer not aligned to its type");
+    return NEON_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kTiny = 127.f * 1.17549435e-38f;  // 127 * FLT_MIN
+
+// ---- a block's rows as float4 pieces in registers ----
+// Thread i holds pieces i, i + 256, ... of the block's 32 * hd / 4, row-major;
+// P = hd / 32 rounded up covers them.
+
+// The largest magnitude of the block, or NaN if a value is not finite.
+template <int P>
+__device__ __forceinline__ float block_amax(const float4 (&x)[P], float* red) {
+    float m = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+        bad = bad || isnan(x[i].x) || isnan(x[i].y) || isnan(x[i].z) || isnan(x[i].w);
+    }
+    if (bad || isinf(m)) m = __int_as_float(0x7fffffff);
+    // as bit patterns: magnitudes order like their bits, and a NaN is above them all
+    const unsigned w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(w);
+    __syncthreads();
+    unsigned r = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) r = max(r, __float_as_uint(red[i]));
+    __syncthreads();
+    return __uint_as_float(r);
+}
+
+__device__ __forceinline__ float block_scale(float amax) {
+    return isnan(amax) ? amax : amax >= kTiny ? __fdiv_rn(amax, 127.f) : 0.f;
+}
+
+__device__ __forceinline__ int quantise(float x, float s, float inv) {
+    float r = rintf(__fmul_rn(x, inv));
+    const float e = __fmaf_rn(-r, s, x);  // exact
+    const float e2 = 2.f * fabsf(e);
+    if (e2 > s || (e2 == s && ((int)r & 1))) r += e > 0.f ? 1.f : -1.f;
+    return (int)r;
+}
+__device__ __forceinline__ char4 quantise4(float4 x, float s, float inv) {
+    if (!(s > 0.f)) return make_char4(0, 0, 0, 0);  // an empty block, or NaN
+    return make_char4((char)quantise(x.x, s, inv), (char)quantise(x.y, s, inv), (char)quantise(x.z, s, inv),
+                      (char)quantise(x.w, s, inv));
+}
+__device__ __forceinline__ float4 dequantise4(char4 c, float s) {
+    return make_float4(__fmul_rn((float)c.x, s), __fmul_rn((float)c.y, s), __fmul_rn((float)c.z, s), __fmul_rn((float)c.w, s));
+}
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, bool vec);
+template <>
+__device__ __forceinline__ float4 load4<float>(const float* p, bool vec) {
+    return vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+}
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, bool vec) {
+    if (!vec) return make_float4(to_f(p[0]), to_f(p[1]), to_f(p[2]), to_f(p[3]));
+    union { uint2 u; T t[4]; } w;
+    w.u = *reinterpret_cast<const uint2*>(p);
+    return make_float4(to_f(w.t[0]), to_f(w.t[1]), to_f(w.t[2]), to_f(w.t[3]));
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+// One CTA per block, head and K or V; the first CTA of a head takes its first
+// block and then its last one, the only two that touch the tail. Memory bounds
+// a prompt's append (8191 new bf16 rows of 8 heads x 128: the figures are in
+// the table of the design notes); one token's is a launch and its latency.
+
+struct AppendArgs {
+    neon_kv8_t c;
+    const void *k, *v;
+    long long ks, vs;
+    int n;
+    bool vec;
+    unsigned* err;
+};
+
+template <typename T, int P>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ float red[kThreads / 32];
+    pdl_wait();
+    pdl_trigger();
+    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, H = (int)a.c.n_kv_head;
+    const int h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+    const int past = *a.c.past;
+    if (past < 0 || (long long)past + a.n > cap) {
+        if (tid == 0 && h == 0 && which == 0 && blockIdx.x == 0) atomicOr(a.err, kErrRows);
+        if (past < 0 || past >= cap) return;
+    }
+    const int end = (int)min((long long)past + a.n, (long long)cap);
+    const int b0 = past >> 5, b1 = (end - 1) >> 5, r0 = past & 31;
+    int b = b0 + (int)blockIdx.x;
+    if (blockIdx.x > 0 && b >= b1) return;
+    const T* src = (const T*)(which ? a.v : a.k);
+    const long long ss = which ? a.vs : a.ks;
+    int8_t* codes = (which ? a.c.v : a.c.k) + (size_t)h * cap * hd;
+    float* scales = (which ? a.c.v_scale : a.c.k_scale) + (size_t)h * (cap >> 5);
+    const size_t slot_floats = (size_t)H * 32 * hd;
+    float* tail = a.c.tail + ((size_t)which * 2 * H + h) * 32 * hd;  // slot s at + s * slot_floats
+    int* tag = a.c.tail_block + ((size_t)which * H + h) * 2;
+
+    // The slots of the first and the last block (the head's first CTA alone
+    // looks at them): the first block's rows are kept if it has earlier rows,
+    // the last block's always, in the other slot.
+    int slot0 = -1, slot1 = -1;
+    bool known = false;
+    if (blockIdx.x == 0) {
+        const int g0 = tag[0], g1 = tag[1];
+        if (r0) {
+            known = g0 == b0 || g1 == b0;
+            slot0 = g0 == b0 ? 0 : g1 == b0 ? 1 : g0 == b0 - 1 ? 1 : 0;
+            if (b1 > b0) slot1 = 1 - slot0;
+        } else if (b1 == b0) {
+            slot0 = g0 == b0 - 1 ? 1 : 0;
+        } else {
+            slot1 = g0 == b1 - 1 ? 1 : 0;
+        }
+        __syncthreads();  // every thread has read the tags
+        if (tid < 2) {
+            const int g = tid ? g1 : g0;
+            // blocks that this call writes are no longer what an older slot holds
+            const int now = tid == slot0 ? b0 : tid == slot1 ? b1 : g >= b0 && g <= b1 ? -1 : g;
+            if (now != g) tag[tid] = now;
+        }
+    }
+    for (;;) {
+        const int rows = min(32, end - 32 * b);  // rows that the block holds after this call
+        const int old = b == b0 ? r0 : 0;        // of them, rows from before
+        const int slot = blockIdx.x == 0 ? (b == b0 ? slot0 : slot1) : -1;
+        float* keep = slot >= 0 ? tail + slot * slot_floats : nullptr;
+        int8_t* bc = codes + (size_t)b * 32 * hd;
+        const float before = old && !known ? scales[b] : 0.f;
+        float4 x[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int e = (i * kThreads + tid) * 4, r = e / hd;
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) {
+                if (r >= old)
+                    x[i] = load4<T>(src + (32LL * b + r - past) * ss + (long long)h * hd + (e - r * hd), a.vec);
+                else if (known)
+                    x[i] = *reinterpret_cast<const float4*>(keep + e);
+                else
+                    x[i] = dequantise4(*reinterpret_cast<const char4*>(bc + e), before);
+            }
+        }
+        const float s = block_scale(block_amax(x, red));
+        const float inv = __fdiv_rn(1.f, s);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int e = (i * kThreads + tid) * 4, r = e / hd;
+            if (r < rows) {
+                *reinterpret_cast<char4*>(bc + e) = quantise4(x[i], s, inv);
+                if (keep && (r >= old || !known)) *reinterpret_cast<float4*>(keep + e) = x[i];
+            }
+        }
+        if (tid == 0) scales[b] = s;
+        if (blockIdx.x > 0 || b == b1) break;
+        b = b1;
+        known = false;
+    }
+}
+
+using AppendKernel = void (*)(AppendArgs);
+template <typename T>
+AppendKernel append_kernel_for(int hd) {
+    return hd <= 64 ? kv8_append_kernel<T, 2> : hd <= 128 ? kv8_append_kernel<T, 4> : kv8_append_kernel<T, 8>;
+}
+
+// ---------------------------------------------------------------------------
+// read
+// ---------------------------------------------------------------------------
+
+__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ neon_kv8_t c, int row0, int n,
+                                                            float* k_out, float* v_out) {
+    pdl_wait();
+    pdl_trigger();
+    const int hd = (int)c.head_dim, cap = (int)c.capacity, H = (int)c.n_kv_head, h = blockIdx.y, which = blockIdx.z;
+    float* out = which ? v_out : k_out;
+    if (!out) return;
+    const int8_t* codes = (which ? c.v : c.k) + ((size_t)h * cap + row0) * hd;
+    const float* scales = (which ? c.v_scale : c.k_scale) + (size_t)h * (cap >> 5);
+    const int per = hd / 4;  // pieces of a row
+    const long long total = (long long)n * per;
+    constexpr int U = 4;
+    for (long long i0 = (long long)blockIdx.x * kThreads * U + threadIdx.x; i0 < total; i0 += (long long)gridDim.x * kThreads * U) {
+        char4 q[U];
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long i = i0 + u * kThreads;
+            if (i < total) {
+                q[u] = *reinterpret_cast<const char4*>(codes + i * 4);
+                s[u] = scales[(row0 + (int)(i / per)) >> 5];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long i = i0 + u * kThreads;
+            if (i < total) {
+                const int r = (int)(i / per);
+                // (a caller's buffer is aligned to its floats only)
+                float* o = out + ((long long)r * H + h) * hd + (i - (long long)r * per) * 4;
+                const float4 x = dequantise4(q[u], s[u]);
+                if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+                    *reinterpret_cast<float4*>(o) = x;
+                } else {
+                    o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// eviction
+// ---------------------------------------------------------------------------
+// Two launches. The first finds each head's kept rows: a cluster of CTAs per
+// head takes the m-th largest weight by four rounds of 8-bit radix counts
+// (weights as ordered bit patterns, so the selection is exact), then writes
+// the rows above it, and the lowest rows equal to it, in order: each warp owns
+// a range of rows, and its place is a prefix sum over the warps. The second
+// gathers: one CTA per new block, head and K or V.
+
+constexpr int kSelCluster = 8;
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+
+// A weight as an unsigned number of the same order; every NaN is the largest.
+__device__ __forceinline__ unsigned order_bits(float w) {
+    const unsigned u = __float_as_uint(w + 0.f);  // -0 as 0
+    if (w != w) return 0xffffffffu;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ unsigned remote_u32(const unsigned* p, int rank) {
+    unsigned a, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+struct SelectArgs {
+    const int* past;
+    const float* w;  // [H][cap]
+    int cap, keep, sink, recent;
+    int* kept;       // [H][keep]
+};
+
+__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_constant__ SelectArgs a) {
+    __shared__ unsigned hist[2][256];
+    __shared__ unsigned sum[256];
+    __shared__ unsigned counts[2 * kSelWarps];       // rows above / equal of this CTA's warps
+    __shared__ unsigned all[2 * kSelWarps * kSelCluster];
+    __shared__ unsigned found[2];
+    pdl_wait();
+    pdl_trigger();
+    const int h = blockIdx.x / kSelCluster, rank = blockIdx.x % kSelCluster;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int len = min(max(*a.past, 0), a.cap);
+    int* kept = a.kept + (size_t)h * a.keep;
+    if (len <= a.keep) {  // everything stays (the whole cluster takes this path)
+        for (int i = rank * kSelThreads + tid; i < a.keep; i += kSelCluster * kSelThreads) kept[i] = i < len ? i : -1;
+        return;
+    }
+    const float* w = a.w + (size_t)h * a.cap;
+    const int lo = a.sink, hi = len - a.recent, m = a.keep - a.sink - a.recent;  // hi - lo > m >= 0
+    for (int i = rank * kSelThreads + tid; i < a.sink; i += kSelCluster * kSelThreads) kept[i] = i;
+    for (int i = rank * kSelThreads + tid; i < a.recent; i += kSelCluster * kSelThreads) kept[a.keep - a.recent + i] = hi + i;
+    if (m == 0) return;
+
+    // the m-th largest, eight bits a round
+    unsigned prefix = 0, left = (unsigned)m;
+    for (int round = 0; round < 4; ++round) {
+        const int shift = 24 - 8 * round;
+        unsigned* hs = hist[round & 1];
+        for (int i = tid; i < 256; i += kSelThreads) hs[i] = 0;
+        __syncthreads();
+        for (int i = lo + rank * kSelThreads + tid; i < hi; i += kSelCluster * kSelThreads) {
+            const unsigned u = order_bits(w[i]);
+            if (round == 0 || (u >> (shift + 8)) == prefix) atomicAdd(&hs[(u >> shift) & 255], 1u);
+        }
+        cluster_barrier();
+        // bin 255 - tid and the bins above it, over the cluster
+        if (tid < 256) {
+            unsigned c = 0;
+#pragma unroll
+            for (int r = 0; r < kSelCluster; ++r) c += remote_u32(&hs[255 - tid], r);
+            unsigned s = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += v;
+            }
+            sum[tid] = s;
+        }
+        __syncthreads();
+        if (tid < 256) {
+            unsigned base = 0;
+            for (int k = 0; k < warp; ++k) base += sum[k * 32 + 31];
+            const unsigned upto = base + sum[tid], above = tid == 0 ? 0u : (lane ? base + sum[tid - 1] : base);
+            if (above < left && left <= upto) {
+                found[0] = 255u - tid;
+                found[1] = left - above;
+            }
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | found[0];
+        left = found[1];
+    }
+    const unsigned T = prefix;  // rows above T stay, and the first `left` rows equal to it
+
+    // the warps' ranges, in row order over the cluster
+    const int nw = kSelCluster * kSelWarps, gw = rank * kSelWarps + warp;
+    const int span = ((hi - lo + nw - 1) / nw + 31) & ~31;
+    const int s0 = min(lo + gw * span, hi), s1 = min(s0 + span, hi);
+    unsigned above = 0, equal = 0;
+    for (int i = s0 + lane; i < s1; i += 32) {
+        const unsigned u = order_bits(w[i]);
+        above += u > T;
+        equal += u == T;
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) {
+        counts[warp] = above;
+        counts[kSelWarps + warp] = equal;
+    }
+    cluster_barrier();
+    for (int i = tid; i < 2 * nw; i += kSelThreads) {
+        const int r = i / (2 * kSelWarps);
+        all[i] = remote_u32(&counts[i % (2 * kSelWarps)], r);
+    }
+    __syncthreads();
+    unsigned before = 0, ties = 0;  // of the warps before this one
+    for (int k = lane; k < gw; k += 32) {
+        before += all[(k / kSelWarps) * 2 * kSelWarps + k % kSelWarps];
+        ties += all[(k / kSelWarps) * 2 * kSelWarps + kSelWarps + k % kSelWarps];
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    for (int i0 = s0; i0 < s1; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned u = i < s1 ? order_bits(w[i]) : 0u;
+        const bool up = i < s1 && u > T, eq = i < s1 && u == T;
+        const unsigned bu = __ballot_sync(0xffffffffu, up), be = __ballot_sync(0xffffffffu, eq);
+        const unsigned mask = (1u << lane) - 1u;
+        const unsigned t = ties + __popc(be & mask);  // equal rows before this one
+        if (up || (eq && t < left)) kept[a.sink + before + __popc(bu & mask) + min(t, left)] = i;
+        before += __popc(bu);
+        ties += __popc(be);
+    }
+    cluster_barrier();  // no CTA leaves while another reads its counts
+}
+
+struct GatherArgs {
+    neon_kv8_t src, dst;
+    const float* w;
+    float* wd;
+    const int* kept;
+    int keep;
+    int pairs, half, rotate;
+    RopeTurns turns;
+};
+
+template <int P>
+__global__ void __launch_bounds__(kThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
+    extern __shared__ float4 rowbuf[];  // with rotation: the block's rows
+    __shared__ float red[kThreads / 32];
+    __shared__ int from[32];
+    pdl_wait();
+    pdl_trigger();
+    const int hd = (int)a.src.head_dim, H = (int)a.src.n_kv_head, cap = (int)a.src.capacity, dcap = (int)a.dst.capacity;
+    const int b = blockIdx.x, h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+    const int len = min(max(*a.src.past, 0), cap), m = min(len, a.keep);
+    if (b == 0) {
+        if (tid < 2) a.dst.tail_block[((size_t)which * H + h) * 2 + tid] = -1;
+        if (h == 0 && which == 0 && tid == 0) *a.dst.past = m;
+    }
+    const int rows = min(32, m - 32 * b);
+    if (rows <= 0) return;
+    if (tid < 32) {
+        const int r = tid < rows ? a.kept[(size_t)h * a.keep + 32 * b + tid] : -1;
+        from[tid] = r;
+        if (which == 0 && tid < rows) a.wd[(size_t)h * dcap + 32 * b + tid] = a.w[(size_t)h * cap + r];
+    }
+    __syncthreads();
+    // kept rows ascend: the last one in place means that all of the block's are
+    const bool stay = from[rows - 1] == 32 * b + rows - 1;
+    const int8_t* sc = (which ? a.src.v : a.src.k) + (size_t)h * cap * hd;
+    const float* ssc = (which ? a.src.v_scale : a.src.k_scale) + (size_t)h * (cap >> 5);
+    int8_t* dc = (which ? a.dst.v : a.dst.k) + ((size_t)h * dcap + 32 * b) * hd;
+    float* dsc = (which ? a.dst.v_scale : a.dst.k_scale) + (size_t)h * (dcap >> 5);
+    char4 q[P];
+    float s[P];
+    float4 x[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int e = (i * kThreads + tid) * 4, r = e / hd;
+        if (r < rows) {
+            const int f = from[r];
+            q[i] = *reinterpret_cast<const char4*>(sc + (size_t)f * hd + (e - r * hd));
+            s[i] = ssc[f >> 5];
+        }
+    }
+    if (stay) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int e = (i * kThreads + tid) * 4;
+            if (e / hd < rows) *reinterpret_cast<char4*>(dc + e) = q[i];
+        }
+        if (tid == 0) dsc[b] = ssc[b];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int e = (i * kThreads + tid) * 4;
+        x[i] = e / hd < rows ? dequantise4(q[i], s[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (a.rotate && which == 0) {
+        float* rb = reinterpret_cast<float*>(rowbuf);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int e = (i * kThreads + tid) * 4;
+            if (e / hd < rows) rowbuf[e / 4] = x[i];
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * a.pairs; i += kThreads) {
+            const int r = i / a.pairs, p = i - r * a.pairs;
+            const int delta = 32 * b + r - from[r];
+            if (delta == 0) continue;
+            const float2 c = turn(a.turns.f[p], delta);
+            float* u = rb + r * hd + (a.half ? p : 2 * p);
+            float* v = u + (a.half ? a.pairs : 1);
+            const float x0 = *u, x1 = *v;
+            *u = __fmaf_rn(x0, c.x, -__fmul_rn(x1, c.y));
+            *v = __fmaf_rn(x0, c.y, __fmul_rn(x1, c.x));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int e = (i * kThreads + tid) * 4;
+            if (e / hd < rows) x[i] = rowbuf[e / 4];
+        }
+    }
+    const float sn = block_scale(block_amax(x, red));
+    const float inv = __fdiv_rn(1.f, sn);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int e = (i * kThreads + tid) * 4;
+        if (e / hd < rows) *reinterpret_cast<char4*>(dc + e) = quantise4(x[i], sn, inv);
+    }
+    if (tid == 0) dsc[b] = sn;
+}
+
+}  // namespace
+
+int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, size_t vs, size_t n, int type, int device,
+               cudaStream_t st) {
+    unsigned* err = neon_internal::device_error_word(device);
+    if (!err) return NEON_ERR_CUDA;
+    const size_t eb = type_bytes(type);
+    AppendArgs a{};
+    a.c = c;
+    a.k = k;
+    a.v = v;
+    a.ks = (long long)ks;
+    a.vs = (long long)vs;
+    a.n = (int)n;
+    a.vec = aligned(k, 4 * eb) && aligned(v, 4 * eb) && ks % 4 == 0 && vs % 4 == 0;
+    a.err = err;
+    AppendKernel kern = type == NEON_GGML_F32   ? append_kernel_for<float>((int)c.head_dim)
+                        : type == NEON_GGML_F16 ? append_kernel_for<__half>((int)c.head_dim)
+                                                : append_kernel_for<__nv_bfloat16>((int)c.head_dim);
+    // rows past .. past + n - 1 touch at most (n + 62) / 32 blocks; the first CTA takes two of them
+    const unsigned blocks = (unsigned)std::max<size_t>(1, (n + 62) / 32 - 1);
+    return launch("kv8_append_kernel", kern, dim3(blocks, c.n_kv_head, 2), kThreads, 0, st, 1, a);
+}
+
+int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
+              size_t recent, const neon_rope_t* rope, int32_t* kept, cudaStream_t st) {
+    SelectArgs s{src.past, w, (int)src.capacity, (int)keep, (int)sink, (int)recent, kept};
+    int rc = launch("kv8_select_kernel", kv8_select_kernel, dim3(src.n_kv_head * kSelCluster), kSelThreads, 0, st,
+                    kSelCluster, s);
+    if (rc) return rc;
+    GatherArgs g{};
+    g.src = src;
+    g.dst = dst;
+    g.w = w;
+    g.wd = wd;
+    g.kept = kept;
+    g.keep = (int)keep;
+    if (rope) {
+        g.rotate = 1;
+        g.pairs = (int)rope->n_dims / 2;
+        g.half = rope->layout == NEON_ROPE_HALF;
+        rope_turns(*rope, &g.turns);
+    }
+    const int hd = (int)src.head_dim;
+    auto kern = hd <= 64 ? kv8_gather_kernel<2> : hd <= 128 ? kv8_gather_kernel<4> : kv8_gather_kernel<8>;
+    return launch("kv8_gather_kernel", kern, dim3((unsigned)((keep + 31) / 32), src.n_kv_head, 2), kThreads,
+                  rope ? (size_t)32 * hd * sizeof(float) : 0, st, 1, g);
+}
+
+}  // namespace longctx
+
+using namespace longctx;
+using neon_internal::error;
+
+extern "C" {
+
+int neon_cuda_kv8_append(const neon_kv8_t* cache, const void* dK, size_t k_stride, const void* dV, size_t v_stride,
+                         size_t n, int type, void* stream) {
+    int rc = kv8_check_buffers(cache);
+    if (rc) return rc;
+    const size_t eb = type_bytes(type);
+    if (!eb) return error(NEON_ERR_UNSUPPORTED, "kv8: type must be F32, F16 or BF16");
+    if (n == 0) return NEON_OK;
+    if (!dK || !dV) return error(NEON_ERR_INVALID, "kv8: null K or V");
+    if (n > cache->capacity) return error(NEON_ERR_INVALID, "kv8: more tokens than the cache's capacity");
+    const size_t row = (size_t)cache->n_kv_head * cache->head_dim;
+    if (n > 1 && (k_stride < row || v_stride < row)) return error(NEON_ERR_INVALID, "kv8: stride smaller than the heads");
+    if (!aligned(dK, eb) || !aligned(dV, eb)) return error(NEON_ERR_INVALID, "kv8: buffer not aligned to its type");
+    OnDevice dev(cache->k);
+    if (dev.rc) return dev.rc;
+    return kv8_append(*cache, dK, k_stride, dV, v_stride, n, type, dev.device, (cudaStream_t)stream);
+}
+
+int neon_cuda_kv8_read(const neon_kv8_t* cache, size_t row0, size_t n, float* dK_out, float* dV_out, void* stream) {
+    int rc = kv8_check_buffers(cache);
+    if (rc) return rc;
+    if (row0 > cache->capacity || n > cache->capacity - row0) return error(NEON_ERR_INVALID, "kv8: rows out of range");
+    if (!aligned(dK_out, 4) || !aligned(dV_out, 4)) return error(NEON_ERR_INVALID, "kv8: buffer not aligned to its type");
+    if (n == 0 || (!dK_out && !dV_out)) return NEON_OK;
+    OnDevice dev(cache->k);
+    if (dev.rc) return dev.rc;
+    const int sms = neon_internal::device_sms(dev.device);
+    if (sms < 0) return NEON_ERR_CUDA;
+    const long long pieces = (long long)n * (cache->head_dim / 4);
+    const long long want = (pieces + kThreads * 4 - 1) / (kThreads * 4);
+    return launch("kv8_read_kernel", kv8_read_kernel, dim3((unsigned)std::min<long long>(want, 1 << 20), cache->n_kv_head, 2),
+                  kThreads, 0, (cudaStream_t)stream, 1, *cache, (int)row0, (int)n, dK_out, dV_out);
+}
+
+int neon_cuda_kv8_evict(const neon_kv8_t* src, const float* d_weight, const neon_kv8_t* dst, float* d_weight_dst,
+                        size_t keep, size_t sink, size_t recent, const neon_rope_t* rope, int32_t* d_kept,
+                        void* stream) {
+    int rc = kv8_check_buffers(src);
+    if (!rc) rc = kv8_check_buffers(dst);
+    if (!rc && rope) rc = rope_check(rope, src->head_dim);
+    if (rc) return rc;
+    if (!d_weight || !d_weight_dst || !d_kept) return error(NEON_ERR_INVALID, "kv8: null weights or kept rows");
+    if (!aligned(d_weight, 4) || !aligned(d_weight_dst, 4) || !aligned(d_kept, 4))
+        return error(NEON_ERR_INVALID, "kv8: buffer not aligned to its type");
+    if (src->n_kv_head != dst->n_kv_head || src->head_dim != dst->head_dim)
+        return error(NEON_ERR_INVALID, "kv8: the caches' heads differ");
+    if (keep == 0 || keep > dst->capacity) return error(NEON_ERR_INVALID, "kv8: keep must be 1 to the new cache's capacity");
+    if (sink > keep || recent > keep - sink) return error(NEON_ERR_INVALID, "kv8: sink + recent above keep");
+    if (src->k == dst->k || src->v == dst->v || src->k_scale == dst->k_scale || src->v_scale == dst->v_scale ||
+        src->past == dst->past || d_weight == d_weight_dst)
+        return error(NEON_ERR_INVALID, "kv8: eviction needs separate buffers");
+    OnDevice dev(src->k);
+    if (dev.rc) return dev.rc;
+    if (neon_internal::device_sms(dev.device) < 0) return NEON_ERR_CUDA;
+    return kv8_evict(*src, d_weight, *dst, d_weight_dst, keep, sink, recent, rope, d_kept, (cudaStream_t)stream);
+}
+
+}  // extern "C"

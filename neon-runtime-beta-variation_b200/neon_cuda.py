@@ -48,6 +48,9 @@ GGML_Q4_K = 12
 GGML_Q5_K = 13
 GGML_Q6_K = 14
 GGML_BF16 = 30
+ROPE_INTERLEAVED = 0
+ROPE_HALF = 1
+KV8_BLOCK = 32
 SHARD_NONE = 0
 SHARD_ROWS = 1
 SHARD_COLS = 2
@@ -72,6 +75,12 @@ C_ENTRY_POINTS = (
     "neon_cuda_sync",
     "neon_cuda_launch_count",
     "neon_cuda_matvec_q4_0_noalloc",
+    "neon_cuda_rope",
+    "neon_cuda_kv8_append",
+    "neon_cuda_kv8_read",
+    "neon_cuda_kv8_attention",
+    "neon_cuda_kv8_attention_workspace",
+    "neon_cuda_kv8_evict",
     "neon_cuda_model_create",
     "neon_cuda_model_set_tensor",
     "neon_cuda_model_set_quantize",
@@ -119,6 +128,21 @@ class _ModelConfig(C.Structure):
                                           "n_ff", "ctx_len")] + [
         ("rope_base", C.c_float), ("rope_scale", C.c_float), ("rope_dim_count", C.c_uint32),
         ("norm_eps", C.c_float), ("plain_ffn", C.c_uint32)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [(f, C.c_uint32) for f in ("n_dims", "layout", "freq_dim", "orig_ctx")] + [
+        (f, C.c_double) for f in ("base", "scale", "yarn", "beta_fast", "beta_slow", "magnitude")] + [
+        ("factors", C.POINTER(C.c_float))]
+
+
+class _RopeTarget(C.Structure):
+    _fields_ = [("X", _vp), ("Y", _vp), ("x_stride", _sz), ("y_stride", _sz), ("n_heads", _sz)]
+
+
+class _Kv8(C.Structure):
+    _fields_ = [(f, C.c_uint32) for f in ("n_kv_head", "head_dim", "capacity")] + [
+        (f, _vp) for f in ("k", "v", "k_scale", "v_scale", "tail", "tail_block", "past")]
 
 
 class NeonError(RuntimeError):
@@ -172,6 +196,14 @@ def load(path: str | None = None) -> C.CDLL:
         L.neon_cuda_set_attn_rows.argtypes = [C.c_int, C.c_int]
         L.neon_cuda_set_attn_head_split.argtypes = [C.c_int]
         L.neon_cuda_matvec_q4_0_noalloc.argtypes = [_vp, _vp, _sz, _vp, _sz, _sz, _vp]
+        L.neon_cuda_rope.argtypes = [C.POINTER(_Rope), C.c_int, _vp, _sz, _sz, C.POINTER(_RopeTarget), _sz, C.c_int, _vp]
+        L.neon_cuda_kv8_append.argtypes = [C.POINTER(_Kv8), _vp, _sz, _vp, _sz, _sz, C.c_int, _vp]
+        L.neon_cuda_kv8_read.argtypes = [C.POINTER(_Kv8), _sz, _sz, _vp, _vp, _vp]
+        L.neon_cuda_kv8_attention.argtypes = [C.POINTER(_Kv8), _vp, _sz, _vp, _sz, _sz, _sz, C.c_float, C.c_int, _vp,
+                                              _vp, _sz, _vp]
+        L.neon_cuda_kv8_attention_workspace.argtypes = [C.POINTER(_Kv8), _sz, _sz, C.POINTER(_sz)]
+        L.neon_cuda_kv8_evict.argtypes = [C.POINTER(_Kv8), _vp, C.POINTER(_Kv8), _vp, _sz, _sz, _sz, C.POINTER(_Rope),
+                                          _vp, _vp]
         L.neon_cuda_model_create.argtypes = [C.POINTER(_ModelConfig), C.POINTER(_vp)]
         L.neon_cuda_model_set_tensor.argtypes = [_vp, C.c_int, C.c_int, _vp, _sz, C.c_int, _sz, _sz]
         L.neon_cuda_model_forward.argtypes = [_vp, _vp, _sz, _vp]
@@ -387,6 +419,117 @@ def quantize_q8_0(X, cols: int, seq: int, d_out, q_out, x_stride: int | None = N
     """Device Q8_0 activation quantisation (bit-exact with quantize_rows_q8_0)."""
     x_stride = cols if x_stride is None else x_stride
     _check(load().neon_cuda_quantize_q8_0(_ptr(X), x_stride, cols, seq, _ptr(d_out), _ptr(q_out),
+                                          _vp(_stream(stream))))
+
+
+# ---------------------------------------------------------------------------
+# long contexts: rotary positions, a KV cache in 8 bits, eviction
+# ---------------------------------------------------------------------------
+
+class Rope:
+    """How positions turn the pairs of a head (neon_rope_t): the first n_dims
+    values of each head, pair i by position * base^(-2i / (freq_dim or n_dims))
+    / factors[i] / scale; interleaved pairs (2i, 2i + 1), or with ``half`` (i,
+    i + n_dims / 2). With yarn > 0 pairs that turn often in the first orig_ctx
+    positions keep their own frequency. ``magnitude`` multiplies what is
+    rotated."""
+
+    def __init__(self, n_dims: int, half: bool = False, base: float = 10000.0, scale: float = 1.0, yarn: float = 0.0,
+                 orig_ctx: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0, magnitude: float = 1.0,
+                 freq_dim: int = 0, factors=None):
+        self._factors = None
+        if factors is not None:
+            self._factors = np.ascontiguousarray(factors, np.float32)
+            if self._factors.shape != (n_dims // 2,):
+                raise NeonError("rope: factors needs one divisor per pair")
+        self._c = _Rope(int(n_dims), ROPE_HALF if half else ROPE_INTERLEAVED, int(freq_dim), int(orig_ctx), float(base),
+                        float(scale), float(yarn), float(beta_fast), float(beta_slow), float(magnitude),
+                        None if self._factors is None else self._factors.ctypes.data_as(C.POINTER(C.c_float)))
+
+
+def rope(spec: Rope, pos, n: int, head_dim: int, targets, type: int = GGML_F32, backward: bool = False,
+         stream=None) -> None:
+    """Rotate n positions (pos: n int32 on the device) of 1 to 4 tensors:
+    targets are (X, Y, n_heads) or (X, Y, n_heads, x_stride, y_stride), device
+    buffers of ``type``; Y may be X. ``backward`` rotates the other way: the
+    gradient with respect to X."""
+    arr = (_RopeTarget * len(targets))()
+    for a, t in zip(arr, targets):
+        row = int(t[2]) * head_dim
+        a.X, a.Y, a.n_heads = _ptr(t[0]), _ptr(t[1]), int(t[2])
+        a.x_stride, a.y_stride = (int(t[3]), int(t[4])) if len(t) > 3 else (row, row)
+    _check(load().neon_cuda_rope(C.byref(spec._c), int(type), _ptr(pos), n, head_dim, arr, len(targets),
+                                 1 if backward else 0, _vp(_stream(stream))))
+
+
+class Kv8Cache:
+    """A KV cache in 8 bits over the caller's device buffers (neon_kv8_t):
+    int8 codes k, v [n_kv_head][capacity][head_dim]; fp32 scales [n_kv_head]
+    [capacity / 32]; tail fp32 [2][2][n_kv_head][32][head_dim]; tail_block int32
+    [2][n_kv_head][2], -1 at the start; past, one int32: the rows held before
+    the current step's tokens. The object keeps the buffers alive."""
+
+    def __init__(self, n_kv_head: int, head_dim: int, capacity: int, k, v, k_scale, v_scale, tail, tail_block, past):
+        self.n_kv_head, self.head_dim, self.capacity = int(n_kv_head), int(head_dim), int(capacity)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.tail, self.tail_block, self.past = tail, tail_block, past
+        self._c = _Kv8(self.n_kv_head, self.head_dim, self.capacity,
+                       *[_ptr(b) for b in (k, v, k_scale, v_scale, tail, tail_block, past)])
+
+    @classmethod
+    def empty(cls, n_kv_head: int, head_dim: int, capacity: int, device="cuda") -> "Kv8Cache":
+        """A new, empty cache in torch tensors."""
+        import torch
+
+        def codes():
+            return torch.zeros(n_kv_head, capacity, head_dim, dtype=torch.int8, device=device)
+
+        def scales():
+            return torch.zeros(n_kv_head, capacity // KV8_BLOCK, device=device)
+
+        return cls(n_kv_head, head_dim, capacity, codes(), codes(), scales(), scales(),
+                   torch.zeros(2, 2, n_kv_head, KV8_BLOCK, head_dim, device=device),
+                   torch.full((2, n_kv_head, 2), -1, dtype=torch.int32, device=device),
+                   torch.zeros(1, dtype=torch.int32, device=device))
+
+    def append(self, K, V, n: int, type: int = GGML_F32, k_stride: int | None = None, v_stride: int | None = None,
+               stream=None) -> None:
+        """K and V rows of n new tokens to rows past .. past + n - 1 (past itself is left)."""
+        row = self.n_kv_head * self.head_dim
+        _check(load().neon_cuda_kv8_append(C.byref(self._c), _ptr(K), row if k_stride is None else k_stride, _ptr(V),
+                                           row if v_stride is None else v_stride, n, int(type), _vp(_stream(stream))))
+
+    def read(self, row0: int, n: int, k_out, v_out, stream=None) -> None:
+        """Rows [row0, row0 + n) as fp32 values [n][n_kv_head][head_dim] (an output may be None)."""
+        _check(load().neon_cuda_kv8_read(C.byref(self._c), row0, n, _ptr(k_out), _ptr(v_out), _vp(_stream(stream))))
+
+    def attention_workspace(self, n_head: int, n: int) -> int:
+        """Bytes of workspace that attention() of up to n tokens needs."""
+        b = _sz()
+        _check(load().neon_cuda_kv8_attention_workspace(C.byref(self._c), n, n_head, C.byref(b)))
+        return b.value
+
+    def attention(self, Q, O, n: int, n_head: int, workspace, type: int = GGML_F32, scale: float = 0.0, weight=None,
+                  q_stride: int | None = None, o_stride: int | None = None, workspace_bytes: int | None = None,
+                  stream=None) -> None:
+        """Causal attention of the n tokens at rows past .. past + n - 1 (already
+        appended); ``weight`` [n_kv_head][capacity] accumulates each cached row's
+        attention weight."""
+        row = n_head * self.head_dim
+        if workspace_bytes is None:
+            workspace_bytes = workspace.nbytes
+        _check(load().neon_cuda_kv8_attention(C.byref(self._c), _ptr(Q), row if q_stride is None else q_stride, _ptr(O),
+                                              row if o_stride is None else o_stride, n, n_head, scale, int(type),
+                                              _ptr(weight), _ptr(workspace), workspace_bytes, _vp(_stream(stream))))
+
+    def evict(self, dst: "Kv8Cache", keep: int, sink: int, recent: int, weight, dst_weight, kept, rope: Rope | None = None,
+              stream=None) -> None:
+        """Into dst: each KV head's first sink rows, last recent rows and, of the
+        others, those of the largest accumulated weight, keep rows in all; kept
+        [n_kv_head][keep] int32 says which. With ``rope`` the K rows that move are
+        rotated by their new row minus their old."""
+        _check(load().neon_cuda_kv8_evict(C.byref(self._c), _ptr(weight), C.byref(dst._c), _ptr(dst_weight), keep, sink,
+                                          recent, None if rope is None else C.byref(rope._c), _ptr(kept),
                                           _vp(_stream(stream))))
 
 
