@@ -27,7 +27,7 @@ NVCC_FLAGS = [
     "--expt-relaxed-constexpr",
 ]
 
-SOURCES = ["neon_cuda.cu", "neon_decode.cu", "neon_comm.cu", "neon_rope.cu", "neon_kv8.cu", "neon_kv8_attn.cu"]
+SOURCES = ["neon_cuda.cu", "neon_decode.cu", "neon_comm.cu", "neon_rope.cu", "neon_kv8.cu", "neon_kv8_attn.cu", "neon_kv8_prompt.cu"]
 
 
 def _nvcc() -> str:

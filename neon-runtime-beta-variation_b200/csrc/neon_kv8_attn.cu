@@ -9,21 +9,17 @@
 // split into two fp16 terms (hi + lo, 22 bits), of which every product is
 // exact. Scales are applied in fp32 to the scores, and to p before the second
 // product, where p is scaled so that its split keeps its bits (see kPUp).
-#include "neon_longctx.cuh"
-#include "neon_kv8.h"
+#include "neon_kv8_attn.cuh"
 
 #include <algorithm>
 
 namespace longctx {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 // p (at most 1, times s_v over the largest s_v so far) is multiplied by 2^14
 // before its split: hi stays below fp16's 65504, and lo keeps values down to
 // 2^-38 of the row's largest.
 constexpr float kPUp = 16384.f, kPDown = 1.f / 16384.f;
-
-// ---- fragments ----
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -31,55 +27,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-
-// 1024 + u is the half 0x6400 | u for a byte u; with u = code + 128 the code is
-// that less 1152, exactly.
-__device__ __forceinline__ uint32_t unbias(uint32_t h) { return h2_bits(__hsub2(bits_h2(h), bits_h2(0x64806480u))); }
-// bytes 0, 1 and 2, 3 of a word of codes + 128 as two half2
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return unbias(__byte_perm(w, 0x64646464u, 0x4140)); }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return unbias(__byte_perm(w, 0x64646464u, 0x4342)); }
-
-// x, y as hi and lo half2 terms
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
-}
-
-__device__ __forceinline__ float q_value(const void* q, int type, long long i) {
-    return type == NEON_GGML_F32   ? ((const float*)q)[i]
-           : type == NEON_GGML_F16 ? __half2float(((const __half*)q)[i])
-                                   : __bfloat162float(((const __nv_bfloat16*)q)[i]);
-}
-__device__ __forceinline__ void o_store(void* o, int type, long long i, float v) {
-    if (type == NEON_GGML_F32) ((float*)o)[i] = v;
-    else if (type == NEON_GGML_F16) ((__half*)o)[i] = __float2half_rn(v);
-    else ((__nv_bfloat16*)o)[i] = __float2bfloat16_rn(v);
-}
-
-// The rows that token t may attend to.
-__device__ __forceinline__ int keys_of(int past, int t, int cap) {
-    return (int)max(0LL, min((long long)past + t + 1, (long long)cap));
-}
-
-// Rows of one KV head: row r is query head r % group of token r / group.
-struct AttnArgs {
-    neon_kv8_t c;
-    const void* q;
-    void* o;
-    long long qs, os;
-    int n, n_head, group, type;
-    float scale;   // softmax scale * log2(e)
-    float* weight;
-    int nsplit;
-    float* stats;  // [H][rows][2]: the row's final m and 1 / l (0 for a row without keys)
-    float* part;   // [H][row groups][nsplit][8][hd + 2]: o, m, l of a split (o unnormalised)
-    unsigned* err;
-};
 
 // ---------------------------------------------------------------------------
 // Eight rows of one KV head over a share of the cache. The MMA's 16 rows hold
@@ -127,15 +74,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
     // the keys of the group's rows, and this warp's share of them in tiles
     const int past = *a.c.past;
     const int row = grp * 8 + g, tok = row / a.group;
-    const int last_tok = min(grp * 8 + 7, rows - 1) / a.group;
-    const int keys = keys_of(past, last_tok, cap);
     const int limit = row < rows ? keys_of(past, tok, cap) : 0;
-    const int tiles = (keys + 31) >> 5;
-    int per_cta = (tiles + a.nsplit - 1) / a.nsplit;
-    per_cta = max(per_cta, min(tiles, 2 * kRowWarps));  // two tiles per warp before another CTA joins
-    const int active = per_cta ? (tiles + per_cta - 1) / per_cta : 1;
-    if (split >= active) return;
-    const int c0 = split * per_cta, c1 = min(c0 + per_cta, tiles);
+    const Shares sh = shares_of(a, past, grp);
+    if (split >= sh.active) return;
+    const int c0 = split * sh.per, c1 = min(c0 + sh.per, sh.tiles);
     const int per_warp = (c1 - c0 + kRowWarps - 1) / kRowWarps;
     const int w0 = min(c0 + warp * per_warp, c1), w1 = min(w0 + per_warp, c1);
 
@@ -231,7 +173,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
         const float mu = mt == -INFINITY ? 0.f : mt;
-        const float down = exp2f(m - mu);
+        const float down = ex2(m - mu);
         float vdown = 1.f;
         if (vs > vref) {
             vdown = vref / vs;
@@ -254,7 +196,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
             for (int hf = 0; hf < 2; ++hf) {
                 const int j = 2 * k + hf;
                 const bool on0 = t[j][0] != -INFINITY, on1 = t[j][1] != -INFINITY;
-                const float p0 = exp2f(t[j][0] - mu), p1 = exp2f(t[j][1] - mu);
+                const float p0 = ex2(t[j][0] - mu), p1 = ex2(t[j][1] - mu);
                 l += p0 + p1;
                 split2(on0 ? p0 * vr : 0.f, on1 ? p1 * vr : 0.f, pf[k][2 * hf], pf[k][2 * hf + 1]);
             }
@@ -320,8 +262,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
         ml[(warp * 8 + g) * 2 + 1] = l;
     }
     __syncthreads();
-    const int nz = (rows + 7) / 8;
-    float* part = a.part + (((size_t)kvh * nz + grp) * a.nsplit + split) * 8 * (hd + 2);
     for (int r = warp; r < 8; r += kRowWarps) {
         const int rr = grp * 8 + r;
         if (rr >= rows) continue;
@@ -331,27 +271,23 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
         float f[kRowWarps], ll = 0.f;
 #pragma unroll
         for (int w = 0; w < kRowWarps; ++w) {
-            f[w] = exp2f(ml[(w * 8 + r) * 2] - mu);
+            f[w] = ex2(ml[(w * 8 + r) * 2] - mu);
             ll += f[w] * ml[(w * 8 + r) * 2 + 1];
         }
-        const float inv = mm == -INFINITY && ll == 0.f ? 0.f : 1.f / ll;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
         const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
+        const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
         for (int d = lane; d < hd; d += 32) {
             float v = 0.f;
 #pragma unroll
             for (int w = 0; w < kRowWarps; ++w) v += f[w] * mo[(w * 8 + r) * HD + d];
-            if (active == 1) o_store(a.o, a.type, ob + d, v * inv);
-            else part[r * (hd + 2) + d] = v;
+            if (sh.active == 1) o_store(a.o, a.type, ob + d, v * inv);
+            else a.part_o[pr * hd + d] = v;
         }
         if (lane == 0) {
-            if (active == 1) {
-                float* st = a.stats + ((size_t)kvh * rows + rr) * 2;
-                st[0] = mu;
-                st[1] = inv;
-            } else {
-                part[r * (hd + 2) + hd] = mm;
-                part[r * (hd + 2) + hd + 1] = ll;
-            }
+            float* st = sh.active == 1 ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
+            st[0] = sh.active == 1 ? mu : mm;
+            st[1] = sh.active == 1 ? inv : ll;
         }
     }
 }
@@ -360,35 +296,29 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
 __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ AttnArgs a) {
     pdl_wait();
     pdl_trigger();
-    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, rows = a.n * a.group, nz = (rows + 7) / 8;
+    const int hd = (int)a.c.head_dim, rows = a.n * a.group;
     const int lane = threadIdx.x & 31;
     const int rr = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y;
     if (rr >= rows) return;
-    const int grp = rr / 8, r = rr & 7;
-    const int past = *a.c.past;
-    const int last_tok = min(grp * 8 + 7, rows - 1) / a.group;
-    const int keys = keys_of(past, last_tok, cap);
-    const int tiles = (keys + 31) >> 5;
-    int per_cta = (tiles + a.nsplit - 1) / a.nsplit;
-    per_cta = max(per_cta, min(tiles, 2 * kRowWarps));
-    const int active = per_cta ? (tiles + per_cta - 1) / per_cta : 1;
-    if (active == 1) return;
-    const size_t step = 8 * (size_t)(hd + 2);
-    const float* part = a.part + ((size_t)kvh * nz + grp) * a.nsplit * step + r * (hd + 2);
+    const Shares sh = shares_of(a, *a.c.past, rr / a.unit);
+    if (sh.active == 1) return;
+    const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit;
+    const float *ml = a.part_ml + pr * 2, *po = a.part_o + pr * hd;
     float mm = -INFINITY;
-    for (int s = lane; s < active; s += 32) mm = fmaxf(mm, part[s * step + hd]);
+    for (int s = lane; s < sh.active; s += 32) mm = fmaxf(mm, ml[2 * s]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
     const float mu = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f, v[8] = {};
-    for (int s = 0; s < active; ++s) {
-        const float f = exp2f(part[s * step + hd] - mu);
-        ll += f * part[s * step + hd + 1];
+#pragma unroll 4
+    for (int s = 0; s < sh.active; ++s) {
+        const float f = ex2(ml[2 * s] - mu);
+        ll += f * ml[2 * s + 1];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd) v[i] += f * part[s * step + lane + 32 * i];
+            if (lane + 32 * i < hd) v[i] += f * po[(size_t)s * hd + lane + 32 * i];
     }
-    const float inv = mm == -INFINITY && ll == 0.f ? 0.f : 1.f / ll;
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
     const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -492,7 +422,7 @@ __global__ void __launch_bounds__(256, 1) kv8_weight_kernel(const __grid_constan
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = tile * 32 + 8 * j + 2 * tq + e;
-                if (key < lim) sum[j][e] += exp2f((sc[j][e] + sc[j][e + 2]) * fac - mrow) * irow;
+                if (key < lim) sum[j][e] += ex2((sc[j][e] + sc[j][e + 2]) * fac - mrow) * irow;
             }
     }
     if (!on) return;
@@ -513,27 +443,55 @@ __global__ void __launch_bounds__(256, 1) kv8_weight_kernel(const __grid_constan
 }
 
 constexpr int kMaxSplit = 64;
+constexpr int kPromptRows = 32;  // query rows of a KV head from which on the prompt kernel takes them
 
-// Splits of the rows kernel: one CTA per SM over the heads and row groups.
-int row_splits(const neon_kv8_t& c, size_t rows) {
-    const size_t units = c.n_kv_head * ((rows + 7) / 8);
-    return (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, (size_t)c.capacity / 512}));
+// The plan of a call, from what the host knows of it (not how many rows the cache holds).
+struct Plan {
+    bool prompt;
+    int unit, nsplit;
+    size_t stats, part_o, part_ml, qt, qfactor, bytes;  // offsets into the workspace
+};
+Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
+    Plan p{};
+    const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head, hd = c.head_dim;
+    p.prompt = rows > (size_t)kPromptRows;
+    p.unit = p.prompt ? prompt_unit((int)hd) : 8;
+    const size_t units = H * ((rows + p.unit - 1) / p.unit);
+    // shares of the keys: as many as fill the SMs once
+    p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, (size_t)c.capacity / 512}));
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at = (at + bytes + 1023) & ~(size_t)1023;
+        return o;
+    };
+    p.stats = take(H * rows * 2 * sizeof(float));
+    p.part_o = take(p.nsplit > 1 ? H * rows * p.nsplit * hd * sizeof(float) : 0);
+    p.part_ml = take(p.nsplit > 1 ? H * rows * p.nsplit * 2 * sizeof(float) : 0);
+    const size_t padded = (rows + 255) / 256 * 256;
+    p.qfactor = take(p.prompt ? H * padded * sizeof(float) : 0);
+    p.qt = take(p.prompt ? prompt_query_bytes(c, rows, type) : 0);
+    p.bytes = at + 1024;  // the caller's 16-byte alignment is rounded up
+    return p;
 }
 
 }  // namespace
 
 size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
-    const size_t rows = n * (n_head / c.n_kv_head), nz = (rows + 7) / 8;
-    const size_t stats = c.n_kv_head * rows * 2 * sizeof(float);
-    const int ns = row_splits(c, rows);
-    const size_t part = ns > 1 ? (size_t)c.n_kv_head * nz * ns * 8 * (c.head_dim + 2) * sizeof(float) : 0;
-    return ((stats + 15) & ~(size_t)15) + part + 16;
+    // Fewer tokens may take more shares, but rows * shares is at most 148 units' rows (plan_of).
+    const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head;
+    const size_t unit = rows > (size_t)kPromptRows ? std::max(8, prompt_unit((int)c.head_dim)) : 8;
+    const size_t padded = (rows + 255) / 256 * 256;
+    return H * rows * 2 * sizeof(float) + 148 * unit * (c.head_dim + 2) * sizeof(float) + H * padded * sizeof(float) +
+           prompt_query_bytes(c, rows, NEON_GGML_F32) + 8 * 1024;
 }
 
 int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t os, size_t n, size_t n_head,
                   float scale, int type, float* weight, void* ws, int device, cudaStream_t st) {
     unsigned* err = neon_internal::device_error_word(device);
     if (!err) return NEON_ERR_CUDA;
+    const Plan p = plan_of(c, n, n_head, type);
+    unsigned char* base = (unsigned char*)(((uintptr_t)ws + 1023) & ~(uintptr_t)1023);
     AttnArgs a{};
     a.c = c;
     a.q = q;
@@ -546,19 +504,31 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     a.type = type;
     a.scale = scale * kLog2e;
     a.weight = weight;
-    const size_t rows = n * a.group;
-    a.nsplit = row_splits(c, rows);
-    a.stats = (float*)ws;
-    a.part = a.stats + ((c.n_kv_head * rows * 2 + 3) & ~(size_t)3);
+    a.nsplit = p.nsplit;
+    a.unit = p.unit;
+    a.stats = (float*)(base + p.stats);
+    a.part_o = (float*)(base + p.part_o);
+    a.part_ml = (float*)(base + p.part_ml);
+    a.qt = base + p.qt;
+    a.qfactor = (float*)(base + p.qfactor);
     a.err = err;
-    const int hd = (int)c.head_dim, nz = (int)((rows + 7) / 8);
-    if (nz > 65535) return neon_internal::error(NEON_ERR_UNSUPPORTED, "kv8: too many query rows in one call");
-    auto rows_kernel = hd <= 64 ? kv8_rows_kernel<64> : hd <= 128 ? kv8_rows_kernel<128> : kv8_rows_kernel<256>;
-    const int smem = hd <= 64 ? RowTile<64>::kSmem : hd <= 128 ? RowTile<128>::kSmem : RowTile<256>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_rows_kernel)");
-    int rc = launch("kv8_rows_kernel", rows_kernel, dim3((unsigned)a.nsplit, c.n_kv_head, (unsigned)nz), kRowThreads,
-                    (size_t)smem, st, 1, a);
+    const size_t rows = n * a.group;
+    const int hd = (int)c.head_dim;
+    int rc;
+    if (p.prompt) {
+        a.tile_keys = prompt_tile_keys(hd);
+        a.min_tiles = 4;
+        rc = launch_prompt(a, st);
+    } else {
+        a.tile_keys = 32;
+        a.min_tiles = 2 * kRowWarps;  // two tiles per warp
+        auto rows_kernel = hd <= 64 ? kv8_rows_kernel<64> : hd <= 128 ? kv8_rows_kernel<128> : kv8_rows_kernel<256>;
+        const int smem = hd <= 64 ? RowTile<64>::kSmem : hd <= 128 ? RowTile<128>::kSmem : RowTile<256>::kSmem;
+        cudaError_t e = cudaFuncSetAttribute(rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_rows_kernel)");
+        rc = launch("kv8_rows_kernel", rows_kernel, dim3((unsigned)a.nsplit, c.n_kv_head, (unsigned)((rows + 7) / 8)),
+                    kRowThreads, (size_t)smem, st, 1, a);
+    }
     if (!rc && a.nsplit > 1)
         rc = launch("kv8_join_kernel", kv8_join_kernel, dim3((unsigned)((rows + 3) / 4), c.n_kv_head), 128, 0, st, 1, a);
     if (!rc && weight) {

@@ -1,0 +1,574 @@
+// neon_kv8_prompt.cu -- attention over the 8-bit KV cache for many query rows
+// (prompts), on tcgen05 with the sums in tensor memory.
+//
+// A CTA takes a unit of query rows of one KV head (MT tiles of 128 rows: row r
+// is query head r % group of token r / group, so all heads of a group share
+// the keys' tiles) and a share of the keys, in tiles of KT:
+//
+//   S = Q K^T    both operands in shared memory: Q as fp16 (fp32 queries as
+//                hi + lo terms, two products into one sum), K's codes as fp16
+//   P            one thread per row: t = s * (row factor * block scale), lazy
+//                running maximum, p = 2^(t - m), rounded to fp16 (types of 16
+//                bits) or split into hi + lo, written over S in tensor memory
+//   O += P V     P from tensor memory, V's codes as fp16 in shared memory
+//
+// Codes are exact in fp16, so a tile of codes is half the traffic of a 16-bit
+// cache and costs a conversion (two permutes and a subtraction for four
+// codes), which four warps do once for all MT tiles. One warp issues the
+// products; the MT tiles alternate, so one's softmax runs under the other's
+// products. What bounds it: exp2 (16 a clock and SM) for types of 16 bits, the
+// products (twice as many) for fp32.
+//
+// The maximum is lazy: O is only rescaled when a row's maximum has grown by
+// more than 2^8 since its m was set (the result does not depend on m), so p is
+// at most 2^8; with V's scale relative to a reference that is kept within a
+// factor of 4 (vr), and 2^5, p times those stays below fp16's 65504, and its
+// lo term has bits down to 2^-30 of a row's largest.
+#include "neon_kv8_attn.cuh"
+
+#include <algorithm>
+
+namespace longctx {
+namespace {
+
+constexpr int kSoftWarps = 8, kConvWarps = 4;
+constexpr int kMmaWarp = kSoftWarps + kConvWarps;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr float kLazy = 8.f;     // log2 of how far p may exceed 1
+constexpr float kPScale = 32.f;  // 2^5
+
+// ---- tcgen05 ----
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// d[tmem] (+)= a b, fp16 operands, fp32 sums: a from shared memory, or from tensor memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t a) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t a) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(a));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand of 128-byte-swizzled panels [rows][64 halves]: groups of eight rows are 1024
+// bytes apart; `lead` is the distance of the panels (used when the panels run along M or N).
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// fp16 x fp16 -> fp32, M = 128; b_mn: B's rows run along the summed dimension
+__device__ __forceinline__ uint32_t instr(int n, bool b_mn) {
+    return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+// ---- waits that end: after 2 s, or once another role has given up ----
+__device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned* err) {
+    if (bar_try(bar, parity)) return true;
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+    for (;;) {
+        if (bar_try(bar, parity)) return true;
+        if (*dead) return false;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        if (t - t0 > 2000000000ull) {
+            atomicOr(err, kErrWait);
+            *dead = 1;
+            return false;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Query tiles: [H][tiles of 128 rows][TERMS][panels of 64 values][128][64] fp16, swizzled as the
+// products read them, row r times 2^-e (its largest value near 2^7) and the sign of the scale; the
+// row's factor |scale| log2(e) 2^e / ... undoes it. Rows beyond the last are zero. One warp per row.
+// ---------------------------------------------------------------------------
+template <int TERMS>
+__global__ void __launch_bounds__(256) kv8_queries_kernel(const __grid_constant__ AttnArgs a, int tiles) {
+    pdl_wait();
+    pdl_trigger();
+    const int hd = (int)a.c.head_dim, panels = (hd + 63) / 64, rows = a.n * a.group;
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long long base = (long long)(r / a.group) * a.qs + (long long)(kvh * a.group + r % a.group) * hd;
+    float x[8];  // values lane * 4 .. + 3, and 128 + those
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = lane * 4 + (i & 3) + 128 * (i >> 2);
+        x[i] = r < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
+        mx = fmaxf(mx, fabsf(x[i]));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const int e = mx > 0.f && !isinf(mx) ? 7 - ilogbf(mx) : 0;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    unsigned char* tile = a.qt + ((size_t)kvh * tiles + r / 128) * TERMS * panels * 16384;
+    const int row = r & 127;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int d = lane * 4 + 128 * half;
+        if (d >= panels * 64) continue;
+        uint2 hi, lo;
+        const float* y = x + 4 * half;
+        split2(ldexpf(y[0], e) * sign, ldexpf(y[1], e) * sign, hi.x, lo.x);
+        split2(ldexpf(y[2], e) * sign, ldexpf(y[3], e) * sign, hi.y, lo.y);
+        // 16-byte piece (d % 64) / 8 of the row moves to piece ^ (row % 8)
+        const size_t at = (size_t)(d / 64) * 16384 + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2;
+        *reinterpret_cast<uint2*>(tile + at) = hi;
+        if (TERMS == 2) *reinterpret_cast<uint2*>(tile + (size_t)panels * 16384 + at) = lo;
+    }
+    if (lane == 0) a.qfactor[(size_t)kvh * tiles * 128 + r] = r < rows ? ldexpf(fabsf(a.scale), -e) : 0.f;
+}
+
+// ---------------------------------------------------------------------------
+// The main kernel
+// ---------------------------------------------------------------------------
+template <int PANELS, int TERMS>
+struct Shape {
+    static constexpr int MT = PANELS <= 2 ? 2 : 1;       // query tiles of 128 rows
+    static constexpr int KT = PANELS <= 2 ? 128 : 64;    // keys of a tile
+    static constexpr int ST = PANELS == 1 || TERMS == 1 ? 2 : 1;  // tiles of K, and of V, held at once
+    static constexpr int QTile = TERMS * PANELS * 16384;
+    static constexpr int Stage = PANELS * KT * 128;
+    static constexpr int Bytes = MT * QTile + 2 * ST * Stage;
+    static constexpr int Smem = Bytes + 1024 + 256;
+    static constexpr int SCols = KT, OCols = PANELS * 64;
+    static_assert(MT * (SCols + OCols) <= 512, "tensor memory");
+    static_assert(Smem <= 232448, "shared memory");
+};
+
+struct Bars {
+    uint64_t q, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drain;
+    uint32_t tmem;
+    int dead;
+};
+static_assert(sizeof(Bars) <= 256, "barriers");
+
+template <int PANELS, int TERMS>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
+    using S = Shape<PANELS, TERMS>;
+    constexpr int MT = S::MT, KT = S::KT, ST = S::ST, NB = KT / 32;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+    unsigned char *qs = smem, *ks = qs + MT * S::QTile, *vs = ks + ST * S::Stage;
+    Bars* bar = reinterpret_cast<Bars*>(vs + ST * S::Stage);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, H = (int)a.c.n_kv_head, rows = a.n * a.group;
+    // the units with the most keys first
+    const int units = (rows + 128 * MT - 1) / (128 * MT);
+    const int kvh = blockIdx.x % H, split = blockIdx.x / H % a.nsplit, unit = units - 1 - blockIdx.x / (H * a.nsplit);
+    if (warp == kMmaWarp) {
+        if (lane == 0) {
+            bar_init(&bar->q, 1);
+            for (int i = 0; i < 2; ++i) {
+                bar_init(&bar->k_full[i], kConvWarps);
+                bar_init(&bar->k_empty[i], 1);
+                bar_init(&bar->v_full[i], kConvWarps);
+                bar_init(&bar->v_empty[i], 1);
+                bar_init(&bar->s_full[i], 1);
+                bar_init(&bar->p_full[i], 4);
+                bar_init(&bar->o_full[i], 1);
+            }
+            bar_init(&bar->drain, 1);
+            bar->dead = 0;
+            bar_init_fence();
+        }
+        __syncwarp();
+        tmem_alloc(&bar->tmem, 512);
+        tc_before();
+    }
+    pdl_wait();
+    pdl_trigger();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = bar->tmem;
+
+    const int past = *a.c.past;
+    const Shares sh = shares_of(a, past, unit);
+    const int j0 = min(split * sh.per, sh.tiles), j1 = min(j0 + sh.per, sh.tiles);
+    // the key tiles of each query tile within the share
+    int nt[MT];
+    int most = 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int first = (unit * MT + m) * 128;
+        const int keys = first < rows ? keys_of(past, min(first + 127, rows - 1) / a.group, cap) : 0;
+        nt[m] = max(0, min(j1, (keys + KT - 1) / KT) - j0);
+        most = max(most, nt[m]);
+    }
+
+    if (warp < kSoftWarps) {
+        // ---- softmax: one thread per row ----
+        const int m = warp >> 2;
+        const int rr = (unit * MT + m) * 128 + (warp & 3) * 32 + lane;
+        if (m < MT && split < sh.active) {
+            const bool on = rr < rows;
+            const int limit = on ? keys_of(past, rr / a.group, cap) : 0;
+            const float factor = a.qfactor[(size_t)kvh * tiles128 * 128 + rr];
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's lanes: 32 (warp % 4) ..
+            const uint32_t st = tmem + lanes + m * S::SCols, ot = tmem + lanes + MT * S::SCols + m * S::OCols;
+            const float* ksc = a.c.k_scale + (size_t)kvh * (cap >> 5);
+            const float* vsc = a.c.v_scale + (size_t)kvh * (cap >> 5);
+            // the keys that every row of the warp sees
+            const int all = __reduce_min_sync(0xffffffffu, limit);
+            float mref = -INFINITY, l = 0.f, vref = 0.f;
+            bool alive = true;
+            float nk[NB], nv[NB];
+            auto scales = [&](int j) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const int blk = j * NB + b;
+                    nk[b] = blk < cap >> 5 ? ksc[blk] : 0.f;
+                    nv[b] = blk < cap >> 5 ? vsc[blk] : 0.f;
+                }
+            };
+            const int n = m < MT ? nt[m < MT ? m : 0] : 0;
+            if (n) scales(j0);
+            for (int i = 0; i < n; ++i) {
+                const int j = j0 + i, key0 = j * KT;
+                float kf[NB], vb[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    kf[b] = factor * nk[b];
+                    vb[b] = nv[b];
+                }
+                if (i + 1 < n) scales(j + 1);
+                alive = wait_or(&bar->s_full[m], (uint32_t)(i & 1), &bar->dead, a.err);
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) break;
+                tc_after();
+                const bool full = key0 + KT <= all;  // no key of the tile is hidden from a row of the warp
+                // the tile's largest score
+                float mt = -INFINITY;
+                float vmax = 0.f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t r[32];
+                    tmem_ld32(r, st + 32 * b);
+                    tmem_wait_ld();
+                    float x = -INFINITY;
+                    if (full) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x = fmaxf(x, __uint_as_float(r[e]));
+                        mt = fmaxf(mt, x * kf[b]);
+                    } else if (key0 + 32 * b < limit) {
+                        const int c = limit - key0 - 32 * b;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (e < c) x = fmaxf(x, __uint_as_float(r[e]));
+                        mt = fmaxf(mt, x * kf[b]);
+                    }
+                    if (key0 + 32 * b < limit) vmax = fmaxf(vmax, vb[b]);
+                }
+                // O and l follow m and the reference of V's scales when those move
+                const float vtop = vmax > 4.f * vref ? vmax : vref;
+                const float mnew = mt > mref + kLazy || mref == -INFINITY ? fmaxf(mt, mref) : mref;
+                if (__any_sync(0xffffffffu, mnew != mref || vtop != vref)) {
+                    const float fl = mref == -INFINITY ? 0.f : ex2(mref - mnew);
+                    const float f = vtop > 0.f ? fl * (vref / vtop) : fl;
+                    if (i > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < hd; c += 16) {
+                            uint32_t r[16];
+                            tmem_ld16(r, ot + c);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                            tmem_st16(ot + c, r);
+                        }
+                    }
+                    l *= fl;
+                    mref = mnew;
+                    vref = vtop;
+                }
+                const float mu = mref == -INFINITY ? 0.f : mref;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t r[32], hi[16], lo[16];
+                    tmem_ld32(r, st + 32 * b);
+                    const float vr = vb[b] == 0.f ? 0.f : vb[b] / vref * kPScale;
+                    tmem_wait_ld();
+                    float bs = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float p0 = ex2(__fmaf_rn(__uint_as_float(r[2 * e]), kf[b], -mu));
+                        float p1 = ex2(__fmaf_rn(__uint_as_float(r[2 * e + 1]), kf[b], -mu));
+                        float w0 = p0 * vr, w1 = p1 * vr;
+                        if (!full) {
+                            const int c = limit - key0 - 32 * b;
+                            if (2 * e >= c) p0 = w0 = 0.f;
+                            if (2 * e + 1 >= c) p1 = w1 = 0.f;
+                        }
+                        bs += p0 + p1;
+                        if (TERMS == 2) split2(w0, w1, hi[e], lo[e]);
+                        else hi[e] = h2_bits(__floats2half2_rn(w0, w1));
+                    }
+                    l += bs;
+                    // over the block's scores: hi in its first 16 columns, lo in the next
+                    tmem_st16(st + 32 * b, hi);
+                    if (TERMS == 2) tmem_st16(st + 32 * b + 16, lo);
+                }
+                tmem_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bar->p_full[m]);
+            }
+            // ---- the row's output, or its part ----
+            if (n && alive) alive = __all_sync(0xffffffffu, wait_or(&bar->o_full[m], 0, &bar->dead, a.err));
+            tc_after();
+            const bool whole = sh.active == 1;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale);
+            const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
+            const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
+            float* po = a.part_o + pr * hd;
+            for (int c = 0; c < hd; c += 16) {
+                uint32_t r[16];
+                if (n) {
+                    tmem_ld16(r, ot + c);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) r[e] = 0;
+                }
+                if (!on) continue;
+                // a row that has seen no key, or only blocks of zeros: 0
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(r[e]) * up;
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(po + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                } else if (a.type == NEON_GGML_F32 && ((reinterpret_cast<uintptr_t>((float*)a.o + ob)) & 15) == 0) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4*>((float*)a.o + ob + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                } else if (a.type == NEON_GGML_BF16 && ((reinterpret_cast<uintptr_t>((__nv_bfloat16*)a.o + ob)) & 15) == 0) {
+                    uint4 w[2];
+                    __nv_bfloat162* q = reinterpret_cast<__nv_bfloat162*>(w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) q[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                    uint4* d = reinterpret_cast<uint4*>((__nv_bfloat16*)a.o + ob + c);
+                    d[0] = w[0];
+                    d[1] = w[1];
+                } else if (a.type == NEON_GGML_F16 && ((reinterpret_cast<uintptr_t>((__half*)a.o + ob)) & 15) == 0) {
+                    uint4 w[2];
+                    __half2* q = reinterpret_cast<__half2*>(w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) q[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                    uint4* d = reinterpret_cast<uint4*>((__half*)a.o + ob + c);
+                    d[0] = w[0];
+                    d[1] = w[1];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o_store(a.o, a.type, ob + c + e, v[e]);
+                }
+            }
+            if (on) {
+                const float mu = mref == -INFINITY ? 0.f : mref;
+                float* d = whole ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
+                d[0] = whole ? mu : mref;
+                d[1] = whole ? inv : l;
+            }
+            tc_before();
+        }
+    } else if (warp < kMmaWarp) {
+        // ---- conversion: codes to fp16, swizzled ----
+        const int ct = tid - kSoftWarps * 32;
+        const int pieces = hd / 16;                 // 16-byte pieces of a row
+        const int total = KT * pieces;
+        constexpr int L = KT * PANELS * 4 / 128;    // pieces per thread at most
+        const int8_t* kc = a.c.k + (size_t)kvh * cap * hd;
+        const int8_t* vc = a.c.v + (size_t)kvh * cap * hd;
+        uint4 kr[L], vr[L];
+        auto load = [&](uint4 (&w)[L], const int8_t* base, int j) {
+            const long long at = (long long)j * total;
+            const long long end = (long long)cap * pieces;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int p = ct + 128 * i;
+                w[i] = make_uint4(0, 0, 0, 0);
+                if (p < total && at + p < end) w[i] = *(reinterpret_cast<const uint4*>(base) + at + p);
+            }
+        };
+        auto store = [&](const uint4 (&w)[L], unsigned char* d) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int p = ct + 128 * i;
+                if (p < total) {
+                    const int r = p / pieces, c = p - r * pieces;  // codes 16 c .. of row r
+                    unsigned char* o = d + (c >> 2) * (KT * 128) + r * 128;
+                    const int at = 2 * (c & 3), x = r & 7;
+                    const uint32_t u[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
+                    *reinterpret_cast<uint4*>(o + ((at ^ x) << 4)) =
+                        make_uint4(codes_lo(u[0]), codes_hi(u[0]), codes_lo(u[1]), codes_hi(u[1]));
+                    *reinterpret_cast<uint4*>(o + (((at + 1) ^ x) << 4)) =
+                        make_uint4(codes_lo(u[2]), codes_hi(u[2]), codes_lo(u[3]), codes_hi(u[3]));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        if (most) {
+            load(kr, kc, j0);
+            load(vr, vc, j0);
+        }
+        for (int i = 0; i < most; ++i) {
+            const int s = i % ST;
+            const uint32_t ph = (uint32_t)((i / ST) & 1);
+            if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->k_empty[s], ph ^ 1, &bar->dead, a.err))) break;
+            store(kr, ks + s * S::Stage);
+            if (lane == 0) bar_arrive(&bar->k_full[s]);
+            if (i + 1 < most) load(kr, kc, j0 + i + 1);
+            if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->v_empty[s], ph ^ 1, &bar->dead, a.err))) break;
+            store(vr, vs + s * S::Stage);
+            if (lane == 0) bar_arrive(&bar->v_full[s]);
+            if (i + 1 < most) load(vr, vc, j0 + i + 1);
+        }
+    } else if (lane == 0 && most && split < sh.active) {
+        // ---- products ----
+        const uint32_t id_s = instr(KT, false), id_o = instr(hd, true);
+        const uint32_t qa = smem_addr(qs), ka = smem_addr(ks), va = smem_addr(vs);
+        const unsigned char* qsrc = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT) * S::QTile;
+        bar_expect(&bar->q, MT * S::QTile);
+        for (int p = 0; p < MT * TERMS * PANELS; ++p) bulk_load(qs + p * 16384, qsrc + (size_t)p * 16384, 16384, &bar->q);
+        bool alive = wait_or(&bar->q, 0, &bar->dead, a.err);
+        const int steps = hd / 16;
+        auto scores = [&](int m, int i) {  // S_m = Q_m K^T of the share's tile i
+            const uint32_t k = ka + (i % ST) * S::Stage, q = qa + m * S::QTile;
+            for (int t = 0; t < TERMS; ++t)
+                for (int s = 0; s < steps; ++s)
+                    mma_ss(tmem + m * S::SCols, operand(q + (t * PANELS + (s >> 2)) * 16384 + (s & 3) * 32, 16),
+                           operand(k + (s >> 2) * (KT * 128) + (s & 3) * 32, 16), id_s, t + s > 0);
+            tc_commit(&bar->s_full[m]);
+        };
+        auto last_of = [&](int i) {  // the last query tile that has tile i
+            int r = -1;
+            for (int m = 0; m < MT; ++m)
+                if (i < nt[m]) r = m;
+            return r;
+        };
+        alive = alive && wait_or(&bar->k_full[0], 0, &bar->dead, a.err);
+        if (alive) {
+            tc_after();
+            for (int m = 0; m < MT; ++m)
+                if (nt[m]) scores(m, 0);
+            tc_commit(&bar->k_empty[0]);
+        }
+        for (int i = 0; alive && i < most; ++i) {
+            const int sv = i % ST, sk = (i + 1) % ST;
+            const int lk = last_of(i + 1);
+            for (int m = 0; alive && m < MT; ++m) {
+                if (i >= nt[m]) continue;
+                alive = wait_or(&bar->p_full[m], (uint32_t)(i & 1), &bar->dead, a.err) &&
+                        wait_or(&bar->v_full[sv], (uint32_t)((i / ST) & 1), &bar->dead, a.err);
+                if (!alive) break;
+                tc_after();
+                // P of key block b: hi at columns 32 b .., lo at 32 b + 16 ..
+                for (int t = 0; t < TERMS; ++t)
+                    for (int s = 0; s < KT / 16; ++s)
+                        mma_ts(tmem + MT * S::SCols + m * S::OCols, tmem + m * S::SCols + 32 * (s >> 1) + 16 * t + 8 * (s & 1),
+                               operand(va + sv * S::Stage + s * 2048, KT * 128), id_o, i > 0 || t + s > 0);
+                if (i + 1 == nt[m]) tc_commit(&bar->o_full[m]);
+                if (i + 1 < nt[m]) {
+                    alive = wait_or(&bar->k_full[sk], (uint32_t)(((i + 1) / ST) & 1), &bar->dead, a.err);
+                    if (!alive) break;
+                    tc_after();
+                    scores(m, i + 1);
+                    if (m == lk) tc_commit(&bar->k_empty[sk]);
+                }
+            }
+            if (alive) tc_commit(&bar->v_empty[sv]);
+        }
+        // every product has ended before tensor memory is freed
+        tc_commit(&bar->drain);
+        volatile int never = 0;
+        wait_or(&bar->drain, 0, &never, a.err);
+    }
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+using PromptKernel = void (*)(AttnArgs, int);
+
+template <int PANELS, int TERMS>
+int launch_shape(const AttnArgs& a, cudaStream_t st) {
+    using S = Shape<PANELS, TERMS>;
+    const int rows = a.n * a.group, H = (int)a.c.n_kv_head;
+    const int tiles = (rows + 255) / 256 * 2;
+    PromptKernel k = kv8_prompt_kernel<PANELS, TERMS>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
+    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_prompt_kernel)");
+    int rc = launch("kv8_queries_kernel", kv8_queries_kernel<TERMS>, dim3((unsigned)tiles * 16, (unsigned)H), 256, 0, st, 1, a, tiles);
+    const int units = (rows + 128 * S::MT - 1) / (128 * S::MT);
+    if (!rc) rc = launch("kv8_prompt_kernel", k, dim3((unsigned)(units * H * a.nsplit)), kThreads, S::Smem, st, 1, a, tiles);
+    return rc;
+}
+
+}  // namespace
+
+int prompt_unit(int hd) { return hd <= 128 ? 256 : 128; }
+int prompt_tile_keys(int hd) { return hd <= 128 ? 128 : 64; }
+
+size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type) {
+    const size_t tiles = (rows + 255) / 256 * 2, panels = (c.head_dim + 63) / 64;
+    return c.n_kv_head * tiles * (type == NEON_GGML_F32 ? 2 : 1) * panels * 16384;
+}
+
+int launch_prompt(const AttnArgs& a, cudaStream_t st) {
+    const int panels = ((int)a.c.head_dim + 63) / 64;
+    const bool two = a.type == NEON_GGML_F32;
+    switch (panels) {
+        case 1: return two ? launch_shape<1, 2>(a, st) : launch_shape<1, 1>(a, st);
+        case 2: return two ? launch_shape<2, 2>(a, st) : launch_shape<2, 1>(a, st);
+        case 3: return two ? launch_shape<3, 2>(a, st) : launch_shape<3, 1>(a, st);
+        default: return two ? launch_shape<4, 2>(a, st) : launch_shape<4, 1>(a, st);
+    }
+}
+
+}  // namespace longctx
