@@ -531,7 +531,9 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     }
     if (!rc && a.nsplit > 1)
         rc = launch("kv8_join_kernel", kv8_join_kernel, dim3((unsigned)((rows + 3) / 4), c.n_kv_head), 128, 0, st, 1, a);
-    if (!rc && weight) {
+    if (!rc && weight && p.prompt) {
+        rc = launch_prompt_weights(a, st);
+    } else if (!rc && weight) {
         auto wk = hd <= 64 ? kv8_weight_kernel<64> : hd <= 128 ? kv8_weight_kernel<128> : kv8_weight_kernel<256>;
         rc = launch("kv8_weight_kernel", wk, dim3((c.capacity + 255) / 256, c.n_kv_head), 256, 0, st, 1, a);
     }

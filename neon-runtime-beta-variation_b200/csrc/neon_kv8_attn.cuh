@@ -94,5 +94,6 @@ size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type);
 int prompt_unit(int hd);
 int prompt_tile_keys(int hd);
 int launch_prompt(const AttnArgs& a, cudaStream_t st);
+int launch_prompt_weights(const AttnArgs& a, cudaStream_t st);  // after launch_prompt and its joins
 
 }  // namespace longctx

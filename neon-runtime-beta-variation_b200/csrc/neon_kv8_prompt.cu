@@ -160,6 +160,16 @@ __global__ void __launch_bounds__(256) kv8_queries_kernel(const __grid_constant_
     if (lane == 0) a.qfactor[(size_t)kvh * tiles * 128 + r] = r < rows ? ldexpf(fabsf(a.scale), -e) : 0.f;
 }
 
+// 16 codes (values 16 c .. of row r) as halves into a swizzled tile of `height` rows
+__device__ __forceinline__ void put_codes(unsigned char* tile, int height, int r, int c, uint4 w) {
+    unsigned char* o = tile + (c >> 2) * (height * 128) + r * 128;
+    const int at = 2 * (c & 3), x = r & 7;
+    const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+    *reinterpret_cast<uint4*>(o + ((at ^ x) << 4)) = make_uint4(codes_lo(u[0]), codes_hi(u[0]), codes_lo(u[1]), codes_hi(u[1]));
+    *reinterpret_cast<uint4*>(o + (((at + 1) ^ x) << 4)) =
+        make_uint4(codes_lo(u[2]), codes_hi(u[2]), codes_lo(u[3]), codes_hi(u[3]));
+}
+
 // ---------------------------------------------------------------------------
 // The main kernel
 // ---------------------------------------------------------------------------
@@ -436,14 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             for (int i = 0; i < L; ++i) {
                 const int p = ct + 128 * i;
                 if (p < total) {
-                    const int r = p / pieces, c = p - r * pieces;  // codes 16 c .. of row r
-                    unsigned char* o = d + (c >> 2) * (KT * 128) + r * 128;
-                    const int at = 2 * (c & 3), x = r & 7;
-                    const uint32_t u[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
-                    *reinterpret_cast<uint4*>(o + ((at ^ x) << 4)) =
-                        make_uint4(codes_lo(u[0]), codes_hi(u[0]), codes_lo(u[1]), codes_hi(u[1]));
-                    *reinterpret_cast<uint4*>(o + (((at + 1) ^ x) << 4)) =
-                        make_uint4(codes_lo(u[2]), codes_hi(u[2]), codes_lo(u[3]), codes_hi(u[3]));
+                    const int r = p / pieces;
+                    put_codes(d, KT, r, p - r * pieces, w[i]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -534,6 +538,202 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     }
 }
 
+// ---------------------------------------------------------------------------
+// The cached rows' weights: a CTA keeps MT tiles of 128 keys (their codes as
+// fp16) and streams the query tiles, S^T = K Q^T, so a thread has one key and
+// sums p = 2^(t - m) / l = 2^(s factor scale - (m + log2 l)) over its columns in
+// registers, in the queries' order. Two buffers of S^T let the products run
+// ahead; exp2 bounds it (one per key and query). Needs the rows' final m, 1 / l.
+// ---------------------------------------------------------------------------
+template <int PANELS>
+struct WShape {
+    static constexpr int MT = PANELS <= 2 ? 2 : 1;
+    static constexpr int KTile = PANELS * 16384;       // a tile of 128 keys
+    static constexpr int Stage = PANELS * 16384;       // a query tile's hi or lo terms
+    static constexpr int ST = PANELS <= 2 ? 4 : 2;
+    static constexpr int Smem = MT * KTile + ST * Stage + 2 * 128 * 8 + 1024 + 256;
+    static_assert(Smem <= 232448, "shared memory");
+};
+constexpr int kWThreads = kThreads + 32;  // and a warp that loads
+
+struct WBars {
+    uint64_t k_full, q_full[4], q_empty[4], s_full[2], s_empty[2], st_full[2], drain;
+    uint32_t tmem;
+    int dead;
+};
+static_assert(sizeof(WBars) <= 256, "barriers");
+
+template <int PANELS, int TERMS>
+__global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
+    using S = WShape<PANELS>;
+    constexpr int MT = S::MT, ST = S::ST;
+    extern __shared__ unsigned char raw[];
+    pdl_wait();
+    pdl_trigger();
+    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, rows = a.n * a.group, kvh = blockIdx.y;
+    const int past = *a.c.past, keys = keys_of(past, a.n - 1, cap);
+    const int key0 = blockIdx.x * MT * 128;
+    if (key0 >= keys) return;
+    unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+    unsigned char *ks = smem, *qs = ks + MT * S::KTile;
+    float2* stat = reinterpret_cast<float2*>(qs + ST * S::Stage);  // [2][128]: factor, m + log2 l
+    WBars* bar = reinterpret_cast<WBars*>(stat + 256);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == kMmaWarp) {
+        if (lane == 0) {
+            bar_init(&bar->k_full, kConvWarps);
+            for (int i = 0; i < ST; ++i) {
+                bar_init(&bar->q_full[i], 1);
+                bar_init(&bar->q_empty[i], 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                bar_init(&bar->s_full[i], 1);
+                bar_init(&bar->s_empty[i], 4 * MT);
+                bar_init(&bar->st_full[i], kConvWarps);
+            }
+            bar_init(&bar->drain, 1);
+            bar->dead = 0;
+            bar_init_fence();
+        }
+        __syncwarp();
+        tmem_alloc(&bar->tmem, 256 * MT);
+        tc_before();
+    }
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = bar->tmem;
+    // query tiles from the first row that sees key0
+    const int first = (int)min((long long)rows - 1, max(0LL, ((long long)key0 - past) * a.group)) / 128;
+    const int n = (rows + 127) / 128 - first;
+
+    if (warp < 4 * MT) {
+        const int m = warp >> 2, key = key0 + m * 128 + (warp & 3) * 32 + lane;
+        const uint32_t st = tmem + ((uint32_t)(warp & 3) << 21) + m * 256;
+        const float scale = key < keys ? a.c.k_scale[(size_t)kvh * (cap >> 5) + (key >> 5)] : 0.f;
+        // the first row that sees this key, and that every key of the warp is seen by
+        const long long seen = key < keys ? ((long long)key - past) * a.group : (1LL << 40);
+        const long long last = max(0LL, ((long long)(key | 31) - past) * a.group);
+        float sum[4] = {};
+        for (int i = 0; i < n; ++i) {
+            const int b = i & 1;
+            const uint32_t ph = (uint32_t)((i >> 1) & 1);
+            bool ok = wait_or(&bar->st_full[b], ph, &bar->dead, a.err) && wait_or(&bar->s_full[b], ph, &bar->dead, a.err);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_after();
+            const long long r0 = (long long)(first + i) * 128;
+            const bool full = r0 >= last && key < keys;
+            const int from = (int)max(0LL, min(128LL, seen - r0));  // columns below are hidden from this key
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(r, st + b * 128 + c);
+                tmem_wait_ld();
+                const float4* sp = reinterpret_cast<const float4*>(stat + b * 128 + c);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float4 q = sp[e / 2];
+                    float p0 = ex2(__fmaf_rn(__uint_as_float(r[e]), q.x * scale, -q.y));
+                    float p1 = ex2(__fmaf_rn(__uint_as_float(r[e + 1]), q.z * scale, -q.w));
+                    if (!full) {
+                        if (c + e < from) p0 = 0.f;
+                        if (c + e + 1 < from) p1 = 0.f;
+                    }
+                    sum[(e & 2)] += p0;
+                    sum[(e & 2) + 1] += p1;
+                }
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bar->s_empty[b]);
+        }
+        if (key < keys) {
+            const float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float* w = a.weight + (size_t)kvh * cap + key;
+            *w = key < past ? *w + v : v;
+        }
+    } else if (warp >= kSoftWarps && warp < kMmaWarp) {
+        const int ct = tid - kSoftWarps * 32, pieces = hd / 16;
+        const uint4* kc = reinterpret_cast<const uint4*>(a.c.k + ((size_t)kvh * cap + key0) * hd);
+        const int held = min(MT * 128, cap - key0) * pieces;
+        for (int p = ct; p < MT * 128 * pieces; p += 128) {
+            const int r = p / pieces;
+            const uint4 w = p < held ? kc[p] : make_uint4(0, 0, 0, 0);
+            put_codes(ks + (r >> 7) * S::KTile, 128, r & 127, p - r * pieces, w);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(&bar->k_full);
+        for (int i = 0; i < n; ++i) {
+            const int b = i & 1, r = (first + i) * 128 + ct;
+            float2 v = make_float2(0.f, INFINITY);
+            if (r < rows) {
+                const float2 s = *reinterpret_cast<const float2*>(a.stats + ((size_t)kvh * rows + r) * 2);
+                v.x = a.qfactor[(size_t)kvh * tiles128 * 128 + r];
+                v.y = s.x - log2f(s.y);  // a row without keys: 1 / l = 0, p = 0
+            }
+            if (i >= 2 && !__all_sync(0xffffffffu, wait_or(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1, &bar->dead, a.err))) break;
+            stat[b * 128 + ct] = v;
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bar->st_full[b]);
+        }
+    } else if (warp == kMmaWarp && lane == 0) {
+        const uint32_t id = instr(128, false), ka = smem_addr(ks), qa = smem_addr(qs);
+        const int steps = hd / 16;
+        bool ok = wait_or(&bar->k_full, 0, &bar->dead, a.err);
+        int it = 0;
+        for (int i = 0; ok && i < n; ++i) {
+            const int b = i & 1;
+            if (i >= 2) ok = wait_or(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1, &bar->dead, a.err);
+            for (int t = 0; ok && t < TERMS; ++t, ++it) {
+                const int sg = it % ST;
+                ok = wait_or(&bar->q_full[sg], (uint32_t)((it / ST) & 1), &bar->dead, a.err);
+                if (!ok) break;
+                tc_after();
+                for (int m = 0; m < MT; ++m)
+                    for (int s = 0; s < steps; ++s)
+                        mma_ss(tmem + m * 256 + b * 128, operand(ka + m * S::KTile + (s >> 2) * 16384 + (s & 3) * 32, 16),
+                               operand(qa + sg * S::Stage + (s >> 2) * 16384 + (s & 3) * 32, 16), id, t + s > 0);
+                tc_commit(&bar->q_empty[sg]);
+            }
+            if (ok) tc_commit(&bar->s_full[b]);
+        }
+        tc_commit(&bar->drain);
+        volatile int never = 0;
+        wait_or(&bar->drain, 0, &never, a.err);
+    } else if (warp == kMmaWarp + 1 && lane == 0) {
+        const unsigned char* src = a.qt + ((size_t)kvh * tiles128 + first) * TERMS * S::Stage;
+        const int total = n * TERMS;
+        int it = 0;
+        for (; it < total; ++it) {
+            const int sg = it % ST;
+            if (it >= ST && !wait_or(&bar->q_empty[sg], (uint32_t)((it / ST) & 1) ^ 1, &bar->dead, a.err)) break;
+            bar_expect(&bar->q_full[sg], S::Stage);
+            bulk_load(qs + sg * S::Stage, src + (size_t)it * S::Stage, S::Stage, &bar->q_full[sg]);
+        }
+        // the copies in flight end before this CTA's shared memory does
+        volatile int never = 0;
+        for (int k = max(0, it - ST); k < it; ++k) wait_or(&bar->q_full[k % ST], (uint32_t)((k / ST) & 1), &never, a.err);
+    }
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_after();
+        tmem_free(tmem, 256 * MT);
+    }
+}
+
+template <int PANELS, int TERMS>
+int launch_weights(const AttnArgs& a, cudaStream_t st) {
+    using S = WShape<PANELS>;
+    auto k = kv8_prompt_weight_kernel<PANELS, TERMS>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
+    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_prompt_weight_kernel)");
+    const int tiles = (a.n * a.group + 255) / 256 * 2;
+    const unsigned grid = (a.c.capacity + 128 * S::MT - 1) / (128 * S::MT);
+    return launch("kv8_prompt_weight_kernel", k, dim3(grid, a.c.n_kv_head), kWThreads, S::Smem, st, 1, a, tiles);
+}
+
 using PromptKernel = void (*)(AttnArgs, int);
 
 template <int PANELS, int TERMS>
@@ -568,6 +768,17 @@ int launch_prompt(const AttnArgs& a, cudaStream_t st) {
         case 2: return two ? launch_shape<2, 2>(a, st) : launch_shape<2, 1>(a, st);
         case 3: return two ? launch_shape<3, 2>(a, st) : launch_shape<3, 1>(a, st);
         default: return two ? launch_shape<4, 2>(a, st) : launch_shape<4, 1>(a, st);
+    }
+}
+
+int launch_prompt_weights(const AttnArgs& a, cudaStream_t st) {
+    const int panels = ((int)a.c.head_dim + 63) / 64;
+    const bool two = a.type == NEON_GGML_F32;
+    switch (panels) {
+        case 1: return two ? launch_weights<1, 2>(a, st) : launch_weights<1, 1>(a, st);
+        case 2: return two ? launch_weights<2, 2>(a, st) : launch_weights<2, 1>(a, st);
+        case 3: return two ? launch_weights<3, 2>(a, st) : launch_weights<3, 1>(a, st);
+        default: return two ? launch_weights<4, 2>(a, st) : launch_weights<4, 1>(a, st);
     }
 }
 
