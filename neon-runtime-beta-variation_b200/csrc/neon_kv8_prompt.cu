@@ -27,13 +27,17 @@
 #include "neon_kv8_attn.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace longctx {
 namespace {
 
-constexpr int kSoftWarps = 8, kConvWarps = 4;
-constexpr int kMmaWarp = kSoftWarps + kConvWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+// Warps 0-7 softmax, 12 the products, 8-11 and 13-15 conversion. The launch's 512 x 128 registers are
+// dealt out again by warpgroup: a softmax thread holds its row of S (128 values) in registers.
+constexpr int kSoftWarps = 8, kMmaWarp = 12, kConvWarps = 7;
+constexpr int kThreads = 512;
+constexpr int kLaunchRegs = 128, kSoftRegs = 184, kOtherRegs = 72;
+static_assert(2 * kSoftRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
 constexpr float kLazy = 8.f;     // log2 of how far p may exceed 1
 constexpr float kPScale = 32.f;  // 2^5
 
@@ -117,57 +121,111 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
     }
 }
 
-// ---------------------------------------------------------------------------
-// Query tiles: [H][tiles of 128 rows][TERMS][panels of 64 values][128][64] fp16, swizzled as the
-// products read them, row r times 2^-e (its largest value near 2^7) and the sign of the scale; the
-// row's factor |scale| log2(e) 2^e / ... undoes it. Rows beyond the last are zero. One warp per row.
-// ---------------------------------------------------------------------------
-template <int TERMS>
-__global__ void __launch_bounds__(256) kv8_queries_kernel(const __grid_constant__ AttnArgs a, int tiles) {
-    pdl_wait();
-    pdl_trigger();
-    const int hd = (int)a.c.head_dim, panels = (hd + 63) / 64, rows = a.n * a.group;
-    const int lane = threadIdx.x & 31, kvh = blockIdx.y;
-    const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const long long base = (long long)(r / a.group) * a.qs + (long long)(kvh * a.group + r % a.group) * hd;
-    float x[8];  // values lane * 4 .. + 3, and 128 + those
-    float mx = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane * 4 + (i & 3) + 128 * (i >> 2);
-        x[i] = r < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
-        mx = fmaxf(mx, fabsf(x[i]));
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const int e = mx > 0.f && !isinf(mx) ? 7 - ilogbf(mx) : 0;
-    const float sign = a.scale < 0.f ? -1.f : 1.f;
-    unsigned char* tile = a.qt + ((size_t)kvh * tiles + r / 128) * TERMS * panels * 16384;
-    const int row = r & 127;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int d = lane * 4 + 128 * half;
-        if (d >= panels * 64) continue;
-        uint2 hi, lo;
-        const float* y = x + 4 * half;
-        split2(ldexpf(y[0], e) * sign, ldexpf(y[1], e) * sign, hi.x, lo.x);
-        split2(ldexpf(y[2], e) * sign, ldexpf(y[3], e) * sign, hi.y, lo.y);
-        // 16-byte piece (d % 64) / 8 of the row moves to piece ^ (row % 8)
-        const size_t at = (size_t)(d / 64) * 16384 + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2;
-        *reinterpret_cast<uint2*>(tile + at) = hi;
-        if (TERMS == 2) *reinterpret_cast<uint2*>(tile + (size_t)panels * 16384 + at) = lo;
-    }
-    if (lane == 0) a.qfactor[(size_t)kvh * tiles * 128 + r] = r < rows ? ldexpf(fabsf(a.scale), -e) : 0.f;
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+
+// fp32 pairs in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
-// 16 codes (values 16 c .. of row r) as halves into a swizzled tile of `height` rows
-__device__ __forceinline__ void put_codes(unsigned char* tile, int height, int r, int c, uint4 w) {
-    unsigned char* o = tile + (c >> 2) * (height * 128) + r * 128;
-    const int at = 2 * (c & 3), x = r & 7;
+// A warp puts 32 query rows of a tile into shared memory as the products read them: [TERMS][panels of
+// 64 values][128 rows][64] fp16, swizzled, row r times 2^e (its largest value near 2^7) and the sign of
+// the scale. Returns each lane's factor |scale| log2(e) 2^-e of row row0 + lane, 0 beyond the last row.
+// (The code runs once per CTA, from a cold instruction cache: little of it, for one type.)
+template <int PANELS, int TERMS, typename T>
+__device__ __forceinline__ float put_queries(const AttnArgs& a, int kvh, int r0, int row0, unsigned char* tile) {
+    const int hd = (int)a.c.head_dim, rows = a.n * a.group, lane = threadIdx.x & 31;
+    constexpr int HALVES = PANELS > 2 ? 2 : 1;  // 128 values at a time
+    constexpr int U = HALVES > 1 ? 8 : 16;      // rows in flight
+    const bool vec = (reinterpret_cast<uintptr_t>(a.q) & (4 * sizeof(T) - 1)) == 0 && (a.qs & 3) == 0;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    float mine = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < 32; i += U) {
+        Vec4<T> w[U][HALVES];  // the loads alone first: all of them in flight before a value is used
+        const T* q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = min(r0 + row0 + i + u, rows - 1);  // rows beyond the last are made zero below
+            q[u] = (const T*)a.q + (long long)(r / a.group) * a.qs + (long long)(kvh * a.group + r % a.group) * hd + lane * 4;
+        }
+        if (vec) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h)
+                    if (lane * 4 + 128 * h < hd) w[u][h].load(q[u] + 128 * h);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h)
+                    if (lane * 4 + 128 * h < hd)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[u][h].t[e] = q[u][128 * h + e];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool on = r0 + row0 + i + u < rows;
+            float mx = 0.f, x[HALVES][4];
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[h][e] = lane * 4 + 128 * h < hd ? to_f(w[u][h].t[e]) : 0.f;
+                    mx = fmaxf(mx, fabsf(x[h][e]));
+                }
+            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23;
+            const int e2 = top >= 255u ? 0 : min(120, 134 - (int)top);
+            const float f = pow2(e2) * sign;
+            const int row = row0 + i + u;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+                const int d = lane * 4 + 128 * h;
+                if (d < PANELS * 64) {
+                    uint2 hi, lo;
+                    split2(x[h][0] * f, x[h][1] * f, hi.x, lo.x);
+                    split2(x[h][2] * f, x[h][3] * f, hi.y, lo.y);
+                    if (!on) hi = lo = make_uint2(0, 0);
+                    // 16-byte piece (d % 64) / 8 of the row moves to piece ^ (row % 8)
+                    const int at = (d / 64) * 16384 + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2;
+                    *reinterpret_cast<uint2*>(tile + at) = hi;
+                    if (TERMS == 2) *reinterpret_cast<uint2*>(tile + PANELS * 16384 + at) = lo;
+                }
+            }
+            if (lane == i + u && on) mine = fabsf(a.scale) * pow2(-e2);
+        }
+    }
+    return mine;
+}
+
+// Where 16 codes (values 16 c .. of row r) begin in a swizzled tile of `height` rows, and putting them
+// there: eight of them as halves fill one 16-byte piece, the other eight the neighbouring one.
+__device__ __forceinline__ int put_at(int height, int r, int c) {
+    return (c >> 2) * (height * 128) + r * 128 + (((2 * (c & 3)) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void put_codes(unsigned char* tile, int at, uint4 w) {
     const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-    *reinterpret_cast<uint4*>(o + ((at ^ x) << 4)) = make_uint4(codes_lo(u[0]), codes_hi(u[0]), codes_lo(u[1]), codes_hi(u[1]));
-    *reinterpret_cast<uint4*>(o + (((at + 1) ^ x) << 4)) =
-        make_uint4(codes_lo(u[2]), codes_hi(u[2]), codes_lo(u[3]), codes_hi(u[3]));
+    *reinterpret_cast<uint4*>(tile + at) = make_uint4(codes_lo(u[0]), codes_hi(u[0]), codes_lo(u[1]), codes_hi(u[1]));
+    *reinterpret_cast<uint4*>(tile + (at ^ 16)) = make_uint4(codes_lo(u[2]), codes_hi(u[2]), codes_lo(u[3]), codes_hi(u[3]));
 }
 
 // ---------------------------------------------------------------------------
@@ -194,7 +252,7 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 256, "barriers");
 
-template <int PANELS, int TERMS>
+template <int PANELS, typename T, int TERMS = sizeof(T) == 4 ? 2 : 1>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
     using S = Shape<PANELS, TERMS>;
     constexpr int MT = S::MT, KT = S::KT, ST = S::ST, NB = KT / 32;
@@ -209,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int kvh = blockIdx.x % H, split = blockIdx.x / H % a.nsplit, unit = units - 1 - blockIdx.x / (H * a.nsplit);
     if (warp == kMmaWarp) {
         if (lane == 0) {
-            bar_init(&bar->q, 1);
+            bar_init(&bar->q, 4 * MT);
             for (int i = 0; i < 2; ++i) {
                 bar_init(&bar->k_full[i], kConvWarps);
                 bar_init(&bar->k_empty[i], 1);
@@ -249,12 +307,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
     if (warp < kSoftWarps) {
         // ---- softmax: one thread per row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int m = warp >> 2;
-        const int rr = (unit * MT + m) * 128 + (warp & 3) * 32 + lane;
-        if (m < MT && split < sh.active) {
+        const int r0 = (unit * MT + m) * 128, rr = r0 + (warp & 3) * 32 + lane;
+        if (m < MT && (split < sh.active || split == 0)) {
             const bool on = rr < rows;
             const int limit = on ? keys_of(past, rr / a.group, cap) : 0;
-            const float factor = a.qfactor[(size_t)kvh * tiles128 * 128 + rr];
+            const float factor = put_queries<PANELS, TERMS, T>(a, kvh, r0, (warp & 3) * 32, qs + m * S::QTile);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bar->q);
+            if (a.weight && split == 0) a.qfactor[(size_t)kvh * tiles128 * 128 + rr] = factor;
             const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's lanes: 32 (warp % 4) ..
             const uint32_t st = tmem + lanes + m * S::SCols, ot = tmem + lanes + MT * S::SCols + m * S::OCols;
             const float* ksc = a.c.k_scale + (size_t)kvh * (cap >> 5);
@@ -268,47 +331,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int blk = j * NB + b;
-                    nk[b] = blk < cap >> 5 ? ksc[blk] : 0.f;
-                    nv[b] = blk < cap >> 5 ? vsc[blk] : 0.f;
+                    nk[b] = blk < (cap >> 5) ? ksc[blk] : 0.f;
+                    nv[b] = blk < (cap >> 5) ? vsc[blk] : 0.f;
                 }
             };
-            const int n = m < MT ? nt[m < MT ? m : 0] : 0;
+            const int n = m == 0 ? nt[0] : nt[MT - 1];
             if (n) scales(j0);
-            for (int i = 0; i < n; ++i) {
-                const int j = j0 + i, key0 = j * KT;
+            // a tile's P from its S; FULL: no key of the tile is hidden from a row of the warp
+            auto tile = [&](auto whole, int i) {
+                constexpr bool FULL = decltype(whole)::value;
+                const int key0 = (j0 + i) * KT, seen = limit - key0;
                 float kf[NB], vb[NB];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     kf[b] = factor * nk[b];
                     vb[b] = nv[b];
                 }
-                if (i + 1 < n) scales(j + 1);
-                alive = wait_or(&bar->s_full[m], (uint32_t)(i & 1), &bar->dead, a.err);
-                alive = __all_sync(0xffffffffu, alive);
-                if (!alive) break;
-                tc_after();
-                const bool full = key0 + KT <= all;  // no key of the tile is hidden from a row of the warp
-                // the tile's largest score
-                float mt = -INFINITY;
-                float vmax = 0.f;
+                if (i + 1 < n) scales(j0 + i + 1);
+                uint32_t r[NB][32];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) tmem_ld32(r[b], st + 32 * b);
+                tmem_wait_ld();
+                float mt = -INFINITY, vmax = 0.f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    uint32_t r[32];
-                    tmem_ld32(r, st + 32 * b);
-                    tmem_wait_ld();
-                    float x = -INFINITY;
-                    if (full) {
+                    float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x = fmaxf(x, __uint_as_float(r[e]));
-                        mt = fmaxf(mt, x * kf[b]);
-                    } else if (key0 + 32 * b < limit) {
-                        const int c = limit - key0 - 32 * b;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (e < c) x = fmaxf(x, __uint_as_float(r[e]));
-                        mt = fmaxf(mt, x * kf[b]);
+                    for (int e = 0; e < 32; e += 2) {
+                        if (FULL || 32 * b + e < seen) x0 = fmaxf(x0, __uint_as_float(r[b][e]));
+                        if (FULL || 32 * b + e + 1 < seen) x1 = fmaxf(x1, __uint_as_float(r[b][e + 1]));
                     }
-                    if (key0 + 32 * b < limit) vmax = fmaxf(vmax, vb[b]);
+                    if (FULL || 32 * b < seen) {
+                        mt = fmaxf(mt, fmaxf(x0, x1) * kf[b]);
+                        vmax = fmaxf(vmax, vb[b]);
+                    }
                 }
                 // O and l follow m and the reference of V's scales when those move
                 const float vtop = vmax > 4.f * vref ? vmax : vref;
@@ -319,12 +375,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     if (i > 0) {
 #pragma unroll 1
                         for (int c = 0; c < hd; c += 16) {
-                            uint32_t r[16];
-                            tmem_ld16(r, ot + c);
+                            uint32_t o[16];
+                            tmem_ld16(o, ot + c);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-                            tmem_st16(ot + c, r);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(ot + c, o);
                         }
                     }
                     l *= fl;
@@ -332,32 +388,48 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     vref = vtop;
                 }
                 const float mu = mref == -INFINITY ? 0.f : mref;
+                const uint64_t mu2 = pair(-mu, -mu);
+                uint64_t sum = pair(0.f, 0.f);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    uint32_t r[32], hi[16], lo[16];
-                    tmem_ld32(r, st + 32 * b);
                     const float vr = vb[b] == 0.f ? 0.f : vb[b] / vref * kPScale;
-                    tmem_wait_ld();
-                    float bs = 0.f;
+                    const uint64_t kf2 = pair(kf[b], kf[b]), vr2 = pair(vr, vr);
+                    uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        float p0 = ex2(__fmaf_rn(__uint_as_float(r[2 * e]), kf[b], -mu));
-                        float p1 = ex2(__fmaf_rn(__uint_as_float(r[2 * e + 1]), kf[b], -mu));
-                        float w0 = p0 * vr, w1 = p1 * vr;
-                        if (!full) {
-                            const int c = limit - key0 - 32 * b;
-                            if (2 * e >= c) p0 = w0 = 0.f;
-                            if (2 * e + 1 >= c) p1 = w1 = 0.f;
+                        float p0, p1, w0, w1;
+                        unpair(fma2(pair(__uint_as_float(r[b][2 * e]), __uint_as_float(r[b][2 * e + 1])), kf2, mu2), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        if (!FULL) {
+                            if (32 * b + 2 * e >= seen) p0 = 0.f;
+                            if (32 * b + 2 * e + 1 >= seen) p1 = 0.f;
                         }
-                        bs += p0 + p1;
+                        const uint64_t p = pair(p0, p1);
+                        sum = add2(sum, p);
+                        unpair(mul2(p, vr2), w0, w1);
+                        if (!FULL) {  // (a scale that is not finite may lie behind a row's keys)
+                            if (32 * b + 2 * e >= seen) w0 = 0.f;
+                            if (32 * b + 2 * e + 1 >= seen) w1 = 0.f;
+                        }
                         if (TERMS == 2) split2(w0, w1, hi[e], lo[e]);
                         else hi[e] = h2_bits(__floats2half2_rn(w0, w1));
                     }
-                    l += bs;
                     // over the block's scores: hi in its first 16 columns, lo in the next
                     tmem_st16(st + 32 * b, hi);
                     if (TERMS == 2) tmem_st16(st + 32 * b + 16, lo);
                 }
+                float s0, s1;
+                unpair(sum, s0, s1);
+                l += s0 + s1;
+            };
+            for (int i = 0; i < n; ++i) {
+                alive = wait_or(&bar->s_full[m], (uint32_t)(i & 1), &bar->dead, a.err);
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) break;
+                tc_after();
+                if ((j0 + i + 1) * KT <= all) tile(std::true_type{}, i);
+                else tile(std::false_type{}, i);
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();
@@ -366,12 +438,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // ---- the row's output, or its part ----
             if (n && alive) alive = __all_sync(0xffffffffu, wait_or(&bar->o_full[m], 0, &bar->dead, a.err));
             tc_after();
-            const bool whole = sh.active == 1;
+            const bool whole = sh.active == 1, out = on && split < sh.active;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale);
             const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
             const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
             float* po = a.part_o + pr * hd;
+#pragma unroll 2
             for (int c = 0; c < hd; c += 16) {
                 uint32_t r[16];
                 if (n) {
@@ -381,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                     for (int e = 0; e < 16; ++e) r[e] = 0;
                 }
-                if (!on) continue;
+                if (!out) continue;
                 // a row that has seen no key, or only blocks of zeros: 0
                 float v[16];
 #pragma unroll
@@ -389,32 +462,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 if (!whole) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(po + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                } else if (a.type == NEON_GGML_F32 && ((reinterpret_cast<uintptr_t>((float*)a.o + ob)) & 15) == 0) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<float4*>((float*)a.o + ob + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                } else if (a.type == NEON_GGML_BF16 && ((reinterpret_cast<uintptr_t>((__nv_bfloat16*)a.o + ob)) & 15) == 0) {
-                    uint4 w[2];
-                    __nv_bfloat162* q = reinterpret_cast<__nv_bfloat162*>(w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                    uint4* d = reinterpret_cast<uint4*>((__nv_bfloat16*)a.o + ob + c);
-                    d[0] = w[0];
-                    d[1] = w[1];
-                } else if (a.type == NEON_GGML_F16 && ((reinterpret_cast<uintptr_t>((__half*)a.o + ob)) & 15) == 0) {
-                    uint4 w[2];
-                    __half2* q = reinterpret_cast<__half2*>(w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-                    uint4* d = reinterpret_cast<uint4*>((__half*)a.o + ob + c);
-                    d[0] = w[0];
-                    d[1] = w[1];
                 } else {
+                    T* d = (T*)a.o + ob + c;
+                    alignas(16) T w[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o_store(a.o, a.type, ob + c + e, v[e]);
+                    for (int e = 0; e < 16; ++e) w[e] = from_f<T>(v[e]);
+                    if ((reinterpret_cast<uintptr_t>(d) & 15) == 0) {
+#pragma unroll
+                        for (int e = 0; e < (int)sizeof(T); ++e) reinterpret_cast<uint4*>(d)[e] = reinterpret_cast<const uint4*>(w)[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) d[e] = w[e];
+                    }
                 }
             }
-            if (on) {
+            if (out) {
                 const float mu = mref == -INFINITY ? 0.f : mref;
                 float* d = whole ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
                 d[0] = whole ? mu : mref;
@@ -422,34 +484,37 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             }
             tc_before();
         }
-    } else if (warp < kMmaWarp) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));  // whole warpgroups
+        if (warp != kMmaWarp) {
         // ---- conversion: codes to fp16, swizzled ----
-        const int ct = tid - kSoftWarps * 32;
+        constexpr int kConv = kConvWarps * 32;
+        const int ct = tid - kSoftWarps * 32 - (warp > kMmaWarp ? 32 : 0);
         const int pieces = hd / 16;                 // 16-byte pieces of a row
         const int total = KT * pieces;
-        constexpr int L = KT * PANELS * 4 / 128;    // pieces per thread at most
-        const int8_t* kc = a.c.k + (size_t)kvh * cap * hd;
-        const int8_t* vc = a.c.v + (size_t)kvh * cap * hd;
+        constexpr int L = (KT * PANELS * 4 + kConv - 1) / kConv;  // pieces per thread at most
+        const uint4* kc = reinterpret_cast<const uint4*>(a.c.k + (size_t)kvh * cap * hd);
+        const uint4* vc = reinterpret_cast<const uint4*>(a.c.v + (size_t)kvh * cap * hd);
+        const long long end = (long long)cap * pieces;
         uint4 kr[L], vr[L];
-        auto load = [&](uint4 (&w)[L], const int8_t* base, int j) {
-            const long long at = (long long)j * total;
-            const long long end = (long long)cap * pieces;
+        int put[L];  // where a piece goes in a tile
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int p = ct + kConv * i, r = p / pieces;
+            put[i] = p < total ? put_at(KT, r, p - r * pieces) : -1;
+        }
+        auto load = [&](uint4 (&w)[L], const uint4* base, int j) {
+            const long long at = (long long)j * total + ct;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const int p = ct + 128 * i;
                 w[i] = make_uint4(0, 0, 0, 0);
-                if (p < total && at + p < end) w[i] = *(reinterpret_cast<const uint4*>(base) + at + p);
+                if (put[i] >= 0 && at + kConv * i < end) w[i] = base[at + kConv * i];
             }
         };
         auto store = [&](const uint4 (&w)[L], unsigned char* d) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const int p = ct + 128 * i;
-                if (p < total) {
-                    const int r = p / pieces;
-                    put_codes(d, KT, r, p - r * pieces, w[i]);
-                }
-            }
+            for (int i = 0; i < L; ++i)
+                if (put[i] >= 0) put_codes(d, put[i], w[i]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
@@ -469,21 +534,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (lane == 0) bar_arrive(&bar->v_full[s]);
             if (i + 1 < most) load(vr, vc, j0 + i + 1);
         }
-    } else if (lane == 0 && most && split < sh.active) {
+        } else if (lane == 0 && (most || (a.weight && split == 0))) {
         // ---- products ----
         const uint32_t id_s = instr(KT, false), id_o = instr(hd, true);
         const uint32_t qa = smem_addr(qs), ka = smem_addr(ks), va = smem_addr(vs);
-        const unsigned char* qsrc = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT) * S::QTile;
-        bar_expect(&bar->q, MT * S::QTile);
-        for (int p = 0; p < MT * TERMS * PANELS; ++p) bulk_load(qs + p * 16384, qsrc + (size_t)p * 16384, 16384, &bar->q);
         bool alive = wait_or(&bar->q, 0, &bar->dead, a.err);
+        const bool keep = a.weight && split == 0 && alive;
+        if (keep) {  // the weights' kernel reads the query tiles
+            unsigned char* dst = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT) * S::QTile;
+            for (int p = 0; p < MT * TERMS * PANELS; ++p)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)p * 16384),
+                             "r"(qa + p * 16384), "r"(16384)
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
         const int steps = hd / 16;
+        // Operands by one addition each (16-byte units into a descriptor's address): the issuing thread's
+        // own instructions would otherwise take longer than the products.
+        const uint64_t qd = operand(qa, 16), kd = operand(ka, 16), vd = operand(va, KT * 128);
         auto scores = [&](int m, int i) {  // S_m = Q_m K^T of the share's tile i
-            const uint32_t k = ka + (i % ST) * S::Stage, q = qa + m * S::QTile;
+            const uint64_t k = kd + (uint32_t)((i % ST) * (S::Stage >> 4)), q = qd + (uint32_t)(m * (S::QTile >> 4));
+            const uint32_t d = tmem + m * S::SCols;
+#pragma unroll
             for (int t = 0; t < TERMS; ++t)
-                for (int s = 0; s < steps; ++s)
-                    mma_ss(tmem + m * S::SCols, operand(q + (t * PANELS + (s >> 2)) * 16384 + (s & 3) * 32, 16),
-                           operand(k + (s >> 2) * (KT * 128) + (s & 3) * 32, 16), id_s, t + s > 0);
+#pragma unroll
+                for (int s = 0; s < PANELS * 4; ++s)
+                    if (s < steps)
+                        mma_ss(d, q + (uint32_t)((t * PANELS + (s >> 2)) * 1024 + (s & 3) * 2), k + (uint32_t)((s >> 2) * (KT * 8) + (s & 3) * 2),
+                               id_s, t + s > 0);
             tc_commit(&bar->s_full[m]);
         };
         auto last_of = [&](int i) {  // the last query tile that has tile i
@@ -492,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 if (i < nt[m]) r = m;
             return r;
         };
-        alive = alive && wait_or(&bar->k_full[0], 0, &bar->dead, a.err);
+        alive = alive && most && wait_or(&bar->k_full[0], 0, &bar->dead, a.err);
         if (alive) {
             tc_after();
             for (int m = 0; m < MT; ++m)
@@ -509,10 +587,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 if (!alive) break;
                 tc_after();
                 // P of key block b: hi at columns 32 b .., lo at 32 b + 16 ..
+                const uint64_t v = vd + (uint32_t)(sv * (S::Stage >> 4));
+                const uint32_t od = tmem + MT * S::SCols + m * S::OCols, pd = tmem + m * S::SCols;
+#pragma unroll
                 for (int t = 0; t < TERMS; ++t)
+#pragma unroll
                     for (int s = 0; s < KT / 16; ++s)
-                        mma_ts(tmem + MT * S::SCols + m * S::OCols, tmem + m * S::SCols + 32 * (s >> 1) + 16 * t + 8 * (s & 1),
-                               operand(va + sv * S::Stage + s * 2048, KT * 128), id_o, i > 0 || t + s > 0);
+                        mma_ts(od, pd + 32 * (s >> 1) + 16 * t + 8 * (s & 1), v + (uint32_t)(s * 128), id_o, i > 0 || t + s > 0);
                 if (i + 1 == nt[m]) tc_commit(&bar->o_full[m]);
                 if (i + 1 < nt[m]) {
                     alive = wait_or(&bar->k_full[sk], (uint32_t)(((i + 1) / ST) & 1), &bar->dead, a.err);
@@ -528,6 +609,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         tc_commit(&bar->drain);
         volatile int never = 0;
         wait_or(&bar->drain, 0, &never, a.err);
+        if (keep) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
     }
     __syncwarp();
     tc_before();
@@ -554,7 +637,8 @@ struct WShape {
     static constexpr int Smem = MT * KTile + ST * Stage + 2 * 128 * 8 + 1024 + 256;
     static_assert(Smem <= 232448, "shared memory");
 };
-constexpr int kWThreads = kThreads + 32;  // and a warp that loads
+// warps 0-7 sum, 8-11 convert the keys and fill in the rows' numbers, 12 the products, 13 loads
+constexpr int kWThreads = 448, kWConvWarps = 4;
 
 struct WBars {
     uint64_t k_full, q_full[4], q_empty[4], s_full[2], s_empty[2], st_full[2], drain;
@@ -581,7 +665,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == kMmaWarp) {
         if (lane == 0) {
-            bar_init(&bar->k_full, kConvWarps);
+            bar_init(&bar->k_full, kWConvWarps);
             for (int i = 0; i < ST; ++i) {
                 bar_init(&bar->q_full[i], 1);
                 bar_init(&bar->q_empty[i], 1);
@@ -589,7 +673,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             for (int i = 0; i < 2; ++i) {
                 bar_init(&bar->s_full[i], 1);
                 bar_init(&bar->s_empty[i], 4 * MT);
-                bar_init(&bar->st_full[i], kConvWarps);
+                bar_init(&bar->st_full[i], kWConvWarps);
             }
             bar_init(&bar->drain, 1);
             bar->dead = 0;
@@ -658,7 +742,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
         for (int p = ct; p < MT * 128 * pieces; p += 128) {
             const int r = p / pieces;
             const uint4 w = p < held ? kc[p] : make_uint4(0, 0, 0, 0);
-            put_codes(ks + (r >> 7) * S::KTile, 128, r & 127, p - r * pieces, w);
+            put_codes(ks + (r >> 7) * S::KTile, put_at(128, r & 127, p - r * pieces), w);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -677,7 +761,8 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             if (lane == 0) bar_arrive(&bar->st_full[b]);
         }
     } else if (warp == kMmaWarp && lane == 0) {
-        const uint32_t id = instr(128, false), ka = smem_addr(ks), qa = smem_addr(qs);
+        const uint32_t id = instr(128, false);
+        const uint64_t kd = operand(smem_addr(ks), 16), qd = operand(smem_addr(qs), 16);
         const int steps = hd / 16;
         bool ok = wait_or(&bar->k_full, 0, &bar->dead, a.err);
         int it = 0;
@@ -689,10 +774,14 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
                 ok = wait_or(&bar->q_full[sg], (uint32_t)((it / ST) & 1), &bar->dead, a.err);
                 if (!ok) break;
                 tc_after();
+                const uint64_t q = qd + (uint32_t)(sg * (S::Stage >> 4));
+#pragma unroll
                 for (int m = 0; m < MT; ++m)
-                    for (int s = 0; s < steps; ++s)
-                        mma_ss(tmem + m * 256 + b * 128, operand(ka + m * S::KTile + (s >> 2) * 16384 + (s & 3) * 32, 16),
-                               operand(qa + sg * S::Stage + (s >> 2) * 16384 + (s & 3) * 32, 16), id, t + s > 0);
+#pragma unroll
+                    for (int s = 0; s < PANELS * 4; ++s)
+                        if (s < steps)
+                            mma_ss(tmem + m * 256 + b * 128, kd + (uint32_t)(m * (S::KTile >> 4) + (s >> 2) * 1024 + (s & 3) * 2),
+                                   q + (uint32_t)((s >> 2) * 1024 + (s & 3) * 2), id, t + s > 0);
                 tc_commit(&bar->q_empty[sg]);
             }
             if (ok) tc_commit(&bar->s_full[b]);
@@ -736,18 +825,21 @@ int launch_weights(const AttnArgs& a, cudaStream_t st) {
 
 using PromptKernel = void (*)(AttnArgs, int);
 
-template <int PANELS, int TERMS>
+template <int PANELS, typename T>
 int launch_shape(const AttnArgs& a, cudaStream_t st) {
-    using S = Shape<PANELS, TERMS>;
+    using S = Shape<PANELS, sizeof(T) == 4 ? 2 : 1>;
     const int rows = a.n * a.group, H = (int)a.c.n_kv_head;
     const int tiles = (rows + 255) / 256 * 2;
-    PromptKernel k = kv8_prompt_kernel<PANELS, TERMS>;
+    PromptKernel k = kv8_prompt_kernel<PANELS, T>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
     if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_prompt_kernel)");
-    int rc = launch("kv8_queries_kernel", kv8_queries_kernel<TERMS>, dim3((unsigned)tiles * 16, (unsigned)H), 256, 0, st, 1, a, tiles);
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, k);
+    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncGetAttributes(kv8_prompt_kernel)");
+    // the kernel's register split waits for registers that the launch has to have
+    if (fa.numRegs < kLaunchRegs) return neon_internal::error(NEON_ERR_UNSUPPORTED, "kv8_prompt_kernel: built with too few registers");
     const int units = (rows + 128 * S::MT - 1) / (128 * S::MT);
-    if (!rc) rc = launch("kv8_prompt_kernel", k, dim3((unsigned)(units * H * a.nsplit)), kThreads, S::Smem, st, 1, a, tiles);
-    return rc;
+    return launch("kv8_prompt_kernel", k, dim3((unsigned)(units * H * a.nsplit)), kThreads, S::Smem, st, 1, a, tiles);
 }
 
 }  // namespace
@@ -760,14 +852,19 @@ size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type) {
     return c.n_kv_head * tiles * (type == NEON_GGML_F32 ? 2 : 1) * panels * 16384;
 }
 
+template <int PANELS>
+static int launch_typed(const AttnArgs& a, cudaStream_t st) {
+    return a.type == NEON_GGML_F32   ? launch_shape<PANELS, float>(a, st)
+           : a.type == NEON_GGML_F16 ? launch_shape<PANELS, __half>(a, st)
+                                     : launch_shape<PANELS, __nv_bfloat16>(a, st);
+}
+
 int launch_prompt(const AttnArgs& a, cudaStream_t st) {
-    const int panels = ((int)a.c.head_dim + 63) / 64;
-    const bool two = a.type == NEON_GGML_F32;
-    switch (panels) {
-        case 1: return two ? launch_shape<1, 2>(a, st) : launch_shape<1, 1>(a, st);
-        case 2: return two ? launch_shape<2, 2>(a, st) : launch_shape<2, 1>(a, st);
-        case 3: return two ? launch_shape<3, 2>(a, st) : launch_shape<3, 1>(a, st);
-        default: return two ? launch_shape<4, 2>(a, st) : launch_shape<4, 1>(a, st);
+    switch (((int)a.c.head_dim + 63) / 64) {
+        case 1: return launch_typed<1>(a, st);
+        case 2: return launch_typed<2>(a, st);
+        case 3: return launch_typed<3>(a, st);
+        default: return launch_typed<4>(a, st);
     }
 }
 
@@ -783,3 +880,4 @@ int launch_prompt_weights(const AttnArgs& a, cudaStream_t st) {
 }
 
 }  // namespace longctx
+

@@ -42,11 +42,19 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 bytes of T as floats, and back.
+// Four values of T in one load.
 template <typename T>
-struct Vec {
-    static constexpr int N = 16 / (int)sizeof(T);
-    union { uint4 u; T t[N]; };
+struct alignas(4 * sizeof(T)) Vec4 {
+    T t[4];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (sizeof(T) == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            *reinterpret_cast<uint4*>(t) = v;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            *reinterpret_cast<uint2*>(t) = v;
+        }
+    }
 };
 
 // ---- mbarriers and bulk copies (one warp or CTA of its own shared memory) ----
