@@ -516,8 +516,8 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     const int hd = (int)c.head_dim;
     int rc;
     if (p.prompt) {
-        a.tile_keys = prompt_tile_keys(hd);
-        a.min_tiles = 4;
+        a.tile_keys = prompt_tile_keys();
+        a.min_tiles = 8;
         rc = launch_prompt(a, st);
     } else {
         a.tile_keys = 32;

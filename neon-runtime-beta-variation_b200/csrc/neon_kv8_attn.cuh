@@ -92,7 +92,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Prompts (neon_kv8_prompt.cu): bytes of the query tiles, and the launches.
 size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type);
 int prompt_unit(int hd);
-int prompt_tile_keys(int hd);
+int prompt_tile_keys();
 int launch_prompt(const AttnArgs& a, cudaStream_t st);
 int launch_prompt_weights(const AttnArgs& a, cudaStream_t st);  // after launch_prompt and its joins
 

@@ -32,12 +32,10 @@
 namespace longctx {
 namespace {
 
-// Warps 0-7 softmax, 12 the products, 8-11 and 13-15 conversion. The launch's 512 x 128 registers are
-// dealt out again by warpgroup: a softmax thread holds its row of S (128 values) in registers.
+// Warps 0-7 softmax, 12 the products, 8-11 and 13-15 conversion.
 constexpr int kSoftWarps = 8, kMmaWarp = 12, kConvWarps = 7;
 constexpr int kThreads = 512;
-constexpr int kLaunchRegs = 128, kSoftRegs = 184, kOtherRegs = 72;
-static_assert(2 * kSoftRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
+constexpr int kTileKeys = 64;
 constexpr float kLazy = 8.f;     // log2 of how far p may exceed 1
 constexpr float kPScale = 32.f;  // 2^5
 
@@ -94,10 +92,22 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory operand of 128-byte-swizzled panels [rows][64 halves]: groups of eight rows are 1024
-// bytes apart; `lead` is the distance of the panels (used when the panels run along M or N).
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// bytes apart; `lead` is the distance of the panels (used when the panels run along M or N). The low
+// word has the address (in 16 bytes) and lead, the high word is the same for all.
+__device__ __forceinline__ uint32_t operand_lo(uint32_t addr, uint32_t lead) {
+    return (addr & 0x3ffff) >> 4 | ((lead >> 4) & 0x3fff) << 16;
+}
+__device__ __forceinline__ uint64_t operand_of(uint32_t lo) {
+    return (uint64_t)(1024 >> 4 | 1u << 14 | 2u << 29) << 32 | lo;
+}
+// The same value in every lane, and known to be.
+template <typename T>
+__device__ __forceinline__ T uniform(T v) { return __shfl_sync(0xffffffffu, v, 0); }
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p != 0;
 }
 // fp16 x fp16 -> fp32, M = 128; b_mn: B's rows run along the summed dimension
 __device__ __forceinline__ uint32_t instr(int n, bool b_mn) {
@@ -234,23 +244,24 @@ __device__ __forceinline__ void put_codes(unsigned char* tile, int at, uint4 w) 
 template <int PANELS, int TERMS>
 struct Shape {
     static constexpr int MT = PANELS <= 2 ? 2 : 1;       // query tiles of 128 rows
-    static constexpr int KT = PANELS <= 2 ? 128 : 64;    // keys of a tile
-    static constexpr int ST = PANELS == 1 || TERMS == 1 ? 2 : 1;  // tiles of K, and of V, held at once
+    static constexpr int KT = kTileKeys;                 // keys of a tile
     static constexpr int QTile = TERMS * PANELS * 16384;
     static constexpr int Stage = PANELS * KT * 128;
-    static constexpr int Bytes = MT * QTile + 2 * ST * Stage;
-    static constexpr int Smem = Bytes + 1024 + 256;
-    static constexpr int SCols = KT, OCols = PANELS * 64;
+    static constexpr int fits(int st) { return MT * QTile + 2 * st * Stage + 1024 + 512 <= 232448; }
+    static constexpr int ST = fits(4) ? 4 : fits(2) ? 2 : 1;  // tiles of K, and of V, held at once
+    static constexpr int Ahead = ST > 1 ? 2 : 1;              // tiles that the scores are ahead of the outputs
+    static constexpr int Smem = MT * QTile + 2 * ST * Stage + 1024 + 512;
+    static constexpr int SCols = 2 * KT, OCols = PANELS * 64;  // two buffers of S
     static_assert(MT * (SCols + OCols) <= 512, "tensor memory");
     static_assert(Smem <= 232448, "shared memory");
 };
 
 struct Bars {
-    uint64_t q, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drain;
+    uint64_t q, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drain;
     uint32_t tmem;
     int dead;
 };
-static_assert(sizeof(Bars) <= 256, "barriers");
+static_assert(sizeof(Bars) <= 512, "barriers");
 
 template <int PANELS, typename T, int TERMS = sizeof(T) == 4 ? 2 : 1>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
@@ -268,13 +279,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     if (warp == kMmaWarp) {
         if (lane == 0) {
             bar_init(&bar->q, 4 * MT);
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 bar_init(&bar->k_full[i], kConvWarps);
                 bar_init(&bar->k_empty[i], 1);
                 bar_init(&bar->v_full[i], kConvWarps);
                 bar_init(&bar->v_empty[i], 1);
-                bar_init(&bar->s_full[i], 1);
-                bar_init(&bar->p_full[i], 4);
+                bar_init(&bar->s_full[i >> 1][i & 1], 1);
+                bar_init(&bar->p_full[i >> 1][i & 1], 4);
+            }
+            for (int i = 0; i < 2; ++i) {
+                bar_init(&bar->o_done[i], 1);
                 bar_init(&bar->o_full[i], 1);
             }
             bar_init(&bar->drain, 1);
@@ -307,7 +321,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
     if (warp < kSoftWarps) {
         // ---- softmax: one thread per row ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int m = warp >> 2;
         const int r0 = (unit * MT + m) * 128, rr = r0 + (warp & 3) * 32 + lane;
         if (m < MT && (split < sh.active || split == 0)) {
@@ -326,43 +339,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             const int all = __reduce_min_sync(0xffffffffu, limit);
             float mref = -INFINITY, l = 0.f, vref = 0.f;
             bool alive = true;
-            float nk[NB], nv[NB];
+            float nk = 0.f, nv = 0.f;  // lane b: the scales of the next tile's block b
             auto scales = [&](int j) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const int blk = j * NB + b;
-                    nk[b] = blk < (cap >> 5) ? ksc[blk] : 0.f;
-                    nv[b] = blk < (cap >> 5) ? vsc[blk] : 0.f;
-                }
+                const int blk = j * NB + lane;
+                const bool in = lane < NB && blk < (cap >> 5);
+                nk = in ? ksc[blk] : 0.f;
+                nv = in ? vsc[blk] : 0.f;
             };
             const int n = m == 0 ? nt[0] : nt[MT - 1];
             if (n) scales(j0);
-            // a tile's P from its S; FULL: no key of the tile is hidden from a row of the warp
+            // A tile's P from its S; FULL: no key of the tile is hidden from a row of the warp.
             auto tile = [&](auto whole, int i) {
                 constexpr bool FULL = decltype(whole)::value;
-                const int key0 = (j0 + i) * KT, seen = limit - key0;
+                const int seen = limit - (j0 + i) * KT;
+                const uint32_t sb = st + (i & 1) * KT;
                 float kf[NB], vb[NB];
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    kf[b] = factor * nk[b];
-                    vb[b] = nv[b];
-                }
-                if (i + 1 < n) scales(j0 + i + 1);
                 uint32_t r[NB][32];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) tmem_ld32(r[b], st + 32 * b);
+                for (int b = 0; b < NB; ++b) tmem_ld32(r[b], sb + 32 * b);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    kf[b] = factor * __shfl_sync(0xffffffffu, nk, b);
+                    vb[b] = __shfl_sync(0xffffffffu, nv, b);
+                }
+                if (i + 1 < n) scales(j0 + i + 1);
                 tmem_wait_ld();
                 float mt = -INFINITY, vmax = 0.f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    float x0 = -INFINITY, x1 = -INFINITY;
+                    const int c = seen - 32 * b;
+                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        if (FULL || 32 * b + e < seen) x0 = fmaxf(x0, __uint_as_float(r[b][e]));
-                        if (FULL || 32 * b + e + 1 < seen) x1 = fmaxf(x1, __uint_as_float(r[b][e + 1]));
-                    }
-                    if (FULL || 32 * b < seen) {
-                        mt = fmaxf(mt, fmaxf(x0, x1) * kf[b]);
+                    for (int e = 0; e < 32; ++e)
+                        if (FULL || e < c) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(r[b][e]));
+                    if (FULL || c > 0) {
+                        mt = fmaxf(mt, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * kf[b]);
                         vmax = fmaxf(vmax, vb[b]);
                     }
                 }
@@ -372,7 +383,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 if (__any_sync(0xffffffffu, mnew != mref || vtop != vref)) {
                     const float fl = mref == -INFINITY ? 0.f : ex2(mref - mnew);
                     const float f = vtop > 0.f ? fl * (vref / vtop) : fl;
+                    // once the tile before has been added: of the outputs, i - 1 or i have ended here (the scores
+                    // of tile i come after output i - 2, output i needs this tile's P), so the parity is clear
                     if (i > 0) {
+                        alive = __all_sync(0xffffffffu, wait_or(&bar->o_done[m], (uint32_t)(i - 1) & 1, &bar->dead, a.err));
+                        tc_after();
 #pragma unroll 1
                         for (int c = 0; c < hd; c += 16) {
                             uint32_t o[16];
@@ -389,12 +404,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 const float mu = mref == -INFINITY ? 0.f : mref;
                 const uint64_t mu2 = pair(-mu, -mu);
-                uint64_t sum = pair(0.f, 0.f);
+                uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const float vr = vb[b] == 0.f ? 0.f : vb[b] / vref * kPScale;
-                    const uint64_t kf2 = pair(kf[b], kf[b]), vr2 = pair(vr, vr);
                     uint32_t hi[16], lo[16];
+                    const float vr = vb[b] == 0.f ? 0.f : __fdividef(vb[b], vref) * kPScale;
+                    const uint64_t kf2 = pair(kf[b], kf[b]), vr2 = pair(vr, vr);
+                    const int c = seen - 32 * b;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float p0, p1, w0, w1;
@@ -402,30 +418,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                         p0 = ex2(p0);
                         p1 = ex2(p1);
                         if (!FULL) {
-                            if (32 * b + 2 * e >= seen) p0 = 0.f;
-                            if (32 * b + 2 * e + 1 >= seen) p1 = 0.f;
+                            if (2 * e >= c) p0 = 0.f;
+                            if (2 * e + 1 >= c) p1 = 0.f;
                         }
                         const uint64_t p = pair(p0, p1);
-                        sum = add2(sum, p);
+                        sum[e & 1] = add2(sum[e & 1], p);
                         unpair(mul2(p, vr2), w0, w1);
                         if (!FULL) {  // (a scale that is not finite may lie behind a row's keys)
-                            if (32 * b + 2 * e >= seen) w0 = 0.f;
-                            if (32 * b + 2 * e + 1 >= seen) w1 = 0.f;
+                            if (2 * e >= c) w0 = 0.f;
+                            if (2 * e + 1 >= c) w1 = 0.f;
                         }
                         if (TERMS == 2) split2(w0, w1, hi[e], lo[e]);
                         else hi[e] = h2_bits(__floats2half2_rn(w0, w1));
                     }
                     // over the block's scores: hi in its first 16 columns, lo in the next
-                    tmem_st16(st + 32 * b, hi);
-                    if (TERMS == 2) tmem_st16(st + 32 * b + 16, lo);
+                    tmem_st16(sb + 32 * b, hi);
+                    if (TERMS == 2) tmem_st16(sb + 32 * b + 16, lo);
                 }
                 float s0, s1;
-                unpair(sum, s0, s1);
+                unpair(add2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
             };
-            for (int i = 0; i < n; ++i) {
-                alive = wait_or(&bar->s_full[m], (uint32_t)(i & 1), &bar->dead, a.err);
-                alive = __all_sync(0xffffffffu, alive);
+            for (int i = 0; i < n && alive; ++i) {
+                alive = __all_sync(0xffffffffu, wait_or(&bar->s_full[m][i & 1], (uint32_t)(i >> 1) & 1, &bar->dead, a.err));
                 if (!alive) break;
                 tc_after();
                 if ((j0 + i + 1) * KT <= all) tile(std::true_type{}, i);
@@ -433,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&bar->p_full[m]);
+                if (lane == 0) bar_arrive(&bar->p_full[m][i & 1]);
             }
             // ---- the row's output, or its part ----
             if (n && alive) alive = __all_sync(0xffffffffu, wait_or(&bar->o_full[m], 0, &bar->dead, a.err));
@@ -485,7 +500,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             tc_before();
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));  // whole warpgroups
         if (warp != kMmaWarp) {
         // ---- conversion: codes to fp16, swizzled ----
         constexpr int kConv = kConvWarps * 32;
@@ -524,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         }
         for (int i = 0; i < most; ++i) {
             const int s = i % ST;
-            const uint32_t ph = (uint32_t)((i / ST) & 1);
+            const uint32_t ph = (uint32_t)(i / ST) & 1;
             if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->k_empty[s], ph ^ 1, &bar->dead, a.err))) break;
             store(kr, ks + s * S::Stage);
             if (lane == 0) bar_arrive(&bar->k_full[s]);
@@ -534,82 +548,109 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (lane == 0) bar_arrive(&bar->v_full[s]);
             if (i + 1 < most) load(vr, vc, j0 + i + 1);
         }
-        } else if (lane == 0 && (most || (a.weight && split == 0))) {
-        // ---- products ----
-        const uint32_t id_s = instr(KT, false), id_o = instr(hd, true);
-        const uint32_t qa = smem_addr(qs), ka = smem_addr(ks), va = smem_addr(vs);
-        bool alive = wait_or(&bar->q, 0, &bar->dead, a.err);
-        const bool keep = a.weight && split == 0 && alive;
-        if (keep) {  // the weights' kernel reads the query tiles
-            unsigned char* dst = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT) * S::QTile;
-            for (int p = 0; p < MT * TERMS * PANELS; ++p)
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)p * 16384),
-                             "r"(qa + p * 16384), "r"(16384)
-                             : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-        const int steps = hd / 16;
-        // Operands by one addition each (16-byte units into a descriptor's address): the issuing thread's
-        // own instructions would otherwise take longer than the products.
-        const uint64_t qd = operand(qa, 16), kd = operand(ka, 16), vd = operand(va, KT * 128);
-        auto scores = [&](int m, int i) {  // S_m = Q_m K^T of the share's tile i
-            const uint64_t k = kd + (uint32_t)((i % ST) * (S::Stage >> 4)), q = qd + (uint32_t)(m * (S::QTile >> 4));
-            const uint32_t d = tmem + m * S::SCols;
+        } else if (most || (a.weight && split == 0)) {
+            // ---- products: the whole warp goes along, one elected lane issues. Descriptors come from one
+            // shuffled word each, so they stay in uniform registers: an issue then takes less than the 64
+            // clocks of its product ----
+            const uint32_t id_s = instr(KT, false), id_o = instr(hd, true);
+            const int steps = hd / 16;
+            const uint32_t base = uniform(smem_addr(qs));
+            const uint32_t kb = base + MT * S::QTile, vb = kb + ST * S::Stage;
+            int n[MT];
 #pragma unroll
-            for (int t = 0; t < TERMS; ++t)
+            for (int m = 0; m < MT; ++m) n[m] = uniform(nt[m]);
+            const int all = uniform(most);
+            const uint32_t tm = uniform(tmem);
+            auto wait = [&](uint64_t* b, uint32_t parity) {
+                bool ok = true;
+                if (lane == 0) ok = wait_or(b, parity, &bar->dead, a.err);
+                return uniform((int)ok) != 0;
+            };
+            auto commit = [&](uint64_t* b) {
+                if (elected()) tc_commit(b);
+            };
+            auto scores = [&](int m, int t) {  // S_m = Q_m K^T of the share's tile t
+                const uint32_t k = uniform(operand_lo(kb + t % ST * S::Stage, 16)), q = uniform(operand_lo(base + m * S::QTile, 16));
+                const uint32_t d = uniform(tm + m * S::SCols + (t & 1) * KT);
+                if (elected()) {
+                    auto step = [&](int x, int s) {
+                        mma_ss(d, operand_of(q + (x * PANELS + (s >> 2)) * 1024 + (s & 3) * 2),
+                               operand_of(k + (s >> 2) * (KT * 8) + (s & 3) * 2), id_s, x + s > 0);
+                    };
+                    if (steps == PANELS * 4) {
 #pragma unroll
-                for (int s = 0; s < PANELS * 4; ++s)
-                    if (s < steps)
-                        mma_ss(d, q + (uint32_t)((t * PANELS + (s >> 2)) * 1024 + (s & 3) * 2), k + (uint32_t)((s >> 2) * (KT * 8) + (s & 3) * 2),
-                               id_s, t + s > 0);
-            tc_commit(&bar->s_full[m]);
-        };
-        auto last_of = [&](int i) {  // the last query tile that has tile i
-            int r = -1;
-            for (int m = 0; m < MT; ++m)
-                if (i < nt[m]) r = m;
-            return r;
-        };
-        alive = alive && most && wait_or(&bar->k_full[0], 0, &bar->dead, a.err);
-        if (alive) {
-            tc_after();
-            for (int m = 0; m < MT; ++m)
-                if (nt[m]) scores(m, 0);
-            tc_commit(&bar->k_empty[0]);
-        }
-        for (int i = 0; alive && i < most; ++i) {
-            const int sv = i % ST, sk = (i + 1) % ST;
-            const int lk = last_of(i + 1);
-            for (int m = 0; alive && m < MT; ++m) {
-                if (i >= nt[m]) continue;
-                alive = wait_or(&bar->p_full[m], (uint32_t)(i & 1), &bar->dead, a.err) &&
-                        wait_or(&bar->v_full[sv], (uint32_t)((i / ST) & 1), &bar->dead, a.err);
-                if (!alive) break;
-                tc_after();
-                // P of key block b: hi at columns 32 b .., lo at 32 b + 16 ..
-                const uint64_t v = vd + (uint32_t)(sv * (S::Stage >> 4));
-                const uint32_t od = tmem + MT * S::SCols + m * S::OCols, pd = tmem + m * S::SCols;
+                        for (int x = 0; x < TERMS; ++x)
 #pragma unroll
-                for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-                    for (int s = 0; s < KT / 16; ++s)
-                        mma_ts(od, pd + 32 * (s >> 1) + 16 * t + 8 * (s & 1), v + (uint32_t)(s * 128), id_o, i > 0 || t + s > 0);
-                if (i + 1 == nt[m]) tc_commit(&bar->o_full[m]);
-                if (i + 1 < nt[m]) {
-                    alive = wait_or(&bar->k_full[sk], (uint32_t)(((i + 1) / ST) & 1), &bar->dead, a.err);
-                    if (!alive) break;
-                    tc_after();
-                    scores(m, i + 1);
-                    if (m == lk) tc_commit(&bar->k_empty[sk]);
+                            for (int s = 0; s < PANELS * 4; ++s) step(x, s);
+                    } else {
+#pragma unroll 1
+                        for (int x = 0; x < TERMS; ++x)
+#pragma unroll 1
+                            for (int s = 0; s < steps; ++s) step(x, s);
+                    }
+                    tc_commit(&bar->s_full[m][t & 1]);
                 }
+            };
+            auto output = [&](int m, int t) {  // O_m (+)= P_m V; P of key block b: hi at columns 32 b, lo 16 on
+                const uint32_t v = uniform(operand_lo(vb + t % ST * S::Stage, KT * 128));
+                const uint32_t p = uniform(tm + m * S::SCols + (t & 1) * KT);
+                if (elected()) {
+#pragma unroll
+                    for (int x = 0; x < TERMS; ++x)
+#pragma unroll
+                        for (int s = 0; s < KT / 16; ++s)
+                            mma_ts(tm + MT * S::SCols + m * S::OCols, p + 32 * (s >> 1) + 16 * x + 8 * (s & 1), operand_of(v + s * 128),
+                                   id_o, t > 0 || x + s > 0);
+                    tc_commit(&bar->o_done[m]);
+                    if (t + 1 == n[m]) tc_commit(&bar->o_full[m]);
+                }
+            };
+            bool alive = wait(&bar->q, 0);
+            const bool keep = a.weight && split == 0 && alive;
+            if (keep && lane == 0) {  // the weights' kernel reads the query tiles
+                unsigned char* dst = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT) * S::QTile;
+                for (int p = 0; p < MT * TERMS * PANELS; ++p)
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)p * 16384),
+                                 "r"(base + p * 16384), "r"(16384)
+                                 : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-            if (alive) tc_commit(&bar->v_empty[sv]);
-        }
-        // every product has ended before tensor memory is freed
-        tc_commit(&bar->drain);
-        volatile int never = 0;
-        wait_or(&bar->drain, 0, &never, a.err);
-        if (keep) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            auto some_scores = [&](int m, int t, bool& got) {
+                if (!alive || t >= n[m]) return;
+                alive = got || wait(&bar->k_full[t % ST], (uint32_t)(t / ST) & 1);
+                if (!alive) return;
+                got = true;
+                tc_after();
+                scores(m, t);
+                if (m == MT - 1 || t >= n[MT - 1]) commit(&bar->k_empty[t % ST]);  // the last to read the tile
+            };
+#pragma unroll 1
+            for (int t = 0; t < S::Ahead; ++t) {
+                bool got = false;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) some_scores(m, t, got);
+            }
+#pragma unroll 1
+            for (int i = 0; alive && i < all; ++i) {
+                bool got_v = false, got_k = false;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if (!alive || i >= n[m]) continue;
+                    alive = wait(&bar->p_full[m][i & 1], (uint32_t)(i >> 1) & 1) &&
+                            (got_v || wait(&bar->v_full[i % ST], (uint32_t)(i / ST) & 1));
+                    if (!alive) continue;
+                    got_v = true;
+                    tc_after();
+                    output(m, i);
+                    some_scores(m, i + S::Ahead, got_k);
+                }
+                if (alive) commit(&bar->v_empty[i % ST]);
+            }
+            // every product has ended before tensor memory is freed
+            commit(&bar->drain);
+            volatile int never = 0;
+            if (lane == 0) wait_or(&bar->drain, 0, &never, a.err);
+            if (keep && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
     }
     __syncwarp();
@@ -760,35 +801,43 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             __syncwarp();
             if (lane == 0) bar_arrive(&bar->st_full[b]);
         }
-    } else if (warp == kMmaWarp && lane == 0) {
-        const uint32_t id = instr(128, false);
-        const uint64_t kd = operand(smem_addr(ks), 16), qd = operand(smem_addr(qs), 16);
-        const int steps = hd / 16;
-        bool ok = wait_or(&bar->k_full, 0, &bar->dead, a.err);
+    } else if (warp == kMmaWarp) {
+        const uint32_t id = instr(128, false), tm = uniform(tmem), base = uniform(smem_addr(ks));
+        const int steps = hd / 16, count = uniform(n);
+        auto wait = [&](uint64_t* w, uint32_t parity) {
+            bool ok = true;
+            if (lane == 0) ok = wait_or(w, parity, &bar->dead, a.err);
+            return uniform((int)ok) != 0;
+        };
+        bool ok = wait(&bar->k_full, 0);
         int it = 0;
-        for (int i = 0; ok && i < n; ++i) {
+        for (int i = 0; ok && i < count; ++i) {
             const int b = i & 1;
-            if (i >= 2) ok = wait_or(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1, &bar->dead, a.err);
+            if (i >= 2) ok = wait(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1);
             for (int t = 0; ok && t < TERMS; ++t, ++it) {
                 const int sg = it % ST;
-                ok = wait_or(&bar->q_full[sg], (uint32_t)((it / ST) & 1), &bar->dead, a.err);
+                ok = wait(&bar->q_full[sg], (uint32_t)((it / ST) & 1));
                 if (!ok) break;
                 tc_after();
-                const uint64_t q = qd + (uint32_t)(sg * (S::Stage >> 4));
+                const uint32_t k = uniform(operand_lo(base, 16)), q = uniform(operand_lo(base + MT * S::KTile + sg * S::Stage, 16));
+                const uint32_t d = uniform(tm + b * 128);
+                const bool add = t > 0;
+                if (elected()) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int s = 0; s < PANELS * 4; ++s)
-                        if (s < steps)
-                            mma_ss(tmem + m * 256 + b * 128, kd + (uint32_t)(m * (S::KTile >> 4) + (s >> 2) * 1024 + (s & 3) * 2),
-                                   q + (uint32_t)((s >> 2) * 1024 + (s & 3) * 2), id, t + s > 0);
-                tc_commit(&bar->q_empty[sg]);
+                        for (int s = 0; s < PANELS * 4; ++s)
+                            if (s < steps)
+                                mma_ss(d + m * 256, operand_of(k + m * (S::KTile >> 4) + (s >> 2) * 1024 + (s & 3) * 2),
+                                       operand_of(q + (s >> 2) * 1024 + (s & 3) * 2), id, add || s > 0);
+                    tc_commit(&bar->q_empty[sg]);
+                }
             }
-            if (ok) tc_commit(&bar->s_full[b]);
+            if (ok && elected()) tc_commit(&bar->s_full[b]);
         }
-        tc_commit(&bar->drain);
+        if (elected()) tc_commit(&bar->drain);
         volatile int never = 0;
-        wait_or(&bar->drain, 0, &never, a.err);
+        if (lane == 0) wait_or(&bar->drain, 0, &never, a.err);
     } else if (warp == kMmaWarp + 1 && lane == 0) {
         const unsigned char* src = a.qt + ((size_t)kvh * tiles128 + first) * TERMS * S::Stage;
         const int total = n * TERMS;
@@ -833,11 +882,6 @@ int launch_shape(const AttnArgs& a, cudaStream_t st) {
     PromptKernel k = kv8_prompt_kernel<PANELS, T>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
     if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_prompt_kernel)");
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, k);
-    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncGetAttributes(kv8_prompt_kernel)");
-    // the kernel's register split waits for registers that the launch has to have
-    if (fa.numRegs < kLaunchRegs) return neon_internal::error(NEON_ERR_UNSUPPORTED, "kv8_prompt_kernel: built with too few registers");
     const int units = (rows + 128 * S::MT - 1) / (128 * S::MT);
     return launch("kv8_prompt_kernel", k, dim3((unsigned)(units * H * a.nsplit)), kThreads, S::Smem, st, 1, a, tiles);
 }
@@ -845,7 +889,7 @@ int launch_shape(const AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int prompt_unit(int hd) { return hd <= 128 ? 256 : 128; }
-int prompt_tile_keys(int hd) { return hd <= 128 ? 128 : 64; }
+int prompt_tile_keys() { return kTileKeys; }
 
 size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type) {
     const size_t tiles = (rows + 255) / 256 * 2, panels = (c.head_dim + 63) / 64;
