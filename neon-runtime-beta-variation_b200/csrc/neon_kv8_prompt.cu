@@ -32,8 +32,8 @@
 namespace longctx {
 namespace {
 
-// Warps 0-7 softmax, 12 the products, 8-11 and 13-15 conversion.
-constexpr int kSoftWarps = 8, kMmaWarp = 12, kConvWarps = 7;
+// Warps 0-7 softmax, 8-13 conversion, 14 and 15 the products, one per query tile.
+constexpr int kSoftWarps = 8, kConvWarps = 6, kMmaWarp = 14;
 constexpr int kThreads = 512;
 constexpr int kTileKeys = 64;
 constexpr float kLazy = 8.f;     // log2 of how far p may exceed 1
@@ -257,7 +257,7 @@ struct Shape {
 };
 
 struct Bars {
-    uint64_t q, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drain;
+    uint64_t q, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drain[2];
     uint32_t tmem;
     int dead;
 };
@@ -281,9 +281,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             bar_init(&bar->q, 4 * MT);
             for (int i = 0; i < 4; ++i) {
                 bar_init(&bar->k_full[i], kConvWarps);
-                bar_init(&bar->k_empty[i], 1);
+                bar_init(&bar->k_empty[i], MT);
                 bar_init(&bar->v_full[i], kConvWarps);
-                bar_init(&bar->v_empty[i], 1);
+                bar_init(&bar->v_empty[i], MT);
                 bar_init(&bar->s_full[i >> 1][i & 1], 1);
                 bar_init(&bar->p_full[i >> 1][i & 1], 4);
             }
@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 bar_init(&bar->o_done[i], 1);
                 bar_init(&bar->o_full[i], 1);
             }
-            bar_init(&bar->drain, 1);
+            bar_init(&bar->drain[0], 1);
+            bar_init(&bar->drain[1], 1);
             bar->dead = 0;
             bar_init_fence();
         }
@@ -500,10 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             tc_before();
         }
     } else {
-        if (warp != kMmaWarp) {
+        if (warp < kMmaWarp) {
         // ---- conversion: codes to fp16, swizzled ----
         constexpr int kConv = kConvWarps * 32;
-        const int ct = tid - kSoftWarps * 32 - (warp > kMmaWarp ? 32 : 0);
+        const int ct = tid - kSoftWarps * 32;
         const int pieces = hd / 16;                 // 16-byte pieces of a row
         const int total = KT * pieces;
         constexpr int L = (KT * PANELS * 4 + kConv - 1) / kConv;  // pieces per thread at most
@@ -548,30 +549,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (lane == 0) bar_arrive(&bar->v_full[s]);
             if (i + 1 < most) load(vr, vc, j0 + i + 1);
         }
-        } else if (most || (a.weight && split == 0)) {
-            // ---- products: the whole warp goes along, one elected lane issues. Descriptors come from one
-            // shuffled word each, so they stay in uniform registers: an issue then takes less than the 64
-            // clocks of its product ----
+        } else if (warp - kMmaWarp < MT && (most || (a.weight && split == 0))) {
+            // ---- products: a warp per query tile (a poll takes some 200 clocks while products read shared
+            // memory; the other tile's products run meanwhile). The whole warp goes along and one elected lane
+            // issues; descriptors come from one shuffled word each, so they stay in uniform registers ----
             const uint32_t id_s = instr(KT, false), id_o = instr(hd, true);
-            const int steps = hd / 16;
-            const uint32_t base = uniform(smem_addr(qs));
+            const int steps = hd / 16, m = uniform(warp - kMmaWarp);
+            const uint32_t base = uniform(smem_addr(qs)), qb = base + m * S::QTile;
             const uint32_t kb = base + MT * S::QTile, vb = kb + ST * S::Stage;
-            int n[MT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) n[m] = uniform(nt[m]);
-            const int all = uniform(most);
-            const uint32_t tm = uniform(tmem);
+            const int n = uniform(m == 0 ? nt[0] : nt[MT - 1]), all = uniform(most);
+            const uint32_t tm = uniform(tmem), ts = tm + m * S::SCols, to = tm + MT * S::SCols + m * S::OCols;
             auto wait = [&](uint64_t* b, uint32_t parity) {
                 bool ok = true;
                 if (lane == 0) ok = wait_or(b, parity, &bar->dead, a.err);
                 return uniform((int)ok) != 0;
             };
-            auto commit = [&](uint64_t* b) {
-                if (elected()) tc_commit(b);
-            };
-            auto scores = [&](int m, int t) {  // S_m = Q_m K^T of the share's tile t
-                const uint32_t k = uniform(operand_lo(kb + t % ST * S::Stage, 16)), q = uniform(operand_lo(base + m * S::QTile, 16));
-                const uint32_t d = uniform(tm + m * S::SCols + (t & 1) * KT);
+            auto wait_k = [&](int t) { return wait(&bar->k_full[t % ST], (uint32_t)(t / ST) & 1); };
+            auto scores = [&](int t) {  // S = Q K^T of the share's tile t
+                const uint32_t k = uniform(operand_lo(kb + t % ST * S::Stage, 16)), q = uniform(operand_lo(qb, 16));
+                const uint32_t d = uniform(ts + (t & 1) * KT);
                 if (elected()) {
                     auto step = [&](int x, int s) {
                         mma_ss(d, operand_of(q + (x * PANELS + (s >> 2)) * 1024 + (s & 3) * 2),
@@ -589,67 +585,62 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                             for (int s = 0; s < steps; ++s) step(x, s);
                     }
                     tc_commit(&bar->s_full[m][t & 1]);
+                    tc_commit(&bar->k_empty[t % ST]);
                 }
             };
-            auto output = [&](int m, int t) {  // O_m (+)= P_m V; P of key block b: hi at columns 32 b, lo 16 on
+            auto output = [&](int t) {  // O (+)= P V; P of key block b: hi at columns 32 b, lo 16 on
                 const uint32_t v = uniform(operand_lo(vb + t % ST * S::Stage, KT * 128));
-                const uint32_t p = uniform(tm + m * S::SCols + (t & 1) * KT);
+                const uint32_t p = uniform(ts + (t & 1) * KT);
                 if (elected()) {
 #pragma unroll
                     for (int x = 0; x < TERMS; ++x)
 #pragma unroll
                         for (int s = 0; s < KT / 16; ++s)
-                            mma_ts(tm + MT * S::SCols + m * S::OCols, p + 32 * (s >> 1) + 16 * x + 8 * (s & 1), operand_of(v + s * 128),
-                                   id_o, t > 0 || x + s > 0);
+                            mma_ts(to, p + 32 * (s >> 1) + 16 * x + 8 * (s & 1), operand_of(v + s * 128), id_o, t > 0 || x + s > 0);
                     tc_commit(&bar->o_done[m]);
-                    if (t + 1 == n[m]) tc_commit(&bar->o_full[m]);
+                    tc_commit(&bar->v_empty[t % ST]);
+                    if (t + 1 == n) tc_commit(&bar->o_full[m]);
                 }
             };
             bool alive = wait(&bar->q, 0);
             const bool keep = a.weight && split == 0 && alive;
             if (keep && lane == 0) {  // the weights' kernel reads the query tiles
-                unsigned char* dst = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT) * S::QTile;
-                for (int p = 0; p < MT * TERMS * PANELS; ++p)
+                unsigned char* dst = a.qt + ((size_t)kvh * tiles128 + (size_t)unit * MT + m) * S::QTile;
+                for (int p = 0; p < TERMS * PANELS; ++p)
                     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)p * 16384),
-                                 "r"(base + p * 16384), "r"(16384)
+                                 "r"(qb + p * 16384), "r"(16384)
                                  : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-            auto some_scores = [&](int m, int t, bool& got) {
-                if (!alive || t >= n[m]) return;
-                alive = got || wait(&bar->k_full[t % ST], (uint32_t)(t / ST) & 1);
-                if (!alive) return;
-                got = true;
+#pragma unroll 1
+            for (int t = 0; t < S::Ahead && t < n && alive; ++t) {
+                alive = wait_k(t);
                 tc_after();
-                scores(m, t);
-                if (m == MT - 1 || t >= n[MT - 1]) commit(&bar->k_empty[t % ST]);  // the last to read the tile
-            };
-#pragma unroll 1
-            for (int t = 0; t < S::Ahead; ++t) {
-                bool got = false;
-#pragma unroll
-                for (int m = 0; m < MT; ++m) some_scores(m, t, got);
+                if (alive) scores(t);
             }
 #pragma unroll 1
-            for (int i = 0; alive && i < all; ++i) {
-                bool got_v = false, got_k = false;
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    if (!alive || i >= n[m]) continue;
-                    alive = wait(&bar->p_full[m][i & 1], (uint32_t)(i >> 1) & 1) &&
-                            (got_v || wait(&bar->v_full[i % ST], (uint32_t)(i / ST) & 1));
-                    if (!alive) continue;
-                    got_v = true;
-                    tc_after();
-                    output(m, i);
-                    some_scores(m, i + S::Ahead, got_k);
+            for (int i = 0; alive && i < n; ++i) {
+                // K of a later tile has come after V of this one
+                const int t = i + S::Ahead;
+                alive = (t < n ? wait_k(t) : wait(&bar->v_full[i % ST], (uint32_t)(i / ST) & 1)) &&
+                        wait(&bar->p_full[m][i & 1], (uint32_t)(i >> 1) & 1);
+                if (!alive) break;
+                tc_after();
+                output(i);
+                if (t < n) scores(t);
+            }
+            // tiles that this query tile does not need: passed on
+            if (alive && lane == 0)
+                for (int t = n; t < all; ++t) {
+                    alive = wait_or(&bar->v_full[t % ST], (uint32_t)(t / ST) & 1, &bar->dead, a.err);
+                    if (!alive) break;
+                    bar_arrive(&bar->k_empty[t % ST]);
+                    bar_arrive(&bar->v_empty[t % ST]);
                 }
-                if (alive) commit(&bar->v_empty[i % ST]);
-            }
             // every product has ended before tensor memory is freed
-            commit(&bar->drain);
+            if (elected()) tc_commit(&bar->drain[m]);
             volatile int never = 0;
-            if (lane == 0) wait_or(&bar->drain, 0, &never, a.err);
+            if (lane == 0) wait_or(&bar->drain[m], 0, &never, a.err);
             if (keep && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
     }
@@ -679,7 +670,7 @@ struct WShape {
     static_assert(Smem <= 232448, "shared memory");
 };
 // warps 0-7 sum, 8-11 convert the keys and fill in the rows' numbers, 12 the products, 13 loads
-constexpr int kWThreads = 448, kWConvWarps = 4;
+constexpr int kWThreads = 448, kWConvWarps = 4, kWMmaWarp = 12;
 
 struct WBars {
     uint64_t k_full, q_full[4], q_empty[4], s_full[2], s_empty[2], st_full[2], drain;
@@ -704,7 +695,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
     float2* stat = reinterpret_cast<float2*>(qs + ST * S::Stage);  // [2][128]: factor, m + log2 l
     WBars* bar = reinterpret_cast<WBars*>(stat + 256);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (warp == kMmaWarp) {
+    if (warp == kWMmaWarp) {
         if (lane == 0) {
             bar_init(&bar->k_full, kWConvWarps);
             for (int i = 0; i < ST; ++i) {
@@ -776,7 +767,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             float* w = a.weight + (size_t)kvh * cap + key;
             *w = key < past ? *w + v : v;
         }
-    } else if (warp >= kSoftWarps && warp < kMmaWarp) {
+    } else if (warp >= kSoftWarps && warp < kWMmaWarp) {
         const int ct = tid - kSoftWarps * 32, pieces = hd / 16;
         const uint4* kc = reinterpret_cast<const uint4*>(a.c.k + ((size_t)kvh * cap + key0) * hd);
         const int held = min(MT * 128, cap - key0) * pieces;
@@ -801,7 +792,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             __syncwarp();
             if (lane == 0) bar_arrive(&bar->st_full[b]);
         }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == kWMmaWarp) {
         const uint32_t id = instr(128, false), tm = uniform(tmem), base = uniform(smem_addr(ks));
         const int steps = hd / 16, count = uniform(n);
         auto wait = [&](uint64_t* w, uint32_t parity) {
@@ -838,7 +829,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
         if (elected()) tc_commit(&bar->drain);
         volatile int never = 0;
         if (lane == 0) wait_or(&bar->drain, 0, &never, a.err);
-    } else if (warp == kMmaWarp + 1 && lane == 0) {
+    } else if (warp == kWMmaWarp + 1 && lane == 0) {
         const unsigned char* src = a.qt + ((size_t)kvh * tiles128 + first) * TERMS * S::Stage;
         const int total = n * TERMS;
         int it = 0;
@@ -855,7 +846,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
     __syncwarp();
     tc_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kWMmaWarp) {
         tc_after();
         tmem_free(tmem, 256 * MT);
     }
