@@ -19,9 +19,9 @@
 // products. What bounds it: exp2 (16 a clock and SM) for types of 16 bits, the
 // products (twice as many) for fp32.
 //
-// The maximum is lazy: O is only rescaled when a row's maximum has grown by
-// more than 2^8 since its m was set (the result does not depend on m), so p is
-// at most 2^8; with V's scale relative to a reference that is kept within a
+// The maximum is lazy: m only moves, and O is only rescaled, when a row's p
+// would sum to more than 2^8 in a tile (the result does not depend on m), so p
+// is at most 2^8; with V's scale relative to a reference that is kept within a
 // factor of 4 (vr), and 2^5, p times those stays below fp16's 65504, and its
 // lo term has bits down to 2^-30 of a row's largest.
 #include "neon_kv8_attn.cuh"
@@ -36,7 +36,7 @@ namespace {
 constexpr int kSoftWarps = 8, kConvWarps = 6, kMmaWarp = 14;
 constexpr int kThreads = 512;
 constexpr int kTileKeys = 64;
-constexpr float kLazy = 8.f;     // log2 of how far p may exceed 1
+constexpr float kMostP = 256.f;  // 2^8: how far p may exceed 1
 constexpr float kPScale = 32.f;  // 2^5
 
 // ---- tcgen05 ----
@@ -349,101 +349,133 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             };
             const int n = m == 0 ? nt[0] : nt[MT - 1];
             if (n) scales(j0);
-            // A tile's P from its S; FULL: no key of the tile is hidden from a row of the warp.
+            // m, and the reference of V's scales, move to what tile i needs: its largest score, and its largest
+            // scale if that is above four times the reference; O and l follow.
+            auto move = [&](int i, const float (&kf)[NB], float vmax) {
+                const int seen = limit - (j0 + i) * KT;
+                float mt = -INFINITY;
+#pragma unroll 1
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t r[32];
+                    tmem_ld32(r, st + (i & 1) * KT + 32 * b);
+                    tmem_wait_ld();
+                    const int c = seen - 32 * b;
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (e < c) x = fmaxf(x, __uint_as_float(r[e]));
+                    if (c > 0) mt = fmaxf(mt, x * (b ? kf[NB - 1] : kf[0]));
+                }
+                const float mnew = fmaxf(mt, mref), vtop = vmax > 4.f * vref ? vmax : vref;
+                const float fl = mref == -INFINITY ? 0.f : ex2(mref - mnew);
+                const float f = vtop > 0.f ? fl * (vref / vtop) : fl;
+                // O once the tile before has been added: of the outputs, i - 1 or i have ended here (the scores of
+                // tile i come after output i - 2, output i needs this tile's P), so the parity is clear
+                if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                    alive = __all_sync(0xffffffffu, wait_or(&bar->o_done[m], (uint32_t)(i - 1) & 1, &bar->dead, a.err));
+                    tc_after();
+#pragma unroll 1
+                    for (int c = 0; c < hd; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o, ot + c);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st16(ot + c, o);
+                    }
+                }
+                l *= fl;
+                mref = mnew;
+                vref = vtop;
+            };
+            // A tile's P from its S; FULL: no key of the tile is hidden from a row of the warp. The maximum is not
+            // taken: p at most 2^8 is all that P needs, and a sum of the row's p at most 2^8 says so. A row whose
+            // sum is above (its m is behind), or without an m yet, moves it and the warp takes the tile again.
+            // Shared memory is slow while products read it (a poll or a shuffle takes some 200 clocks), so what does
+            // not need S is done before the wait, and the next S is looked for in mid-tile.
+            float kf[NB], vr[NB], vmax = 0.f;
+            bool ready = false;
             auto tile = [&](auto whole, int i) {
                 constexpr bool FULL = decltype(whole)::value;
                 const int seen = limit - (j0 + i) * KT;
                 const uint32_t sb = st + (i & 1) * KT;
-                float kf[NB], vb[NB];
-                uint32_t r[NB][32];
+                constexpr int AT = TERMS == 1 ? NB : 1;  // blocks read at once, as registers allow
+                uint32_t hi[NB][16], lo[NB][16];
+                float add;
+                for (;;) {
+                    const float mu = mref == -INFINITY ? 0.f : mref;
+                    const uint64_t mu2 = pair(-mu, -mu);
+                    uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                    uint32_t r[AT][32];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) tmem_ld32(r[b], sb + 32 * b);
+                    for (int b = 0; b < NB; ++b) {
+                        if (b % AT == 0) {
+#pragma unroll
+                            for (int k = 0; k < AT; ++k) tmem_ld32(r[k], sb + 32 * (b + k));
+                            tmem_wait_ld();
+                        }
+                        if (b == NB - 1 && !ready && i + 1 < n) ready = bar_test(&bar->s_full[m][(i + 1) & 1], (uint32_t)((i + 1) >> 1) & 1);
+                        const uint64_t kf2 = pair(kf[b], kf[b]), vr2 = pair(vr[b], vr[b]);
+                        const int c = seen - 32 * b;
+                        const uint32_t(&x)[32] = r[b % AT];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float p0, p1, w0, w1;
+                            unpair(fma2(pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), kf2, mu2), p0, p1);
+                            p0 = ex2(p0);
+                            p1 = ex2(p1);
+                            if (!FULL) {
+                                if (2 * e >= c) p0 = 0.f;
+                                if (2 * e + 1 >= c) p1 = 0.f;
+                            }
+                            const uint64_t p = pair(p0, p1);
+                            sum[e & 1] = add2(sum[e & 1], p);
+                            unpair(mul2(p, vr2), w0, w1);
+                            if (!FULL) {  // (a scale that is not finite may lie behind a row's keys)
+                                if (2 * e >= c) w0 = 0.f;
+                                if (2 * e + 1 >= c) w1 = 0.f;
+                            }
+                            if (TERMS == 2) split2(w0, w1, hi[b][e], lo[b][e]);
+                            else hi[b][e] = h2_bits(__floats2half2_rn(w0, w1));
+                        }
+                    }
+                    float s0, s1;
+                    unpair(add2(sum[0], sum[1]), s0, s1);
+                    add = s0 + s1;
+                    const float before = mref;
+                    if (!__any_sync(0xffffffffu, add > kMostP)) break;
+                    move(i, kf, vmax);
+                    // (a score that is infinite leaves m where it is: its row is not a number)
+                    if (!__any_sync(0xffffffffu, mref != before)) break;
+                }
+                l += add;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {  // over the block's scores: hi in its first 16 columns, lo in the next
+                    tmem_st16(sb + 32 * b, hi[b]);
+                    if (TERMS == 2) tmem_st16(sb + 32 * b + 16, lo[b]);
+                }
+            };
+            for (int i = 0; i < n && alive; ++i) {
+                const int seen = limit - (j0 + i) * KT;
+                float vb[NB];
+                vmax = 0.f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     kf[b] = factor * __shfl_sync(0xffffffffu, nk, b);
                     vb[b] = __shfl_sync(0xffffffffu, nv, b);
+                    if (seen > 32 * b) vmax = fmaxf(vmax, vb[b]);
                 }
                 if (i + 1 < n) scales(j0 + i + 1);
-                tmem_wait_ld();
-                float mt = -INFINITY, vmax = 0.f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const int c = seen - 32 * b;
-                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (FULL || e < c) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(r[b][e]));
-                    if (FULL || c > 0) {
-                        mt = fmaxf(mt, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * kf[b]);
-                        vmax = fmaxf(vmax, vb[b]);
-                    }
+                const bool moves = __any_sync(0xffffffffu, (mref == -INFINITY && seen > 0) || vmax > 4.f * vref);
+                if (!__all_sync(0xffffffffu, ready)) {
+                    alive = __all_sync(0xffffffffu, wait_or(&bar->s_full[m][i & 1], (uint32_t)(i >> 1) & 1, &bar->dead, a.err));
+                    if (!alive) break;
                 }
-                // O and l follow m and the reference of V's scales when those move
-                const float vtop = vmax > 4.f * vref ? vmax : vref;
-                const float mnew = mt > mref + kLazy || mref == -INFINITY ? fmaxf(mt, mref) : mref;
-                if (__any_sync(0xffffffffu, mnew != mref || vtop != vref)) {
-                    const float fl = mref == -INFINITY ? 0.f : ex2(mref - mnew);
-                    const float f = vtop > 0.f ? fl * (vref / vtop) : fl;
-                    // once the tile before has been added: of the outputs, i - 1 or i have ended here (the scores
-                    // of tile i come after output i - 2, output i needs this tile's P), so the parity is clear
-                    if (i > 0) {
-                        alive = __all_sync(0xffffffffu, wait_or(&bar->o_done[m], (uint32_t)(i - 1) & 1, &bar->dead, a.err));
-                        tc_after();
-#pragma unroll 1
-                        for (int c = 0; c < hd; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o, ot + c);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st16(ot + c, o);
-                        }
-                    }
-                    l *= fl;
-                    mref = mnew;
-                    vref = vtop;
-                }
-                const float mu = mref == -INFINITY ? 0.f : mref;
-                const uint64_t mu2 = pair(-mu, -mu);
-                uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    uint32_t hi[16], lo[16];
-                    const float vr = vb[b] == 0.f ? 0.f : __fdividef(vb[b], vref) * kPScale;
-                    const uint64_t kf2 = pair(kf[b], kf[b]), vr2 = pair(vr, vr);
-                    const int c = seen - 32 * b;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float p0, p1, w0, w1;
-                        unpair(fma2(pair(__uint_as_float(r[b][2 * e]), __uint_as_float(r[b][2 * e + 1])), kf2, mu2), p0, p1);
-                        p0 = ex2(p0);
-                        p1 = ex2(p1);
-                        if (!FULL) {
-                            if (2 * e >= c) p0 = 0.f;
-                            if (2 * e + 1 >= c) p1 = 0.f;
-                        }
-                        const uint64_t p = pair(p0, p1);
-                        sum[e & 1] = add2(sum[e & 1], p);
-                        unpair(mul2(p, vr2), w0, w1);
-                        if (!FULL) {  // (a scale that is not finite may lie behind a row's keys)
-                            if (2 * e >= c) w0 = 0.f;
-                            if (2 * e + 1 >= c) w1 = 0.f;
-                        }
-                        if (TERMS == 2) split2(w0, w1, hi[e], lo[e]);
-                        else hi[e] = h2_bits(__floats2half2_rn(w0, w1));
-                    }
-                    // over the block's scores: hi in its first 16 columns, lo in the next
-                    tmem_st16(sb + 32 * b, hi);
-                    if (TERMS == 2) tmem_st16(sb + 32 * b + 16, lo);
-                }
-                float s0, s1;
-                unpair(add2(sum[0], sum[1]), s0, s1);
-                l += s0 + s1;
-            };
-            for (int i = 0; i < n && alive; ++i) {
-                alive = __all_sync(0xffffffffu, wait_or(&bar->s_full[m][i & 1], (uint32_t)(i >> 1) & 1, &bar->dead, a.err));
-                if (!alive) break;
+                ready = false;
                 tc_after();
+                if (moves) move(i, kf, vmax);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) vr[b] = vb[b] == 0.f ? 0.f : __fdividef(vb[b], vref) * kPScale;
                 if ((j0 + i + 1) * KT <= all) tile(std::true_type{}, i);
                 else tile(std::false_type{}, i);
                 tmem_wait_st();

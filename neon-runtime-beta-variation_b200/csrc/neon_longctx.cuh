@@ -85,6 +85,15 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
                  : "memory");
     return done != 0;
 }
+// Whether a phase has completed, without waiting.
+__device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(done)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
 // Waits for a phase; gives up after about 2 s, notes it in *err and returns false.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, unsigned* err) {
     if (bar_try(bar, parity)) return true;
