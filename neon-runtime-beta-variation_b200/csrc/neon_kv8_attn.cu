@@ -33,38 +33,78 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // the eight rows' hi terms and below them their lo terms, so the split costs
 // no extra products: a row's score is the sum of its two halves, and its
 // output likewise. Each warp streams its own tiles of 32 rows (a block of the
-// cache: K and V codes as two bulk copies) through its own ring in shared
+// cache: K's codes, then V's, a bulk copy each) through its own ring in shared
 // memory, with no barrier between the warps until their results are merged.
 // The order of the summed dimension is free, so each lane reads whole 16-byte
-// pieces of a K row and the query fragments are laid out to match; of V, lane
-// group g takes columns [g HD / 8, (g + 1) HD / 8) of four rows.
+// pieces of a K row and the query fragments (in shared memory, the same for
+// all warps) are laid out to match; of V, lane group g takes columns [g HD / 8,
+// (g + 1) HD / 8) of four rows. HBM bounds it at length; the arithmetic (some
+// 800 instructions a warp for 8 KB of codes) needs 16 warps per SM to hide its
+// latencies: with 8, and the query fragments in registers, 131071 rows of 8
+// heads x 128 took 68 us (3.9 TB/s).
 // ---------------------------------------------------------------------------
-constexpr int kRowWarps = 8;
-constexpr int kRowThreads = kRowWarps * 32;
-
 template <int HD>
 struct RowTile {
-    static constexpr int kStages = HD <= 64 ? 4 : HD <= 128 ? 3 : 1;
-    static constexpr int kStageBytes = 2 * 32 * HD;
-    static constexpr int kRingBytes = kRowWarps * kStages * kStageBytes;
-    static constexpr int kMergeBytes = kRowWarps * 8 * (HD + 2) * 4;
-    static constexpr int kSmem = (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes) + 128 + kRowWarps * kStages * 8;
+    static constexpr int kWarps = HD <= 128 ? 16 : 8;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kSlots = HD <= 64 ? 6 : 3;
+    static constexpr int kSlotBytes = 32 * HD;
+    static constexpr int kRing = kWarps * kSlots * kSlotBytes;
+    static constexpr int kMerge = kWarps * 8 * (HD + 2) * 4;
+    static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
+    static constexpr int kQuery = HD / 16 * 512;
+    static constexpr int kSmem = kBody + kQuery + 8 * 4 + kWarps * kSlots * 8;
+    static_assert(kSmem <= 232448, "shared memory");
 };
 
+// The query fragments of rows 8 grp .. of a KV head: lane (g, tq) holds values tq HD / 4 + 4 s .. + 3 of row g for
+// step s, times 2^e so that the row's largest is near 2^7 (its lo terms then stay normal halves). One warp; the
+// row's factor scale log2(e) 2^-e is returned to its four lanes.
 template <int HD>
-__global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_constant__ AttnArgs a) {
+__device__ __forceinline__ float row_queries(const AttnArgs& a, int kvh, int grp, uint4* out) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3, hd = (int)a.c.head_dim, rows = a.n * a.group;
+    const int row = grp * 8 + g;
+    const long long base = (long long)(row / a.group) * a.qs + (long long)(kvh * a.group + row % a.group) * hd;
+    float x[HD / 4];
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) {
+        const int d = tq * (HD / 4) + i;
+        x[i] = row < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
+        mx = fmaxf(mx, fabsf(x[i]));
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const unsigned top = __float_as_uint(mx) >> 23;
+    const int e = top >= 255u ? 0 : min(120, 134 - (int)top);
+    const float f = pow2(e);
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) {
+        uint4 q;
+        split2(x[4 * s] * f, x[4 * s + 1] * f, q.x, q.y);
+        split2(x[4 * s + 2] * f, x[4 * s + 3] * f, q.z, q.w);
+        out[s * 32 + lane] = q;
+    }
+    return a.scale * pow2(-e);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(const __grid_constant__ AttnArgs a) {
     using R = RowTile<HD>;
     constexpr int KS = HD / 16;   // k-steps of the score product
     constexpr int NT = HD / 8;    // column tiles of the output
+    constexpr int W = R::kWarps, S = R::kSlots;
     extern __shared__ __align__(128) unsigned char smem[];
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (R::kRingBytes > R::kMergeBytes ? R::kRingBytes : R::kMergeBytes));
+    uint4* qf = reinterpret_cast<uint4*>(smem + R::kBody);
+    float* qfac = reinterpret_cast<float*>(smem + R::kBody + R::kQuery);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qfac + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
     const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity;
     const int split = blockIdx.x, kvh = blockIdx.y, grp = blockIdx.z, rows = a.n * a.group;
-    unsigned char* ring = smem + warp * R::kStages * R::kStageBytes;
-    uint64_t* bar = bars + warp * R::kStages;
+    unsigned char* ring = smem + warp * S * R::kSlotBytes;
+    uint64_t* bar = bars + warp * S;
     if (lane == 0) {
-        for (int s = 0; s < R::kStages; ++s) bar_init(&bar[s], 1);
+        for (int s = 0; s < S; ++s) bar_init(&bar[s], 1);
         bar_init_fence();
     }
     __syncwarp();
@@ -73,12 +113,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
 
     // the keys of the group's rows, and this warp's share of them in tiles
     const int past = *a.c.past;
-    const int row = grp * 8 + g, tok = row / a.group;
-    const int limit = row < rows ? keys_of(past, tok, cap) : 0;
+    const int row = grp * 8 + g;
+    const int limit = row < rows ? keys_of(past, row / a.group, cap) : 0;
     const Shares sh = shares_of(a, past, grp);
     if (split >= sh.active) return;
     const int c0 = split * sh.per, c1 = min(c0 + sh.per, sh.tiles);
-    const int per_warp = (c1 - c0 + kRowWarps - 1) / kRowWarps;
+    const int per_warp = (c1 - c0 + W - 1) / W;
     const int w0 = min(c0 + warp * per_warp, c1), w1 = min(w0 + per_warp, c1);
 
     const int8_t* kc = a.c.k + (size_t)kvh * cap * hd;
@@ -86,40 +126,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
     const float* ksc = a.c.k_scale + (size_t)kvh * (cap >> 5);
     const float* vsc = a.c.v_scale + (size_t)kvh * (cap >> 5);
     const uint32_t bytes = 32u * hd;
-    auto issue = [&](int tile) {
-        const int s = (tile - w0) % R::kStages;
-        unsigned char* d = ring + s * R::kStageBytes;
-        bar_expect(&bar[s], 2 * bytes);
-        bulk_load(d, kc + (size_t)tile * bytes, bytes, &bar[s]);
-        bulk_load(d + 32 * HD, vc + (size_t)tile * bytes, bytes, &bar[s]);
+    const int items = 2 * (w1 - w0);  // K of a tile, then its V
+    auto issue = [&](int it, int slot) {
+        bar_expect(&bar[slot], bytes);
+        bulk_load(ring + slot * R::kSlotBytes, (it & 1 ? vc : kc) + (size_t)(w0 + (it >> 1)) * bytes, bytes, &bar[slot]);
     };
     if (lane == 0)
-        for (int t = w0; t < min(w0 + R::kStages, w1); ++t) issue(t);
-
-    // Query fragments: lane (g, tq) holds values tq HD / 4 + 4 s .. + 3 of row g for step s, times
-    // 2^-e so that the row's largest is near 2^7 (its lo terms then stay normal halves).
-    uint32_t qf[KS][4];
-    float factor;
-    {
-        float x[HD / 4];
-        float mx = 0.f;
-        const long long base = (long long)tok * a.qs + (long long)(kvh * a.group + row % a.group) * hd;
-#pragma unroll
-        for (int i = 0; i < HD / 4; ++i) {
-            const int d = tq * (HD / 4) + i;
-            x[i] = row < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
-            mx = fmaxf(mx, fabsf(x[i]));
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = mx > 0.f && !isinf(mx) ? 7 - ilogbf(mx) : 0;
-        factor = ldexpf(a.scale, -e);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            split2(ldexpf(x[4 * s], e), ldexpf(x[4 * s + 1], e), qf[s][0], qf[s][1]);
-            split2(ldexpf(x[4 * s + 2], e), ldexpf(x[4 * s + 3], e), qf[s][2], qf[s][3]);
-        }
+        for (int it = 0; it < min(S, items); ++it) issue(it, it);
+    if (warp == 0) {
+        const float f = row_queries<HD>(a, kvh, grp, qf);
+        if (tq == 0) qfac[g] = f;
     }
+    __syncthreads();
+    const float factor = qfac[g];
+    float* scores = a.scores ? a.scores + (((size_t)kvh * gridDim.z + grp) * 8 + g) * cap : nullptr;
 
     float acc[NT][4];
 #pragma unroll
@@ -129,36 +149,59 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
     float m = -INFINITY, l = 0.f, vref = 0.f;
     float my_ks = 0.f, my_vs = 0.f;  // the scales of 32 tiles, one per lane
     bool ok = true;
+    int slot = 0;
+    uint32_t phase = 0;
+    auto take = [&]() {  // waits for the next item
+        ok = __all_sync(0xffffffffu, bar_wait(&bar[slot], phase, a.err));
+        return ring + slot * R::kSlotBytes;
+    };
+    auto give = [&](int it) {  // its slot goes to the item S further on
+        __syncwarp();
+        if (lane == 0 && it + S < items) issue(it + S, slot);
+        if (++slot == S) {
+            slot = 0;
+            phase ^= 1;
+        }
+    };
+    int it = 0;
     for (int tile = w0; tile < w1; ++tile) {
-        const int it = tile - w0, s = it % R::kStages;
-        if ((it & 31) == 0) {
+        const int at = (tile - w0) & 31;
+        if (at == 0) {
             const int b = tile + lane;
             my_ks = b < w1 ? ksc[b] : 0.f;
             my_vs = b < w1 ? vsc[b] : 0.f;
         }
-        const float ks = __shfl_sync(0xffffffffu, my_ks, it & 31), vs = __shfl_sync(0xffffffffu, my_vs, it & 31);
-        ok = ok && bar_wait(&bar[s], (uint32_t)((it / R::kStages) & 1), a.err);
-        ok = __all_sync(0xffffffffu, ok);
+        const float ks = __shfl_sync(0xffffffffu, my_ks, at), vs = __shfl_sync(0xffffffffu, my_vs, at);
+        const unsigned char* kt = take();
         if (!ok) break;
-        const unsigned char* kt = ring + s * R::kStageBytes;
-        const unsigned char* vt = kt + 32 * HD;
 
         // scores of 32 keys: key 8 j + g of column tile j
         float sc[4][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
-            const unsigned char* kr = kt + (8 * j + g) * hd + tq * (HD / 4);
 #pragma unroll
-            for (int p = 0; p < HD / 64; ++p) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (tq * (HD / 4) + 16 * p < hd) w = *reinterpret_cast<const uint4*>(kr + 16 * p);
-                const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+        for (int p = 0; p < HD / 64; ++p) {
+            uint4 w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mma16816(sc[j], qf[4 * p + i], codes_lo(u[i]), codes_hi(u[i]));
+            for (int j = 0; j < 4; ++j) {
+                w[j] = make_uint4(0, 0, 0, 0);
+                if (tq * (HD / 4) + 16 * p < hd)
+                    w[j] = *reinterpret_cast<const uint4*>(kt + (8 * j + g) * hd + tq * (HD / 4) + 16 * p);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 qv = qf[(4 * p + i) * 32 + lane];
+                const uint32_t q[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t u = (i == 0 ? w[j].x : i == 1 ? w[j].y : i == 2 ? w[j].z : w[j].w) ^ 0x80808080u;
+                    mma16816(sc[j], q, codes_lo(u), codes_hi(u));
+                }
             }
         }
+        give(it++);
         // online softmax of row g: the lane has keys 8 j + 2 tq and + 1
         const float kf = factor * ks;
         float t[4][2], mt = m;
@@ -170,6 +213,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
                 t[j][e] = key < limit ? (sc[j][e] + sc[j][e + 2]) * kf : -INFINITY;
                 mt = fmaxf(mt, t[j][e]);
             }
+        if (scores && row < rows)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float2*>(scores + tile * 32 + 8 * j + 2 * tq) = make_float2(t[j][0], t[j][1]);
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
         const float mu = mt == -INFINITY ? 0.f : mt;
@@ -201,23 +248,25 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
                 split2(on0 ? p0 * vr : 0.f, on1 ? p1 * vr : 0.f, pf[k][2 * hf], pf[k][2 * hf + 1]);
             }
         }
+        const unsigned char* vt = take();
+        if (!ok) break;
         // o += p V: lane (g, tq) reads columns g HD / 8 .. of rows 16 k + 2 tq, + 1, + 8, + 9
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const unsigned char* vrow = vt + (16 * k + 2 * tq) * hd + g * (HD / 8);
-            constexpr int W = HD / 32;  // words of a lane's columns
-            uint32_t w[4][W];
+            constexpr int WD = HD / 32;  // words of a lane's columns
+            uint32_t w[4][WD];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const unsigned char* src = vrow + ((r & 1) + 8 * (r >> 1)) * hd;
-                if constexpr (W == 2) {
+                if constexpr (WD == 2) {
                     uint2 v = make_uint2(0, 0);
                     if (g * 8 < hd) v = *reinterpret_cast<const uint2*>(src);
                     w[r][0] = v.x ^ 0x80808080u;
                     w[r][1] = v.y ^ 0x80808080u;
                 } else {
 #pragma unroll
-                    for (int p = 0; p < W / 4; ++p) {
+                    for (int p = 0; p < WD / 4; ++p) {
                         uint4 v = make_uint4(0, 0, 0, 0);
                         if (g * (HD / 8) + 16 * p < hd) v = *reinterpret_cast<const uint4*>(src + 16 * p);
                         w[r][4 * p] = v.x ^ 0x80808080u;
@@ -228,7 +277,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
                 }
             }
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
+            for (int i = 0; i < WD; ++i) {
                 // bytes (r0 c0, r1 c0, r0 c1, r1 c1) and (.. c2, .. c3) of both row pairs
                 const uint32_t a01 = __byte_perm(w[0][i], w[1][i], 0x5140), a23 = __byte_perm(w[0][i], w[1][i], 0x7362);
                 const uint32_t b01 = __byte_perm(w[2][i], w[3][i], 0x5140), b23 = __byte_perm(w[2][i], w[3][i], 0x7362);
@@ -238,18 +287,23 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
                 mma16816(acc[4 * i + 3], pf[k], codes_hi(a23), codes_hi(b23));
             }
         }
-        __syncwarp();
-        if (lane == 0 && tile + R::kStages < w1) issue(tile + R::kStages);
+        give(it++);
     }
-    if (!ok)  // let this warp's copies end (each wait bounded) before shared memory is reused
-        for (int s = 0; s < R::kStages; ++s) bar_wait(&bar[s], 0, a.err);
+    if (!ok)  // this warp's copies in flight end (each wait bounded) before shared memory is reused
+        for (int s = 0; s < min(S - 1, items - it - 1); ++s) {
+            if (++slot == S) {
+                slot = 0;
+                phase ^= 1;
+            }
+            bar_wait(&bar[slot], phase, a.err);
+        }
 
     // merge the warps: o (times s_v), m, l of each row
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();
     float* mo = reinterpret_cast<float*>(smem);             // [warps][8][HD]
-    float* ml = mo + kRowWarps * 8 * HD;                     // [warps][8][2]
+    float* ml = mo + W * 8 * HD;                            // [warps][8][2]
     const float up = vref * kPDown;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -262,194 +316,130 @@ __global__ void __launch_bounds__(kRowThreads, 1) kv8_rows_kernel(const __grid_c
         ml[(warp * 8 + g) * 2 + 1] = l;
     }
     __syncthreads();
-    for (int r = warp; r < 8; r += kRowWarps) {
-        const int rr = grp * 8 + r;
-        if (rr >= rows) continue;
-        float mm = -INFINITY;
-        for (int w = 0; w < kRowWarps; ++w) mm = fmaxf(mm, ml[(w * 8 + r) * 2]);
-        const float mu = mm == -INFINITY ? 0.f : mm;
-        float f[kRowWarps], ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
-            f[w] = ex2(ml[(w * 8 + r) * 2] - mu);
-            ll += f[w] * ml[(w * 8 + r) * 2 + 1];
-        }
-        const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
-        const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
-        for (int d = lane; d < hd; d += 32) {
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) v += f[w] * mo[(w * 8 + r) * HD + d];
-            if (sh.active == 1) o_store(a.o, a.type, ob + d, v * inv);
-            else a.part_o[pr * hd + d] = v;
-        }
-        if (lane == 0) {
-            float* st = sh.active == 1 ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
-            st[0] = sh.active == 1 ? mu : mm;
-            st[1] = sh.active == 1 ? inv : ll;
-        }
-    }
-}
-
-// Joins a row's splits, in their order. One warp per row.
-__global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ AttnArgs a) {
-    pdl_wait();
-    pdl_trigger();
-    const int hd = (int)a.c.head_dim, rows = a.n * a.group;
-    const int lane = threadIdx.x & 31;
-    const int rr = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y;
+    const int used = min(W, per_warp ? (c1 - c0 + per_warp - 1) / per_warp : 0);  // warps that had tiles
+    constexpr int PARTS = W / 8;  // warps of a row, each with a part of its columns
+    const int r = warp / PARTS, rr = grp * 8 + r;
     if (rr >= rows) return;
-    const Shares sh = shares_of(a, *a.c.past, rr / a.unit);
-    if (sh.active == 1) return;
-    const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit;
-    const float *ml = a.part_ml + pr * 2, *po = a.part_o + pr * hd;
     float mm = -INFINITY;
-    for (int s = lane; s < sh.active; s += 32) mm = fmaxf(mm, ml[2 * s]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    for (int w = 0; w < used; ++w) mm = fmaxf(mm, ml[(w * 8 + r) * 2]);
     const float mu = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, v[8] = {};
-#pragma unroll 4
-    for (int s = 0; s < sh.active; ++s) {
-        const float f = ex2(ml[2 * s] - mu);
-        ll += f * ml[2 * s + 1];
+    float ll = 0.f;
+    constexpr int D = HD / 32 / PARTS > 0 ? HD / 32 / PARTS : 1;
+    float v[D] = {};
+    const int d0 = (warp % PARTS) * (HD / PARTS) + lane;
+    for (int w = 0; w < used; ++w) {
+        const float f = ex2(ml[(w * 8 + r) * 2] - mu);
+        ll += f * ml[(w * 8 + r) * 2 + 1];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd) v[i] += f * po[(size_t)s * hd + lane + 32 * i];
+        for (int i = 0; i < D; ++i) v[i] += f * mo[(w * 8 + r) * HD + d0 + 32 * i];
     }
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
     const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
+    const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < hd) o_store(a.o, a.type, ob + lane + 32 * i, v[i] * inv);
-    if (lane == 0) {
-        float* st = a.stats + ((size_t)kvh * rows + rr) * 2;
-        st[0] = mu;
-        st[1] = inv;
+    for (int i = 0; i < D; ++i) {
+        const int d = d0 + 32 * i;
+        if (d >= hd) continue;
+        if (sh.active == 1) o_store(a.o, a.type, ob + d, v[i] * inv);
+        else a.part_o[pr * hd + d] = v[i];
+    }
+    if (lane == 0 && warp % PARTS == 0) {
+        float* st = sh.active == 1 ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
+        st[0] = sh.active == 1 ? mu : mm;
+        st[1] = sh.active == 1 ? inv : ll;
     }
 }
 
-// ---------------------------------------------------------------------------
-// The rows' weights: a warp owns 32 cached rows (one block), keeps their codes
-// as fragments, goes through the query rows in groups of eight and sums each
-// column of p. Needs the rows' final m and 1 / l.
-// ---------------------------------------------------------------------------
-template <int HD>
-__global__ void __launch_bounds__(256, 1) kv8_weight_kernel(const __grid_constant__ AttnArgs a) {
-    constexpr int KS = HD / 16;
-    __shared__ uint32_t qs[KS][32][4];
-    __shared__ float qfac[8], qm[8], qi[8];
-    __shared__ int qlim[8];
+// A row's final m and 1 / l from its splits (or from the only one).
+__device__ __forceinline__ float2 row_stats(const AttnArgs& a, int kvh, int rr, const Shares& sh) {
+    const int rows = a.n * a.group;
+    if (sh.active == 1) return *reinterpret_cast<const float2*>(a.stats + ((size_t)kvh * rows + rr) * 2);
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + ((size_t)kvh * rows + rr) * a.nsplit;
+    float mm = -INFINITY, ll = 0.f;
+    for (int s = 0; s < sh.active; ++s) mm = fmaxf(mm, ml[s].x);
+    const float mu = mm == -INFINITY ? 0.f : mm;
+    for (int s = 0; s < sh.active; ++s) ll += ex2(ml[s].x - mu) * ml[s].y;
+    return make_float2(mu, ll == 0.f ? 0.f : 1.f / ll);
+}
+
+// After the splits: the first `joins` CTAs of a KV head join rows' splits, in their order (a warp per row); the
+// others, with weights kept and few rows, add up the rows' weights from the stored scores (1024 keys a CTA).
+__global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ AttnArgs a, int joins) {
+    __shared__ float2 st[kPromptRows];
+    __shared__ int lim[kPromptRows];
     pdl_wait();
     pdl_trigger();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
-    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, kvh = blockIdx.y, rows = a.n * a.group;
-    const int past = *a.c.past;
+    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, rows = a.n * a.group;
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y, past = *a.c.past;
+    if ((int)blockIdx.x < joins) {
+        const int rr = blockIdx.x * 8 + (threadIdx.x >> 5);
+        if (rr >= rows) return;
+        const Shares sh = shares_of(a, past, rr / a.unit);
+        if (sh.active == 1) return;
+        const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit;
+        const float *ml = a.part_ml + pr * 2, *po = a.part_o + pr * hd;
+        float mm = -INFINITY;
+        for (int s = lane; s < sh.active; s += 32) mm = fmaxf(mm, ml[2 * s]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+        const float mu = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f, v[8] = {};
+#pragma unroll 4
+        for (int s = 0; s < sh.active; ++s) {
+            const float f = ex2(ml[2 * s] - mu);
+            ll += f * ml[2 * s + 1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 32 * i < hd) v[i] += f * po[(size_t)s * hd + lane + 32 * i];
+        }
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (lane + 32 * i < hd) o_store(a.o, a.type, ob + lane + 32 * i, v[i] * inv);
+        if (lane == 0 && !a.scores) {  // (the weights' CTAs of few rows take their own)
+            float* d = a.stats + ((size_t)kvh * rows + rr) * 2;
+            d[0] = mu;
+            d[1] = inv;
+        }
+        return;
+    }
     const int keys = keys_of(past, a.n - 1, cap);
-    if ((int)blockIdx.x * 256 >= keys) return;
-    const int tile = blockIdx.x * 8 + warp;  // this warp's block
-    const bool on = tile * 32 < keys;
-    uint32_t kf[4][KS][2];
-    float ks = 0.f;
-    if (on) {
-        ks = a.c.k_scale[(size_t)kvh * (cap >> 5) + tile];
-        const int8_t* kc = a.c.k + ((size_t)kvh * cap + 32 * tile) * hd;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int p = 0; p < HD / 64; ++p) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (tq * (HD / 4) + 16 * p < hd)
-                    w = *reinterpret_cast<const uint4*>(kc + (8 * j + g) * hd + tq * (HD / 4) + 16 * p);
-                const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    kf[j][4 * p + i][0] = codes_lo(u[i]);
-                    kf[j][4 * p + i][1] = codes_hi(u[i]);
-                }
-            }
+    const int key = ((int)blockIdx.x - joins) * 1024 + (int)threadIdx.x * 4;
+    if (((int)blockIdx.x - joins) * 1024 >= keys) return;
+    if ((int)threadIdx.x < rows) {
+        st[threadIdx.x] = row_stats(a, kvh, (int)threadIdx.x, shares_of(a, past, (int)threadIdx.x / a.unit));
+        lim[threadIdx.x] = keys_of(past, (int)threadIdx.x / a.group, cap);
     }
-    float sum[4][2] = {};
-    // the first row that sees any key of the CTA
-    const int first = (int)max(0LL, min((long long)rows, ((long long)blockIdx.x * 256 - past) * a.group)) / 8;
-    for (int grp = first; grp * 8 < rows; ++grp) {
-        __syncthreads();
-        if (warp == 0) {
-            const int row = grp * 8 + g, tok = row / a.group;
-            float x[HD / 4];
-            float mx = 0.f;
-            const long long base = (long long)tok * a.qs + (long long)(kvh * a.group + row % a.group) * hd;
-#pragma unroll
-            for (int i = 0; i < HD / 4; ++i) {
-                const int d = tq * (HD / 4) + i;
-                x[i] = row < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
-                mx = fmaxf(mx, fabsf(x[i]));
-            }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const int e = mx > 0.f && !isinf(mx) ? 7 - ilogbf(mx) : 0;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                split2(ldexpf(x[4 * s], e), ldexpf(x[4 * s + 1], e), qs[s][lane][0], qs[s][lane][1]);
-                split2(ldexpf(x[4 * s + 2], e), ldexpf(x[4 * s + 3], e), qs[s][lane][2], qs[s][lane][3]);
-            }
-            if (tq == 0) {
-                const float* st = a.stats + ((size_t)kvh * rows + min(row, rows - 1)) * 2;
-                qfac[g] = ldexpf(a.scale, -e);
-                qm[g] = st[0];
-                qi[g] = row < rows ? st[1] : 0.f;
-                qlim[g] = row < rows ? keys_of(past, tok, cap) : 0;
-            }
-        }
-        __syncthreads();
-        if (!on) continue;
-        const float fac = qfac[g] * ks, mrow = qm[g], irow = qi[g];
-        const int lim = qlim[g];
-        float sc[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const uint32_t q[4] = {qs[s][lane][0], qs[s][lane][1], qs[s][lane][2], qs[s][lane][3]};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma16816(sc[j], q, kf[j][s][0], kf[j][s][1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int key = tile * 32 + 8 * j + 2 * tq + e;
-                if (key < lim) sum[j][e] += ex2((sc[j][e] + sc[j][e + 2]) * fac - mrow) * irow;
-            }
+    __syncthreads();
+    if (key >= keys) return;
+    const int nz = (rows + 7) / 8;
+    const float* t = a.scores + (size_t)kvh * nz * 8 * cap + key;
+    float sum[4] = {};
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+        // a row that sees none of the four keys may not have stored them
+        if (key >= lim[r]) continue;
+        const float4 x = *reinterpret_cast<const float4*>(t + (size_t)r * cap);
+        const float mr = st[r].x, ir = st[r].y;
+        sum[0] += ex2(x.x - mr) * ir;
+        sum[1] += ex2(x.y - mr) * ir;
+        sum[2] += ex2(x.z - mr) * ir;
+        sum[3] += ex2(x.w - mr) * ir;
     }
-    if (!on) return;
+    float* w = a.weight + (size_t)kvh * cap + key;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float v = sum[j][e];
-            v += __shfl_xor_sync(0xffffffffu, v, 4);
-            v += __shfl_xor_sync(0xffffffffu, v, 8);
-            v += __shfl_xor_sync(0xffffffffu, v, 16);
-            const int key = tile * 32 + 8 * j + 2 * tq + e;
-            if (g == 0 && key < keys) {
-                float* w = a.weight + (size_t)kvh * cap + key;
-                *w = key < past ? *w + v : v;
-            }
-        }
+    for (int e = 0; e < 4; ++e)
+        if (key + e < keys) w[e] = key + e < past ? w[e] + sum[e] : sum[e];
 }
 
 constexpr int kMaxSplit = 64;
-constexpr int kPromptRows = 32;  // query rows of a KV head from which on the prompt kernel takes them
 
 // The plan of a call, from what the host knows of it (not how many rows the cache holds).
 struct Plan {
     bool prompt;
     int unit, nsplit;
-    size_t stats, part_o, part_ml, qt, qfactor, bytes;  // offsets into the workspace
+    size_t stats, part_o, part_ml, scores, qt, qfactor, bytes;  // offsets into the workspace
 };
 Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     Plan p{};
@@ -468,6 +458,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     p.stats = take(H * rows * 2 * sizeof(float));
     p.part_o = take(p.nsplit > 1 ? H * rows * p.nsplit * hd * sizeof(float) : 0);
     p.part_ml = take(p.nsplit > 1 ? H * rows * p.nsplit * 2 * sizeof(float) : 0);
+    p.scores = take(p.prompt ? 0 : H * ((rows + 7) / 8) * 8 * c.capacity * sizeof(float));
     const size_t padded = (rows + 255) / 256 * 256;
     p.qfactor = take(p.prompt ? H * padded * sizeof(float) : 0);
     p.qt = take(p.prompt ? prompt_query_bytes(c, rows, type) : 0);
@@ -483,7 +474,8 @@ size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
     const size_t unit = rows > (size_t)kPromptRows ? std::max(8, prompt_unit((int)c.head_dim)) : 8;
     const size_t padded = (rows + 255) / 256 * 256;
     return H * rows * 2 * sizeof(float) + 148 * unit * (c.head_dim + 2) * sizeof(float) + H * padded * sizeof(float) +
-           prompt_query_bytes(c, rows, NEON_GGML_F32) + 8 * 1024;
+           prompt_query_bytes(c, rows, NEON_GGML_F32) +
+           H * ((std::min<size_t>(rows, kPromptRows) + 7) / 8 * 8) * c.capacity * sizeof(float) + 10 * 1024;
 }
 
 int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t os, size_t n, size_t n_head,
@@ -521,22 +513,21 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
         rc = launch_prompt(a, st);
     } else {
         a.tile_keys = 32;
-        a.min_tiles = 2 * kRowWarps;  // two tiles per warp
+        if (weight) a.scores = (float*)(base + p.scores);
         auto rows_kernel = hd <= 64 ? kv8_rows_kernel<64> : hd <= 128 ? kv8_rows_kernel<128> : kv8_rows_kernel<256>;
         const int smem = hd <= 64 ? RowTile<64>::kSmem : hd <= 128 ? RowTile<128>::kSmem : RowTile<256>::kSmem;
+        const int warps = hd <= 128 ? RowTile<128>::kWarps : RowTile<256>::kWarps;
+        a.min_tiles = warps;  // a tile per warp before another CTA joins
         cudaError_t e = cudaFuncSetAttribute(rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_rows_kernel)");
         rc = launch("kv8_rows_kernel", rows_kernel, dim3((unsigned)a.nsplit, c.n_kv_head, (unsigned)((rows + 7) / 8)),
-                    kRowThreads, (size_t)smem, st, 1, a);
+                    warps * 32, (size_t)smem, st, 1, a);
     }
-    if (!rc && a.nsplit > 1)
-        rc = launch("kv8_join_kernel", kv8_join_kernel, dim3((unsigned)((rows + 3) / 4), c.n_kv_head), 128, 0, st, 1, a);
-    if (!rc && weight && p.prompt) {
-        rc = launch_prompt_weights(a, st);
-    } else if (!rc && weight) {
-        auto wk = hd <= 64 ? kv8_weight_kernel<64> : hd <= 128 ? kv8_weight_kernel<128> : kv8_weight_kernel<256>;
-        rc = launch("kv8_weight_kernel", wk, dim3((c.capacity + 255) / 256, c.n_kv_head), 256, 0, st, 1, a);
-    }
+    const unsigned joins = a.nsplit > 1 ? (unsigned)((rows + 7) / 8) : 0;
+    const unsigned sums = a.scores ? (c.capacity + 1023) / 1024 : 0;
+    if (!rc && joins + sums)
+        rc = launch("kv8_join_kernel", kv8_join_kernel, dim3(joins + sums, c.n_kv_head), 256, 0, st, 1, a, (int)joins);
+    if (!rc && weight && p.prompt) rc = launch_prompt_weights(a, st);
     return rc;
 }
 

@@ -46,6 +46,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+
 // The rows that token t may attend to.
 __device__ __forceinline__ int keys_of(int past, int t, int cap) {
     return (int)max(0LL, min((long long)past + t + 1, (long long)cap));
@@ -67,6 +69,7 @@ struct AttnArgs {
     float* stats;    // [H][rows][2]: a row's final m and 1 / l (0 for a row without keys)
     float* part_o;   // [H][rows][nsplit][hd]: o of a split, not normalised, in units of
     float* part_ml;  // [H][rows][nsplit][2]: 2^m with m, and l
+    float* scores;   // few rows, weights kept: [H][row groups][8][capacity] scores * log2(e), or null
     // prompts: query tiles of 128 rows as fp16 (see kv8_queries_kernel), and the rows' factors
     unsigned char* qt;
     float* qfactor;
@@ -86,6 +89,8 @@ __device__ __forceinline__ Shares shares_of(const AttnArgs& a, int past, int uni
     s.active = s.per ? (s.tiles + s.per - 1) / s.per : 1;
     return s;
 }
+
+constexpr int kPromptRows = 32;  // query rows of a KV head above which the prompt kernel takes them
 
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -131,8 +131,6 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
     }
 }
 
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
-
 // fp32 pairs in one instruction
 __device__ __forceinline__ uint64_t pair(float x, float y) {
     uint64_t r;
