@@ -4,8 +4,8 @@
 //
 // A block is 32 rows of one KV head: codes c = rint(x / s), s = amax / 127. A
 // code is the nearest integer to the exact quotient: the quotient is first
-// taken with the reciprocal of s, then the remainder e = x - r s, which one
-// FMA gives exactly (r is at most one off the nearest integer, so e is a
+// taken with the reciprocal of s, which settles it unless it is near a tie.
+// There the remainder e = x - r s, which one FMA gives exactly (r is at most one off the nearest integer, so e is a
 // multiple of the smaller ulp and below s), moves r by one where |e| > s / 2
 // and to the even side where |e| = s / 2. So the codes do not depend on how a
 // quotient is rounded, and a block's codes are a function of its rows.
@@ -42,76 +42,52 @@ int kv8_check_buffers(const neon_kv8_t* c) {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kTiny = 127.f * 1.17549435e-38f;  // 127 * FLT_MIN
 
-// ---- a block's rows as float4 pieces in registers ----
-// Thread i holds pieces i, i + 256, ... of the block's 32 * hd / 4, row-major;
-// P = hd / 32 rounded up covers them.
-
-// The largest magnitude of the block, or NaN if a value is not finite.
-template <int P>
-__device__ __forceinline__ float block_amax(const float4 (&x)[P], float* red) {
-    float m = 0.f;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-        bad = bad || isnan(x[i].x) || isnan(x[i].y) || isnan(x[i].z) || isnan(x[i].w);
-    }
-    if (bad || isinf(m)) m = __int_as_float(0x7fffffff);
-    // as bit patterns: magnitudes order like their bits, and a NaN is above them all
-    const unsigned w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(w);
-    __syncthreads();
-    unsigned r = 0;
-#pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) r = max(r, __float_as_uint(red[i]));
-    __syncthreads();
-    return __uint_as_float(r);
-}
-
+// A block's scale from its largest magnitude (NaN: a value is not finite).
 __device__ __forceinline__ float block_scale(float amax) {
     return isnan(amax) ? amax : amax >= kTiny ? __fdiv_rn(amax, 127.f) : 0.f;
 }
 
-__device__ __forceinline__ int quantise(float x, float s, float inv) {
+// The nearest integer to x / s, ties to even, from x times the reciprocal: as is where that is clear of a tie
+// (the product is off by less than 2^-15 of an integer), else by the exact remainder.
+__device__ __forceinline__ int quantise_exact(float x, float s, float inv) {
     float r = rintf(__fmul_rn(x, inv));
     const float e = __fmaf_rn(-r, s, x);  // exact
     const float e2 = 2.f * fabsf(e);
     if (e2 > s || (e2 == s && ((int)r & 1))) r += e > 0.f ? 1.f : -1.f;
     return (int)r;
 }
-__device__ __forceinline__ char4 quantise4(float4 x, float s, float inv) {
-    if (!(s > 0.f)) return make_char4(0, 0, 0, 0);  // an empty block, or NaN
-    return make_char4((char)quantise(x.x, s, inv), (char)quantise(x.y, s, inv), (char)quantise(x.z, s, inv),
-                      (char)quantise(x.w, s, inv));
-}
-__device__ __forceinline__ float4 dequantise4(char4 c, float s) {
-    return make_float4(__fmul_rn((float)c.x, s), __fmul_rn((float)c.y, s), __fmul_rn((float)c.z, s), __fmul_rn((float)c.w, s));
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, which the low byte then holds
+// Four values as four codes.
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[4], float s, float inv) {
+    float t[4], far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = __fmul_rn(x[i], inv);
+        t[i] = __fadd_rn(y, kMagic);
+        far = fmaxf(far, fabsf(__fadd_rn(y, -__fadd_rn(t[i], -kMagic))));
+    }
+    if (far > 0.4999f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = kMagic + (float)quantise_exact(x[i], s, inv);
+    }
+    return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                       __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, bool vec);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float* p, bool vec) {
-    return vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
-}
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, bool vec) {
-    if (!vec) return make_float4(to_f(p[0]), to_f(p[1]), to_f(p[2]), to_f(p[3]));
-    union { uint2 u; T t[4]; } w;
-    w.u = *reinterpret_cast<const uint2*>(p);
-    return make_float4(to_f(w.t[0]), to_f(w.t[1]), to_f(w.t[2]), to_f(w.t[3]));
+__device__ __forceinline__ float code_value(uint32_t w, int i, float s) {
+    return __fmul_rn((float)(int8_t)(w >> (8 * i)), s);
 }
 
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// One CTA per block, head and K or V; the first CTA of a head takes its first
-// block and then its last one, the only two that touch the tail. Memory bounds
-// a prompt's append (8191 new bf16 rows of 8 heads x 128: the figures are in
-// the table of the design notes); one token's is a launch and its latency.
+// A CTA of four warps per block, head and K or V; the first CTA of a head
+// takes its first block and then its last one, the only two that touch the
+// tail. A thread has 8 pieces of 4 values at head_dim 128, all loaded before
+// the first is used; memory bounds a prompt's append, one token's is a launch
+// and its latency.
 
 struct AppendArgs {
     neon_kv8_t c;
@@ -121,10 +97,11 @@ struct AppendArgs {
     bool vec;
     unsigned* err;
 };
+constexpr int kAppThreads = 128;
 
 template <typename T, int P>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
-    __shared__ float red[kThreads / 32];
+__global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ unsigned red[2][kAppThreads / 32];
     pdl_wait();
     pdl_trigger();
     const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, H = (int)a.c.n_kv_head;
@@ -170,35 +147,69 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
             if (now != g) tag[tid] = now;
         }
     }
-    for (;;) {
+    for (int pass = 0;; ++pass) {
         const int rows = min(32, end - 32 * b);  // rows that the block holds after this call
         const int old = b == b0 ? r0 : 0;        // of them, rows from before
         const int slot = blockIdx.x == 0 ? (b == b0 ? slot0 : slot1) : -1;
         float* keep = slot >= 0 ? tail + slot * slot_floats : nullptr;
-        int8_t* bc = codes + (size_t)b * 32 * hd;
-        const float before = old && !known ? scales[b] : 0.f;
-        float4 x[P];
+        uint32_t* bc = reinterpret_cast<uint32_t*>(codes + (size_t)b * 32 * hd);
+        const int per = hd / 4;  // pieces of a row
+        Vec4<T> w[P];
+        int row[P];
+        // the new rows' loads alone first, all in flight together
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int e = (i * kThreads + tid) * 4, r = e / hd;
-            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows) {
-                if (r >= old)
-                    x[i] = load4<T>(src + (32LL * b + r - past) * ss + (long long)h * hd + (e - r * hd), a.vec);
-                else if (known)
-                    x[i] = *reinterpret_cast<const float4*>(keep + e);
-                else
-                    x[i] = dequantise4(*reinterpret_cast<const char4*>(bc + e), before);
+            const int p = i * kAppThreads + tid;
+            row[i] = p / per;
+            if (row[i] >= old && row[i] < rows) {
+                const T* q = src + (32LL * b + row[i] - past) * ss + (long long)h * hd + (p - row[i] * per) * 4;
+                if (a.vec) {
+                    w[i].load(q);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[i].t[e] = q[e];
+                }
             }
         }
-        const float s = block_scale(block_amax(x, red));
+        const float before = old && !known ? scales[b] : 0.f;
+        float x[P][4];
+        float m = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int p = i * kAppThreads + tid;
+            if (row[i] >= old && row[i] < rows) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = to_f(w[i].t[e]);
+            } else if (row[i] < old && known) {
+                const float4 v = *reinterpret_cast<const float4*>(keep + 4 * p);
+                x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+            } else {
+                const uint32_t c = row[i] < old ? bc[p] : 0u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = code_value(c, e, before);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m = fmaxf(m, fabsf(x[i][e]));
+                bad = bad || isnan(x[i][e]);
+            }
+        }
+        if (bad || isinf(m)) m = __int_as_float(0x7fffffff);
+        // as bit patterns: magnitudes order like their bits, and a NaN is above them all
+        const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+        if ((tid & 31) == 0) red[pass & 1][tid >> 5] = top;
+        __syncthreads();
+        const unsigned* rd = red[pass & 1];
+        const float s = block_scale(__uint_as_float(max(max(rd[0], rd[1]), max(rd[2], rd[3]))));
         const float inv = __fdiv_rn(1.f, s);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int e = (i * kThreads + tid) * 4, r = e / hd;
-            if (r < rows) {
-                *reinterpret_cast<char4*>(bc + e) = quantise4(x[i], s, inv);
-                if (keep && (r >= old || !known)) *reinterpret_cast<float4*>(keep + e) = x[i];
+            const int p = i * kAppThreads + tid;
+            if (row[i] < rows) {
+                bc[p] = s > 0.f ? quantise4(x[i], s, inv) : 0u;  // an empty block, or NaN: 0
+                if (keep && (row[i] >= old || !known))
+                    *reinterpret_cast<float4*>(keep + 4 * p) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
             }
         }
         if (tid == 0) scales[b] = s;
@@ -211,49 +222,54 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
 using AppendKernel = void (*)(AppendArgs);
 template <typename T>
 AppendKernel append_kernel_for(int hd) {
-    return hd <= 64 ? kv8_append_kernel<T, 2> : hd <= 128 ? kv8_append_kernel<T, 4> : kv8_append_kernel<T, 8>;
+    return hd <= 64 ? kv8_append_kernel<T, 4> : hd <= 128 ? kv8_append_kernel<T, 8> : kv8_append_kernel<T, 16>;
 }
 
 // ---------------------------------------------------------------------------
 // read
 // ---------------------------------------------------------------------------
+// A piece of four codes per lane, so that a warp's loads and stores are whole
+// lines; eight pieces in flight a thread.
+constexpr int kReadThreads = 256, kReadRows = 64;  // rows of a CTA
 
-__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ neon_kv8_t c, int row0, int n,
-                                                            float* k_out, float* v_out) {
+__global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const __grid_constant__ neon_kv8_t c, int row0, int n,
+                                                                float* k_out, float* v_out) {
     pdl_wait();
     pdl_trigger();
     const int hd = (int)c.head_dim, cap = (int)c.capacity, H = (int)c.n_kv_head, h = blockIdx.y, which = blockIdx.z;
     float* out = which ? v_out : k_out;
     if (!out) return;
-    const int8_t* codes = (which ? c.v : c.k) + ((size_t)h * cap + row0) * hd;
+    const int first = row0 + (int)blockIdx.x * kReadRows, rows = min(kReadRows, row0 + n - first);
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>((which ? c.v : c.k) + ((size_t)h * cap + first) * hd);
     const float* scales = (which ? c.v_scale : c.k_scale) + (size_t)h * (cap >> 5);
-    const int per = hd / 4;  // pieces of a row
-    const long long total = (long long)n * per;
-    constexpr int U = 4;
-    for (long long i0 = (long long)blockIdx.x * kThreads * U + threadIdx.x; i0 < total; i0 += (long long)gridDim.x * kThreads * U) {
-        char4 q[U];
+    float* to = out + ((size_t)(first - row0) * H + h) * hd;
+    const int per = hd / 4, total = rows * per;
+    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;  // (a caller's buffer is aligned to its floats only)
+    constexpr int U = 8;
+    for (int i0 = threadIdx.x; i0 < total; i0 += kReadThreads * U) {
+        uint32_t q[U];
         float s[U];
+        int r[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long i = i0 + u * kThreads;
+            const int i = i0 + u * kReadThreads;
+            r[u] = i / per;
             if (i < total) {
-                q[u] = *reinterpret_cast<const char4*>(codes + i * 4);
-                s[u] = scales[(row0 + (int)(i / per)) >> 5];
+                q[u] = codes[i];
+                s[u] = scales[(first + r[u]) >> 5];
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long i = i0 + u * kThreads;
-            if (i < total) {
-                const int r = (int)(i / per);
-                // (a caller's buffer is aligned to its floats only)
-                float* o = out + ((long long)r * H + h) * hd + (i - (long long)r * per) * 4;
-                const float4 x = dequantise4(q[u], s[u]);
-                if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-                    *reinterpret_cast<float4*>(o) = x;
-                } else {
-                    o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
-                }
+            const int i = i0 + u * kReadThreads;
+            if (i >= total) continue;
+            float* o = to + (size_t)r[u] * H * hd + (i - r[u] * per) * 4;
+            const float4 x = make_float4(code_value(q[u], 0, s[u]), code_value(q[u], 1, s[u]), code_value(q[u], 2, s[u]),
+                                         code_value(q[u], 3, s[u]));
+            if (vec) {
+                *reinterpret_cast<float4*>(o) = x;
+            } else {
+                o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
             }
         }
     }
@@ -270,8 +286,9 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constan
 // gathers: one CTA per new block, head and K or V.
 
 constexpr int kSelCluster = 8;
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelHeld = 16;  // weights that a thread holds (131072 rows of a head); any others are read again
 
 // A weight as an unsigned number of the same order; every NaN is the largest.
 __device__ __forceinline__ unsigned order_bits(float w) {
@@ -319,6 +336,24 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     for (int i = rank * kSelThreads + tid; i < a.recent; i += kSelCluster * kSelThreads) kept[a.keep - a.recent + i] = hi + i;
     if (m == 0) return;
 
+    // Held weights are this warp's: rows s0 + 32 j + lane.
+    const int nw = kSelCluster * kSelWarps, gw = rank * kSelWarps + warp;
+    const int span = ((hi - lo + nw - 1) / nw + 31) & ~31;
+    const int s0 = min(lo + gw * span, hi), s1 = min(s0 + span, hi);
+    unsigned held[kSelHeld];
+#pragma unroll
+    for (int j = 0; j < kSelHeld; ++j) held[j] = s0 + 32 * j + lane < s1 ? order_bits(w[s0 + 32 * j + lane]) : 0u;
+    // f(row, its ordered weight, whether it is one of the warp's), for whole warps and in row order
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < kSelHeld; ++j)
+            if (s0 + 32 * j < s1) f(s0 + 32 * j + lane, held[j], s0 + 32 * j + lane < s1);
+        for (int i0 = s0 + 32 * kSelHeld; i0 < s1; i0 += 32) {
+            const bool on = i0 + lane < s1;
+            f(i0 + lane, on ? order_bits(w[i0 + lane]) : 0u, on);
+        }
+    };
+
     // the m-th largest, eight bits a round
     unsigned prefix = 0, left = (unsigned)m;
     for (int round = 0; round < 4; ++round) {
@@ -326,10 +361,9 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         unsigned* hs = hist[round & 1];
         for (int i = tid; i < 256; i += kSelThreads) hs[i] = 0;
         __syncthreads();
-        for (int i = lo + rank * kSelThreads + tid; i < hi; i += kSelCluster * kSelThreads) {
-            const unsigned u = order_bits(w[i]);
-            if (round == 0 || (u >> (shift + 8)) == prefix) atomicAdd(&hs[(u >> shift) & 255], 1u);
-        }
+        each([&](int, unsigned u, bool on) {
+            if (on && (round == 0 || (u >> (shift + 8)) == prefix)) atomicAdd(&hs[(u >> shift) & 255], 1u);
+        });
         cluster_barrier();
         // bin 255 - tid and the bins above it, over the cluster
         if (tid < 256) {
@@ -360,16 +394,11 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     }
     const unsigned T = prefix;  // rows above T stay, and the first `left` rows equal to it
 
-    // the warps' ranges, in row order over the cluster
-    const int nw = kSelCluster * kSelWarps, gw = rank * kSelWarps + warp;
-    const int span = ((hi - lo + nw - 1) / nw + 31) & ~31;
-    const int s0 = min(lo + gw * span, hi), s1 = min(s0 + span, hi);
     unsigned above = 0, equal = 0;
-    for (int i = s0 + lane; i < s1; i += 32) {
-        const unsigned u = order_bits(w[i]);
-        above += u > T;
-        equal += u == T;
-    }
+    each([&](int, unsigned u, bool on) {
+        above += on && u > T;
+        equal += on && u == T;
+    });
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) {
@@ -389,17 +418,15 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     }
     before = __reduce_add_sync(0xffffffffu, before);
     ties = __reduce_add_sync(0xffffffffu, ties);
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned u = i < s1 ? order_bits(w[i]) : 0u;
-        const bool up = i < s1 && u > T, eq = i < s1 && u == T;
+    each([&](int i, unsigned u, bool on) {
+        const bool up = on && u > T, eq = on && u == T;
         const unsigned bu = __ballot_sync(0xffffffffu, up), be = __ballot_sync(0xffffffffu, eq);
         const unsigned mask = (1u << lane) - 1u;
         const unsigned t = ties + __popc(be & mask);  // equal rows before this one
         if (up || (eq && t < left)) kept[a.sink + before + __popc(bu & mask) + min(t, left)] = i;
         before += __popc(bu);
         ties += __popc(be);
-    }
+    });
     cluster_barrier();  // no CTA leaves while another reads its counts
 }
 
@@ -412,93 +439,113 @@ struct GatherArgs {
     int pairs, half, rotate;
     RopeTurns turns;
 };
+constexpr int kGatherThreads = 128;
 
+// A CTA of four warps per new block, head and K or V; a warp has eight rows in pieces of four codes, P of them a
+// lane (P = hd / 16 rounded up to 4, 8 or 16). The largest magnitude is a row's largest code times its scale.
 template <int P>
-__global__ void __launch_bounds__(kThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
-    extern __shared__ float4 rowbuf[];  // with rotation: the block's rows
-    __shared__ float red[kThreads / 32];
+__global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
+    extern __shared__ float rowbuf[];  // with rotation: the block's rows
+    __shared__ unsigned red[kGatherThreads / 32];
     __shared__ int from[32];
+    __shared__ float fs[32];
     pdl_wait();
     pdl_trigger();
     const int hd = (int)a.src.head_dim, H = (int)a.src.n_kv_head, cap = (int)a.src.capacity, dcap = (int)a.dst.capacity;
     const int b = blockIdx.x, h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
-    const int len = min(max(*a.src.past, 0), cap), m = min(len, a.keep);
+    const float* ssc = (which ? a.src.v_scale : a.src.k_scale) + (size_t)h * (cap >> 5);
+    const int r_ = tid < 32 && 32 * b + tid < a.keep ? a.kept[(size_t)h * a.keep + 32 * b + tid] : -1;  // -1 behind the last
     if (b == 0) {
+        const int m = min(min(max(*a.src.past, 0), cap), a.keep);
         if (tid < 2) a.dst.tail_block[((size_t)which * H + h) * 2 + tid] = -1;
         if (h == 0 && which == 0 && tid == 0) *a.dst.past = m;
     }
-    const int rows = min(32, m - 32 * b);
-    if (rows <= 0) return;
     if (tid < 32) {
-        const int r = tid < rows ? a.kept[(size_t)h * a.keep + 32 * b + tid] : -1;
-        from[tid] = r;
-        if (which == 0 && tid < rows) a.wd[(size_t)h * dcap + 32 * b + tid] = a.w[(size_t)h * cap + r];
+        from[tid] = r_;
+        if (r_ >= 0) {
+            fs[tid] = ssc[r_ >> 5];
+            if (which == 0) a.wd[(size_t)h * dcap + 32 * b + tid] = a.w[(size_t)h * cap + r_];
+        }
     }
     __syncthreads();
+    int rows = 32;
+    if (from[31] < 0) {  // the last block
+        rows = 0;
+        while (rows < 32 && from[rows] >= 0) ++rows;
+        if (rows == 0) return;
+    }
     // kept rows ascend: the last one in place means that all of the block's are
     const bool stay = from[rows - 1] == 32 * b + rows - 1;
     const int8_t* sc = (which ? a.src.v : a.src.k) + (size_t)h * cap * hd;
-    const float* ssc = (which ? a.src.v_scale : a.src.k_scale) + (size_t)h * (cap >> 5);
-    int8_t* dc = (which ? a.dst.v : a.dst.k) + ((size_t)h * dcap + 32 * b) * hd;
+    uint32_t* dc = reinterpret_cast<uint32_t*>((which ? a.dst.v : a.dst.k) + ((size_t)h * dcap + 32 * b) * hd);
     float* dsc = (which ? a.dst.v_scale : a.dst.k_scale) + (size_t)h * (dcap >> 5);
-    char4 q[P];
-    float s[P];
-    float4 x[P];
+    const int per = hd / 4;
+    uint32_t q[P];
+    int row[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int e = (i * kThreads + tid) * 4, r = e / hd;
-        if (r < rows) {
-            const int f = from[r];
-            q[i] = *reinterpret_cast<const char4*>(sc + (size_t)f * hd + (e - r * hd));
-            s[i] = ssc[f >> 5];
-        }
+        const int p = i * kGatherThreads + tid;
+        row[i] = p / per;
+        q[i] = 0;
+        if (row[i] < rows) q[i] = *reinterpret_cast<const uint32_t*>(sc + (size_t)from[row[i]] * hd + (p - row[i] * per) * 4);
     }
     if (stay) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int e = (i * kThreads + tid) * 4;
-            if (e / hd < rows) *reinterpret_cast<char4*>(dc + e) = q[i];
-        }
-        if (tid == 0) dsc[b] = ssc[b];
+        for (int i = 0; i < P; ++i)
+            if (row[i] < rows) dc[i * kGatherThreads + tid] = q[i];
+        if (tid == 0) dsc[b] = fs[0];
         return;
     }
+    const bool turned = a.rotate && which == 0;
+    float m = 0.f;
+    if (!turned) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int e = (i * kThreads + tid) * 4;
-        x[i] = e / hd < rows ? dequantise4(q[i], s[i]) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    if (a.rotate && which == 0) {
-        float* rb = reinterpret_cast<float*>(rowbuf);
+        for (int i = 0; i < P; ++i)
+            if (row[i] < rows) {
+                const uint32_t u = __vabs4(q[i]);  // (codes are -127 .. 127)
+                const unsigned top = max(max(u & 255, (u >> 8) & 255), max((u >> 16) & 255, u >> 24));
+                const float x = __fmul_rn((float)top, fs[row[i]]);
+                m = x != x ? __int_as_float(0x7fffffff) : __uint_as_float(max(__float_as_uint(m), __float_as_uint(x)));
+            }
+    } else {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int e = (i * kThreads + tid) * 4;
-            if (e / hd < rows) rowbuf[e / 4] = x[i];
-        }
+        for (int i = 0; i < P; ++i)
+            if (row[i] < rows)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rowbuf[4 * (i * kGatherThreads + tid) + e] = code_value(q[i], e, fs[row[i]]);
         __syncthreads();
-        for (int i = tid; i < rows * a.pairs; i += kThreads) {
+        for (int i = tid; i < rows * a.pairs; i += kGatherThreads) {
             const int r = i / a.pairs, p = i - r * a.pairs;
             const int delta = 32 * b + r - from[r];
             if (delta == 0) continue;
             const float2 c = turn(a.turns.f[p], delta);
-            float* u = rb + r * hd + (a.half ? p : 2 * p);
+            float* u = rowbuf + r * hd + (a.half ? p : 2 * p);
             float* v = u + (a.half ? a.pairs : 1);
             const float x0 = *u, x1 = *v;
             *u = __fmaf_rn(x0, c.x, -__fmul_rn(x1, c.y));
             *v = __fmaf_rn(x0, c.y, __fmul_rn(x1, c.x));
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int e = (i * kThreads + tid) * 4;
-            if (e / hd < rows) x[i] = rowbuf[e / 4];
+        bool bad = false;
+        for (int i = tid; i < rows * hd; i += kGatherThreads) {
+            m = fmaxf(m, fabsf(rowbuf[i]));
+            bad = bad || isnan(rowbuf[i]);
         }
+        if (bad || isinf(m)) m = __int_as_float(0x7fffffff);
     }
-    const float sn = block_scale(block_amax(x, red));
+    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if ((tid & 31) == 0) red[tid >> 5] = top;
+    __syncthreads();
+    const float sn = block_scale(__uint_as_float(max(max(red[0], red[1]), max(red[2], red[3]))));
     const float inv = __fdiv_rn(1.f, sn);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int e = (i * kThreads + tid) * 4;
-        if (e / hd < rows) *reinterpret_cast<char4*>(dc + e) = quantise4(x[i], sn, inv);
+        if (row[i] >= rows) continue;
+        const int p = i * kGatherThreads + tid;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = turned ? rowbuf[4 * p + e] : code_value(q[i], e, fs[row[i]]);
+        dc[p] = sn > 0.f ? quantise4(x, sn, inv) : 0u;
     }
     if (tid == 0) dsc[b] = sn;
 }
@@ -524,7 +571,7 @@ int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, siz
                                                 : append_kernel_for<__nv_bfloat16>((int)c.head_dim);
     // rows past .. past + n - 1 touch at most (n + 62) / 32 blocks; the first CTA takes two of them
     const unsigned blocks = (unsigned)std::max<size_t>(1, (n + 62) / 32 - 1);
-    return launch("kv8_append_kernel", kern, dim3(blocks, c.n_kv_head, 2), kThreads, 0, st, 1, a);
+    return launch("kv8_append_kernel", kern, dim3(blocks, c.n_kv_head, 2), kAppThreads, 0, st, 1, a);
 }
 
 int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
@@ -547,8 +594,8 @@ int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, floa
         rope_turns(*rope, &g.turns);
     }
     const int hd = (int)src.head_dim;
-    auto kern = hd <= 64 ? kv8_gather_kernel<2> : hd <= 128 ? kv8_gather_kernel<4> : kv8_gather_kernel<8>;
-    return launch("kv8_gather_kernel", kern, dim3((unsigned)((keep + 31) / 32), src.n_kv_head, 2), kThreads,
+    auto kern = hd <= 64 ? kv8_gather_kernel<4> : hd <= 128 ? kv8_gather_kernel<8> : kv8_gather_kernel<16>;
+    return launch("kv8_gather_kernel", kern, dim3((unsigned)((keep + 31) / 32), src.n_kv_head, 2), kGatherThreads,
                   rope ? (size_t)32 * hd * sizeof(float) : 0, st, 1, g);
 }
 
@@ -584,12 +631,9 @@ int neon_cuda_kv8_read(const neon_kv8_t* cache, size_t row0, size_t n, float* dK
     if (n == 0 || (!dK_out && !dV_out)) return NEON_OK;
     OnDevice dev(cache->k);
     if (dev.rc) return dev.rc;
-    const int sms = neon_internal::device_sms(dev.device);
-    if (sms < 0) return NEON_ERR_CUDA;
-    const long long pieces = (long long)n * (cache->head_dim / 4);
-    const long long want = (pieces + kThreads * 4 - 1) / (kThreads * 4);
-    return launch("kv8_read_kernel", kv8_read_kernel, dim3((unsigned)std::min<long long>(want, 1 << 20), cache->n_kv_head, 2),
-                  kThreads, 0, (cudaStream_t)stream, 1, *cache, (int)row0, (int)n, dK_out, dV_out);
+    if (neon_internal::device_sms(dev.device) < 0) return NEON_ERR_CUDA;
+    return launch("kv8_read_kernel", kv8_read_kernel, dim3((unsigned)((n + kReadRows - 1) / kReadRows), cache->n_kv_head, 2),
+                  kReadThreads, 0, (cudaStream_t)stream, 1, *cache, (int)row0, (int)n, dK_out, dV_out);
 }
 
 int neon_cuda_kv8_evict(const neon_kv8_t* src, const float* d_weight, const neon_kv8_t* dst, float* d_weight_dst,

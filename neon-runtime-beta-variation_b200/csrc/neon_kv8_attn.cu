@@ -57,35 +57,40 @@ struct RowTile {
     static_assert(kSmem <= 232448, "shared memory");
 };
 
-// The query fragments of rows 8 grp .. of a KV head: lane (g, tq) holds values tq HD / 4 + 4 s .. + 3 of row g for
-// step s, times 2^e so that the row's largest is near 2^7 (its lo terms then stay normal halves). One warp; the
-// row's factor scale log2(e) 2^-e is returned to its four lanes.
+// The query fragments of rows 8 grp .. of a KV head, one warp per row: lane (g, tq) of the products holds values
+// tq HD / 4 + 4 s .. + 3 of row g for step s, as hi and lo terms, times 2^e so that the row's largest is near 2^7 (its
+// lo terms then stay normal halves). The row's factor is scale log2(e) 2^-e.
 template <int HD>
-__device__ __forceinline__ float row_queries(const AttnArgs& a, int kvh, int grp, uint4* out) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3, hd = (int)a.c.head_dim, rows = a.n * a.group;
-    const int row = grp * 8 + g;
+__device__ __forceinline__ void row_queries(const AttnArgs& a, int kvh, int grp, int g, uint4* out, float* factor) {
+    const int lane = threadIdx.x & 31, hd = (int)a.c.head_dim, rows = a.n * a.group, row = grp * 8 + g;
     const long long base = (long long)(row / a.group) * a.qs + (long long)(kvh * a.group + row % a.group) * hd;
-    float x[HD / 4];
+    constexpr int V = (HD + 127) / 128;  // pieces of four values a lane
+    float x[V][4];
     float mx = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD / 4; ++i) {
-        const int d = tq * (HD / 4) + i;
-        x[i] = row < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
-        mx = fmaxf(mx, fabsf(x[i]));
-    }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const unsigned top = __float_as_uint(mx) >> 23;
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 4 * (lane + 32 * v) + i;
+            x[v][i] = row < rows && d < hd ? q_value(a.q, a.type, base + d) : 0.f;
+        }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fabsf(x[v][i]));
+    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23;
     const int e = top >= 255u ? 0 : min(120, 134 - (int)top);
     const float f = pow2(e);
 #pragma unroll
-    for (int s = 0; s < HD / 16; ++s) {
+    for (int v = 0; v < V; ++v) {
+        const int d = 4 * (lane + 32 * v);
+        if (d >= HD) continue;
         uint4 q;
-        split2(x[4 * s] * f, x[4 * s + 1] * f, q.x, q.y);
-        split2(x[4 * s + 2] * f, x[4 * s + 3] * f, q.z, q.w);
-        out[s * 32 + lane] = q;
+        split2(x[v][0] * f, x[v][1] * f, q.x, q.y);
+        split2(x[v][2] * f, x[v][3] * f, q.z, q.w);
+        out[d % (HD / 4) / 4 * 32 + g * 4 + d / (HD / 4)] = q;
     }
-    return a.scale * pow2(-e);
+    if (lane == 0) factor[g] = a.scale * pow2(-e);
 }
 
 template <int HD>
@@ -133,10 +138,7 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     };
     if (lane == 0)
         for (int it = 0; it < min(S, items); ++it) issue(it, it);
-    if (warp == 0) {
-        const float f = row_queries<HD>(a, kvh, grp, qf);
-        if (tq == 0) qfac[g] = f;
-    }
+    if (warp < 8) row_queries<HD>(a, kvh, grp, warp, qf, qfac);
     __syncthreads();
     const float factor = qfac[g];
     float* scores = a.scores ? a.scores + (((size_t)kvh * gridDim.z + grp) * 8 + g) * cap : nullptr;
@@ -320,16 +322,22 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     constexpr int PARTS = W / 8;  // warps of a row, each with a part of its columns
     const int r = warp / PARTS, rr = grp * 8 + r;
     if (rr >= rows) return;
-    float mm = -INFINITY;
-    for (int w = 0; w < used; ++w) mm = fmaxf(mm, ml[(w * 8 + r) * 2]);
+    // lane w has warp w's m and l
+    float2 own = lane < used ? *reinterpret_cast<const float2*>(ml + (lane * 8 + r) * 2) : make_float2(-INFINITY, 0.f);
+    float mm = own.x;
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    mm = __shfl_sync(0xffffffffu, mm, 0);
     const float mu = mm == -INFINITY ? 0.f : mm;
+    const float fw = ex2(own.x - mu);
     float ll = 0.f;
     constexpr int D = HD / 32 / PARTS > 0 ? HD / 32 / PARTS : 1;
     float v[D] = {};
     const int d0 = (warp % PARTS) * (HD / PARTS) + lane;
+#pragma unroll 8
     for (int w = 0; w < used; ++w) {
-        const float f = ex2(ml[(w * 8 + r) * 2] - mu);
-        ll += f * ml[(w * 8 + r) * 2 + 1];
+        const float f = __shfl_sync(0xffffffffu, fw, w);
+        ll += f * __shfl_sync(0xffffffffu, own.y, w);
 #pragma unroll
         for (int i = 0; i < D; ++i) v[i] += f * mo[(w * 8 + r) * HD + d0 + 32 * i];
     }
