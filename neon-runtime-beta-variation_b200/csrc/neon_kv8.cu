@@ -44,9 +44,17 @@ namespace {
 
 constexpr float kTiny = 127.f * 1.17549435e-38f;  // 127 * FLT_MIN
 
-// A block's scale from its largest magnitude (NaN: a value is not finite).
-__device__ __forceinline__ float block_scale(float amax) {
-    return isnan(amax) ? amax : amax >= kTiny ? __fdiv_rn(amax, 127.f) : 0.f;
+// A block's scale from its largest magnitude (as bits).
+__device__ __forceinline__ float block_scale(unsigned top) {
+    const float amax = __uint_as_float(top);
+    return top >= 0x7f800000u ? __int_as_float(0x7fffffff) : amax >= kTiny ? __fdiv_rn(amax, 127.f) : 0.f;
+}
+// The largest of a CTA of four warps.
+__device__ __forceinline__ unsigned block_top(unsigned m, unsigned* red) {
+    const unsigned top = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    return max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
 // The nearest integer to x / s, ties to even, from x times the reciprocal: as is where that is clear of a tie
@@ -76,8 +84,20 @@ __device__ __forceinline__ uint32_t quantise4(const float (&x)[4], float s, floa
                        __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
-__device__ __forceinline__ float code_value(uint32_t w, int i, float s) {
-    return __fmul_rn((float)(int8_t)(w >> (8 * i)), s);
+// The values of four codes: 0x4b0000uu is 2^23 + u, with u = code + 128 (an int-to-float conversion has a
+// quarter of the rate).
+__device__ __forceinline__ void code_values(uint32_t w, float s, float (&x)[4]) {
+    const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        x[e] = __fmul_rn(__fadd_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 | e)), -8388736.f), s);
+}
+// Magnitudes as bit patterns order like numbers, and what is not finite is at or above 0x7f800000.
+__device__ __forceinline__ unsigned magnitude(const float (&x)[4]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    return m;
 }
 
 // ---------------------------------------------------------------------------
@@ -99,12 +119,13 @@ struct AppendArgs {
 };
 constexpr int kAppThreads = 128;
 
-template <typename T, int P>
+// HD: the head dimension, known to the compiler, or 0 (then P covers a.c.head_dim).
+template <typename T, int HD, int P = HD ? HD / 16 : 16>
 __global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ unsigned red[2][kAppThreads / 32];
     pdl_wait();
     pdl_trigger();
-    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, H = (int)a.c.n_kv_head;
+    const int hd = HD ? HD : (int)a.c.head_dim, cap = (int)a.c.capacity, H = (int)a.c.n_kv_head;
     const int h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
     const int past = *a.c.past;
     if (past < 0 || (long long)past + a.n > cap) {
@@ -154,6 +175,34 @@ __global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_co
         float* keep = slot >= 0 ? tail + slot * slot_floats : nullptr;
         uint32_t* bc = reinterpret_cast<uint32_t*>(codes + (size_t)b * 32 * hd);
         const int per = hd / 4;  // pieces of a row
+        if (old == 0 && rows == 32 && a.vec && !keep) {  // a new, whole block: most of a prompt's
+            Vec4<T> w[P];
+            const T* q = src + (32LL * b - past) * ss + (long long)h * hd;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int p = i * kAppThreads + tid, r = p / per;
+                if (r < 32) w[i].load(q + r * ss + (p - r * per) * 4);
+            }
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if ((i * kAppThreads + tid) / per < 32) {
+                    const float x[4] = {to_f(w[i].t[0]), to_f(w[i].t[1]), to_f(w[i].t[2]), to_f(w[i].t[3])};
+                    m = max(m, magnitude(x));
+                }
+            const float s = block_scale(block_top(m, red[pass & 1])), inv = __fdiv_rn(1.f, s);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if ((i * kAppThreads + tid) / per < 32) {
+                    const float x[4] = {to_f(w[i].t[0]), to_f(w[i].t[1]), to_f(w[i].t[2]), to_f(w[i].t[3])};
+                    bc[i * kAppThreads + tid] = s > 0.f ? quantise4(x, s, inv) : 0u;
+                }
+            if (tid == 0) scales[b] = s;
+            if (blockIdx.x > 0 || b == b1) break;
+            b = b1;
+            known = false;
+            continue;
+        }
         Vec4<T> w[P];
         int row[P];
         // the new rows' loads alone first, all in flight together
@@ -173,8 +222,7 @@ __global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_co
         }
         const float before = old && !known ? scales[b] : 0.f;
         float x[P][4];
-        float m = 0.f;
-        bool bad = false;
+        unsigned m = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int p = i * kAppThreads + tid;
@@ -184,24 +232,14 @@ __global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_co
             } else if (row[i] < old && known) {
                 const float4 v = *reinterpret_cast<const float4*>(keep + 4 * p);
                 x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+            } else if (row[i] < old) {
+                code_values(bc[p], before, x[i]);
             } else {
-                const uint32_t c = row[i] < old ? bc[p] : 0u;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] = code_value(c, e, before);
+                x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                m = fmaxf(m, fabsf(x[i][e]));
-                bad = bad || isnan(x[i][e]);
-            }
+            m = max(m, magnitude(x[i]));
         }
-        if (bad || isinf(m)) m = __int_as_float(0x7fffffff);
-        // as bit patterns: magnitudes order like their bits, and a NaN is above them all
-        const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-        if ((tid & 31) == 0) red[pass & 1][tid >> 5] = top;
-        __syncthreads();
-        const unsigned* rd = red[pass & 1];
-        const float s = block_scale(__uint_as_float(max(max(rd[0], rd[1]), max(rd[2], rd[3]))));
+        const float s = block_scale(block_top(m, red[pass & 1]));
         const float inv = __fdiv_rn(1.f, s);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -222,7 +260,7 @@ __global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_co
 using AppendKernel = void (*)(AppendArgs);
 template <typename T>
 AppendKernel append_kernel_for(int hd) {
-    return hd <= 64 ? kv8_append_kernel<T, 4> : hd <= 128 ? kv8_append_kernel<T, 8> : kv8_append_kernel<T, 16>;
+    return hd == 64 ? kv8_append_kernel<T, 64> : hd == 128 ? kv8_append_kernel<T, 128> : kv8_append_kernel<T, 0>;
 }
 
 // ---------------------------------------------------------------------------
@@ -264,12 +302,12 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const __grid_con
             const int i = i0 + u * kReadThreads;
             if (i >= total) continue;
             float* o = to + (size_t)r[u] * H * hd + (i - r[u] * per) * 4;
-            const float4 x = make_float4(code_value(q[u], 0, s[u]), code_value(q[u], 1, s[u]), code_value(q[u], 2, s[u]),
-                                         code_value(q[u], 3, s[u]));
+            float x[4];
+            code_values(q[u], s[u], x);
             if (vec) {
-                *reinterpret_cast<float4*>(o) = x;
+                *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
             } else {
-                o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
+                o[0] = x[0]; o[1] = x[1]; o[2] = x[2]; o[3] = x[3];
             }
         }
     }
@@ -441,17 +479,17 @@ struct GatherArgs {
 };
 constexpr int kGatherThreads = 128;
 
-// A CTA of four warps per new block, head and K or V; a warp has eight rows in pieces of four codes, P of them a
-// lane (P = hd / 16 rounded up to 4, 8 or 16). The largest magnitude is a row's largest code times its scale.
-template <int P>
+// A CTA of four warps per new block, head and K or V, in pieces of four codes, P a thread. The largest magnitude is
+// a row's largest code times its scale. HD as for the append.
+template <int HD, int P = HD ? HD / 16 : 16>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
-    extern __shared__ float rowbuf[];  // with rotation: the block's rows
+    extern __shared__ __align__(16) float rowbuf[];  // with rotation: the block's rows
     __shared__ unsigned red[kGatherThreads / 32];
     __shared__ int from[32];
     __shared__ float fs[32];
     pdl_wait();
     pdl_trigger();
-    const int hd = (int)a.src.head_dim, H = (int)a.src.n_kv_head, cap = (int)a.src.capacity, dcap = (int)a.dst.capacity;
+    const int hd = HD ? HD : (int)a.src.head_dim, H = (int)a.src.n_kv_head, cap = (int)a.src.capacity, dcap = (int)a.dst.capacity;
     const int b = blockIdx.x, h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
     const float* ssc = (which ? a.src.v_scale : a.src.k_scale) + (size_t)h * (cap >> 5);
     const int r_ = tid < 32 && 32 * b + tid < a.keep ? a.kept[(size_t)h * a.keep + 32 * b + tid] : -1;  // -1 behind the last
@@ -497,22 +535,23 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid
         return;
     }
     const bool turned = a.rotate && which == 0;
-    float m = 0.f;
+    unsigned m = 0;
     if (!turned) {
 #pragma unroll
         for (int i = 0; i < P; ++i)
             if (row[i] < rows) {
                 const uint32_t u = __vabs4(q[i]);  // (codes are -127 .. 127)
                 const unsigned top = max(max(u & 255, (u >> 8) & 255), max((u >> 16) & 255, u >> 24));
-                const float x = __fmul_rn((float)top, fs[row[i]]);
-                m = x != x ? __int_as_float(0x7fffffff) : __uint_as_float(max(__float_as_uint(m), __float_as_uint(x)));
+                m = max(m, __float_as_uint(__fmul_rn((float)top, fs[row[i]])));  // scales are not negative
             }
     } else {
 #pragma unroll
         for (int i = 0; i < P; ++i)
-            if (row[i] < rows)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) rowbuf[4 * (i * kGatherThreads + tid) + e] = code_value(q[i], e, fs[row[i]]);
+            if (row[i] < rows) {
+                float x[4];
+                code_values(q[i], fs[row[i]], x);
+                *reinterpret_cast<float4*>(rowbuf + 4 * (i * kGatherThreads + tid)) = make_float4(x[0], x[1], x[2], x[3]);
+            }
         __syncthreads();
         for (int i = tid; i < rows * a.pairs; i += kGatherThreads) {
             const int r = i / a.pairs, p = i - r * a.pairs;
@@ -526,25 +565,19 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid
             *v = __fmaf_rn(x0, c.y, __fmul_rn(x1, c.x));
         }
         __syncthreads();
-        bool bad = false;
-        for (int i = tid; i < rows * hd; i += kGatherThreads) {
-            m = fmaxf(m, fabsf(rowbuf[i]));
-            bad = bad || isnan(rowbuf[i]);
-        }
-        if (bad || isinf(m)) m = __int_as_float(0x7fffffff);
+        for (int i = tid; i < rows * hd; i += kGatherThreads) m = max(m, __float_as_uint(rowbuf[i]) & 0x7fffffffu);
     }
-    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    if ((tid & 31) == 0) red[tid >> 5] = top;
-    __syncthreads();
-    const float sn = block_scale(__uint_as_float(max(max(red[0], red[1]), max(red[2], red[3]))));
+    const float sn = block_scale(block_top(m, red));
     const float inv = __fdiv_rn(1.f, sn);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         if (row[i] >= rows) continue;
         const int p = i * kGatherThreads + tid;
         float x[4];
+        code_values(q[i], fs[row[i]], x);
+        if (turned)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = turned ? rowbuf[4 * p + e] : code_value(q[i], e, fs[row[i]]);
+            for (int e = 0; e < 4; ++e) x[e] = rowbuf[4 * p + e];
         dc[p] = sn > 0.f ? quantise4(x, sn, inv) : 0u;
     }
     if (tid == 0) dsc[b] = sn;
@@ -594,7 +627,7 @@ int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, floa
         rope_turns(*rope, &g.turns);
     }
     const int hd = (int)src.head_dim;
-    auto kern = hd <= 64 ? kv8_gather_kernel<4> : hd <= 128 ? kv8_gather_kernel<8> : kv8_gather_kernel<16>;
+    auto kern = hd == 64 ? kv8_gather_kernel<64> : hd == 128 ? kv8_gather_kernel<128> : kv8_gather_kernel<0>;
     return launch("kv8_gather_kernel", kern, dim3((unsigned)((keep + 31) / 32), src.n_kv_head, 2), kGatherThreads,
                   rope ? (size_t)32 * hd * sizeof(float) : 0, st, 1, g);
 }
