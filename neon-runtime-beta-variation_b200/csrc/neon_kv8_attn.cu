@@ -16,10 +16,10 @@
 namespace longctx {
 namespace {
 
-// p (at most 1, times s_v over the largest s_v so far) is multiplied by 2^14
-// before its split: hi stays below fp16's 65504, and lo keeps values down to
-// 2^-38 of the row's largest.
-constexpr float kPUp = 16384.f, kPDown = 1.f / 16384.f;
+// p (at most 2^8, times s_v over a reference that it is at most four times of)
+// is multiplied by 2^5 before its split: hi stays below fp16's 65504, and lo
+// keeps values down to 2^-30 of the row's largest.
+constexpr float kPUp = 32.f, kPDown = 1.f / 32.f;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -93,7 +93,8 @@ __device__ __forceinline__ void row_queries(const AttnArgs& a, int kvh, int grp,
     if (lane == 0) factor[g] = a.scale * pow2(-e);
 }
 
-template <int HD>
+// FULL: head_dim is HD itself, not less.
+template <int HD, bool FULL>
 __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(const __grid_constant__ AttnArgs a) {
     using R = RowTile<HD>;
     constexpr int KS = HD / 16;   // k-steps of the score product
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     float* qfac = reinterpret_cast<float*>(smem + R::kBody + R::kQuery);
     uint64_t* bars = reinterpret_cast<uint64_t*>(qfac + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
-    const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity;
+    const int hd = FULL ? HD : (int)a.c.head_dim, cap = (int)a.c.capacity;
     const int split = blockIdx.x, kvh = blockIdx.y, grp = blockIdx.z, rows = a.n * a.group;
     unsigned char* ring = smem + warp * S * R::kSlotBytes;
     uint64_t* bar = bars + warp * S;
@@ -221,23 +222,21 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
                 *reinterpret_cast<float2*>(scores + tile * 32 + 8 * j + 2 * tq) = make_float2(t[j][0], t[j][1]);
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
         mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-        const float mu = mt == -INFINITY ? 0.f : mt;
-        const float down = ex2(m - mu);
-        float vdown = 1.f;
-        if (vs > vref) {
-            vdown = vref / vs;
-            vref = vs;
-        }
-        const float vr = vs == 0.f ? 0.f : vs / vref * kPUp;
-        l *= down;
-        m = mt;
-        if (__any_sync(0xffffffffu, down * vdown != 1.f)) {
-            const float f = down * vdown;
+        // m follows when p would pass 2^8 (the result does not depend on m): O is seldom rescaled
+        const float mnew = mt > m + 8.f || m == -INFINITY ? mt : m;
+        const float mu = mnew == -INFINITY ? 0.f : mnew;
+        if (__any_sync(0xffffffffu, mnew != m || vs > 4.f * vref)) {
+            const float down = ex2(m - mu), vtop = vs > 4.f * vref ? vs : vref;
+            const float f = vtop > 0.f ? down * (vref / vtop) : down;
+            l *= down;
+            m = mnew;
+            vref = vtop;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[n][e] *= f;
         }
+        const float vr = vs == 0.f ? 0.f : vs / vref * kPUp;
         uint32_t pf[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -522,7 +521,12 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     } else {
         a.tile_keys = 32;
         if (weight) a.scores = (float*)(base + p.scores);
-        auto rows_kernel = hd <= 64 ? kv8_rows_kernel<64> : hd <= 128 ? kv8_rows_kernel<128> : kv8_rows_kernel<256>;
+        auto rows_kernel = hd == 64    ? kv8_rows_kernel<64, true>
+                           : hd < 64   ? kv8_rows_kernel<64, false>
+                           : hd == 128 ? kv8_rows_kernel<128, true>
+                           : hd < 128  ? kv8_rows_kernel<128, false>
+                           : hd == 256 ? kv8_rows_kernel<256, true>
+                                       : kv8_rows_kernel<256, false>;
         const int smem = hd <= 64 ? RowTile<64>::kSmem : hd <= 128 ? RowTile<128>::kSmem : RowTile<256>::kSmem;
         const int warps = hd <= 128 ? RowTile<128>::kWarps : RowTile<256>::kWarps;
         a.min_tiles = warps;  // a tile per warp before another CTA joins
