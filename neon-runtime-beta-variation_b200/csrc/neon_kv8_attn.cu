@@ -28,6 +28,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+constexpr int kMaxSplit = 64;
+
 // ---------------------------------------------------------------------------
 // Eight rows of one KV head over a share of the cache. The MMA's 16 rows hold
 // the eight rows' hi terms and below them their lo terms, so the split costs
@@ -50,7 +52,8 @@ struct RowTile {
     static constexpr int kSlots = HD <= 64 ? 6 : 3;
     static constexpr int kSlotBytes = 32 * HD;
     static constexpr int kRing = kWarps * kSlots * kSlotBytes;
-    static constexpr int kMerge = kWarps * 8 * (HD + 2) * 4;
+    static constexpr int kPitch = HD + 8;  // floats of a row in the merge: eight rows in different banks
+    static constexpr int kMerge = kWarps * 8 * (kPitch + 2) * 4;
     static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
     static constexpr int kQuery = HD / 16 * 512;
     static constexpr int kSmem = kBody + kQuery + 8 * 4 + kWarps * kSlots * 8;
@@ -63,7 +66,8 @@ struct RowTile {
 template <int HD>
 __device__ __forceinline__ void row_queries(const AttnArgs& a, int kvh, int grp, int g, uint4* out, float* factor) {
     const int lane = threadIdx.x & 31, hd = (int)a.c.head_dim, rows = a.n * a.group, row = grp * 8 + g;
-    const long long base = (long long)(row / a.group) * a.qs + (long long)(kvh * a.group + row % a.group) * hd;
+    const int tok = token_of(a, row);
+    const long long base = tok * a.qs + (long long)(kvh * a.group + row - tok * a.group) * hd;
     constexpr int V = (HD + 127) / 128;  // pieces of four values a lane
     float x[V][4];
     float mx = 0.f;
@@ -120,9 +124,9 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     // the keys of the group's rows, and this warp's share of them in tiles
     const int past = *a.c.past;
     const int row = grp * 8 + g;
-    const int limit = row < rows ? keys_of(past, row / a.group, cap) : 0;
+    const int limit = row < rows ? keys_of(past, token_of(a, row), cap) : 0;
     const Shares sh = shares_of(a, past, grp);
-    if (split >= sh.active) return;
+    if (!sh.has(split)) return;
     const int c0 = split * sh.per, c1 = min(c0 + sh.per, sh.tiles);
     const int per_warp = (c1 - c0 + W - 1) / W;
     const int w0 = min(c0 + warp * per_warp, c1), w1 = min(w0 + per_warp, c1);
@@ -303,15 +307,13 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();
-    float* mo = reinterpret_cast<float*>(smem);             // [warps][8][HD]
-    float* ml = mo + W * 8 * HD;                            // [warps][8][2]
+    float* mo = reinterpret_cast<float*>(smem);             // [warps][8][HD]: place 8 t + c has column c HD / 8 + t
+    float* ml = mo + W * 8 * R::kPitch;                     // [warps][8][2]
     const float up = vref * kPDown;
+    float* mine = mo + (warp * 8 + g) * R::kPitch + 2 * tq;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        float* o = mo + (warp * 8 + g) * HD;
-        o[2 * tq * (HD / 8) + t] = (acc[t][0] + acc[t][2]) * up;
-        o[(2 * tq + 1) * (HD / 8) + t] = (acc[t][1] + acc[t][3]) * up;
-    }
+    for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<float2*>(mine + 8 * t) = make_float2((acc[t][0] + acc[t][2]) * up, (acc[t][1] + acc[t][3]) * up);
     if (tq == 0) {
         ml[(warp * 8 + g) * 2] = m;
         ml[(warp * 8 + g) * 2 + 1] = l;
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     const int r = warp / PARTS, rr = grp * 8 + r;
     if (rr >= rows) return;
     // lane w has warp w's m and l
-    float2 own = lane < used ? *reinterpret_cast<const float2*>(ml + (lane * 8 + r) * 2) : make_float2(-INFINITY, 0.f);
+    const float2 own = lane < used ? *reinterpret_cast<const float2*>(ml + (lane * 8 + r) * 2) : make_float2(-INFINITY, 0.f);
     float mm = own.x;
 #pragma unroll
     for (int o = W / 2; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
@@ -338,34 +340,46 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
         const float f = __shfl_sync(0xffffffffu, fw, w);
         ll += f * __shfl_sync(0xffffffffu, own.y, w);
 #pragma unroll
-        for (int i = 0; i < D; ++i) v[i] += f * mo[(w * 8 + r) * HD + d0 + 32 * i];
+        for (int i = 0; i < D; ++i) v[i] += f * mo[(w * 8 + r) * R::kPitch + d0 + 32 * i];
     }
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
+    const int tok = token_of(a, rr);
+    const long long ob = tok * a.os + (long long)(kvh * a.group + rr - tok * a.group) * hd;
     const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
 #pragma unroll
     for (int i = 0; i < D; ++i) {
-        const int d = d0 + 32 * i;
+        const int p = d0 + 32 * i, d = (p & 7) * (HD / 8) + (p >> 3);
         if (d >= hd) continue;
-        if (sh.active == 1) o_store(a.o, a.type, ob + d, v[i] * inv);
+        if (sh.whole()) o_store(a.o, a.type, ob + d, v[i] * inv);
         else a.part_o[pr * hd + d] = v[i];
     }
     if (lane == 0 && warp % PARTS == 0) {
-        float* st = sh.active == 1 ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
-        st[0] = sh.active == 1 ? mu : mm;
-        st[1] = sh.active == 1 ? inv : ll;
+        float* st = sh.whole() ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
+        st[0] = sh.whole() ? mu : mm;
+        st[1] = sh.whole() ? inv : ll;
     }
 }
 
-// A row's final m and 1 / l from its splits (or from the only one).
+// A row's final m and 1 / l from its splits (or from the only one), by a warp.
 __device__ __forceinline__ float2 row_stats(const AttnArgs& a, int kvh, int rr, const Shares& sh) {
-    const int rows = a.n * a.group;
-    if (sh.active == 1) return *reinterpret_cast<const float2*>(a.stats + ((size_t)kvh * rows + rr) * 2);
+    const int rows = a.n * a.group, lane = threadIdx.x & 31;
+    if (sh.whole()) return *reinterpret_cast<const float2*>(a.stats + ((size_t)kvh * rows + rr) * 2);
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + ((size_t)kvh * rows + rr) * a.nsplit;
+    const int n = sh.count();
+    float2 x[kMaxSplit / 32];
     float mm = -INFINITY, ll = 0.f;
-    for (int s = 0; s < sh.active; ++s) mm = fmaxf(mm, ml[s].x);
+#pragma unroll
+    for (int i = 0; i < kMaxSplit / 32; ++i) {
+        x[i] = lane + 32 * i < n ? ml[lane + 32 * i] : make_float2(-INFINITY, 0.f);
+        mm = fmaxf(mm, x[i].x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
     const float mu = mm == -INFINITY ? 0.f : mm;
-    for (int s = 0; s < sh.active; ++s) ll += ex2(ml[s].x - mu) * ml[s].y;
+#pragma unroll
+    for (int i = 0; i < kMaxSplit / 32; ++i) ll += ex2(x[i].x - mu) * x[i].y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
     return make_float2(mu, ll == 0.f ? 0.f : 1.f / ll);
 }
 
@@ -373,7 +387,6 @@ __device__ __forceinline__ float2 row_stats(const AttnArgs& a, int kvh, int rr, 
 // others, with weights kept and few rows, add up the rows' weights from the stored scores (1024 keys a CTA).
 __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ AttnArgs a, int joins) {
     __shared__ float2 st[kPromptRows];
-    __shared__ int lim[kPromptRows];
     pdl_wait();
     pdl_trigger();
     const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, rows = a.n * a.group;
@@ -382,17 +395,18 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
         const int rr = blockIdx.x * 8 + (threadIdx.x >> 5);
         if (rr >= rows) return;
         const Shares sh = shares_of(a, past, rr / a.unit);
-        if (sh.active == 1) return;
+        if (sh.whole()) return;
         const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit;
         const float *ml = a.part_ml + pr * 2, *po = a.part_o + pr * hd;
+        const int n = sh.count();
         float mm = -INFINITY;
-        for (int s = lane; s < sh.active; s += 32) mm = fmaxf(mm, ml[2 * s]);
+        for (int s = lane; s < n; s += 32) mm = fmaxf(mm, ml[2 * s]);
 #pragma unroll
         for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
         const float mu = mm == -INFINITY ? 0.f : mm;
         float ll = 0.f, v[8] = {};
 #pragma unroll 4
-        for (int s = 0; s < sh.active; ++s) {
+        for (int s = 0; s < n; ++s) {
             const float f = ex2(ml[2 * s] - mu);
             ll += f * ml[2 * s + 1];
 #pragma unroll
@@ -400,7 +414,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
                 if (lane + 32 * i < hd) v[i] += f * po[(size_t)s * hd + lane + 32 * i];
         }
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
+        const int tok = token_of(a, rr);
+        const long long ob = tok * a.os + (long long)(kvh * a.group + rr - tok * a.group) * hd;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (lane + 32 * i < hd) o_store(a.o, a.type, ob + lane + 32 * i, v[i] * inv);
@@ -414,33 +429,40 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
     const int keys = keys_of(past, a.n - 1, cap);
     const int key = ((int)blockIdx.x - joins) * 1024 + (int)threadIdx.x * 4;
     if (((int)blockIdx.x - joins) * 1024 >= keys) return;
-    if ((int)threadIdx.x < rows) {
-        st[threadIdx.x] = row_stats(a, kvh, (int)threadIdx.x, shares_of(a, past, (int)threadIdx.x / a.unit));
-        lim[threadIdx.x] = keys_of(past, (int)threadIdx.x / a.group, cap);
-    }
-    __syncthreads();
-    if (key >= keys) return;
     const int nz = (rows + 7) / 8;
     const float* t = a.scores + (size_t)kvh * nz * 8 * cap + key;
     float sum[4] = {};
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-        // a row that sees none of the four keys may not have stored them
-        if (key >= lim[r]) continue;
-        const float4 x = *reinterpret_cast<const float4*>(t + (size_t)r * cap);
-        const float mr = st[r].x, ir = st[r].y;
-        sum[0] += ex2(x.x - mr) * ir;
-        sum[1] += ex2(x.y - mr) * ir;
-        sum[2] += ex2(x.z - mr) * ir;
-        sum[3] += ex2(x.w - mr) * ir;
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+        float4 x[8];  // loaded before the statistics that they wait for
+#pragma unroll
+        for (int r = 0; r < 8; ++r)  // a row that sees none of the four keys may not have stored them
+            x[r] = r0 + r < rows && key < keys_of(past, token_of(a, r0 + r), cap)
+                       ? *reinterpret_cast<const float4*>(t + (size_t)(r0 + r) * cap)
+                       : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (r0 == 0) {
+            for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+                const float2 y = row_stats(a, kvh, r, shares_of(a, past, r / a.unit));
+                if (lane == 0) st[r] = y;
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (r0 + r >= rows) continue;
+            const float mr = st[r0 + r].x, ir = st[r0 + r].y;
+            const float v[4] = {x[r].x, x[r].y, x[r].z, x[r].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // (a row that is not a number spoils the keys that it sees, no others)
+                if (v[e] != -INFINITY) sum[e] += ex2(v[e] - mr) * ir;
+        }
     }
+    if (key >= keys) return;
     float* w = a.weight + (size_t)kvh * cap + key;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (key + e < keys) w[e] = key + e < past ? w[e] + sum[e] : sum[e];
 }
 
-constexpr int kMaxSplit = 64;
 
 // The plan of a call, from what the host knows of it (not how many rows the cache holds).
 struct Plan {
@@ -515,11 +537,11 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     const int hd = (int)c.head_dim;
     int rc;
     if (p.prompt) {
-        a.tile_keys = prompt_tile_keys();
+        a.tile_shift = prompt_tile_shift();
         a.min_tiles = 8;
         rc = launch_prompt(a, st);
     } else {
-        a.tile_keys = 32;
+        a.tile_shift = 5;
         if (weight) a.scores = (float*)(base + p.scores);
         auto rows_kernel = hd == 64    ? kv8_rows_kernel<64, true>
                            : hd < 64   ? kv8_rows_kernel<64, false>

@@ -64,8 +64,8 @@ struct AttnArgs {
     float* weight;
     int nsplit;      // shares of a unit's keys at most
     int unit;        // rows of a CTA of the main kernel (8, or a prompt unit)
-    int min_tiles;   // tiles of 32 (of a prompt: of its key tile) before another CTA joins
-    int tile_keys;
+    int min_tiles;   // tiles before another CTA joins
+    int tile_shift;  // log2 of a tile's keys
     float* stats;    // [H][rows][2]: a row's final m and 1 / l (0 for a row without keys)
     float* part_o;   // [H][rows][nsplit][hd]: o of a split, not normalised, in units of
     float* part_ml;  // [H][rows][nsplit][2]: 2^m with m, and l
@@ -76,17 +76,21 @@ struct AttnArgs {
     unsigned* err;
 };
 
-// How the keys of a unit of rows are shared out: `per` tiles a CTA, `active` CTAs.
+// How the keys of a unit of rows are shared out: `per` tiles a CTA, as many CTAs as that takes (split * per < tiles;
+// one at least). Few divisions: they are a good part of a short call.
 struct Shares {
-    int tiles, per, active;
+    int tiles, per;
+    __device__ __forceinline__ bool whole() const { return per >= tiles; }
+    __device__ __forceinline__ bool has(int split) const { return split == 0 || split * per < tiles; }
+    __device__ __forceinline__ int count() const { return whole() ? 1 : (tiles + per - 1) / per; }
 };
+__device__ __forceinline__ int token_of(const AttnArgs& a, int row) { return a.n == 1 ? 0 : row / a.group; }
 __device__ __forceinline__ Shares shares_of(const AttnArgs& a, int past, int unit) {
     const int rows = a.n * a.group;
-    const int last = min(unit * a.unit + a.unit - 1, rows - 1) / a.group;
+    const int last = token_of(a, min(unit * a.unit + a.unit - 1, rows - 1));
     Shares s;
-    s.tiles = (keys_of(past, last, (int)a.c.capacity) + a.tile_keys - 1) / a.tile_keys;
-    s.per = max((s.tiles + a.nsplit - 1) / a.nsplit, min(s.tiles, a.min_tiles));
-    s.active = s.per ? (s.tiles + s.per - 1) / s.per : 1;
+    s.tiles = (keys_of(past, last, (int)a.c.capacity) + (1 << a.tile_shift) - 1) >> a.tile_shift;
+    s.per = a.nsplit == 1 ? s.tiles : max((s.tiles + a.nsplit - 1) / a.nsplit, min(s.tiles, a.min_tiles));
     return s;
 }
 
@@ -97,7 +101,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Prompts (neon_kv8_prompt.cu): bytes of the query tiles, and the launches.
 size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type);
 int prompt_unit(int hd);
-int prompt_tile_keys();
+int prompt_tile_shift();
 int launch_prompt(const AttnArgs& a, cudaStream_t st);
 int launch_prompt_weights(const AttnArgs& a, cudaStream_t st);  // after launch_prompt and its joins
 

@@ -35,7 +35,7 @@ namespace {
 // Warps 0-7 softmax, 8-13 conversion, 14 and 15 the products, one per query tile.
 constexpr int kSoftWarps = 8, kConvWarps = 6, kMmaWarp = 14;
 constexpr int kThreads = 512;
-constexpr int kTileKeys = 64;
+constexpr int kTileShift = 6, kTileKeys = 1 << kTileShift;
 constexpr float kMostP = 256.f;  // 2^8: how far p may exceed 1
 constexpr float kPScale = 32.f;  // 2^5
 
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         // ---- softmax: one thread per row ----
         const int m = warp >> 2;
         const int r0 = (unit * MT + m) * 128, rr = r0 + (warp & 3) * 32 + lane;
-        if (m < MT && (split < sh.active || split == 0)) {
+        if (m < MT && (sh.has(split))) {
             const bool on = rr < rows;
             const int limit = on ? keys_of(past, rr / a.group, cap) : 0;
             const float factor = put_queries<PANELS, TERMS, T>(a, kvh, r0, (warp & 3) * 32, qs + m * S::QTile);
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // ---- the row's output, or its part ----
             if (n && alive) alive = __all_sync(0xffffffffu, wait_or(&bar->o_full[m], 0, &bar->dead, a.err));
             tc_after();
-            const bool whole = sh.active == 1, out = on && split < sh.active;
+            const bool whole = sh.whole(), out = on;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale);
             const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
@@ -910,7 +910,7 @@ int launch_shape(const AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 int prompt_unit(int hd) { return hd <= 128 ? 256 : 128; }
-int prompt_tile_keys() { return kTileKeys; }
+int prompt_tile_shift() { return kTileShift; }
 
 size_t prompt_query_bytes(const neon_kv8_t& c, size_t rows, int type) {
     const size_t tiles = (rows + 255) / 256 * 2, panels = (c.head_dim + 63) / 64;

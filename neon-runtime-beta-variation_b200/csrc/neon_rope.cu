@@ -6,8 +6,7 @@
 // Each value is read and written once, so memory bounds it. A CTA takes some
 // heads of some positions: it first puts the positions' cos and sin into
 // shared memory (once for all heads; the 64-bit reduction of the angle is the
-// costly part), then streams the heads in 16-byte pieces, four loads in
-// flight per thread.
+// costly part), then streams the heads in 16-byte pieces.
 #include "neon_longctx.cuh"
 
 #include <algorithm>
@@ -44,10 +43,13 @@ void rope_turns(const neon_rope_t& r, RopeTurns* t) {
         lo = std::max(0.0, std::floor(at(r.beta_fast)));
         hi = std::min((double)r.n_dims - 1, std::ceil(at(r.beta_slow)));
     }
-    for (uint32_t i = 0; i < 128; ++i) {
+    // the powers by products in 80 bits (64 of them lose 2^-58): a pow for each would be half of a short call
+    const long double step = powl((long double)r.base, -2.0L / den);
+    long double power = 1;
+    for (uint32_t i = 0; i < 128; ++i, power *= step) {
         t->f[i] = 0;
         if (i >= r.n_dims / 2) continue;
-        double f = std::pow(r.base, -2.0 * i / den);
+        double f = (double)power;
         if (r.factors) f /= r.factors[i];
         double own = 0;
         if (r.yarn > 0)
@@ -79,7 +81,7 @@ struct RopeArgs {
 // layout V values of the first half with their partners, and after those the
 // V-value pieces that are copied.
 template <typename T, int V, bool HALF>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
     extern __shared__ float2 cs[];
     pdl_wait();
     pdl_trigger();
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     int v = threadIdx.x % per, h = threadIdx.x / per, t = h / nh;
     h -= t * nh;
     const int dv = kThreads % per, dh = kThreads / per;
-    constexpr int U = 4;
+    constexpr int U = 2;
     for (int i = threadIdx.x; i < total; i += U * kThreads) {
         alignas(16) T lo[U][V], hi[U][V];
         T *dst[U];
@@ -246,10 +248,10 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
     a.back = backward != 0;
     a.mag = (float)rope->magnitude;
     rope_turns(*rope, &a.turns);
-    // Pieces per CTA: enough CTAs for four on every SM, one to eight pieces per thread.
+    // Pieces per CTA: one to four a thread, so that CTAs in their table and CTAs in their heads share the SMs.
     const int V1 = vec ? (int)V : half ? 1 : 2;
     const long long per = half ? (a.hd - a.pairs) / V1 : a.hd / V1, row = per * (long long)heads;
-    const long long want = std::min<long long>(std::max<long long>((long long)n * row / (sms * 4), kThreads), 8 * kThreads);
+    const long long want = std::min<long long>(std::max<long long>((long long)n * row / (sms * 4), kThreads), 4 * kThreads);
     a.tile = (int)std::min<long long>({std::max<long long>(1, want / row), (long long)kMaxTile, (long long)n});
     a.heads = row <= want ? (int)heads : (int)std::max<long long>(std::min<long long>(want / per, (long long)heads), 1);
     if (heads > 65535 && a.heads == 1) a.heads = (int)((heads + 65534) / 65535);

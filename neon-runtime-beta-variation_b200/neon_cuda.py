@@ -136,10 +136,6 @@ class _Rope(C.Structure):
         ("factors", C.POINTER(C.c_float))]
 
 
-class _RopeTarget(C.Structure):
-    _fields_ = [("X", _vp), ("Y", _vp), ("x_stride", _sz), ("y_stride", _sz), ("n_heads", _sz)]
-
-
 class _Kv8(C.Structure):
     _fields_ = [(f, C.c_uint32) for f in ("n_kv_head", "head_dim", "capacity")] + [
         (f, _vp) for f in ("k", "v", "k_scale", "v_scale", "tail", "tail_block", "past")]
@@ -156,6 +152,8 @@ _lock = threading.Lock()
 def load(path: str | None = None) -> C.CDLL:
     """Load libneon_cuda.so (building it first if it is missing)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -196,7 +194,7 @@ def load(path: str | None = None) -> C.CDLL:
         L.neon_cuda_set_attn_rows.argtypes = [C.c_int, C.c_int]
         L.neon_cuda_set_attn_head_split.argtypes = [C.c_int]
         L.neon_cuda_matvec_q4_0_noalloc.argtypes = [_vp, _vp, _sz, _vp, _sz, _sz, _vp]
-        L.neon_cuda_rope.argtypes = [C.POINTER(_Rope), C.c_int, _vp, _sz, _sz, C.POINTER(_RopeTarget), _sz, C.c_int, _vp]
+        L.neon_cuda_rope.argtypes = [C.POINTER(_Rope), C.c_int, _vp, _sz, _sz, C.c_char_p, _sz, C.c_int, _vp]
         L.neon_cuda_kv8_append.argtypes = [C.POINTER(_Kv8), _vp, _sz, _vp, _sz, _sz, C.c_int, _vp]
         L.neon_cuda_kv8_read.argtypes = [C.POINTER(_Kv8), _sz, _sz, _vp, _vp, _vp]
         L.neon_cuda_kv8_attention.argtypes = [C.POINTER(_Kv8), _vp, _sz, _vp, _sz, _sz, _sz, C.c_float, C.c_int, _vp,
@@ -309,6 +307,10 @@ def sync(stream: int = 0) -> None:
 
 def _ptr(a) -> int:
     """Address of a numpy array, a torch tensor or an int."""
+    try:
+        return a.data_ptr()  # a torch tensor, the usual case of a short call
+    except AttributeError:
+        pass
     if a is None:
         return 0
     if isinstance(a, int):
@@ -445,6 +447,7 @@ class Rope:
         self._c = _Rope(int(n_dims), ROPE_HALF if half else ROPE_INTERLEAVED, int(freq_dim), int(orig_ctx), float(base),
                         float(scale), float(yarn), float(beta_fast), float(beta_slow), float(magnitude),
                         None if self._factors is None else self._factors.ctypes.data_as(C.POINTER(C.c_float)))
+        self._ref = C.byref(self._c)
 
 
 def rope(spec: Rope, pos, n: int, head_dim: int, targets, type: int = GGML_F32, backward: bool = False,
@@ -453,12 +456,12 @@ def rope(spec: Rope, pos, n: int, head_dim: int, targets, type: int = GGML_F32, 
     targets are (X, Y, n_heads) or (X, Y, n_heads, x_stride, y_stride), device
     buffers of ``type``; Y may be X. ``backward`` rotates the other way: the
     gradient with respect to X."""
-    arr = (_RopeTarget * len(targets))()
-    for a, t in zip(arr, targets):
-        row = int(t[2]) * head_dim
-        a.X, a.Y, a.n_heads = _ptr(t[0]), _ptr(t[1]), int(t[2])
-        a.x_stride, a.y_stride = (int(t[3]), int(t[4])) if len(t) > 3 else (row, row)
-    _check(load().neon_cuda_rope(C.byref(spec._c), int(type), _ptr(pos), n, head_dim, arr, len(targets),
+    flat = []  # neon_rope_target_t: X, Y, x_stride, y_stride, n_heads
+    for t in targets:
+        row = t[2] * head_dim
+        flat += [_ptr(t[0]), _ptr(t[1]), *(t[3:5] if len(t) > 3 else (row, row)), t[2]]
+    arr = struct.pack("%dQ" % len(flat), *flat)
+    _check(load().neon_cuda_rope(spec._ref, int(type), _ptr(pos), n, head_dim, arr, len(targets),
                                  1 if backward else 0, _vp(_stream(stream))))
 
 
@@ -475,6 +478,7 @@ class Kv8Cache:
         self.tail, self.tail_block, self.past = tail, tail_block, past
         self._c = _Kv8(self.n_kv_head, self.head_dim, self.capacity,
                        *[_ptr(b) for b in (k, v, k_scale, v_scale, tail, tail_block, past)])
+        self._ref = C.byref(self._c)
 
     @classmethod
     def empty(cls, n_kv_head: int, head_dim: int, capacity: int, device="cuda") -> "Kv8Cache":
@@ -496,17 +500,17 @@ class Kv8Cache:
                stream=None) -> None:
         """K and V rows of n new tokens to rows past .. past + n - 1 (past itself is left)."""
         row = self.n_kv_head * self.head_dim
-        _check(load().neon_cuda_kv8_append(C.byref(self._c), _ptr(K), row if k_stride is None else k_stride, _ptr(V),
+        _check(load().neon_cuda_kv8_append(self._ref, _ptr(K), row if k_stride is None else k_stride, _ptr(V),
                                            row if v_stride is None else v_stride, n, int(type), _vp(_stream(stream))))
 
     def read(self, row0: int, n: int, k_out, v_out, stream=None) -> None:
         """Rows [row0, row0 + n) as fp32 values [n][n_kv_head][head_dim] (an output may be None)."""
-        _check(load().neon_cuda_kv8_read(C.byref(self._c), row0, n, _ptr(k_out), _ptr(v_out), _vp(_stream(stream))))
+        _check(load().neon_cuda_kv8_read(self._ref, row0, n, _ptr(k_out), _ptr(v_out), _vp(_stream(stream))))
 
     def attention_workspace(self, n_head: int, n: int) -> int:
         """Bytes of workspace that attention() of up to n tokens needs."""
         b = _sz()
-        _check(load().neon_cuda_kv8_attention_workspace(C.byref(self._c), n, n_head, C.byref(b)))
+        _check(load().neon_cuda_kv8_attention_workspace(self._ref, n, n_head, C.byref(b)))
         return b.value
 
     def attention(self, Q, O, n: int, n_head: int, workspace, type: int = GGML_F32, scale: float = 0.0, weight=None,
@@ -518,7 +522,7 @@ class Kv8Cache:
         row = n_head * self.head_dim
         if workspace_bytes is None:
             workspace_bytes = workspace.nbytes
-        _check(load().neon_cuda_kv8_attention(C.byref(self._c), _ptr(Q), row if q_stride is None else q_stride, _ptr(O),
+        _check(load().neon_cuda_kv8_attention(self._ref, _ptr(Q), row if q_stride is None else q_stride, _ptr(O),
                                               row if o_stride is None else o_stride, n, n_head, scale, int(type),
                                               _ptr(weight), _ptr(workspace), workspace_bytes, _vp(_stream(stream))))
 
@@ -528,8 +532,8 @@ class Kv8Cache:
         others, those of the largest accumulated weight, keep rows in all; kept
         [n_kv_head][keep] int32 says which. With ``rope`` the K rows that move are
         rotated by their new row minus their old."""
-        _check(load().neon_cuda_kv8_evict(C.byref(self._c), _ptr(weight), C.byref(dst._c), _ptr(dst_weight), keep, sink,
-                                          recent, None if rope is None else C.byref(rope._c), _ptr(kept),
+        _check(load().neon_cuda_kv8_evict(self._ref, _ptr(weight), dst._ref, _ptr(dst_weight), keep, sink,
+                                          recent, None if rope is None else rope._ref, _ptr(kept),
                                           _vp(_stream(stream))))
 
 

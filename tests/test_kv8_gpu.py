@@ -322,7 +322,10 @@ def test_not_finite_stays_in_its_rows(n):
     d.append(torch.nan_to_num(k, nan=1.0).cuda(), v.cuda(), past + n)
     c.past.fill_(past)
     d.past.fill_(past)
-    o, ref = attend(c, q.cuda(), "f32"), attend(d, clean.cuda(), "f32")
+    w = torch.zeros(H, 224, device="cuda")
+    o, ref = attend(c, q.cuda(), "f32", weight=w), attend(d, clean.cuda(), "f32")
+    # a weight is not a number where such a query sees the row: those of tokens 1 and 2 see up to row past + 2
+    assert torch.isnan(w[0, :past + 3]).all() and torch.isfinite(w[0, past + 3:]).all() and torch.isnan(w[1, :past + n]).all()
     assert torch.isnan(o[:, 2:]).all()            # KV head 1: every token sees block 1
     assert torch.isnan(o[1, 0]).all() and torch.isnan(o[2, 1]).all()
     fine = torch.ones(n, 2, dtype=torch.bool, device="cuda")

@@ -1,6 +1,7 @@
 """The long-context operators' argument checks, on a host without a GPU: each
 refusal has its code and message and comes before any device use."""
 import ctypes as C
+import struct
 
 import numpy as np
 import pytest
@@ -18,7 +19,7 @@ def err():
 def rope_call(spec=None, type=0, pos=P, n=4, dim=64, targets=None, nt=None, **kw):
     s = N.Rope(64, **kw)._c if spec is None else spec
     t = [(P, 1 << 30, 256, 256, 4)] if targets is None else targets
-    arr = (N._RopeTarget * max(1, len(t)))(*[N._RopeTarget(*v) for v in t])
+    arr = struct.pack("%dQ" % (5 * len(t)), *[x or 0 for v in t for x in v])
     return N.load().neon_cuda_rope(C.byref(s), type, pos, n, dim, arr, len(t) if nt is None else nt, 0, None)
 
 
