@@ -357,6 +357,16 @@ typedef struct neon_model* neon_model_t;
  * + KVCache (NEON-3.cpp:535-564). */
 NEON_API int neon_cuda_model_create(const neon_model_config_t* cfg, neon_model_t* out);
 
+/* A decoder whose KV cache is held in 8 bits (neon_kv8_t per layer: a quarter
+ * of the fp32 cache's bytes; ctx_len up to 131072). `comm` as for
+ * neon_cuda_model_create_tp, or NULL. With keep_weights the accumulated
+ * attention weight of every cached row is kept for neon_cuda_model_kv_evict
+ * (queries that are rewound later, or lie behind the end token of a generate,
+ * have counted). Everything else is as for neon_cuda_model_create; read_kv
+ * gives the values that the codes stand for. */
+NEON_API int neon_cuda_model_create_kv8(const neon_model_config_t* cfg, struct neon_comm* comm, int keep_weights,
+                                        neon_model_t* out);
+
 /* Upload one tensor (GGUF bytes; ne1 = 0 for a 1-D norm weight). Projection,
  * embedding and lm_head tensors may be any NEON_GGML_* type above (ffn_gate
  * and ffn_up of one layer share theirs). A norm weight may be any of them too
@@ -399,6 +409,14 @@ NEON_API int neon_cuda_model_set_length(neon_model_t m, size_t length);
  * positions and both K and V moved down; length shrinks by discard. A no-op
  * when discard is 0 or the cache holds no more than keep+discard positions. */
 NEON_API int neon_cuda_model_kv_shift(neon_model_t m, size_t keep, size_t discard);
+
+/* Make room by accumulated attention weight instead (a model made with
+ * keep_weights): in each layer and KV head the first `sink` rows, the last
+ * `recent` and, of the others, those of the largest weight stay, `keep` in
+ * all; K rows are rotated to their new positions as kv_shift does, and length
+ * becomes `keep`. A no-op when the cache holds no more than `keep`. See
+ * neon_cuda_kv8_evict. */
+NEON_API int neon_cuda_model_kv_evict(neon_model_t m, size_t keep, size_t sink, size_t recent);
 
 /* Copy the K and V rows of `layer` for positions [0, n) to the host
  * (n x n_kv_head*head_dim floats each). */

@@ -27,6 +27,7 @@
 #include "neon_cuda.h"
 #include "neon_internal.h"
 #include "neon_attn_layout.h"
+#include "neon_kv8.h"
 
 namespace neon {
 // epilogue kinds of the one-position matvec kernel (see neon_kernels.cuh)
@@ -54,6 +55,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxChunk = 256;      // positions per forward chunk (prefill)
 constexpr int kMaxCtx = 16384;      // attention scores live in shared memory
+constexpr int kMaxCtxKv8 = 131072;  // with the KV cache in 8 bits (the RoPE table has a row per position)
 
 // neon_cuda_set_attn_rows: the decode attention's cache rows per CTA at
 // least (read when a step is launched), and the share of ctx_len per CTA the
@@ -557,11 +559,11 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_kernel(const float* __restri
 
 // RoPE on q and k of position pos = *d_pos + blockIdx.x (fwd::rope_apply,
 // rawllm_forward.hpp:767-782, with the reference's cos/sin from `cs`), then
-// K/V cache rows at pos (transformer_forward :1104-1107).
-__global__ void rope_kv_kernel(float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+// K/V cache rows at pos (transformer_forward :1104-1107). Without a cache of
+// floats (Kc null) k is rotated where it is, and v left.
+__global__ void rope_kv_kernel(float* __restrict__ q, float* k, const float* __restrict__ v,
                                const float2* __restrict__ cs, const int* __restrict__ d_pos, int n_head, int n_kv,
-                               int hd, int rope_half, int q_dim, int kv_dim, float* __restrict__ Kc,
-                               float* __restrict__ Vc) {
+                               int hd, int rope_half, int q_dim, int kv_dim, float* Kc, float* __restrict__ Vc) {
     const int t = blockIdx.x;
     const int pos = *d_pos + t;
     const int half = hd / 2;
@@ -578,7 +580,7 @@ __global__ void rope_kv_kernel(float* __restrict__ q, const float* __restrict__ 
         }
     }
     const float* kt = k + (long long)t * kv_dim;
-    float* kc = Kc + (long long)pos * kv_dim;
+    float* kc = Kc ? Kc + (long long)pos * kv_dim : k + (long long)t * kv_dim;
     for (int idx = threadIdx.x; idx < n_kv * half; idx += blockDim.x) {
         const int h = idx / half, i = idx % half;
         const float x0 = kt[h * hd + 2 * i], x1 = kt[h * hd + 2 * i + 1];
@@ -591,6 +593,7 @@ __global__ void rope_kv_kernel(float* __restrict__ q, const float* __restrict__ 
             kc[h * hd + 2 * i + 1] = x1;
         }
     }
+    if (!Kc) return;
     const float* vt = v + (long long)t * kv_dim;
     float* vc = Vc + (long long)pos * kv_dim;
     for (int j = threadIdx.x; j < kv_dim; j += blockDim.x) vc[j] = vt[j];
@@ -1193,6 +1196,18 @@ struct neon_model {
     };
     std::vector<Layer> layers;
     float *K = nullptr, *V = nullptr;   // [layer][ctx][kv_dim]
+    // neon_cuda_model_create_kv8: the caches in 8 bits instead, one per layer; with weights kept,
+    // [layer][n_kv_l][kv8_cap] of them; a spare cache for eviction and shifts
+    bool kv8 = false;
+    size_t kv8_cap = 0;
+    std::vector<neon_kv8_t> kv8_layers;
+    float* kv8_weight = nullptr;
+    void* kv8_ws = nullptr;
+    neon_kv8_t kv8_spare{};
+    float* kv8_spare_weight = nullptr;
+    int32_t* kv8_kept = nullptr;
+    int* kv8_one = nullptr;  // the spare cache's length
+    float* kv8_read = nullptr;  // rows read as floats
     float2* rope_cs = nullptr;          // [ctx][rope_half]
     float *h = nullptr, *xn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *att = nullptr;
     float *gu = nullptr, *act = nullptr, *logits = nullptr;
@@ -1461,6 +1476,81 @@ int launch_attn_decode(neon_model* m, uint32_t li) {
     return neon_internal::launched(1);
 }
 
+// The new rows of `seq` positions (in k and v) into layer li's cache in 8
+// bits, then the attention of their queries over it.
+int kv8_layer(neon_model* m, uint32_t li, int seq) {
+    const neon_kv8_t& c = m->kv8_layers[li];
+    int rc = longctx::kv8_append(c, m->k, m->kv_dim, m->v, m->kv_dim, (size_t)seq, NEON_GGML_F32, m->device, m->stream);
+    if (rc) return rc;
+    float* w = m->kv8_weight ? m->kv8_weight + (size_t)li * m->n_kv_l * m->kv8_cap : nullptr;
+    return longctx::kv8_attention(c, m->q, m->q_dim, m->att, m->q_dim, (size_t)seq, m->n_head_l,
+                                  1.0f / std::sqrt((float)m->cfg.head_dim), NEON_GGML_F32, w, m->kv8_ws, m->device,
+                                  m->stream);
+}
+
+// A cache in 8 bits of the model's shape in one allocation, `past` apart.
+int kv8_alloc(neon_model* m, int32_t* past, neon_kv8_t* c) {
+    const size_t H = m->n_kv_l, hd = m->cfg.head_dim, cap = m->kv8_cap;
+    const size_t codes = H * cap * hd, scales = H * (cap / 32) * sizeof(float), tail = 4 * H * 32 * hd * sizeof(float);
+    auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+    unsigned char* p = nullptr;
+    int rc = dev_alloc(m, (void**)&p, 2 * up(codes) + 2 * up(scales) + up(tail) + up(4 * H * sizeof(int32_t)));
+    if (rc) return rc;
+    c->n_kv_head = (uint32_t)H;
+    c->head_dim = (uint32_t)hd;
+    c->capacity = (uint32_t)cap;
+    c->k = (int8_t*)p;
+    c->v = (int8_t*)(p + up(codes));
+    c->k_scale = (float*)(p + 2 * up(codes));
+    c->v_scale = (float*)(p + 2 * up(codes) + up(scales));
+    c->tail = (float*)(p + 2 * up(codes) + 2 * up(scales));
+    c->tail_block = (int32_t*)(p + 2 * up(codes) + 2 * up(scales) + up(tail));
+    c->past = past;
+    return cuda_error_if(cudaMemset(c->tail_block, 0xff, 4 * H * sizeof(int32_t)), "cudaMemset");
+}
+
+// The spare cache, made by the first eviction or shift.
+int kv8_need_spare(neon_model* m) {
+    if (m->kv8_spare.k) return NEON_OK;
+    int rc = dev_alloc(m, (void**)&m->kv8_one, sizeof(int));
+    if (!rc) rc = dev_alloc(m, (void**)&m->kv8_spare_weight, m->n_kv_l * m->kv8_cap * sizeof(float));
+    if (!rc) rc = dev_alloc(m, (void**)&m->kv8_kept, m->n_kv_l * m->kv8_cap * sizeof(int32_t));
+    neon_kv8_t c{};
+    if (!rc) rc = kv8_alloc(m, m->kv8_one, &c);
+    if (!rc) m->kv8_spare = c;
+    return rc;
+}
+
+// Layer li's first `n` rows, and their weights, from the spare cache.
+int kv8_from_spare(neon_model* m, uint32_t li, size_t n) {
+    const neon_kv8_t &d = m->kv8_layers[li], &s = m->kv8_spare;
+    const size_t H = m->n_kv_l, hd = m->cfg.head_dim, cap = m->kv8_cap, row = cap / 32 * sizeof(float),
+                 blocks = (n + 31) / 32 * sizeof(float);
+    const auto kind = cudaMemcpyDeviceToDevice;
+    DEC_TRY(cudaMemcpy2DAsync(d.k, cap * hd, s.k, cap * hd, n * hd, H, kind, m->stream));
+    DEC_TRY(cudaMemcpy2DAsync(d.v, cap * hd, s.v, cap * hd, n * hd, H, kind, m->stream));
+    DEC_TRY(cudaMemcpy2DAsync(d.k_scale, row, s.k_scale, row, blocks, H, kind, m->stream));
+    DEC_TRY(cudaMemcpy2DAsync(d.v_scale, row, s.v_scale, row, blocks, H, kind, m->stream));
+    DEC_TRY(cudaMemcpyAsync(d.tail_block, s.tail_block, 4 * H * sizeof(int32_t), kind, m->stream));
+    if (m->kv8_weight)
+        DEC_TRY(cudaMemcpy2DAsync(m->kv8_weight + (size_t)li * H * cap, cap * sizeof(float), m->kv8_spare_weight,
+                                  cap * sizeof(float), n * sizeof(float), H, kind, m->stream));
+    return NEON_OK;
+}
+
+// The rotation of the model's RoPE (rope_rotate_by_delta): pairs interleaved,
+// frequencies base^(-2i / head_dim) / scale.
+neon_rope_t kv8_rope(const neon_model* m) {
+    neon_rope_t r{};
+    r.n_dims = (uint32_t)(2 * m->rope_half);
+    r.layout = NEON_ROPE_INTERLEAVED;
+    r.freq_dim = m->cfg.head_dim;
+    r.base = m->cfg.rope_base;
+    r.scale = m->cfg.rope_scale;
+    r.magnitude = 1.0;
+    return r;
+}
+
 int rmsnorm(neon_model* m, const float* x, const float* w, float* out, int rows) {
     rmsnorm_kernel<<<rows, kThreads, 0, m->stream>>>(x, w, out, (int)m->cfg.n_embd, m->cfg.norm_eps);
     return check_launch("rmsnorm_kernel");
@@ -1493,8 +1583,8 @@ int run_layers(neon_model* m, const int* toks, int seq) {
     const size_t attn_smem = sizeof(float) * c.ctx_len;
     for (uint32_t li = 0; li < c.n_layer && !rc; ++li) {
         auto& L = m->layers[li];
-        float* Kl = m->K + (size_t)li * c.ctx_len * kv_dim;
-        float* Vl = m->V + (size_t)li * c.ctx_len * kv_dim;
+        float* Kl = m->kv8 ? nullptr : m->K + (size_t)li * c.ctx_len * kv_dim;
+        float* Vl = m->kv8 ? nullptr : m->V + (size_t)li * c.ctx_len * kv_dim;
         rc = rmsnorm(m, m->h, L.attn_norm, m->xn, seq);
         if (!rc) rc = proj(m, {{L.w[0], m->q, q_dim}, {L.w[1], m->k, kv_dim}, {L.w[2], m->v, kv_dim}}, m->xn, n_embd, seq, 0);
         if (!rc) {
@@ -1503,7 +1593,9 @@ int run_layers(neon_model* m, const int* toks, int seq) {
                                                             (int)q_dim, (int)kv_dim, Kl, Vl);
             rc = check_launch("rope_kv_kernel");
         }
-        if (!rc && (c.head_dim == 64 || c.head_dim == 128)) {
+        if (!rc && m->kv8) {
+            rc = kv8_layer(m, li, seq);
+        } else if (!rc && (c.head_dim == 64 || c.head_dim == 128)) {
             // register-tiled fp32 tiles of 64 positions per query head
             const dim3 grid((unsigned)m->n_head_l, (unsigned)((seq + kPfRows - 1) / kPfRows));
             if (c.head_dim == 128)
@@ -1585,13 +1677,15 @@ int run_step(neon_model* m) {
     };
     for (uint32_t li = 0; li < c.n_layer && !rc; ++li) {
         auto& L = m->layers[li];
-        float* Kl = m->K + (size_t)li * c.ctx_len * kv_dim;
-        float* Vl = m->V + (size_t)li * c.ctx_len * kv_dim;
+        // (with the cache in 8 bits k and v are written beside q, and appended from there)
+        float* Kl = m->kv8 ? m->k : m->K + (size_t)li * c.ctx_len * kv_dim;
+        float* Vl = m->kv8 ? m->v : m->V + (size_t)li * c.ctx_len * kv_dim;
         {
             // q, k, v = W x with x = rms_norm(h); RoPE on q and k; k and v into the cache
             const neon_proj_target_t t[3] = {{L.w[0], m->q, q_dim}, {L.w[1], Kl, kv_dim}, {L.w[2], Vl, kv_dim}};
             const int epi[3] = {neon::kEpiRope, neon::kEpiRope, neon::kEpiAtPos};
-            const long long stride[3] = {0, (long long)kv_dim, (long long)kv_dim};
+            const long long row = m->kv8 ? 0 : (long long)kv_dim;
+            const long long stride[3] = {0, row, row};
             neon_internal::MatvecExt ext;
             ext.norm_w = L.attn_norm;
             ext.norm_eps = c.norm_eps;
@@ -1603,7 +1697,7 @@ int run_step(neon_model* m) {
             ext.pos_stride = stride;
             rc = neon_internal::matvec(t, 3, hc, n_embd, 1, m->stream, 0, &ext);
         }
-        if (!rc) rc = launch_attn_decode(m, li);
+        if (!rc) rc = m->kv8 ? kv8_layer(m, li, 1) : launch_attn_decode(m, li);
         if (!rc) rc = residual(L.w[3], m->att, q_dim);
         if (!rc) {
             // act = silu(gate) * up, (gate, up) = W x with x = rms_norm(h); or silu(up)
@@ -1696,6 +1790,8 @@ int forward_device(neon_model* m, const int32_t* tokens_host, size_t n) {
     return NEON_OK;
 }
 
+int create_model(const neon_model_config_t* cfg, neon_comm_t comm, bool kv8, bool kv8_weights, neon_model_t* out);
+
 }  // namespace
 
 extern "C" {
@@ -1716,6 +1812,18 @@ int neon_cuda_model_create(const neon_model_config_t* cfg, neon_model_t* out) {
 }
 
 int neon_cuda_model_create_tp(const neon_model_config_t* cfg, neon_comm_t comm, neon_model_t* out) {
+    return create_model(cfg, comm, false, false, out);
+}
+
+int neon_cuda_model_create_kv8(const neon_model_config_t* cfg, neon_comm_t comm, int keep_weights, neon_model_t* out) {
+    return create_model(cfg, comm, true, keep_weights != 0, out);
+}
+
+}  // extern "C"
+
+namespace {
+
+int create_model(const neon_model_config_t* cfg, neon_comm_t comm, bool kv8, bool kv8_weights, neon_model_t* out) {
     if (!cfg || !out) return error(NEON_ERR_INVALID, "null argument");
     *out = nullptr;
     const auto& c = *cfg;
@@ -1726,7 +1834,8 @@ int neon_cuda_model_create_tp(const neon_model_config_t* cfg, neon_comm_t comm, 
         return error(NEON_ERR_INVALID, "NANITY: attention.head_count must be an exact multiple of attention.head_count_kv");
     if (c.head_dim % 32 != 0 || c.head_dim > 256 || c.n_embd % 32 != 0 || c.n_ff % 32 != 0)
         return error(NEON_ERR_UNSUPPORTED, "head_dim must be a multiple of 32 up to 256; n_embd and n_ff multiples of 32");
-    if (c.ctx_len > (uint32_t)kMaxCtx) return error(NEON_ERR_UNSUPPORTED, "ctx_len above 16384");
+    if (!kv8 && c.ctx_len > (uint32_t)kMaxCtx) return error(NEON_ERR_UNSUPPORTED, "ctx_len above 16384");
+    if (kv8 && c.ctx_len > (uint32_t)kMaxCtxKv8) return error(NEON_ERR_UNSUPPORTED, "ctx_len above 131072");
     if (c.n_head / c.n_kv_head > 8) return error(NEON_ERR_UNSUPPORTED, "more than 8 query heads per KV head");
     if (c.rope_dim_count > c.head_dim) return error(NEON_ERR_INVALID, "rope dimension count above head_dim");
     const int world = comm ? comm->peers.world : 1, rank = comm ? comm->peers.rank : 0;
@@ -1772,9 +1881,12 @@ int neon_cuda_model_create_tp(const neon_model_config_t* cfg, neon_comm_t comm, 
     auto A = [&](void** p, size_t bytes) {
         if (!rc) rc = dev_alloc(m, p, bytes);
     };
-    const size_t kv_bytes = sizeof(float) * (size_t)c.n_layer * c.ctx_len * m->kv_dim;
-    A((void**)&m->K, kv_bytes);
-    A((void**)&m->V, kv_bytes);
+    m->kv8 = kv8;
+    const size_t kv_bytes = kv8 ? 0 : sizeof(float) * (size_t)c.n_layer * c.ctx_len * m->kv_dim;
+    if (!kv8) {
+        A((void**)&m->K, kv_bytes);
+        A((void**)&m->V, kv_bytes);
+    }
     A((void**)&m->rope_cs, sizeof(float2) * (size_t)c.ctx_len * std::max<size_t>(1, m->rope_half));
     A((void**)&m->h, sizeof(float) * S * c.n_embd);
     A((void**)&m->xn, sizeof(float) * S * c.n_embd);
@@ -1796,7 +1908,17 @@ int neon_cuda_model_create_tp(const neon_model_config_t* cfg, neon_comm_t comm, 
     A((void**)&m->d_pos, sizeof(int));
     A((void**)&m->d_step, sizeof(int));
     A((void**)&m->d_err, sizeof(unsigned));
-    if (!rc) rc = plan_attention(m);
+    if (!rc && kv8) {
+        m->kv8_cap = ((size_t)c.ctx_len + 31) / 32 * 32;
+        m->kv8_layers.resize(c.n_layer);
+        for (auto& layer : m->kv8_layers)
+            if (!rc) rc = kv8_alloc(m, m->d_pos, &layer);
+        size_t ws = 0;
+        if (!rc) ws = longctx::kv8_attention_workspace(m->kv8_layers[0], std::min(S, m->kv8_cap), m->n_head_l);
+        A(&m->kv8_ws, ws);
+        if (kv8_weights) A((void**)&m->kv8_weight, sizeof(float) * c.n_layer * m->n_kv_l * m->kv8_cap);
+    }
+    if (!rc && !kv8) rc = plan_attention(m);
     if (!rc) rc = cudaStreamCreateWithFlags(&m->stream, cudaStreamNonBlocking) == cudaSuccess ? NEON_OK : error(NEON_ERR_CUDA, "cudaStreamCreate");
     if (!rc) rc = (cudaEventCreate(&m->ev0) == cudaSuccess && cudaEventCreate(&m->ev1) == cudaSuccess &&
                    cudaEventCreate(&m->evf0) == cudaSuccess && cudaEventCreate(&m->evf1) == cudaSuccess)
@@ -1816,14 +1938,15 @@ int neon_cuda_model_create_tp(const neon_model_config_t* cfg, neon_comm_t comm, 
             }
         }
         if (cudaMemcpy(m->rope_cs, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice) != cudaSuccess ||
-            cudaMemset(m->d_err, 0, sizeof(unsigned)) != cudaSuccess || cudaMemset(m->K, 0, kv_bytes) != cudaSuccess ||
+            cudaMemset(m->d_err, 0, sizeof(unsigned)) != cudaSuccess ||
+            (!kv8 && cudaMemset(m->K, 0, kv_bytes) != cudaSuccess) ||
             cudaMemset(m->am_key, 0, sizeof(unsigned long long)) != cudaSuccess ||
             cudaMemset(m->am_count, 0, sizeof(unsigned int)) != cudaSuccess ||
-            cudaMemset(m->V, 0, kv_bytes) != cudaSuccess)
+            (!kv8 && cudaMemset(m->V, 0, kv_bytes) != cudaSuccess))
             rc = error(NEON_ERR_CUDA, "model initialisation copies failed");
     }
-    if (!rc) rc = build_kv_maps(m);
-    if (!rc && c.ctx_len * sizeof(float) > 48 * 1024) {
+    if (!rc && !kv8) rc = build_kv_maps(m);
+    if (!rc && !kv8 && c.ctx_len * sizeof(float) > 48 * 1024) {
         if (cudaFuncSetAttribute(attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(c.ctx_len * sizeof(float))) != cudaSuccess)
             rc = error(NEON_ERR_CUDA, "cudaFuncSetAttribute(attention_kernel)");
     }
@@ -1843,6 +1966,10 @@ int neon_cuda_model_create_tp(const neon_model_config_t* cfg, neon_comm_t comm, 
     *out = m;
     return NEON_OK;
 }
+
+}  // namespace
+
+extern "C" {
 
 int neon_cuda_set_attn_head_split(int max_split) {
     if (max_split < 1 || max_split > kAttnMaxGroup || (max_split & (max_split - 1)))
@@ -2133,6 +2260,27 @@ int neon_cuda_model_kv_shift(neon_model_t m, size_t keep, size_t discard) {
     ModelDevice md(m->device);
     const auto& c = m->cfg;
     const size_t kv_dim = m->kv_dim, tail = m->length - keep - discard;
+    if (m->kv8) {  // the same rows of every head move, into the spare cache and back
+        int rc = kv8_need_spare(m);
+        if (rc) return rc;
+        const size_t left = keep + tail, H = m->n_kv_l;
+        std::vector<int32_t> kept(H * left);
+        for (size_t h = 0; h < H; ++h)
+            for (size_t i = 0; i < left; ++i) kept[h * left + i] = (int32_t)(i < keep ? i : i + discard);
+        const int len = (int)m->length;
+        DEC_TRY(cudaMemcpyAsync(m->kv8_kept, kept.data(), kept.size() * sizeof(int32_t), cudaMemcpyHostToDevice, m->stream));
+        DEC_TRY(cudaMemcpyAsync(m->d_pos, &len, sizeof(int), cudaMemcpyHostToDevice, m->stream));
+        const neon_rope_t rope = kv8_rope(m);
+        for (uint32_t li = 0; li < c.n_layer && !rc; ++li) {
+            const float* w = m->kv8_weight ? m->kv8_weight + (size_t)li * H * m->kv8_cap : nullptr;
+            rc = longctx::kv8_move(m->kv8_layers[li], w, m->kv8_spare, w ? m->kv8_spare_weight : nullptr, left,
+                                   m->rope_half ? &rope : nullptr, m->kv8_kept, m->stream);
+            if (!rc) rc = kv8_from_spare(m, li, left);
+        }
+        if (!rc) rc = cuda_error_if(cudaStreamSynchronize(m->stream), "cudaStreamSynchronize");
+        if (!rc) m->length = left;
+        return rc;
+    }
     if (!m->shift_scratch) {
         int rc = dev_alloc(m, (void**)&m->shift_scratch, sizeof(float) * (size_t)c.ctx_len * kv_dim);
         if (!rc) rc = dev_alloc(m, (void**)&m->shift_cs, sizeof(float2) * std::max<size_t>(1, m->rope_half));
@@ -2168,10 +2316,47 @@ int neon_cuda_model_kv_shift(neon_model_t m, size_t keep, size_t discard) {
     return NEON_OK;
 }
 
+int neon_cuda_model_kv_evict(neon_model_t m, size_t keep, size_t sink, size_t recent) {
+    if (!m) return error(NEON_ERR_INVALID, "null model");
+    if (!m->kv8_weight)
+        return error(NEON_ERR_INVALID, "kv_evict: the model does not keep attention weights (neon_cuda_model_create_kv8)");
+    if (keep == 0 || keep > m->cfg.ctx_len) return error(NEON_ERR_INVALID, "kv_evict: keep must be 1 to ctx_len");
+    if (sink > keep || recent > keep - sink) return error(NEON_ERR_INVALID, "kv_evict: sink + recent above keep");
+    if (m->length <= keep) return NEON_OK;
+    ModelDevice md(m->device);
+    int rc = kv8_need_spare(m);
+    if (rc) return rc;
+    const int len = (int)m->length;
+    DEC_TRY(cudaMemcpyAsync(m->d_pos, &len, sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    const neon_rope_t rope = kv8_rope(m);
+    for (uint32_t li = 0; li < m->cfg.n_layer && !rc; ++li) {
+        rc = longctx::kv8_evict(m->kv8_layers[li], m->kv8_weight + (size_t)li * m->n_kv_l * m->kv8_cap, m->kv8_spare,
+                                m->kv8_spare_weight, keep, sink, recent, m->rope_half ? &rope : nullptr, m->kv8_kept,
+                                m->stream);
+        if (!rc) rc = kv8_from_spare(m, li, keep);
+    }
+    if (!rc) rc = sync_and_check(m);
+    if (!rc) m->length = keep;
+    return rc;
+}
+
 int neon_cuda_model_read_kv(neon_model_t m, int layer, size_t n, float* k_host, float* v_host) {
     if (!m || !k_host || !v_host) return error(NEON_ERR_INVALID, "null argument");
     if (layer < 0 || (uint32_t)layer >= m->cfg.n_layer || n > m->cfg.ctx_len) return error(NEON_ERR_INVALID, "layer or n out of range");
     ModelDevice md(m->device);
+    if (m->kv8) {
+        if (n == 0) return NEON_OK;
+        if (!m->kv8_read) {
+            int rc = dev_alloc(m, (void**)&m->kv8_read, 2 * sizeof(float) * (size_t)m->cfg.ctx_len * m->kv_dim);
+            if (rc) return rc;
+        }
+        float* v = m->kv8_read + (size_t)m->cfg.ctx_len * m->kv_dim;
+        int rc = neon_cuda_kv8_read(&m->kv8_layers[layer], 0, n, m->kv8_read, v, m->stream);
+        if (rc) return rc;
+        DEC_TRY(cudaMemcpyAsync(k_host, m->kv8_read, sizeof(float) * n * m->kv_dim, cudaMemcpyDeviceToHost, m->stream));
+        DEC_TRY(cudaMemcpyAsync(v_host, v, sizeof(float) * n * m->kv_dim, cudaMemcpyDeviceToHost, m->stream));
+        return cuda_error_if(cudaStreamSynchronize(m->stream), "cudaStreamSynchronize");
+    }
     const size_t off = (size_t)layer * m->cfg.ctx_len * m->kv_dim;
     DEC_TRY(cudaMemcpy(k_host, m->K + off, sizeof(float) * n * m->kv_dim, cudaMemcpyDeviceToHost));
     DEC_TRY(cudaMemcpy(v_host, m->V + off, sizeof(float) * n * m->kv_dim, cudaMemcpyDeviceToHost));

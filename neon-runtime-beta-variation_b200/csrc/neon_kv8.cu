@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid
         from[tid] = r_;
         if (r_ >= 0) {
             fs[tid] = ssc[r_ >> 5];
-            if (which == 0) a.wd[(size_t)h * dcap + 32 * b + tid] = a.w[(size_t)h * cap + r_];
+            if (which == 0 && a.wd) a.wd[(size_t)h * dcap + 32 * b + tid] = a.w[(size_t)h * cap + r_];
         }
     }
     __syncthreads();
@@ -607,12 +607,8 @@ int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, siz
     return launch("kv8_append_kernel", kern, dim3(blocks, c.n_kv_head, 2), kAppThreads, 0, st, 1, a);
 }
 
-int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
-              size_t recent, const neon_rope_t* rope, int32_t* kept, cudaStream_t st) {
-    SelectArgs s{src.past, w, (int)src.capacity, (int)keep, (int)sink, (int)recent, kept};
-    int rc = launch("kv8_select_kernel", kv8_select_kernel, dim3(src.n_kv_head * kSelCluster), kSelThreads, 0, st,
-                    kSelCluster, s);
-    if (rc) return rc;
+int kv8_move(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, const neon_rope_t* rope,
+             const int32_t* kept, cudaStream_t st) {
     GatherArgs g{};
     g.src = src;
     g.dst = dst;
@@ -630,6 +626,14 @@ int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, floa
     auto kern = hd == 64 ? kv8_gather_kernel<64> : hd == 128 ? kv8_gather_kernel<128> : kv8_gather_kernel<0>;
     return launch("kv8_gather_kernel", kern, dim3((unsigned)((keep + 31) / 32), src.n_kv_head, 2), kGatherThreads,
                   rope ? (size_t)32 * hd * sizeof(float) : 0, st, 1, g);
+}
+
+int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
+              size_t recent, const neon_rope_t* rope, int32_t* kept, cudaStream_t st) {
+    SelectArgs s{src.past, w, (int)src.capacity, (int)keep, (int)sink, (int)recent, kept};
+    int rc = launch("kv8_select_kernel", kv8_select_kernel, dim3(src.n_kv_head * kSelCluster), kSelThreads, 0, st,
+                    kSelCluster, s);
+    return rc ? rc : kv8_move(src, w, dst, wd, keep, rope, kept, st);
 }
 
 }  // namespace longctx

@@ -17,5 +17,8 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
                   float scale, int type, float* weight, void* ws, int device, cudaStream_t st);
 int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
               size_t recent, const neon_rope_t* rope, int32_t* kept, cudaStream_t st);
+// The rows kept[n_kv_head][keep] (ascending, -1 behind the last) of src into dst; weights too unless null.
+int kv8_move(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, const neon_rope_t* rope,
+             const int32_t* kept, cudaStream_t st);
 
 }  // namespace longctx

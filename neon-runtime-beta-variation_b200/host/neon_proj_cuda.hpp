@@ -217,11 +217,16 @@ class Decoder {
 public:
     // `quantize_to` (a NEON_GGML_* type, -1 for none): float weight tensors --
     // a loader::NCTRLoader's, F32/F16 GGUF tensors -- are quantised on load to
-    // that type, as the exporters' gguf-py would have written them.
+    // that type, as the exporters' gguf-py would have written them. `kv`: the
+    // KV cache in fp32, in 8 bits, or in 8 bits with the weights that kv_evict
+    // goes by.
+    enum KvCache { kKvF32, kKv8, kKv8Weights };
     template <class ConfigT, class LoaderT>
-    Decoder(const ConfigT& cfg, const LoaderT& loader, neon_comm_t comm = nullptr, int quantize_to = -1) {
+    Decoder(const ConfigT& cfg, const LoaderT& loader, neon_comm_t comm = nullptr, int quantize_to = -1,
+            KvCache kv = kKvF32) {
         const neon_model_config_t c = model_config(cfg);
-        check(neon_cuda_model_create_tp(&c, comm, &m_));
+        if (kv == kKvF32) check(neon_cuda_model_create_tp(&c, comm, &m_));
+        else check(neon_cuda_model_create_kv8(&c, comm, kv == kKv8Weights, &m_));
         try {
             if (quantize_to >= 0) check(neon_cuda_model_set_quantize(m_, quantize_to));
             for (const auto& t : loader.tensors) {
@@ -266,6 +271,8 @@ public:
     void set_length(size_t n) { check(neon_cuda_model_set_length(m_, n)); }
     // fwd::kv_cache_shift: ensure_cache_room's slide of the window (NEON-3.cpp:590-630)
     void kv_shift(size_t keep, size_t discard) { check(neon_cuda_model_kv_shift(m_, keep, discard)); }
+    // room by accumulated attention weight (a kKv8Weights cache): neon_cuda_model_kv_evict
+    void kv_evict(size_t keep, size_t sink, size_t recent) { check(neon_cuda_model_kv_evict(m_, keep, sink, recent)); }
     neon_model_t handle() const { return m_; }
 
 private:

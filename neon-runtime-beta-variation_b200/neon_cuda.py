@@ -82,6 +82,7 @@ C_ENTRY_POINTS = (
     "neon_cuda_kv8_attention_workspace",
     "neon_cuda_kv8_evict",
     "neon_cuda_model_create",
+    "neon_cuda_model_create_kv8",
     "neon_cuda_model_set_tensor",
     "neon_cuda_model_set_quantize",
     "neon_cuda_model_forward",
@@ -89,6 +90,7 @@ C_ENTRY_POINTS = (
     "neon_cuda_model_length",
     "neon_cuda_model_set_length",
     "neon_cuda_model_kv_shift",
+    "neon_cuda_model_kv_evict",
     "neon_cuda_model_read_kv",
     "neon_cuda_model_decode_ms",
     "neon_cuda_model_forward_ms",
@@ -203,12 +205,14 @@ def load(path: str | None = None) -> C.CDLL:
         L.neon_cuda_kv8_evict.argtypes = [C.POINTER(_Kv8), _vp, C.POINTER(_Kv8), _vp, _sz, _sz, _sz, C.POINTER(_Rope),
                                           _vp, _vp]
         L.neon_cuda_model_create.argtypes = [C.POINTER(_ModelConfig), C.POINTER(_vp)]
+        L.neon_cuda_model_create_kv8.argtypes = [C.POINTER(_ModelConfig), _vp, C.c_int, C.POINTER(_vp)]
         L.neon_cuda_model_set_tensor.argtypes = [_vp, C.c_int, C.c_int, _vp, _sz, C.c_int, _sz, _sz]
         L.neon_cuda_model_forward.argtypes = [_vp, _vp, _sz, _vp]
         L.neon_cuda_model_generate.argtypes = [_vp, _vp, _sz, _sz, C.c_int32, _vp, C.POINTER(_sz)]
         L.neon_cuda_model_length.argtypes = [_vp, C.POINTER(_sz)]
         L.neon_cuda_model_set_length.argtypes = [_vp, _sz]
         L.neon_cuda_model_kv_shift.argtypes = [_vp, _sz, _sz]
+        L.neon_cuda_model_kv_evict.argtypes = [_vp, _sz, _sz, _sz]
         L.neon_cuda_model_read_kv.argtypes = [_vp, C.c_int, _sz, _vp, _vp]
         L.neon_cuda_model_decode_ms.argtypes = [_vp, C.POINTER(C.c_float)]
         L.neon_cuda_model_forward_ms.argtypes = [_vp, C.POINTER(C.c_float)]
@@ -996,16 +1000,25 @@ class Model:
     n_embd, n_layer, n_head, n_kv_head, head_dim, n_ff, ctx_len, rope_base,
     rope_scale, rope_dim_count, norm_eps); ``tensors`` yields (role, layer,
     GGUF bytes, ggml type, ne0, ne1); ``quantize`` (a GGML type) quantises
-    float matrices on load. With a connected :class:`Comm`, the
+    float matrices on load. ``kv8`` holds the KV cache in 8 bits; with
+    ``kv_weights`` it also keeps each cached row's accumulated attention
+    weight, for :meth:`kv_evict`. With a connected :class:`Comm`, the
     model is this rank's tensor-parallel share; every rank passes the WHOLE
     tensors and makes the same calls in the same order."""
 
-    def __init__(self, cfg, tensors=(), comm: Comm | None = None, quantize: int | None = None):
+    def __init__(self, cfg, tensors=(), comm: Comm | None = None, quantize: int | None = None, kv8: bool = False,
+                 kv_weights: bool = False):
         L = load()
         self.cfg = cfg
         self.comm = comm
         h = _vp()
-        _check(L.neon_cuda_model_create_tp(C.byref(_config(cfg)), comm.handle if comm else None, C.byref(h)))
+        if kv8:
+            _check(L.neon_cuda_model_create_kv8(C.byref(_config(cfg)), comm.handle if comm else None,
+                                                1 if kv_weights else 0, C.byref(h)))
+        elif kv_weights:
+            raise NeonError("Model: kv_weights needs kv8")
+        else:
+            _check(L.neon_cuda_model_create_tp(C.byref(_config(cfg)), comm.handle if comm else None, C.byref(h)))
         self.handle = h.value
         self._fin = weakref.finalize(self, L.neon_cuda_model_free, self.handle)
         if quantize is not None:
@@ -1047,6 +1060,11 @@ class Model:
     def kv_shift(self, keep: int, discard: int) -> None:
         """fwd::kv_cache_shift: forget positions [keep, keep+discard), slide the rest down."""
         _check(load().neon_cuda_model_kv_shift(self.handle, int(keep), int(discard)))
+
+    def kv_evict(self, keep: int, sink: int, recent: int) -> None:
+        """Keep `keep` rows of each head's cache: the first `sink`, the last
+        `recent`, and the others of the largest accumulated attention weight."""
+        _check(load().neon_cuda_model_kv_evict(self.handle, int(keep), int(sink), int(recent)))
 
     def read_kv(self, layer: int, n: int):
         """K and V cache rows [0, n) of `layer` (this rank's KV heads)."""
