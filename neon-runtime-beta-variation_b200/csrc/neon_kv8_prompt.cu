@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // the keys that every row of the warp sees
             const int all = __reduce_min_sync(0xffffffffu, limit);
             float mref = -INFINITY, l = 0.f, vref = 0.f;
+            float lw = 0.f, lz = 0.f;  // the sum of p's terms, and the same as the products sum it (below)
             bool alive = true;
             float nk = 0.f, nv = 0.f;  // lane b: the scales of the next tile's block b
             auto scales = [&](int j) {
@@ -383,6 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     }
                 }
                 l *= fl;
+                lw *= f;
+                lz *= f;
                 mref = mnew;
                 vref = vtop;
             };
@@ -399,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 const uint32_t sb = st + (i & 1) * KT;
                 constexpr int AT = TERMS == 1 ? NB : 1;  // blocks read at once, as registers allow
                 uint32_t hi[NB][16], lo[NB][16];
+                uint64_t hs[2 * NB], ls[2 * NB];
                 float add;
                 for (;;) {
                     const float mu = mref == -INFINITY ? 0.f : mref;
@@ -433,8 +437,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                                 if (2 * e >= c) w0 = 0.f;
                                 if (2 * e + 1 >= c) w1 = 0.f;
                             }
-                            if (TERMS == 2) split2(w0, w1, hi[b][e], lo[b][e]);
-                            else hi[b][e] = h2_bits(__floats2half2_rn(w0, w1));
+                            const __half2 h = __floats2half2_rn(w0, w1);
+                            hi[b][e] = h2_bits(h);
+                            if (TERMS == 2) {
+                                const float2 f = __half22float2(h);
+                                const float d0 = w0 - f.x, d1 = w1 - f.y;
+                                lo[b][e] = h2_bits(__floats2half2_rn(d0, d1));
+                                const int s = 2 * b + e / 8;
+                                hs[s] = e % 8 ? add2(hs[s], pair(f.x, f.y)) : pair(f.x, f.y);
+                                ls[s] = e % 8 ? add2(ls[s], pair(d0, d1)) : pair(d0, d1);
+                            }
                         }
                     }
                     float s0, s1;
@@ -447,6 +459,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     if (!__any_sync(0xffffffffu, mref != before)) break;
                 }
                 l += add;
+                if (TERMS == 2) {
+                    // The products cut each of their sums off towards zero (measured: half an ulp per 16 keys and
+                    // term, -2e-6 of an output after 512 keys). lz is cut off the same way, in the same order, and
+                    // lw / lz takes that out of the output: all of it where the values agree, most where they do not.
+                    float all = 0.f;
+#pragma unroll
+                    for (int s = 0; s < 2 * NB; ++s) {
+                        float x0, x1;
+                        unpair(hs[s], x0, x1);
+                        lz = __fadd_rz(lz, x0 + x1);
+                        all += x0 + x1;
+                    }
+#pragma unroll
+                    for (int s = 0; s < 2 * NB; ++s) {
+                        float x0, x1;
+                        unpair(ls[s], x0, x1);
+                        lz = __fadd_rz(lz, x0 + x1);
+                        all += x0 + x1;
+                    }
+                    lw += all;
+                }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {  // over the block's scores: hi in its first 16 columns, lo in the next
                     tmem_st16(sb + 32 * b, hi[b]);
@@ -486,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             tc_after();
             const bool whole = sh.whole(), out = on;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale);
+            const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale) * (TERMS == 2 && lz != 0.f ? lw / lz : 1.f);
             const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
             const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
             float* po = a.part_o + pr * hd;
@@ -599,8 +632,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 const uint32_t k = uniform(operand_lo(kb + t % ST * S::Stage, 16)), q = uniform(operand_lo(qb, 16));
                 const uint32_t d = uniform(ts + (t & 1) * KT);
                 if (elected()) {
+                    // the lo terms first: each product's sum is cut off, which then costs them nothing
                     auto step = [&](int x, int s) {
-                        mma_ss(d, operand_of(q + (x * PANELS + (s >> 2)) * 1024 + (s & 3) * 2),
+                        mma_ss(d, operand_of(q + ((TERMS - 1 - x) * PANELS + (s >> 2)) * 1024 + (s & 3) * 2),
                                operand_of(k + (s >> 2) * (KT * 8) + (s & 3) * 2), id_s, x + s > 0);
                     };
                     if (steps == PANELS * 4) {
@@ -860,14 +894,14 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
         volatile int never = 0;
         if (lane == 0) wait_or(&bar->drain, 0, &never, a.err);
     } else if (warp == kWMmaWarp + 1 && lane == 0) {
-        const unsigned char* src = a.qt + ((size_t)kvh * tiles128 + first) * TERMS * S::Stage;
+        const unsigned char* src = a.qt + ((size_t)kvh * tiles128 + first) * TERMS * S::Stage;  // (a tile's lo terms first)
         const int total = n * TERMS;
         int it = 0;
         for (; it < total; ++it) {
             const int sg = it % ST;
             if (it >= ST && !wait_or(&bar->q_empty[sg], (uint32_t)((it / ST) & 1) ^ 1, &bar->dead, a.err)) break;
             bar_expect(&bar->q_full[sg], S::Stage);
-            bulk_load(qs + sg * S::Stage, src + (size_t)it * S::Stage, S::Stage, &bar->q_full[sg]);
+            bulk_load(qs + sg * S::Stage, src + (size_t)(it / TERMS * TERMS + TERMS - 1 - it % TERMS) * S::Stage, S::Stage, &bar->q_full[sg]);
         }
         // the copies in flight end before this CTA's shared memory does
         volatile int never = 0;
