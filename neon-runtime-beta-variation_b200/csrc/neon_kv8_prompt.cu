@@ -32,9 +32,12 @@
 namespace longctx {
 namespace {
 
-// Warps 0-7 softmax, 8-13 conversion, 14 and 15 the products, one per query tile.
+// Warps 0-7 softmax, 8-13 conversion, 14 and 15 the products, one per query tile. The launch's 512 x 128
+// registers are dealt out again by warpgroup: a softmax thread holds 64 scores, their P and its sums.
 constexpr int kSoftWarps = 8, kConvWarps = 6, kMmaWarp = 14;
 constexpr int kThreads = 512;
+constexpr int kLaunchRegs = 128, kSoftRegs = 168, kOtherRegs = 88;
+static_assert(2 * kSoftRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
 constexpr int kTileShift = 6, kTileKeys = 1 << kTileShift;
 constexpr float kMostP = 256.f;  // 2^8: how far p may exceed 1
 constexpr float kPScale = 32.f;  // 2^5
@@ -320,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
     if (warp < kSoftWarps) {
         // ---- softmax: one thread per row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int m = warp >> 2;
         const int r0 = (unit * MT + m) * 128, rr = r0 + (warp & 3) * 32 + lane;
         if (m < MT && (sh.has(split))) {
@@ -564,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             tc_before();
         }
     } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));  // whole warpgroups
         if (warp < kMmaWarp) {
         // ---- conversion: codes to fp16, swizzled ----
         constexpr int kConv = kConvWarps * 32;
@@ -937,6 +942,11 @@ int launch_shape(const AttnArgs& a, cudaStream_t st) {
     PromptKernel k = kv8_prompt_kernel<PANELS, T>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
     if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_prompt_kernel)");
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, k);
+    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncGetAttributes(kv8_prompt_kernel)");
+    // the register split would wait for registers that the launch did not bring
+    if (fa.numRegs < kLaunchRegs) return neon_internal::error(NEON_ERR_UNSUPPORTED, "kv8_prompt_kernel: built with too few registers");
     const int units = (rows + 128 * S::MT - 1) / (128 * S::MT);
     return launch("kv8_prompt_kernel", k, dim3((unsigned)(units * H * a.nsplit)), kThreads, S::Smem, st, 1, a, tiles);
 }
