@@ -323,10 +323,9 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const __grid_con
 // a range of rows, and its place is a prefix sum over the warps. The second
 // gathers: one CTA per new block, head and K or V.
 
-constexpr int kSelCluster = 8;
 constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelHeld = 16;  // weights that a thread holds (131072 rows of a head); any others are read again
+constexpr int kSelHeld = 16;  // weights that a thread holds (16384 rows of a head and CTA); any others are read again
 
 // A weight as an unsigned number of the same order; every NaN is the largest.
 __device__ __forceinline__ unsigned order_bits(float w) {
@@ -352,30 +351,33 @@ struct SelectArgs {
     int* kept;       // [H][keep]
 };
 
+// CL: CTAs of a head, a cluster. One takes 1024 rows in 6 us where eight, with their barriers, take 11; eight take
+// 131071 rows in 24 us.
+template <int CL>
 __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_constant__ SelectArgs a) {
     __shared__ unsigned hist[2][256];
     __shared__ unsigned sum[256];
     __shared__ unsigned counts[2 * kSelWarps];       // rows above / equal of this CTA's warps
-    __shared__ unsigned all[2 * kSelWarps * kSelCluster];
+    __shared__ unsigned all[2 * kSelWarps * CL];
     __shared__ unsigned found[2];
     pdl_wait();
     pdl_trigger();
-    const int h = blockIdx.x / kSelCluster, rank = blockIdx.x % kSelCluster;
+    const int h = blockIdx.x / CL, rank = blockIdx.x % CL;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int len = min(max(*a.past, 0), a.cap);
     int* kept = a.kept + (size_t)h * a.keep;
     if (len <= a.keep) {  // everything stays (the whole cluster takes this path)
-        for (int i = rank * kSelThreads + tid; i < a.keep; i += kSelCluster * kSelThreads) kept[i] = i < len ? i : -1;
+        for (int i = rank * kSelThreads + tid; i < a.keep; i += CL * kSelThreads) kept[i] = i < len ? i : -1;
         return;
     }
     const float* w = a.w + (size_t)h * a.cap;
     const int lo = a.sink, hi = len - a.recent, m = a.keep - a.sink - a.recent;  // hi - lo > m >= 0
-    for (int i = rank * kSelThreads + tid; i < a.sink; i += kSelCluster * kSelThreads) kept[i] = i;
-    for (int i = rank * kSelThreads + tid; i < a.recent; i += kSelCluster * kSelThreads) kept[a.keep - a.recent + i] = hi + i;
+    for (int i = rank * kSelThreads + tid; i < a.sink; i += CL * kSelThreads) kept[i] = i;
+    for (int i = rank * kSelThreads + tid; i < a.recent; i += CL * kSelThreads) kept[a.keep - a.recent + i] = hi + i;
     if (m == 0) return;
 
     // Held weights are this warp's: rows s0 + 32 j + lane.
-    const int nw = kSelCluster * kSelWarps, gw = rank * kSelWarps + warp;
+    const int nw = CL * kSelWarps, gw = rank * kSelWarps + warp;
     const int span = ((hi - lo + nw - 1) / nw + 31) & ~31;
     const int s0 = min(lo + gw * span, hi), s1 = min(s0 + span, hi);
     unsigned held[kSelHeld];
@@ -402,12 +404,13 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         each([&](int, unsigned u, bool on) {
             if (on && (round == 0 || (u >> (shift + 8)) == prefix)) atomicAdd(&hs[(u >> shift) & 255], 1u);
         });
-        cluster_barrier();
+        if (CL > 1) cluster_barrier();
+        else __syncthreads();
         // bin 255 - tid and the bins above it, over the cluster
         if (tid < 256) {
             unsigned c = 0;
 #pragma unroll
-            for (int r = 0; r < kSelCluster; ++r) c += remote_u32(&hs[255 - tid], r);
+            for (int r = 0; r < CL; ++r) c += CL > 1 ? remote_u32(&hs[255 - tid], r) : hs[255 - tid];
             unsigned s = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -443,10 +446,11 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         counts[warp] = above;
         counts[kSelWarps + warp] = equal;
     }
-    cluster_barrier();
+    if (CL > 1) cluster_barrier();
+    else __syncthreads();
     for (int i = tid; i < 2 * nw; i += kSelThreads) {
         const int r = i / (2 * kSelWarps);
-        all[i] = remote_u32(&counts[i % (2 * kSelWarps)], r);
+        all[i] = CL > 1 ? remote_u32(&counts[i % (2 * kSelWarps)], r) : counts[i];
     }
     __syncthreads();
     unsigned before = 0, ties = 0;  // of the warps before this one
@@ -465,7 +469,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         before += __popc(bu);
         ties += __popc(be);
     });
-    cluster_barrier();  // no CTA leaves while another reads its counts
+    if (CL > 1) cluster_barrier();  // no CTA leaves while another reads its counts
 }
 
 struct GatherArgs {
@@ -631,8 +635,9 @@ int kv8_move(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float
 int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
               size_t recent, const neon_rope_t* rope, int32_t* kept, cudaStream_t st) {
     SelectArgs s{src.past, w, (int)src.capacity, (int)keep, (int)sink, (int)recent, kept};
-    int rc = launch("kv8_select_kernel", kv8_select_kernel, dim3(src.n_kv_head * kSelCluster), kSelThreads, 0, st,
-                    kSelCluster, s);
+    const bool one = src.capacity <= kSelThreads * kSelHeld;  // a CTA holds all of a head's weights
+    int rc = one ? launch("kv8_select_kernel", kv8_select_kernel<1>, dim3(src.n_kv_head), kSelThreads, 0, st, 1, s)
+                 : launch("kv8_select_kernel", kv8_select_kernel<8>, dim3(src.n_kv_head * 8), kSelThreads, 0, st, 8, s);
     return rc ? rc : kv8_move(src, w, dst, wd, keep, rope, kept, st);
 }
 

@@ -577,6 +577,7 @@ int check_heads(const neon_kv8_t* c, size_t n, size_t n_head) {
     if (n_head == 0 || n_head % c->n_kv_head) return error(NEON_ERR_INVALID, "kv8: n_head must be a multiple of n_kv_head");
     if (n_head / c->n_kv_head > 64) return error(NEON_ERR_UNSUPPORTED, "kv8: more than 64 query heads per KV head");
     if (n > c->capacity) return error(NEON_ERR_INVALID, "kv8: more tokens than the cache's capacity");
+    if (n * (n_head / c->n_kv_head) > (1u << 26)) return error(NEON_ERR_UNSUPPORTED, "kv8: more than 2^26 query rows per KV head");
     return NEON_OK;
 }
 }  // namespace

@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
     if (key0 >= keys) return;
     unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     unsigned char *ks = smem, *qs = ks + MT * S::KTile;
-    float2* stat = reinterpret_cast<float2*>(qs + ST * S::Stage);  // [2][128]: factor, m + log2 l
+    float2* stat = reinterpret_cast<float2*>(qs + ST * S::Stage);  // [2][128 queries]: factors and -(m + log2 l)
     WBars* bar = reinterpret_cast<WBars*>(stat + 256);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == kWMmaWarp) {
@@ -798,7 +798,8 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
         // the first row that sees this key, and that every key of the warp is seen by
         const long long seen = key < keys ? ((long long)key - past) * a.group : (1LL << 40);
         const long long last = max(0LL, ((long long)(key | 31) - past) * a.group);
-        float sum[4] = {};
+        const uint64_t scale2 = pair(scale, scale);
+        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
         for (int i = 0; i < n; ++i) {
             const int b = i & 1;
             const uint32_t ph = (uint32_t)((i >> 1) & 1);
@@ -813,18 +814,19 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
                 uint32_t r[32];
                 tmem_ld32(r, st + b * 128 + c);
                 tmem_wait_ld();
-                const float4* sp = reinterpret_cast<const float4*>(stat + b * 128 + c);
+                const ulonglong2* sp = reinterpret_cast<const ulonglong2*>(stat + b * 128 + c);
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                    const float4 q = sp[e / 2];
-                    float p0 = ex2(__fmaf_rn(__uint_as_float(r[e]), q.x * scale, -q.y));
-                    float p1 = ex2(__fmaf_rn(__uint_as_float(r[e + 1]), q.z * scale, -q.w));
+                    const ulonglong2 q = sp[e / 2];  // the factors of two queries, then minus their m + log2 l
+                    float p0, p1;
+                    unpair(fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), mul2(q.x, scale2), q.y), p0, p1);
+                    p0 = ex2(p0);
+                    p1 = ex2(p1);
                     if (!full) {
                         if (c + e < from) p0 = 0.f;
                         if (c + e + 1 < from) p1 = 0.f;
                     }
-                    sum[(e & 2)] += p0;
-                    sum[(e & 2) + 1] += p1;
+                    sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(p0, p1));
                 }
             }
             tc_before();
@@ -832,7 +834,9 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             if (lane == 0) bar_arrive(&bar->s_empty[b]);
         }
         if (key < keys) {
-            const float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float s0, s1;
+            unpair(add2(sum[0], sum[1]), s0, s1);
+            const float v = s0 + s1;
             float* w = a.weight + (size_t)kvh * cap + key;
             *w = key < past ? *w + v : v;
         }
@@ -857,7 +861,10 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
                 v.y = s.x - log2f(s.y);  // a row without keys: 1 / l = 0, p = 0
             }
             if (i >= 2 && !__all_sync(0xffffffffu, wait_or(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1, &bar->dead, a.err))) break;
-            stat[b * 128 + ct] = v;
+            // two queries side by side: f, f, -M, -M
+            float* to = reinterpret_cast<float*>(stat + b * 128) + ct / 2 * 4 + (ct & 1);
+            to[0] = v.x;
+            to[2] = -v.y;
             __syncwarp();
             if (lane == 0) bar_arrive(&bar->st_full[b]);
         }

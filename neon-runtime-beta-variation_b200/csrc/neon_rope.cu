@@ -200,7 +200,7 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
     if (!targets || n_targets == 0 || n_targets > (size_t)kMaxTargets)
         return error(NEON_ERR_INVALID, "rope: 1 to 4 targets");
     if (n == 0) return NEON_OK;
-    if (!d_pos) return error(NEON_ERR_INVALID, "rope: null positions");
+    if (!d_pos || !aligned(d_pos, 4)) return error(NEON_ERR_INVALID, "rope: null or unaligned positions");
     if (n > (size_t)INT32_MAX / 2) return error(NEON_ERR_INVALID, "rope: too many positions");
     RopeArgs a{};
     const bool half = rope->layout == NEON_ROPE_HALF;
