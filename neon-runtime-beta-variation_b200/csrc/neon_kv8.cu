@@ -67,30 +67,46 @@ __device__ __forceinline__ int quantise_exact(float x, float s, float inv) {
     return (int)r;
 }
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, which the low byte then holds
+constexpr float kNearTie = 0.4999f;
+
+// Four quotients (as two pairs) as rounded codes; far: how far one is from its code.
+__device__ __forceinline__ uint32_t round4(uint64_t y01, uint64_t y23, float& far) {
+    const uint64_t up = pair(kMagic, kMagic), down = pair(-kMagic, -kMagic), minus = pair(-1.f, -1.f);
+    const uint64_t t01 = add2(y01, up), t23 = add2(y23, up);
+    float d0, d1, d2, d3, t0, t1, t2, t3;
+    unpair(fma2(add2(t01, down), minus, y01), d0, d1);
+    unpair(fma2(add2(t23, down), minus, y23), d2, d3);
+    far = fmaxf(fmaxf(fabsf(d0), fabsf(d1)), fmaxf(fabsf(d2), fabsf(d3)));
+    unpair(t01, t0, t1);
+    unpair(t23, t2, t3);
+    return __byte_perm(__byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040),
+                       __byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x0040), 0x5410);
+}
+__device__ __noinline__ uint32_t exact4(float4 x, float s, float inv) {
+    return (uint32_t)(quantise_exact(x.x, s, inv) & 255) | (uint32_t)(quantise_exact(x.y, s, inv) & 255) << 8 |
+           (uint32_t)(quantise_exact(x.z, s, inv) & 255) << 16 | (uint32_t)(quantise_exact(x.w, s, inv) & 255) << 24;
+}
 // Four values as four codes.
 __device__ __forceinline__ uint32_t quantise4(const float (&x)[4], float s, float inv) {
-    float t[4], far = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = __fmul_rn(x[i], inv);
-        t[i] = __fadd_rn(y, kMagic);
-        far = fmaxf(far, fabsf(__fadd_rn(y, -__fadd_rn(t[i], -kMagic))));
-    }
-    if (far > 0.4999f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = kMagic + (float)quantise_exact(x[i], s, inv);
-    }
-    return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
-                       __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+    const uint64_t i2 = pair(inv, inv);
+    float far;
+    const uint32_t c = round4(mul2(pair(x[0], x[1]), i2), mul2(pair(x[2], x[3]), i2), far);
+    return far > kNearTie ? exact4(make_float4(x[0], x[1], x[2], x[3]), s, inv) : c;
 }
 
-// The values of four codes: 0x4b0000uu is 2^23 + u, with u = code + 128 (an int-to-float conversion has a
-// quarter of the rate).
-__device__ __forceinline__ void code_values(uint32_t w, float s, float (&x)[4]) {
+// Four codes as floats: 0x4b0000uu is 2^23 + u, with u = code + 128 (an int-to-float conversion has a quarter of
+// the rate).
+__device__ __forceinline__ void code_pairs(uint32_t w, uint64_t& c01, uint64_t& c23) {
     const uint32_t u = w ^ 0x80808080u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        x[e] = __fmul_rn(__fadd_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 | e)), -8388736.f), s);
+    const uint64_t bias = pair(-8388736.f, -8388736.f);
+    c01 = add2(pair(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541))), bias);
+    c23 = add2(pair(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7542)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7543))), bias);
+}
+__device__ __forceinline__ void code_values(uint32_t w, float s, float (&x)[4]) {
+    uint64_t c01, c23;
+    code_pairs(w, c01, c23);
+    unpair(mul2(c01, pair(s, s)), x[0], x[1]);
+    unpair(mul2(c23, pair(s, s)), x[2], x[3]);
 }
 // Magnitudes as bit patterns order like numbers, and what is not finite is at or above 0x7f800000.
 __device__ __forceinline__ unsigned magnitude(const float (&x)[4]) {
@@ -577,12 +593,24 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid
     for (int i = 0; i < P; ++i) {
         if (row[i] >= rows) continue;
         const int p = i * kGatherThreads + tid;
-        float x[4];
-        code_values(q[i], fs[row[i]], x);
-        if (turned)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = rowbuf[4 * p + e];
-        dc[p] = sn > 0.f ? quantise4(x, sn, inv) : 0u;
+        if (turned) {
+            const float4 v = *reinterpret_cast<const float4*>(rowbuf + 4 * p);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+            dc[p] = sn > 0.f ? quantise4(x, sn, inv) : 0u;
+        } else {
+            // a code times the row's scale over the new one; the value itself only where that is near a tie
+            const float s = fs[row[i]], rho = __fmul_rn(s, inv);
+            uint64_t c01, c23;
+            code_pairs(q[i], c01, c23);
+            float far;
+            uint32_t c = round4(mul2(c01, pair(rho, rho)), mul2(c23, pair(rho, rho)), far);
+            if (far > kNearTie) {
+                float x[4];
+                code_values(q[i], s, x);
+                c = exact4(make_float4(x[0], x[1], x[2], x[3]), sn, inv);
+            }
+            dc[p] = sn > 0.f ? c : 0u;
+        }
     }
     if (tid == 0) dsc[b] = sn;
 }

@@ -134,29 +134,6 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
     }
 }
 
-// fp32 pairs in one instruction
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // A warp puts 32 query rows of a tile into shared memory as the products read them: [TERMS][panels of
 // 64 values][128 rows][64] fp16, swizzled, row r times 2^e (its largest value near 2^7) and the sign of
 // the scale. Returns each lane's factor |scale| log2(e) 2^-e of row row0 + lane, 0 beyond the last row.
