@@ -286,7 +286,7 @@ NEON_API int neon_cuda_kv8_read(const neon_kv8_t* cache, size_t row0, size_t n, 
  * appended, over the cache: query head h of token t (dQ[t * q_stride + h *
  * head_dim + d]) attends to rows 0 .. *past + t of KV head h / (n_head /
  * n_kv_head), with scores times `scale` (0: 1 / sqrt(head_dim)). Writes
- * dO[t * o_stride + h * head_dim + d]; a token with no row to attend to
+ * dO[t * o_stride + h * head_dim + d] (dO does not overlap dQ); a token with no row to attend to
  * (*past + t < 0) gets zeros. d_weight (or NULL): [n_kv_head][capacity] floats,
  * the accumulated attention weight of each cached row: the probabilities that
  * the queries of its group give a row are added for rows before *past and

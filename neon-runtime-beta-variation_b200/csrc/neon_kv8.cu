@@ -721,7 +721,7 @@ int neon_cuda_kv8_evict(const neon_kv8_t* src, const float* d_weight, const neon
     if (keep == 0 || keep > dst->capacity) return error(NEON_ERR_INVALID, "kv8: keep must be 1 to the new cache's capacity");
     if (sink > keep || recent > keep - sink) return error(NEON_ERR_INVALID, "kv8: sink + recent above keep");
     if (src->k == dst->k || src->v == dst->v || src->k_scale == dst->k_scale || src->v_scale == dst->v_scale ||
-        src->past == dst->past || d_weight == d_weight_dst)
+        src->past == dst->past || src->tail_block == dst->tail_block || d_weight == d_weight_dst)
         return error(NEON_ERR_INVALID, "kv8: eviction needs separate buffers");
     OnDevice dev(src->k);
     if (dev.rc) return dev.rc;

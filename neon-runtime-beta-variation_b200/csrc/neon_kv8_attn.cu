@@ -602,6 +602,7 @@ int neon_cuda_kv8_attention(const neon_kv8_t* cache, const void* dQ, size_t q_st
     if (!eb) return error(NEON_ERR_UNSUPPORTED, "kv8: type must be F32, F16 or BF16");
     if (n == 0) return NEON_OK;
     if (!dQ || !dO || !workspace) return error(NEON_ERR_INVALID, "kv8: null Q, O or workspace");
+    if (dQ == dO) return error(NEON_ERR_INVALID, "kv8: Q and O must not be the same buffer");
     const size_t row = n_head * cache->head_dim;
     if (n > 1 && (q_stride < row || o_stride < row)) return error(NEON_ERR_INVALID, "kv8: stride smaller than the heads");
     if (!aligned(dQ, eb) || !aligned(dO, eb) || !aligned(d_weight, 4) || !aligned(workspace, 16))

@@ -28,6 +28,13 @@ def device():
     N.init(0)
 
 
+@pytest.fixture(autouse=True)
+def no_device_errors():
+    """Every test leaves the device's error word clear: no wait ran out."""
+    yield
+    N.sync()
+
+
 def cpu(t):
     return t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
 
@@ -263,7 +270,9 @@ def test_attention_of_few_tokens(kind, H, D, heads, past, n):
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("H,D,heads,past,n", [(2, 128, 4, 0, 130), (1, 64, 8, 0, 257), (2, 64, 2, 300, 65),
                                               (1, 128, 3, 33, 200), (1, 80, 2, 95, 129), (1, 256, 2, 20, 140),
-                                              (1, 128, 1, 1, 300), (2, 112, 10, 64, 64)])
+                                              (1, 128, 1, 1, 300), (2, 112, 10, 64, 64), (1, 16, 2, 40, 70),
+                                               (2, 48, 4, 0, 90), (1, 144, 3, 64, 50), (1, 192, 2, 31, 97),
+                                               (1, 240, 4, 10, 33), (1, 128, 64, 77, 1), (2, 64, 24, 500, 3)])
 def test_attention_of_prompts(kind, H, D, heads, past, n):
     check_attention(H, D, heads, past, n, kind)
 
@@ -338,6 +347,70 @@ def test_not_finite_stays_in_its_rows(n):
         c.append(k.cuda()[past:], v.cuda()[past:], n)
         o = attend(c, clean.cuda(), "f32")
         assert torch.isnan(o[32:, 2:]).all() and torch.isfinite(o[:32]).all() and torch.isfinite(o[:, :2]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_long_share_of_keys(kind):
+    """Many key tiles per CTA, scores that rise along the cache (m moves again and again) and values that agree."""
+    H, D, heads, past, n = 1, 64, 2, 7000, 100
+    k, v = rows(past + n, H, D, 60), rows(past + n, H, D, 61) + 3.0
+    k *= torch.linspace(0.05, 3.0, past + n)[:, None, None]
+    c = junk(N.Kv8Cache.empty(H, D, 7168))
+    c.append(k.cuda(), v.cuda(), past + n)
+    c.past.fill_(past)
+    kk, vv = torch.empty(past + n, H, D, device="cuda"), torch.empty(past + n, H, D, device="cuda")
+    c.read(0, past + n, kk, vv)
+    q = torch.randn(n, heads, D, generator=torch.Generator().manual_seed(5)).to(getattr(torch, TYPES[kind][1])).cuda()
+    w = torch.zeros(H, 7168, device="cuda")
+    o = attend(c, q, kind, weight=w)
+    kn, vn = cpu(kk).transpose(1, 0, 2), cpu(vv).transpose(1, 0, 2)
+    want, ww, big = O.attention(cpu(q), kn, vn, past, D ** -0.5)
+    to, tw = tolerances(kind, want, big, vn, ww)
+    assert (np.abs(cpu(o) - want) <= to).all()
+    assert (np.abs(cpu(w[:, :past + n]) - ww) <= tw + 2.0 ** -23).all()
+
+
+def test_offsets_beyond_32_bits():
+    """The second head of a cache whose codes fill 2^33 bytes, its last rows: the others are zeros, that weigh 1 each."""
+    H, D, cap, n = 2, 256, 1 << 24, 3
+    c = N.Kv8Cache.empty(H, D, cap)
+    past = cap - n
+    c.past.fill_(past)
+    k, v = rows(n, H, D, 70), rows(n, H, D, 71)
+    c.append(k.cuda(), v.cuda(), n)
+    kk, vv = torch.empty(n, H, D, device="cuda"), torch.empty(n, H, D, device="cuda")
+    c.read(past, n, kk, vv)
+    for h in range(H):  # (the block's earlier rows are zeros)
+        want = O.quantise(np.concatenate([np.zeros((29, D), np.float32), k[:, h].numpy()]))
+        assert np.array_equal(cpu(c.k[h, past:]), want[0][29:])
+    q = torch.randn(n, 2, D, generator=torch.Generator().manual_seed(6)).cuda() * 3
+    w = torch.zeros(H, cap, device="cuda")
+    o = attend(c, q, "f32", weight=w)
+    for t in range(n):
+        for h in range(H):
+            s = (cpu(kk)[:t + 1, h] @ cpu(q)[t, h]) * D ** -0.5
+            p = np.exp(s) / (past + np.exp(s).sum())
+            want = p @ cpu(vv)[:t + 1, h]
+            assert np.abs(cpu(o[t, h]) - want).max() <= 2.0 ** -10 * np.abs(p[:, None] * cpu(vv)[:t + 1, h]).max() * (t + 1)
+    total = 1.0 / (past + np.exp((cpu(kk)[:1, 1] @ cpu(q)[0, 1]) * D ** -0.5).sum())
+    assert abs(w[1, 12345].item() / (3 * total) - 1) < 1e-2 and w[1, past - 1].item() > 0
+    del c, w
+    torch.cuda.empty_cache()
+
+
+def test_a_prompt_of_tokens_without_rows():
+    c, k, v = filled(2, 64, 200, 224, 1)
+    q = torch.randn(140, 4, 64, generator=torch.Generator().manual_seed(7)).cuda()
+    w = torch.full((2, 224), 3.0, device="cuda")
+    c.past.fill_(-20)
+    o = attend(c, q, "f32", weight=w)
+    assert (o[:20] == 0).all()
+    want, ww, big = O.attention(cpu(q[20:]), k[:, :120], v[:, :120], 0, 64 ** -0.5)
+    to, tw = tolerances("f32", want, big, v, ww)
+    assert (np.abs(cpu(o[20:]) - want) <= to).all()
+    assert (np.abs(cpu(w[:, :120]) - ww) <= tw + 2.0 ** -23).all() and (w[:, 120:] == 3).all()
+    c.past.fill_(-1000)
+    assert (attend(c, q, "f32", weight=w) == 0).all()
 
 
 def test_no_rows_to_attend_to():

@@ -77,7 +77,7 @@ BAD = [(dict(n_kv_head=0), INVALID), (dict(n_kv_head=20000), INVALID), (dict(hea
 @pytest.mark.parametrize("bad,code", BAD)
 def test_cache_is_checked_everywhere(bad, code):
     L, c = N.load(), C.byref(cache(**bad))
-    good = C.byref(cache(k=P * 8, v=P * 9, k_scale=P * 10, v_scale=P * 11, past=P * 12))
+    good = C.byref(cache(k=P * 8, v=P * 9, k_scale=P * 10, v_scale=P * 11, tail_block=P * 13, past=P * 12))
     assert L.neon_cuda_kv8_append(c, P, 128, P, 128, 1, 0, None) == code
     assert L.neon_cuda_kv8_read(c, 0, 1, P, P, None) == code
     assert L.neon_cuda_kv8_attention(c, P, 128, P, 128, 1, 2, 0.0, 0, None, P, 1 << 20, None) == code
@@ -110,24 +110,25 @@ def test_attention_arguments():
     b = C.c_size_t()
     assert L.neon_cuda_kv8_attention_workspace(c, 4, 6, C.byref(b)) == 0 and b.value > 0
     assert L.neon_cuda_kv8_attention_workspace(c, 4, 6, None) == INVALID
-    assert f(c, P, 384, P, 384, 4, 6, 0.0, 0, None, P, b.value - 1, None) == INVALID and "workspace" in err()
-    assert f(c, P, 384, P, 384, 4, 6, 0.0, 0, None, P + 8, b.value, None) == INVALID and "16 bytes" in err()
-    assert f(c, P, 384, P, 384, 4, 6, 0.0, 0, None, None, b.value, None) == INVALID
-    assert f(c, P, 383, P, 384, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "stride" in err()
-    assert f(c, P, 384, P, 383, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "stride" in err()
-    assert f(c, P, 384, P, 384, 4, 5, 0.0, 0, None, P, b.value, None) == INVALID and "n_kv_head" in err()
-    assert f(c, P, 384, P, 384, 4, 0, 0.0, 0, None, P, b.value, None) == INVALID
-    assert f(c, P, 384, P, 384, 4, 260, 0.0, 0, None, P, b.value, None) == UNSUPPORTED
-    assert f(c, P, 384, P, 384, 97, 6, 0.0, 0, None, P, 1 << 40, None) == INVALID and "capacity" in err()
-    assert f(c, P, 384, P, 384, 4, 6, float("nan"), 0, None, P, b.value, None) == INVALID and "scale" in err()
-    assert f(c, P, 384, P, 384, 4, 6, 0.0, 3, None, P, b.value, None) == UNSUPPORTED
+    assert f(c, P, 384, P * 2, 384, 4, 6, 0.0, 0, None, P, b.value - 1, None) == INVALID and "workspace" in err()
+    assert f(c, P, 384, P * 2, 384, 4, 6, 0.0, 0, None, P + 8, b.value, None) == INVALID and "16 bytes" in err()
+    assert f(c, P, 384, P * 2, 384, 4, 6, 0.0, 0, None, None, b.value, None) == INVALID
+    assert f(c, P, 384, P, 384, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "same buffer" in err()
+    assert f(c, P, 383, P * 2, 384, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "stride" in err()
+    assert f(c, P, 384, P * 2, 383, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "stride" in err()
+    assert f(c, P, 384, P * 2, 384, 4, 5, 0.0, 0, None, P, b.value, None) == INVALID and "n_kv_head" in err()
+    assert f(c, P, 384, P * 2, 384, 4, 0, 0.0, 0, None, P, b.value, None) == INVALID
+    assert f(c, P, 384, P * 2, 384, 4, 260, 0.0, 0, None, P, b.value, None) == UNSUPPORTED
+    assert f(c, P, 384, P * 2, 384, 97, 6, 0.0, 0, None, P, 1 << 40, None) == INVALID and "capacity" in err()
+    assert f(c, P, 384, P * 2, 384, 4, 6, float("nan"), 0, None, P, b.value, None) == INVALID and "scale" in err()
+    assert f(c, P, 384, P * 2, 384, 4, 6, 0.0, 3, None, P, b.value, None) == UNSUPPORTED
     assert f(c, None, 0, None, 0, 0, 6, 0.0, 0, None, None, 0, None) == 0
 
 
 def test_evict_arguments():
     L = N.load()
     src = cache()
-    other = dict(k=P * 8, v=P * 9, k_scale=P * 10, v_scale=P * 11, past=P * 12)
+    other = dict(k=P * 8, v=P * 9, k_scale=P * 10, v_scale=P * 11, tail_block=P * 13, past=P * 12)
 
     def f(dst=None, keep=8, sink=2, recent=2, w=P, wd=P * 20, kept=P, rope=None):
         return L.neon_cuda_kv8_evict(C.byref(src), w, C.byref(cache(**(other if dst is None else dst))), wd, keep, sink,
@@ -137,7 +138,7 @@ def test_evict_arguments():
     assert f(sink=9) == INVALID and f(sink=7, recent=2) == INVALID and "sink" in err()
     assert f(w=None) == INVALID and f(wd=None) == INVALID and f(kept=None) == INVALID
     assert f(dst=dict(other, head_dim=128)) == INVALID and f(dst=dict(other, n_kv_head=4)) == INVALID
-    for same in ("k", "v", "k_scale", "v_scale", "past"):
+    for same in ("k", "v", "k_scale", "v_scale", "tail_block", "past"):
         assert f(dst=dict(other, **{same: getattr(src, same)})) == INVALID and "separate" in err()
     assert f(wd=P) == INVALID and "separate" in err()
     assert f(rope=C.byref(N.Rope(128)._c)) == INVALID and "n_dims" in err()
