@@ -137,72 +137,97 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
 // A warp puts 32 query rows of a tile into shared memory as the products read them: [TERMS][panels of
 // 64 values][128 rows][64] fp16, swizzled, row r times 2^e (its largest value near 2^7) and the sign of
 // the scale. Returns each lane's factor |scale| log2(e) 2^-e of row row0 + lane, 0 beyond the last row.
-// (The code runs once per CTA, from a cold instruction cache: little of it, for one type.)
+// A lane has eight values, one 16-byte piece, of one of R rows at a time. (This code runs once per CTA, from
+// a cold instruction cache, and with the output takes a third of a short prompt: little of it, loads first.)
 template <int PANELS, int TERMS, typename T>
 __device__ __forceinline__ float put_queries(const AttnArgs& a, int kvh, int r0, int row0, unsigned char* tile) {
     const int hd = (int)a.c.head_dim, rows = a.n * a.group, lane = threadIdx.x & 31;
-    constexpr int HALVES = PANELS > 2 ? 2 : 1;  // 128 values at a time
-    constexpr int U = HALVES > 1 ? 8 : 16;      // rows in flight
-    const bool vec = (reinterpret_cast<uintptr_t>(a.q) & (4 * sizeof(T) - 1)) == 0 && (a.qs & 3) == 0;
-    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    constexpr int LPR = PANELS == 1 ? 8 : PANELS == 2 ? 16 : 32, R = 32 / LPR;  // lanes of a row, rows at a time
+    constexpr int U = TERMS == 1 ? 8 : 4;                                       // of those in flight
+    constexpr int Q = sizeof(T) / 2;                                            // 16-byte loads of a lane
+    const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qs * sizeof(T)) % 16 == 0;
+    const float sign = a.scale < 0.f ? -1.f : 1.f, size = fabsf(a.scale);
+    const int d = lane % LPR * 8, sub = lane / LPR;
+    const unsigned row_lanes = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << (sub * LPR);
+    // token and head of the warp's first row; those of the next 32 by a product (below 2^7 rows: exact)
+    const int tok0 = (r0 + row0) / a.group, head0 = r0 + row0 - tok0 * a.group;
+    const unsigned magic = 65536u / (unsigned)a.group + 1u;
     float mine = 0.f;
 #pragma unroll 1
-    for (int i = 0; i < 32; i += U) {
-        Vec4<T> w[U][HALVES];  // the loads alone first: all of them in flight before a value is used
-        const T* q[U];
+    for (int i = 0; i < 32; i += R * U) {
+        union { uint4 v[Q]; T t[8]; } w[U];  // the loads alone first: all of them in flight before a value is used
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = min(r0 + row0 + i + u, rows - 1);  // rows beyond the last are made zero below
-            q[u] = (const T*)a.q + (long long)(r / a.group) * a.qs + (long long)(kvh * a.group + r % a.group) * hd + lane * 4;
-        }
-        if (vec) {
+            const int k = i + u * R + sub;
+            const int up = (int)(((unsigned)(head0 + k) * magic) >> 16);
+            const T* q = (const T*)a.q + (long long)(tok0 + up) * a.qs + (long long)(kvh * a.group + head0 + k - up * a.group) * hd + d;
+            const bool on = d < hd && r0 + row0 + k < rows;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int e = 0; e < Q; ++e) w[u].v[e] = make_uint4(0, 0, 0, 0);
+            if (vec) {
+                if (on)
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h)
-                    if (lane * 4 + 128 * h < hd) w[u][h].load(q[u] + 128 * h);
-        } else {
+                    for (int e = 0; e < Q; ++e) w[u].v[e] = reinterpret_cast<const uint4*>(q)[e];
+            } else if (on) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int h = 0; h < HALVES; ++h)
-                    if (lane * 4 + 128 * h < hd)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[u][h].t[e] = q[u][128 * h + e];
+                for (int e = 0; e < 8; ++e) w[u].t[e] = q[e];
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool on = r0 + row0 + i + u < rows;
-            float mx = 0.f, x[HALVES][4];
+            float x[8], mx = 0.f;
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[h][e] = lane * 4 + 128 * h < hd ? to_f(w[u][h].t[e]) : 0.f;
-                    mx = fmaxf(mx, fabsf(x[h][e]));
-                }
-            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23;
+            for (int e = 0; e < 8; ++e) {
+                x[e] = to_f(w[u].t[e]);
+                mx = fmaxf(mx, fabsf(x[e]));
+            }
+            const unsigned top = __reduce_max_sync(row_lanes, __float_as_uint(mx)) >> 23;
             const int e2 = top >= 255u ? 0 : min(120, 134 - (int)top);
             const float f = pow2(e2) * sign;
-            const int row = row0 + i + u;
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) {
-                const int d = lane * 4 + 128 * h;
-                if (d < PANELS * 64) {
-                    uint2 hi, lo;
-                    split2(x[h][0] * f, x[h][1] * f, hi.x, lo.x);
-                    split2(x[h][2] * f, x[h][3] * f, hi.y, lo.y);
-                    if (!on) hi = lo = make_uint2(0, 0);
-                    // 16-byte piece (d % 64) / 8 of the row moves to piece ^ (row % 8)
-                    const int at = (d / 64) * 16384 + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2;
-                    *reinterpret_cast<uint2*>(tile + at) = hi;
-                    if (TERMS == 2) *reinterpret_cast<uint2*>(tile + PANELS * 16384 + at) = lo;
-                }
+            if (d < PANELS * 64) {
+                uint4 hi, lo;
+                split2(x[0] * f, x[1] * f, hi.x, lo.x);
+                split2(x[2] * f, x[3] * f, hi.y, lo.y);
+                split2(x[4] * f, x[5] * f, hi.z, lo.z);
+                split2(x[6] * f, x[7] * f, hi.w, lo.w);
+                // piece (d % 64) / 8 of the row moves to piece ^ (row % 8)
+                const int row = row0 + i + u * R + sub;
+                const int at = (d >> 6) * 16384 + row * 128 + (((d & 63) >> 3 ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(tile + at) = hi;
+                if (TERMS == 2) *reinterpret_cast<uint4*>(tile + PANELS * 16384 + at) = lo;
             }
-            if (lane == i + u && on) mine = fabsf(a.scale) * pow2(-e2);
+            // lane k takes the factor of row k
+            const float got = __shfl_sync(0xffffffffu, size * pow2(-e2), lane % R * LPR);
+            if (lane / R * R == i + u * R && r0 + row0 + lane < rows) mine = got;
         }
     }
     return mine;
+}
+
+// 16 values of a thread's row, in whole 32-byte sectors where the address allows.
+template <typename T>
+__device__ __forceinline__ void store16(T* d, const T (&w)[16]) {
+    constexpr int N = sizeof(T) * 4;  // words
+    uint32_t x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (sizeof(T) == 4) x[i] = __float_as_uint(w[i]);
+        else x[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&w[2 * i]) | (uint32_t)*reinterpret_cast<const uint16_t*>(&w[2 * i + 1]) << 16;
+    }
+    if ((reinterpret_cast<uintptr_t>(d) & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(d) + i),
+                         "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), "r"(x[i + 6]),
+                         "r"(x[i + 7])
+                         : "memory");
+    } else if ((reinterpret_cast<uintptr_t>(d) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) reinterpret_cast<uint4*>(d)[i / 4] = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] = w[i];
+    }
 }
 
 // Where 16 codes (values 16 c .. of row r) begin in a swizzled tile of `height` rows, and putting them
@@ -522,20 +547,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(r[e]) * up;
                 if (!whole) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(po + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    store16(po + c, v);
                 } else {
                     T* d = (T*)a.o + ob + c;
                     alignas(16) T w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) w[e] = from_f<T>(v[e]);
-                    if ((reinterpret_cast<uintptr_t>(d) & 15) == 0) {
-#pragma unroll
-                        for (int e = 0; e < (int)sizeof(T); ++e) reinterpret_cast<uint4*>(d)[e] = reinterpret_cast<const uint4*>(w)[e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) d[e] = w[e];
-                    }
+                    store16(d, w);
                 }
             }
             if (out) {
