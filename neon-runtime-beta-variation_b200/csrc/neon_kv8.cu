@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     __shared__ unsigned sum[256];
     __shared__ unsigned counts[2 * kSelWarps];       // rows above / equal of this CTA's warps
     __shared__ unsigned all[2 * kSelWarps * CL];
-    __shared__ unsigned found[2];
+    __shared__ unsigned found[3];
     pdl_wait();
     pdl_trigger();
     const int h = blockIdx.x / CL, rank = blockIdx.x % CL;
@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
 
     // the m-th largest, eight bits a round
     unsigned prefix = 0, left = (unsigned)m;
-    for (int round = 0; round < 4; ++round) {
+    bool closed = false;  // every row from the threshold on stays: no need to look further down
+    for (int round = 0; round < 4 && !closed; ++round) {
         const int shift = 24 - 8 * round;
         unsigned* hs = hist[round & 1];
         for (int i = tid; i < 256; i += kSelThreads) hs[i] = 0;
@@ -443,18 +444,23 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
             if (above < left && left <= upto) {
                 found[0] = 255u - tid;
                 found[1] = left - above;
+                found[2] = upto - above;
             }
         }
         __syncthreads();
         prefix = (prefix << 8) | found[0];
         left = found[1];
+        closed = left == found[2];
+        if (closed) prefix <<= shift;
     }
-    const unsigned T = prefix;  // rows above T stay, and the first `left` rows equal to it
+    // rows above T stay, and the first `left` rows equal to it; closed: rows from T on
+    const unsigned T = prefix;
+    if (closed) left = 0;
 
     unsigned above = 0, equal = 0;
     each([&](int, unsigned u, bool on) {
-        above += on && u > T;
-        equal += on && u == T;
+        above += on && (u > T || (closed && u == T));
+        equal += on && u == T && !closed;
     });
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     before = __reduce_add_sync(0xffffffffu, before);
     ties = __reduce_add_sync(0xffffffffu, ties);
     each([&](int i, unsigned u, bool on) {
-        const bool up = on && u > T, eq = on && u == T;
+        const bool up = on && (u > T || (closed && u == T)), eq = on && u == T && !closed;
         const unsigned bu = __ballot_sync(0xffffffffu, up), be = __ballot_sync(0xffffffffu, eq);
         const unsigned mask = (1u << lane) - 1u;
         const unsigned t = ties + __popc(be & mask);  // equal rows before this one
