@@ -806,7 +806,11 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             const long long r0 = (long long)(first + i) * 128;
             const bool full = r0 >= last && key < keys;
             const int from = (int)max(0LL, min(128LL, seen - r0));  // columns below are hidden from this key
-            auto add = [&](const uint32_t (&r)[32], int c) {
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(r, st + b * 128 + c);
+                tmem_wait_ld();
                 const ulonglong2* sp = reinterpret_cast<const ulonglong2*>(stat + b * 128 + c);
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
@@ -821,18 +825,6 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
                     }
                     sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(p0, p1));
                 }
-            };
-            // the next 32 columns are read while these are summed
-            uint32_t ra[32], rb[32];
-            tmem_ld32(ra, st + b * 128);
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 64) {
-                tmem_wait_ld();
-                tmem_ld32(rb, st + b * 128 + c + 32);
-                add(ra, c);
-                tmem_wait_ld();
-                if (c == 0) tmem_ld32(ra, st + b * 128 + 64);
-                add(rb, c + 32);
             }
             tc_before();
             __syncwarp();
