@@ -721,25 +721,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
 // ---------------------------------------------------------------------------
 // The cached rows' weights: a CTA keeps MT tiles of 128 keys (their codes as
-// fp16) and streams the query tiles, S^T = K Q^T, so a thread has one key and
-// sums p = 2^(t - m) / l = 2^(s factor scale - (m + log2 l)) over its columns in
-// registers, in the queries' order. Two buffers of S^T let the products run
-// ahead; exp2 bounds it (one per key and query). Needs the rows' final m, 1 / l.
+// fp16) and streams the query tiles, S = Q K^T. A thread has one query of each
+// tile and 32 MT keys; it adds p = 2^(t - m) / l = 2^(s factor scale - (m + log2 l))
+// to its keys' sums in registers, over all tiles, and the 128 queries of a key
+// are added up once, at the end, in a fixed order. The keys are two halves with
+// two buffers of S each, and the second half follows a tile behind, so the
+// warps of one take the exponentials while those of the other wait. Needs the
+// rows' final m, 1 / l.
+// exp2 bounds it, one per key and query: 4008 rows over 30501 keys of four heads
+// take 232 us where the exponentials alone are 115 us (16 a clock and SM); the
+// last of four waves of CTAs is a quarter full, and a tile takes 3300 cycles of
+// which 2050 are exponentials. A thread with one key and all queries (S^T)
+// reads each query's numbers from shared memory: 255 us, and 247 us with twice
+// the warps; both halves of the keys in step 240 us.
 // ---------------------------------------------------------------------------
 template <int PANELS>
 struct WShape {
     static constexpr int MT = PANELS <= 2 ? 2 : 1;
-    static constexpr int KTile = PANELS * 16384;       // a tile of 128 keys
+    static constexpr int Keys = MT * 128;
+    static constexpr int KTile = PANELS * Keys * 128;  // the keys
     static constexpr int Stage = PANELS * 16384;       // a query tile's hi or lo terms
     static constexpr int ST = PANELS <= 2 ? 4 : 2;
-    static constexpr int Smem = MT * KTile + ST * Stage + 2 * 128 * 8 + 1024 + 256;
+    static constexpr int Smem = KTile + ST * Stage + 4 * Keys * 4 + 1024 + 256;
     static_assert(Smem <= 232448, "shared memory");
 };
-// warps 0-7 sum, 8-11 convert the keys and fill in the rows' numbers, 12 the products, 13 loads
-constexpr int kWThreads = 448, kWConvWarps = 4, kWMmaWarp = 12;
+// warps 0-15 convert the keys, then sum: four of them share a quarter of the keys; 16 the products, 17 loads
+constexpr int kWSumWarps = 16, kWMmaWarp = 16, kWThreads = 576;
 
 struct WBars {
-    uint64_t k_full, q_full[4], q_empty[4], s_full[2], s_empty[2], st_full[2], drain;
+    uint64_t k_full, q_full[4], q_empty[4], s_full[2][2], s_empty[2][2], drain;
     uint32_t tmem;
     int dead;
 };
@@ -748,37 +758,37 @@ static_assert(sizeof(WBars) <= 256, "barriers");
 template <int PANELS, int TERMS>
 __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
     using S = WShape<PANELS>;
-    constexpr int MT = S::MT, ST = S::ST;
+    constexpr int ST = S::ST, Keys = S::Keys, KC = Keys / 4;
+    constexpr int Lag = 2 * TERMS <= ST ? 1 : 0;  // (the ring holds two query tiles)
     extern __shared__ unsigned char raw[];
     pdl_wait();
     pdl_trigger();
     const int hd = (int)a.c.head_dim, cap = (int)a.c.capacity, rows = a.n * a.group, kvh = blockIdx.y;
     const int past = *a.c.past, keys = keys_of(past, a.n - 1, cap);
-    const int key0 = blockIdx.x * MT * 128;
+    const int key0 = blockIdx.x * Keys;
     if (key0 >= keys) return;
     unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-    unsigned char *ks = smem, *qs = ks + MT * S::KTile;
-    float2* stat = reinterpret_cast<float2*>(qs + ST * S::Stage);  // [2][128 queries]: factors and -(m + log2 l)
-    WBars* bar = reinterpret_cast<WBars*>(stat + 256);
+    unsigned char *ks = smem, *qs = ks + S::KTile;
+    float* part = reinterpret_cast<float*>(qs + ST * S::Stage);  // [4][Keys]
+    WBars* bar = reinterpret_cast<WBars*>(part + 4 * Keys);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == kWMmaWarp) {
         if (lane == 0) {
-            bar_init(&bar->k_full, kWConvWarps);
+            bar_init(&bar->k_full, kWSumWarps);
             for (int i = 0; i < ST; ++i) {
                 bar_init(&bar->q_full[i], 1);
                 bar_init(&bar->q_empty[i], 1);
             }
-            for (int i = 0; i < 2; ++i) {
-                bar_init(&bar->s_full[i], 1);
-                bar_init(&bar->s_empty[i], 4 * MT);
-                bar_init(&bar->st_full[i], kWConvWarps);
+            for (int i = 0; i < 4; ++i) {
+                bar_init(&bar->s_full[i >> 1][i & 1], 1);
+                bar_init(&bar->s_empty[i >> 1][i & 1], kWSumWarps / 2);
             }
             bar_init(&bar->drain, 1);
             bar->dead = 0;
             bar_init_fence();
         }
         __syncwarp();
-        tmem_alloc(&bar->tmem, 256 * MT);
+        tmem_alloc(&bar->tmem, 2 * Keys);
         tc_before();
     }
     __syncthreads();
@@ -788,85 +798,98 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
     const int first = (int)min((long long)rows - 1, max(0LL, ((long long)key0 - past) * a.group)) / 128;
     const int n = (rows + 127) / 128 - first;
 
-    if (warp < 4 * MT) {
-        const int m = warp >> 2, key = key0 + m * 128 + (warp & 3) * 32 + lane;
-        const uint32_t st = tmem + ((uint32_t)(warp & 3) << 21) + m * 256;
-        const float scale = key < keys ? a.c.k_scale[(size_t)kvh * (cap >> 5) + (key >> 5)] : 0.f;
-        // the first row that sees this key, and that every key of the warp is seen by
-        const long long seen = key < keys ? ((long long)key - past) * a.group : (1LL << 40);
-        const long long last = max(0LL, ((long long)(key | 31) - past) * a.group);
-        const uint64_t scale2 = pair(scale, scale);
-        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-        for (int i = 0; i < n; ++i) {
-            const int b = i & 1;
-            const uint32_t ph = (uint32_t)((i >> 1) & 1);
-            bool ok = wait_or(&bar->st_full[b], ph, &bar->dead, a.err) && wait_or(&bar->s_full[b], ph, &bar->dead, a.err);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            tc_after();
-            const long long r0 = (long long)(first + i) * 128;
-            const bool full = r0 >= last && key < keys;
-            const int from = (int)max(0LL, min(128LL, seen - r0));  // columns below are hidden from this key
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(r, st + b * 128 + c);
-                tmem_wait_ld();
-                const ulonglong2* sp = reinterpret_cast<const ulonglong2*>(stat + b * 128 + c);
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const ulonglong2 q = sp[e / 2];  // the factors of two queries, then minus their m + log2 l
-                    float p0, p1;
-                    unpair(fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), mul2(q.x, scale2), q.y), p0, p1);
-                    p0 = ex2(p0);
-                    p1 = ex2(p1);
-                    if (!full) {
-                        if (c + e < from) p0 = 0.f;
-                        if (c + e + 1 < from) p1 = 0.f;
-                    }
-                    sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(p0, p1));
-                }
-            }
-            tc_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(&bar->s_empty[b]);
-        }
-        if (key < keys) {
-            float s0, s1;
-            unpair(add2(sum[0], sum[1]), s0, s1);
-            const float v = s0 + s1;
-            float* w = a.weight + (size_t)kvh * cap + key;
-            *w = key < past ? *w + v : v;
-        }
-    } else if (warp >= kSoftWarps && warp < kWMmaWarp) {
-        const int ct = tid - kSoftWarps * 32, pieces = hd / 16;
+    if (warp < kWSumWarps) {
+        const int pieces = hd / 16;
         const uint4* kc = reinterpret_cast<const uint4*>(a.c.k + ((size_t)kvh * cap + key0) * hd);
-        const int held = min(MT * 128, cap - key0) * pieces;
-        for (int p = ct; p < MT * 128 * pieces; p += 128) {
+        const int held = min(Keys, cap - key0) * pieces;
+        for (int p = tid; p < Keys * pieces; p += kWSumWarps * 32) {
             const int r = p / pieces;
             const uint4 w = p < held ? kc[p] : make_uint4(0, 0, 0, 0);
-            put_codes(ks + (r >> 7) * S::KTile, put_at(128, r & 127, p - r * pieces), w);
+            put_codes(ks, put_at(Keys, r, p - r * pieces), w);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(&bar->k_full);
-        for (int i = 0; i < n; ++i) {
-            const int b = i & 1, r = (first + i) * 128 + ct;
-            float2 v = make_float2(0.f, INFINITY);
-            if (r < rows) {
-                const float2 s = *reinterpret_cast<const float2*>(a.stats + ((size_t)kvh * rows + r) * 2);
-                v.x = a.qfactor[(size_t)kvh * tiles128 * 128 + r];
-                v.y = s.x - log2f(s.y);  // a row without keys: 1 / l = 0, p = 0
+
+        const int quarter = warp & 3, half = warp >> 3, cols = (warp >> 2) * KC, base = key0 + cols;
+        const uint32_t st = tmem + ((uint32_t)quarter << 21) + cols;
+        float scale[KC / 32];
+#pragma unroll
+        for (int h = 0; h < KC / 32; ++h) scale[h] = base + 32 * h < keys ? a.c.k_scale[(size_t)kvh * (cap >> 5) + (base >> 5) + h] : 0.f;
+        uint64_t sum[KC / 2];
+#pragma unroll
+        for (int e = 0; e < KC / 2; ++e) sum[e] = pair(0.f, 0.f);
+        // a row's factor, m and 1 / l (0 for a row without keys: p = 0); the next tile's are on their way while a
+        // tile is summed
+        float factor;
+        float2 ml;
+        auto numbers = [&](int i) {
+            const int r = (first + i) * 128 + quarter * 32 + lane;
+            factor = 0.f;
+            ml = make_float2(0.f, 0.f);
+            if (i < n && r < rows) {
+                ml = *reinterpret_cast<const float2*>(a.stats + ((size_t)kvh * rows + r) * 2);
+                factor = a.qfactor[(size_t)kvh * tiles128 * 128 + r];
             }
-            if (i >= 2 && !__all_sync(0xffffffffu, wait_or(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1, &bar->dead, a.err))) break;
-            // two queries side by side: f, f, -M, -M
-            float* to = reinterpret_cast<float*>(stat + b * 128) + ct / 2 * 4 + (ct & 1);
-            to[0] = v.x;
-            to[2] = -v.y;
+        };
+        numbers(0);
+        for (int i = 0; i < n; ++i) {
+            const int b = i & 1, r0 = (first + i) * 128 + quarter * 32;
+            const float mine = factor, less = log2f(ml.y) - ml.x;  // -(m + log2 l)
+            numbers(i + 1);
+            const bool ok = wait_or(&bar->s_full[half][b], (uint32_t)((i >> 1) & 1), &bar->dead, a.err);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_after();
+            const bool full = (long long)past + r0 / a.group >= base + KC - 1;
+            const long long left = (long long)past + (r0 + lane) / a.group - base;  // the last column that this row sees
+            const uint64_t minus = pair(less, less);
+#pragma unroll
+            for (int h = 0; h < KC / 16; ++h) {
+                uint32_t r[16];
+                tmem_ld16(r, st + b * Keys + 16 * h);
+                const float f = mine * scale[h / 2];
+                const uint64_t ff = pair(f, f);
+                tmem_wait_ld();
+                if (full) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float p0, p1;
+                        unpair(fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), ff, minus), p0, p1);
+                        sum[8 * h + e / 2] = add2(sum[8 * h + e / 2], pair(ex2(p0), ex2(p1)));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float p0, p1;
+                        unpair(fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), ff, minus), p0, p1);
+                        p0 = 16 * h + e <= left ? ex2(p0) : 0.f;
+                        p1 = 16 * h + e + 1 <= left ? ex2(p1) : 0.f;
+                        sum[8 * h + e / 2] = add2(sum[8 * h + e / 2], pair(p0, p1));
+                    }
+                }
+            }
+            tc_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(&bar->st_full[b]);
+            if (lane == 0) bar_arrive(&bar->s_empty[half][b]);
         }
+        // the warp's 32 rows: each step adds the lanes that differ in one bit and halves what a lane has
+        float v[KC];
+#pragma unroll
+        for (int e = 0; e < KC / 2; ++e) unpair(sum[e], v[2 * e], v[2 * e + 1]);
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) {
+            const int c = KC * w / 32;
+            const bool up = lane & w;
+#pragma unroll
+            for (int e = 0; e < c; ++e) {
+                const float keep = up ? v[e + c] : v[e], give = up ? v[e] : v[e + c];
+                v[e] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < KC / 32; ++e) part[quarter * Keys + cols + lane * (KC / 32) + e] = v[e];
     } else if (warp == kWMmaWarp) {
-        const uint32_t id = instr(128, false), tm = uniform(tmem), base = uniform(smem_addr(ks));
+        const uint32_t id = instr(Keys / 2, false), tm = uniform(tmem), base = uniform(smem_addr(ks));
         const int steps = hd / 16, count = uniform(n);
         auto wait = [&](uint64_t* w, uint32_t parity) {
             bool ok = true;
@@ -874,35 +897,35 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
             return uniform((int)ok) != 0;
         };
         bool ok = wait(&bar->k_full, 0);
-        int it = 0;
-        for (int i = 0; ok && i < count; ++i) {
-            const int b = i & 1;
-            if (i >= 2) ok = wait(&bar->s_empty[b], (uint32_t)((i >> 1) & 1) ^ 1);
-            for (int t = 0; ok && t < TERMS; ++t, ++it) {
-                const int sg = it % ST;
+        for (int j = 0; ok && j < 2 * (count + Lag); ++j) {
+            const int half = j & 1, i = (j >> 1) - half * Lag, b = i & 1;
+            if (i < 0 || i >= count) continue;
+            if (i >= 2) ok = wait(&bar->s_empty[half][b], (uint32_t)((i >> 1) & 1) ^ 1);
+            for (int t = 0; ok && t < TERMS; ++t) {
+                const int it = i * TERMS + t, sg = it % ST;
                 ok = wait(&bar->q_full[sg], (uint32_t)((it / ST) & 1));
                 if (!ok) break;
                 tc_after();
-                const uint32_t k = uniform(operand_lo(base, 16)), q = uniform(operand_lo(base + MT * S::KTile + sg * S::Stage, 16));
-                const uint32_t d = uniform(tm + b * 128);
+                // (a row is 8 of the operand's units: to the half's first row)
+                const uint32_t k = uniform(operand_lo(base, 16) + half * (Keys / 2 * 8));
+                const uint32_t q = uniform(operand_lo(base + S::KTile + sg * S::Stage, 16));
+                const uint32_t d = uniform(tm + b * Keys + half * (Keys / 2));
                 const bool add = t > 0;
                 if (elected()) {
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int s = 0; s < PANELS * 4; ++s)
-                            if (s < steps)
-                                mma_ss(d + m * 256, operand_of(k + m * (S::KTile >> 4) + (s >> 2) * 1024 + (s & 3) * 2),
-                                       operand_of(q + (s >> 2) * 1024 + (s & 3) * 2), id, add || s > 0);
-                    tc_commit(&bar->q_empty[sg]);
+                    for (int s = 0; s < PANELS * 4; ++s)
+                        if (s < steps)
+                            mma_ss(d, operand_of(q + (s >> 2) * 1024 + (s & 3) * 2), operand_of(k + (s >> 2) * (Keys * 8) + (s & 3) * 2), id,
+                                   add || s > 0);
+                    if (half) tc_commit(&bar->q_empty[sg]);
                 }
             }
-            if (ok && elected()) tc_commit(&bar->s_full[b]);
+            if (ok && elected()) tc_commit(&bar->s_full[half][b]);
         }
         if (elected()) tc_commit(&bar->drain);
         volatile int never = 0;
         if (lane == 0) wait_or(&bar->drain, 0, &never, a.err);
-    } else if (warp == kWMmaWarp + 1 && lane == 0) {
+    } else if (lane == 0) {
         const unsigned char* src = a.qt + ((size_t)kvh * tiles128 + first) * TERMS * S::Stage;  // (a tile's lo terms first)
         const int total = n * TERMS;
         int it = 0;
@@ -919,9 +942,14 @@ __global__ void __launch_bounds__(kWThreads, 1) kv8_prompt_weight_kernel(const _
     __syncwarp();
     tc_before();
     __syncthreads();
+    if (tid < Keys && key0 + tid < keys) {
+        const float v = (part[tid] + part[Keys + tid]) + (part[2 * Keys + tid] + part[3 * Keys + tid]);
+        float* w = a.weight + (size_t)kvh * cap + key0 + tid;
+        *w = key0 + tid < past ? *w + v : v;
+    }
     if (warp == kWMmaWarp) {
         tc_after();
-        tmem_free(tmem, 256 * MT);
+        tmem_free(tmem, 2 * Keys);
     }
 }
 
@@ -932,7 +960,7 @@ int launch_weights(const AttnArgs& a, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::Smem);
     if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_prompt_weight_kernel)");
     const int tiles = (a.n * a.group + 255) / 256 * 2;
-    const unsigned grid = (a.c.capacity + 128 * S::MT - 1) / (128 * S::MT);
+    const unsigned grid = (a.c.capacity + S::Keys - 1) / S::Keys;
     return launch("kv8_prompt_weight_kernel", k, dim3(grid, a.c.n_kv_head), kWThreads, S::Smem, st, 1, a, tiles);
 }
 
