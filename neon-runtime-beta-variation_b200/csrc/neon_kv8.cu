@@ -367,8 +367,8 @@ struct SelectArgs {
     int* kept;       // [H][keep]
 };
 
-// CL: CTAs of a head, a cluster. One takes 1024 rows in 6 us where eight, with their barriers, take 11; eight take
-// 131071 rows in 24 us.
+// CL: CTAs of a head, a cluster. One takes 1024 rows in 8 us and 8192 in 13.6 where eight, with their barriers, take
+// 11 and 13.7; eight take 131071 rows in 27 us. Loads, counts in shared memory and barriers bound it, in rounds.
 template <int CL>
 __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_constant__ SelectArgs a) {
     __shared__ unsigned hist[2][256];

@@ -31,10 +31,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 constexpr int kMaxSplit = 64;
 
 // ---------------------------------------------------------------------------
-// Eight rows of one KV head over a share of the cache. The MMA's 16 rows hold
-// the eight rows' hi terms and below them their lo terms, so the split costs
-// no extra products: a row's score is the sum of its two halves, and its
-// output likewise. Each warp streams its own tiles of 32 rows (a block of the
+// Eight or sixteen rows of one KV head over a share of the cache. The MMA's 16
+// rows hold eight rows' hi terms and below them their lo terms, so the split
+// costs no extra products: a row's score is the sum of its two halves, and its
+// output likewise. Of more than eight rows in a 16-bit type they hold sixteen
+// rows' single terms (q is exact in one, up to values far below the row's
+// largest; p is rounded to 2^-11 of itself, as for prompts): 16 rows over
+// 120000 of 8 heads x 128 take 68 us where two passes of eight took 95, and 32
+// rows 102 where four took 186. Each warp streams its own tiles of 32 rows (a block of the
 // cache: K's codes, then V's, a bulk copy each) through its own ring in shared
 // memory, with no barrier between the warps until their results are merged.
 // The order of the summed dimension is free, so each lane reads whole 16-byte
@@ -42,10 +46,12 @@ constexpr int kMaxSplit = 64;
 // all warps) are laid out to match; of V, lane group g takes columns [g HD / 8,
 // (g + 1) HD / 8) of four rows. HBM bounds it at length; the arithmetic (some
 // 800 instructions a warp for 8 KB of codes) needs 16 warps per SM to hide its
-// latencies: with 8, and the query fragments in registers, 131071 rows of 8
-// heads x 128 took 68 us (3.9 TB/s).
+// latencies: 131071 rows of 8 heads x 128 take 66 us with the weights' scores
+// stored, of which the stream is 47 (5.8 TB/s) and the rest prologue, merge and
+// the last warps; with 8 warps, and the query fragments in registers, 68 us
+// without.
 // ---------------------------------------------------------------------------
-template <int HD>
+template <int HD, int ROWS>
 struct RowTile {
     static constexpr int kWarps = HD <= 128 ? 16 : 8;
     static constexpr int kThreads = kWarps * 32;
@@ -53,19 +59,20 @@ struct RowTile {
     static constexpr int kSlotBytes = 32 * HD;
     static constexpr int kRing = kWarps * kSlots * kSlotBytes;
     static constexpr int kPitch = HD + 8;  // floats of a row in the merge: eight rows in different banks
-    static constexpr int kMerge = kWarps * 8 * (kPitch + 2) * 4;
+    static constexpr int kMerge = kWarps * ROWS * (kPitch + 2) * 4;
     static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
     static constexpr int kQuery = HD / 16 * 512;
-    static constexpr int kSmem = kBody + kQuery + 8 * 4 + kWarps * kSlots * 8;
+    static constexpr int kSmem = kBody + kQuery + 16 * 4 + kWarps * kSlots * 8;
     static_assert(kSmem <= 232448, "shared memory");
 };
 
-// The query fragments of rows 8 grp .. of a KV head, one warp per row: lane (g, tq) of the products holds values
-// tq HD / 4 + 4 s .. + 3 of row g for step s, as hi and lo terms, times 2^e so that the row's largest is near 2^7 (its
-// lo terms then stay normal halves). The row's factor is scale log2(e) 2^-e.
-template <int HD>
+// The query fragments of row g of a group, by a warp: lane (g % 8, tq) of the products holds values
+// tq HD / 4 + 4 s .. + 3 of row g for step s, as hi and lo terms (of 16 rows: row g's and row g + 8's values), times
+// 2^e so that the row's largest is near 2^7 (its lo terms then stay normal halves, and of a 16-bit type only values
+// below 2^-20 of the row's largest lose bits). The row's factor is scale log2(e) 2^-e.
+template <int HD, int ROWS>
 __device__ __forceinline__ void row_queries(const AttnArgs& a, int kvh, int grp, int g, uint4* out, float* factor) {
-    const int lane = threadIdx.x & 31, hd = (int)a.c.head_dim, rows = a.n * a.group, row = grp * 8 + g;
+    const int lane = threadIdx.x & 31, hd = (int)a.c.head_dim, rows = a.n * a.group, row = grp * ROWS + g;
     const int tok = token_of(a, row);
     const long long base = tok * a.qs + (long long)(kvh * a.group + row - tok * a.group) * hd;
     constexpr int V = (HD + 127) / 128;  // pieces of four values a lane
@@ -92,22 +99,30 @@ __device__ __forceinline__ void row_queries(const AttnArgs& a, int kvh, int grp,
         uint4 q;
         split2(x[v][0] * f, x[v][1] * f, q.x, q.y);
         split2(x[v][2] * f, x[v][3] * f, q.z, q.w);
-        out[d % (HD / 4) / 4 * 32 + g * 4 + d / (HD / 4)] = q;
+        uint4* to = out + d % (HD / 4) / 4 * 32 + g % 8 * 4 + d / (HD / 4);
+        if (ROWS == 8) {
+            *to = q;
+        } else {
+            uint32_t* half = reinterpret_cast<uint32_t*>(to) + g / 8;
+            half[0] = q.x;
+            half[2] = q.z;
+        }
     }
     if (lane == 0) factor[g] = a.scale * pow2(-e);
 }
 
 // FULL: head_dim is HD itself, not less.
-template <int HD, bool FULL>
-__global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(const __grid_constant__ AttnArgs a) {
-    using R = RowTile<HD>;
+template <int HD, bool FULL, int ROWS>
+__global__ void __launch_bounds__(RowTile<HD, ROWS>::kThreads, 1) kv8_rows_kernel(const __grid_constant__ AttnArgs a) {
+    using R = RowTile<HD, ROWS>;
+    constexpr int RL = ROWS / 8;  // rows of a lane: g, and of 16 g + 8
     constexpr int KS = HD / 16;   // k-steps of the score product
     constexpr int NT = HD / 8;    // column tiles of the output
     constexpr int W = R::kWarps, S = R::kSlots;
     extern __shared__ __align__(128) unsigned char smem[];
     uint4* qf = reinterpret_cast<uint4*>(smem + R::kBody);
     float* qfac = reinterpret_cast<float*>(smem + R::kBody + R::kQuery);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(qfac + 8);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qfac + 16);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
     const int hd = FULL ? HD : (int)a.c.head_dim, cap = (int)a.c.capacity;
     const int split = blockIdx.x, kvh = blockIdx.y, grp = blockIdx.z, rows = a.n * a.group;
@@ -123,8 +138,12 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
 
     // the keys of the group's rows, and this warp's share of them in tiles
     const int past = *a.c.past;
-    const int row = grp * 8 + g;
-    const int limit = row < rows ? keys_of(past, token_of(a, row), cap) : 0;
+    int limit[RL];
+#pragma unroll
+    for (int h = 0; h < RL; ++h) {
+        const int row = grp * ROWS + 8 * h + g;
+        limit[h] = row < rows ? keys_of(past, token_of(a, row), cap) : 0;
+    }
     const Shares sh = shares_of(a, past, grp);
     if (!sh.has(split)) return;
     const int c0 = split * sh.per, c1 = min(c0 + sh.per, sh.tiles);
@@ -143,17 +162,24 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
     };
     if (lane == 0)
         for (int it = 0; it < min(S, items); ++it) issue(it, it);
-    if (warp < 8) row_queries<HD>(a, kvh, grp, warp, qf, qfac);
+    for (int r = warp; r < ROWS; r += W) row_queries<HD, ROWS>(a, kvh, grp, r, qf, qfac);
     __syncthreads();
-    const float factor = qfac[g];
-    float* scores = a.scores ? a.scores + (((size_t)kvh * gridDim.z + grp) * 8 + g) * cap : nullptr;
+    float factor[RL];
+#pragma unroll
+    for (int h = 0; h < RL; ++h) factor[h] = qfac[8 * h + g];
+    float* scores = a.scores ? a.scores + (((size_t)kvh * gridDim.z + grp) * ROWS + g) * cap : nullptr;
 
     float acc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-    float m = -INFINITY, l = 0.f, vref = 0.f;
+    float m[RL], l[RL], vref = 0.f;
+#pragma unroll
+    for (int h = 0; h < RL; ++h) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+    }
     float my_ks = 0.f, my_vs = 0.f;  // the scales of 32 tiles, one per lane
     bool ok = true;
     int slot = 0;
@@ -209,36 +235,49 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
             }
         }
         give(it++);
-        // online softmax of row g: the lane has keys 8 j + 2 tq and + 1
-        const float kf = factor * ks;
-        float t[4][2], mt = m;
+        // online softmax of the lane's rows: it has keys 8 j + 2 tq and + 1
+        float t[RL][4][2], mu[RL], down[RL];
+        bool moves = vs > 4.f * vref;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int key = tile * 32 + 8 * j + 2 * tq + e;
-                t[j][e] = key < limit ? (sc[j][e] + sc[j][e + 2]) * kf : -INFINITY;
-                mt = fmaxf(mt, t[j][e]);
-            }
-        if (scores && row < rows)
+        for (int h = 0; h < RL; ++h) {
+            const float kf = factor[h] * ks;
+            float mt = m[h];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float2*>(scores + tile * 32 + 8 * j + 2 * tq) = make_float2(t[j][0], t[j][1]);
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-        // m follows when p would pass 2^8 (the result does not depend on m): O is seldom rescaled
-        const float mnew = mt > m + 8.f || m == -INFINITY ? mt : m;
-        const float mu = mnew == -INFINITY ? 0.f : mnew;
-        if (__any_sync(0xffffffffu, mnew != m || vs > 4.f * vref)) {
-            const float down = ex2(m - mu), vtop = vs > 4.f * vref ? vs : vref;
-            const float f = vtop > 0.f ? down * (vref / vtop) : down;
-            l *= down;
-            m = mnew;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = tile * 32 + 8 * j + 2 * tq + e;
+                    t[h][j][e] = key < limit[h] ? (ROWS == 8 ? sc[j][e] + sc[j][e + 2] : sc[j][e + 2 * h]) * kf : -INFINITY;
+                    mt = fmaxf(mt, t[h][j][e]);
+                }
+            if (scores && grp * ROWS + 8 * h + g < rows)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<float2*>(scores + (size_t)(8 * h) * cap + tile * 32 + 8 * j + 2 * tq) =
+                        make_float2(t[h][j][0], t[h][j][1]);
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+            // m follows when p would pass 2^8 (the result does not depend on m): O is seldom rescaled
+            const float mnew = mt > m[h] + 8.f || m[h] == -INFINITY ? mt : m[h];
+            mu[h] = mnew == -INFINITY ? 0.f : mnew;
+            down[h] = ex2(m[h] - mu[h]);
+            moves |= mnew != m[h];
+            m[h] = mnew;
+        }
+        if (__any_sync(0xffffffffu, moves)) {
+            const float vtop = vs > 4.f * vref ? vs : vref;
+            const float vdown = vtop > 0.f ? vref / vtop : 1.f;
             vref = vtop;
+            float f[RL];
+#pragma unroll
+            for (int h = 0; h < RL; ++h) {
+                l[h] *= down[h];
+                f[h] = down[h] * vdown;
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][e] *= f;
+                for (int e = 0; e < 4; ++e) acc[n][e] *= f[ROWS == 8 ? 0 : e >> 1];
         }
         const float vr = vs == 0.f ? 0.f : vs / vref * kPUp;
         uint32_t pf[2][4];
@@ -247,10 +286,15 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 const int j = 2 * k + hf;
-                const bool on0 = t[j][0] != -INFINITY, on1 = t[j][1] != -INFINITY;
-                const float p0 = ex2(t[j][0] - mu), p1 = ex2(t[j][1] - mu);
-                l += p0 + p1;
-                split2(on0 ? p0 * vr : 0.f, on1 ? p1 * vr : 0.f, pf[k][2 * hf], pf[k][2 * hf + 1]);
+#pragma unroll
+                for (int h = 0; h < RL; ++h) {
+                    const bool on0 = t[h][j][0] != -INFINITY, on1 = t[h][j][1] != -INFINITY;
+                    const float p0 = ex2(t[h][j][0] - mu[h]), p1 = ex2(t[h][j][1] - mu[h]);
+                    l[h] += p0 + p1;
+                    const float x0 = on0 ? p0 * vr : 0.f, x1 = on1 ? p1 * vr : 0.f;
+                    if (ROWS == 8) split2(x0, x1, pf[k][2 * hf], pf[k][2 * hf + 1]);
+                    else pf[k][2 * hf + h] = h2_bits(__floats2half2_rn(x0, x1));
+                }
             }
         }
         const unsigned char* vt = take();
@@ -304,59 +348,67 @@ __global__ void __launch_bounds__(RowTile<HD>::kThreads, 1) kv8_rows_kernel(cons
         }
 
     // merge the warps: o (times s_v), m, l of each row
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();
-    float* mo = reinterpret_cast<float*>(smem);             // [warps][8][HD]: place 8 t + c has column c HD / 8 + t
-    float* ml = mo + W * 8 * R::kPitch;                     // [warps][8][2]
+    float* mo = reinterpret_cast<float*>(smem);             // [warps][ROWS][HD]: place 8 t + c has column c HD / 8 + t
+    float* ml = mo + W * ROWS * R::kPitch;                  // [warps][ROWS][2]
     const float up = vref * kPDown;
-    float* mine = mo + (warp * 8 + g) * R::kPitch + 2 * tq;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-        *reinterpret_cast<float2*>(mine + 8 * t) = make_float2((acc[t][0] + acc[t][2]) * up, (acc[t][1] + acc[t][3]) * up);
-    if (tq == 0) {
-        ml[(warp * 8 + g) * 2] = m;
-        ml[(warp * 8 + g) * 2 + 1] = l;
+    for (int h = 0; h < RL; ++h) {
+        const int at = warp * ROWS + 8 * h + g;
+        float* mine = mo + at * R::kPitch + 2 * tq;
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            *reinterpret_cast<float2*>(mine + 8 * t) =
+                ROWS == 8 ? make_float2((acc[t][0] + acc[t][2]) * up, (acc[t][1] + acc[t][3]) * up)
+                          : make_float2(acc[t][2 * h] * up, acc[t][2 * h + 1] * up);
+        if (tq == 0) {
+            ml[at * 2] = m[h];
+            ml[at * 2 + 1] = l[h];
+        }
     }
     __syncthreads();
     const int used = min(W, per_warp ? (c1 - c0 + per_warp - 1) / per_warp : 0);  // warps that had tiles
-    constexpr int PARTS = W / 8;  // warps of a row, each with a part of its columns
-    const int r = warp / PARTS, rr = grp * 8 + r;
-    if (rr >= rows) return;
-    // lane w has warp w's m and l
-    const float2 own = lane < used ? *reinterpret_cast<const float2*>(ml + (lane * 8 + r) * 2) : make_float2(-INFINITY, 0.f);
-    float mm = own.x;
+    constexpr int PARTS = W > ROWS ? W / ROWS : 1;  // warps of a row, each with a part of its columns
+    for (int r = warp / PARTS; r < ROWS; r += W / PARTS) {
+        const int rr = grp * ROWS + r;
+        if (rr >= rows) return;
+        // lane w has warp w's m and l
+        const float2 own = lane < used ? *reinterpret_cast<const float2*>(ml + (lane * ROWS + r) * 2) : make_float2(-INFINITY, 0.f);
+        float mm = own.x;
 #pragma unroll
-    for (int o = W / 2; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    mm = __shfl_sync(0xffffffffu, mm, 0);
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    const float fw = ex2(own.x - mu);
-    float ll = 0.f;
-    constexpr int D = HD / 32 / PARTS > 0 ? HD / 32 / PARTS : 1;
-    float v[D] = {};
-    const int d0 = (warp % PARTS) * (HD / PARTS) + lane;
+        for (int o = W / 2; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+        mm = __shfl_sync(0xffffffffu, mm, 0);
+        const float mu = mm == -INFINITY ? 0.f : mm;
+        const float fw = ex2(own.x - mu);
+        float ll = 0.f;
+        constexpr int D = HD / 32 / PARTS > 0 ? HD / 32 / PARTS : 1;
+        float v[D] = {};
+        const int d0 = (warp % PARTS) * (HD / PARTS) + lane;
 #pragma unroll 8
-    for (int w = 0; w < used; ++w) {
-        const float f = __shfl_sync(0xffffffffu, fw, w);
-        ll += f * __shfl_sync(0xffffffffu, own.y, w);
+        for (int w = 0; w < used; ++w) {
+            const float f = __shfl_sync(0xffffffffu, fw, w);
+            ll += f * __shfl_sync(0xffffffffu, own.y, w);
 #pragma unroll
-        for (int i = 0; i < D; ++i) v[i] += f * mo[(w * 8 + r) * R::kPitch + d0 + 32 * i];
-    }
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    const int tok = token_of(a, rr);
-    const long long ob = tok * a.os + (long long)(kvh * a.group + rr - tok * a.group) * hd;
-    const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
+            for (int i = 0; i < D; ++i) v[i] += f * mo[(w * ROWS + r) * R::kPitch + d0 + 32 * i];
+        }
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        const int tok = token_of(a, rr);
+        const long long ob = tok * a.os + (long long)(kvh * a.group + rr - tok * a.group) * hd;
+        const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
 #pragma unroll
-    for (int i = 0; i < D; ++i) {
-        const int p = d0 + 32 * i, d = (p & 7) * (HD / 8) + (p >> 3);
-        if (d >= hd) continue;
-        if (sh.whole()) o_store(a.o, a.type, ob + d, v[i] * inv);
-        else a.part_o[pr * hd + d] = v[i];
-    }
-    if (lane == 0 && warp % PARTS == 0) {
-        float* st = sh.whole() ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
-        st[0] = sh.whole() ? mu : mm;
-        st[1] = sh.whole() ? inv : ll;
+        for (int i = 0; i < D; ++i) {
+            const int p = d0 + 32 * i, d = (p & 7) * (HD / 8) + (p >> 3);
+            if (d >= hd) continue;
+            if (sh.whole()) o_store(a.o, a.type, ob + d, v[i] * inv);
+            else a.part_o[pr * hd + d] = v[i];
+        }
+        if (lane == 0 && warp % PARTS == 0) {
+            float* st = sh.whole() ? a.stats + ((size_t)kvh * rows + rr) * 2 : a.part_ml + pr * 2;
+            st[0] = sh.whole() ? mu : mm;
+            st[1] = sh.whole() ? inv : ll;
+        }
     }
 }
 
@@ -399,26 +451,48 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
         const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit;
         const float *ml = a.part_ml + pr * 2, *po = a.part_o + pr * hd;
         const int n = sh.count();
+        // lane s has share s's (and s + 32's) m and l
+        float2 own[kMaxSplit / 32];
         float mm = -INFINITY;
-        for (int s = lane; s < n; s += 32) mm = fmaxf(mm, ml[2 * s]);
+#pragma unroll
+        for (int i = 0; i < kMaxSplit / 32; ++i) {
+            own[i] = lane + 32 * i < n ? *reinterpret_cast<const float2*>(ml + 2 * (lane + 32 * i)) : make_float2(-INFINITY, 0.f);
+            mm = fmaxf(mm, own[i].x);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
         const float mu = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f, v[8] = {};
-#pragma unroll 4
-        for (int s = 0; s < n; ++s) {
-            const float f = ex2(ml[2 * s] - mu);
-            ll += f * ml[2 * s + 1];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (lane + 32 * i < hd) v[i] += f * po[(size_t)s * hd + lane + 32 * i];
-        }
+        for (int i = 0; i < kMaxSplit / 32; ++i) own[i].x = ex2(own[i].x - mu);
+        float ll = 0.f, v[8] = {};
+        // four columns of a share a lane and load; eight shares in flight (hd is a multiple of 16)
+        auto add = [&](int s, int from, float f) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (4 * lane + 128 * i < hd) {
+                    const float4 x = *reinterpret_cast<const float4*>(po + (size_t)(from + s) * hd + 4 * lane + 128 * i);
+                    v[4 * i] += f * x.x;
+                    v[4 * i + 1] += f * x.y;
+                    v[4 * i + 2] += f * x.z;
+                    v[4 * i + 3] += f * x.w;
+                }
+        };
+#pragma unroll
+        for (int i = 0; i < kMaxSplit / 32; ++i)
+#pragma unroll 8
+            for (int s = 0; s < min(32, n - 32 * i); ++s) {
+                const float f = __shfl_sync(0xffffffffu, own[i].x, s);
+                ll += f * __shfl_sync(0xffffffffu, own[i].y, s);
+                add(s, 32 * i, f);
+            }
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         const int tok = token_of(a, rr);
         const long long ob = tok * a.os + (long long)(kvh * a.group + rr - tok * a.group) * hd;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd) o_store(a.o, a.type, ob + lane + 32 * i, v[i] * inv);
+        for (int i = 0; i < 8; ++i) {
+            const int d = 4 * lane + 128 * (i / 4) + i % 4;
+            if (d < hd) o_store(a.o, a.type, ob + d, v[i] * inv);
+        }
         if (lane == 0 && !a.scores) {  // (the weights' CTAs of few rows take their own)
             float* d = a.stats + ((size_t)kvh * rows + rr) * 2;
             d[0] = mu;
@@ -429,8 +503,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
     const int keys = keys_of(past, a.n - 1, cap);
     const int key = ((int)blockIdx.x - joins) * 1024 + (int)threadIdx.x * 4;
     if (((int)blockIdx.x - joins) * 1024 >= keys) return;
-    const int nz = (rows + 7) / 8;
-    const float* t = a.scores + (size_t)kvh * nz * 8 * cap + key;
+    const float* t = a.scores + (size_t)kvh * ((rows + a.unit - 1) / a.unit * a.unit) * cap + key;
     float sum[4] = {};
     for (int r0 = 0; r0 < rows; r0 += 8) {
         float4 x[8];  // loaded before the statistics that they wait for
@@ -474,7 +547,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     Plan p{};
     const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head, hd = c.head_dim;
     p.prompt = rows > (size_t)kPromptRows;
-    p.unit = p.prompt ? prompt_unit((int)hd) : 8;
+    p.unit = p.prompt ? prompt_unit((int)hd) : rows > 8 && type != NEON_GGML_F32 ? 16 : 8;
     const size_t units = H * ((rows + p.unit - 1) / p.unit);
     // shares of the keys: as many as fill the SMs once
     p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, (size_t)c.capacity / 512}));
@@ -487,7 +560,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     p.stats = take(H * rows * 2 * sizeof(float));
     p.part_o = take(p.nsplit > 1 ? H * rows * p.nsplit * hd * sizeof(float) : 0);
     p.part_ml = take(p.nsplit > 1 ? H * rows * p.nsplit * 2 * sizeof(float) : 0);
-    p.scores = take(p.prompt ? 0 : H * ((rows + 7) / 8) * 8 * c.capacity * sizeof(float));
+    p.scores = take(p.prompt ? 0 : H * ((rows + p.unit - 1) / p.unit) * p.unit * c.capacity * sizeof(float));
     const size_t padded = (rows + 255) / 256 * 256;
     p.qfactor = take(p.prompt ? H * padded * sizeof(float) : 0);
     p.qt = take(p.prompt ? prompt_query_bytes(c, rows, type) : 0);
@@ -495,16 +568,38 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     return p;
 }
 
+template <int ROWS>
+int launch_rows(AttnArgs& a, cudaStream_t st) {
+    const int hd = (int)a.c.head_dim;
+    auto k = hd == 64    ? kv8_rows_kernel<64, true, ROWS>
+             : hd < 64   ? kv8_rows_kernel<64, false, ROWS>
+             : hd == 128 ? kv8_rows_kernel<128, true, ROWS>
+             : hd < 128  ? kv8_rows_kernel<128, false, ROWS>
+             : hd == 256 ? kv8_rows_kernel<256, true, ROWS>
+                         : kv8_rows_kernel<256, false, ROWS>;
+    const int smem = hd <= 64    ? RowTile<64, ROWS>::kSmem
+                     : hd <= 128 ? RowTile<128, ROWS>::kSmem
+                                 : RowTile<256, ROWS>::kSmem;
+    const int warps = hd <= 128 ? RowTile<128, ROWS>::kWarps : RowTile<256, ROWS>::kWarps;
+    // a tile per warp before another CTA joins (one token over 512 and 1500 rows takes 7.7 and 11.4 us; with no
+    // least share 7.6 and 11.3, with four tiles a warp 7.6 and 15.1: the fewer shares to join are free)
+    a.min_tiles = warps;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_rows_kernel)");
+    const unsigned groups = (unsigned)((a.n * a.group + ROWS - 1) / ROWS);
+    return launch("kv8_rows_kernel", k, dim3((unsigned)a.nsplit, a.c.n_kv_head, groups), warps * 32, (size_t)smem, st, 1, a);
+}
+
 }  // namespace
 
 size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
     // Fewer tokens may take more shares, but rows * shares is at most 148 units' rows (plan_of).
     const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head;
-    const size_t unit = rows > (size_t)kPromptRows ? std::max(8, prompt_unit((int)c.head_dim)) : 8;
+    const size_t unit = rows > (size_t)kPromptRows ? prompt_unit((int)c.head_dim) : 16;
     const size_t padded = (rows + 255) / 256 * 256;
     return H * rows * 2 * sizeof(float) + 148 * unit * (c.head_dim + 2) * sizeof(float) + H * padded * sizeof(float) +
            prompt_query_bytes(c, rows, NEON_GGML_F32) +
-           H * ((std::min<size_t>(rows, kPromptRows) + 7) / 8 * 8) * c.capacity * sizeof(float) + 10 * 1024;
+           H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * c.capacity * sizeof(float) + 10 * 1024;
 }
 
 int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t os, size_t n, size_t n_head,
@@ -534,7 +629,6 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     a.qfactor = (float*)(base + p.qfactor);
     a.err = err;
     const size_t rows = n * a.group;
-    const int hd = (int)c.head_dim;
     int rc;
     if (p.prompt) {
         a.tile_shift = prompt_tile_shift();
@@ -543,19 +637,7 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     } else {
         a.tile_shift = 5;
         if (weight) a.scores = (float*)(base + p.scores);
-        auto rows_kernel = hd == 64    ? kv8_rows_kernel<64, true>
-                           : hd < 64   ? kv8_rows_kernel<64, false>
-                           : hd == 128 ? kv8_rows_kernel<128, true>
-                           : hd < 128  ? kv8_rows_kernel<128, false>
-                           : hd == 256 ? kv8_rows_kernel<256, true>
-                                       : kv8_rows_kernel<256, false>;
-        const int smem = hd <= 64 ? RowTile<64>::kSmem : hd <= 128 ? RowTile<128>::kSmem : RowTile<256>::kSmem;
-        const int warps = hd <= 128 ? RowTile<128>::kWarps : RowTile<256>::kWarps;
-        a.min_tiles = warps;  // a tile per warp before another CTA joins
-        cudaError_t e = cudaFuncSetAttribute(rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return neon_internal::cuda_error(e, "cudaFuncSetAttribute(kv8_rows_kernel)");
-        rc = launch("kv8_rows_kernel", rows_kernel, dim3((unsigned)a.nsplit, c.n_kv_head, (unsigned)((rows + 7) / 8)),
-                    warps * 32, (size_t)smem, st, 1, a);
+        rc = p.unit == 8 ? launch_rows<8>(a, st) : launch_rows<16>(a, st);
     }
     const unsigned joins = a.nsplit > 1 ? (unsigned)((rows + 7) / 8) : 0;
     const unsigned sums = a.scores ? (c.capacity + 1023) / 1024 : 0;

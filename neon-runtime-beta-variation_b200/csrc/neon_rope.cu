@@ -248,7 +248,8 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
     a.back = backward != 0;
     a.mag = (float)rope->magnitude;
     rope_turns(*rope, &a.turns);
-    // Pieces per CTA: one to four a thread, so that CTAs in their table and CTAs in their heads share the SMs.
+    // Pieces per CTA: one to four a thread, so that CTAs in their table and CTAs in their heads share the SMs (4099
+    // positions of 32 heads: 16 us; always one 28, always four 16; one position of 24 heads: 2.2, always four 2.7).
     const int V1 = vec ? (int)V : half ? 1 : 2;
     const long long per = half ? (a.hd - a.pairs) / V1 : a.hd / V1, row = per * (long long)heads;
     const long long want = std::min<long long>(std::max<long long>((long long)n * row / (sms * 4), kThreads), 4 * kThreads);

@@ -277,6 +277,15 @@ def test_attention_of_prompts(kind, H, D, heads, past, n):
     check_attention(H, D, heads, past, n, kind)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("H,D,heads,past,n", [(2, 64, 22, 400, 1), (1, 48, 9, 5000, 1), (1, 128, 32, 3000, 1),
+                                              (1, 256, 31, 900, 1), (1, 64, 3, 20, 3), (1, 16, 16, 33, 2),
+                                              (3, 112, 51, 31, 1), (1, 64, 1, 0, 17), (150, 16, 1350, 70, 1)])
+def test_attention_of_shared_passes(kind, H, D, heads, past, n):
+    """9 to 32 rows of a KV head in 16 bits: sixteen share a pass."""
+    check_attention(H, D, heads, past, n, kind)
+
+
 @pytest.mark.parametrize("past,cap", [(5000, 6016), (3, 8192), (8000, 8032)])
 def test_attention_long(past, cap):
     check_attention(2, 64, 8, past, 1, "f32", cap=cap)
