@@ -1494,7 +1494,11 @@ int kv8_alloc(neon_model* m, int32_t* past, neon_kv8_t* c) {
     const size_t codes = H * cap * hd, scales = H * (cap / 32) * sizeof(float), tail = 4 * H * 32 * hd * sizeof(float);
     auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
     unsigned char* p = nullptr;
-    int rc = dev_alloc(m, (void**)&p, 2 * up(codes) + 2 * up(scales) + up(tail) + up(4 * H * sizeof(int32_t)));
+    const size_t bytes = 2 * up(codes) + 2 * up(scales) + up(tail) + up(4 * H * sizeof(int32_t));
+    int rc = dev_alloc(m, (void**)&p, bytes);
+    if (rc) return rc;
+    // (rows that set_length goes over before they are written are zeros, as in the fp32 cache)
+    rc = cuda_error_if(cudaMemset(p, 0, bytes), "cudaMemset");
     if (rc) return rc;
     c->n_kv_head = (uint32_t)H;
     c->head_dim = (uint32_t)hd;
@@ -1940,6 +1944,7 @@ int create_model(const neon_model_config_t* cfg, neon_comm_t comm, bool kv8, boo
         if (cudaMemcpy(m->rope_cs, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice) != cudaSuccess ||
             cudaMemset(m->d_err, 0, sizeof(unsigned)) != cudaSuccess ||
             (!kv8 && cudaMemset(m->K, 0, kv_bytes) != cudaSuccess) ||
+            (m->kv8_weight && cudaMemset(m->kv8_weight, 0, sizeof(float) * c.n_layer * m->n_kv_l * m->kv8_cap) != cudaSuccess) ||
             cudaMemset(m->am_key, 0, sizeof(unsigned long long)) != cudaSuccess ||
             cudaMemset(m->am_count, 0, sizeof(unsigned int)) != cudaSuccess ||
             (!kv8 && cudaMemset(m->V, 0, kv_bytes) != cudaSuccess))

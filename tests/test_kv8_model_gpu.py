@@ -113,6 +113,23 @@ def test_logits_over_the_cached_values(kw):
     close_logits(logits, one.forward(tokens, 75, *rows_of(m, 0, 78))[0])
 
 
+@pytest.mark.parametrize("start", [5, 32, 45, 159])
+def test_rows_gone_over_are_zeros(start):
+    """set_length beyond what was written: those rows are zeros, as in the fp32 cache, and have no weight yet."""
+    one = OneLayer()
+    m = N.Model(one.cfg, one.tensors(), kv8=True, kv_weights=True)
+    m.set_length(start)
+    out = m.forward([7])
+    k, v = rows_of(m, 0, start + 1)
+    assert not k[:start].any() and not v[:start].any()
+    want, _ = one.forward([7], start, k, v)
+    close_logits(out, want)
+    if start > 8:
+        m.kv_evict(8, 2, 2)
+        k, v = rows_of(m, 0, 8)
+        assert not k[:7].any() and k[7].any()
+
+
 def test_generate_is_forward_step_by_step():
     tensors = list(S.model_tensors(TINY, seed=3))
     prompt = S.prompt_tokens(12, TINY.n_vocab, 4)
