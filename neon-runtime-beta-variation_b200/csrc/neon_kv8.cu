@@ -122,8 +122,9 @@ __device__ __forceinline__ unsigned magnitude(const float (&x)[4]) {
 // A CTA of four warps per block, head and K or V; the first CTA of a head
 // takes its first block and then its last one, the only two that touch the
 // tail. A thread has 8 pieces of 4 values at head_dim 128, all loaded before
-// the first is used; memory bounds a prompt's append, one token's is a launch
-// and its latency.
+// the first is used. 8191 rows of 8 heads x 128 in bf16 take 19 us where their
+// bytes are 8: loads, the block's largest value, then the rounding, one after
+// the other in each CTA; one token's is a launch and its latency (4.4 us).
 
 struct AppendArgs {
     neon_kv8_t c;
@@ -283,7 +284,8 @@ AppendKernel append_kernel_for(int hd) {
 // read
 // ---------------------------------------------------------------------------
 // A piece of four codes per lane, so that a warp's loads and stores are whole
-// lines; eight pieces in flight a thread.
+// lines; eight pieces in flight a thread. The fp32 rows that it writes bound it:
+// 32768 rows of 8 heads x 128 take 60 us (5.6 TB/s).
 constexpr int kReadThreads = 256, kReadRows = 64;  // rows of a CTA
 
 __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const __grid_constant__ neon_kv8_t c, int row0, int n,
@@ -506,7 +508,9 @@ struct GatherArgs {
 constexpr int kGatherThreads = 128;
 
 // A CTA of four warps per new block, head and K or V, in pieces of four codes, P a thread. The largest magnitude is
-// a row's largest code times its scale. HD as for the append.
+// a row's largest code times its scale. HD as for the append. 32768 of 131071 rows of 8 heads x 128 take 55 us where
+// their bytes are 20: rows of 128 bytes from anywhere, and the rounding. CTAs that take several blocks, the next
+// one's rows loaded while one is quantised, are no faster (an eviction of 148 to 158 us against 146).
 template <int HD, int P = HD ? HD / 16 : 16>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
     extern __shared__ __align__(16) float rowbuf[];  // with rotation: the block's rows

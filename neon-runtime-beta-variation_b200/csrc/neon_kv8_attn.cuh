@@ -70,7 +70,7 @@ struct AttnArgs {
     float* part_o;   // [H][rows][nsplit][hd]: o of a split, not normalised, in units of
     float* part_ml;  // [H][rows][nsplit][2]: 2^m with m, and l
     float* scores;   // few rows, weights kept: [H][rows, to whole units][capacity] scores * log2(e), or null
-    // prompts: query tiles of 128 rows as fp16 (see kv8_queries_kernel), and the rows' factors
+    // prompts: query tiles of 128 rows as fp16 (put_queries in neon_kv8_prompt.cu), and the rows' factors
     unsigned char* qt;
     float* qfactor;
     unsigned* err;

@@ -14,10 +14,17 @@
 //
 // Codes are exact in fp16, so a tile of codes is half the traffic of a 16-bit
 // cache and costs a conversion (two permutes and a subtraction for four
-// codes), which four warps do once for all MT tiles. One warp issues the
-// products; the MT tiles alternate, so one's softmax runs under the other's
-// products. What bounds it: exp2 (16 a clock and SM) for types of 16 bits, the
-// products (twice as many) for fp32.
+// codes), which six warps do once for all MT tiles. A warp per query tile issues
+// its products; one tile's softmax runs under the other's products.
+//
+// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 360 us in bf16, 2048
+// in fp32 179: 0.76 PFLOP/s of products in bf16. Neither unit is full (tensor
+// pipe 36 %, exp2 at 40 % of its rate, issue 50 %): what bounds it is the chain
+// score product, read, softmax, write, output product of a row tile, of which
+// tensor memory holds two, and about a quarter of a CTA's time in its queries'
+// conversion before and the outputs after it. Reading the next tile's scores
+// early, into registers dealt out again for it, took 419 us where this order
+// took 369.
 //
 // The maximum is lazy: m only moves, and O is only rescaled, when a row's p
 // would sum to more than 2^8 in a tile (the result does not depend on m), so p
@@ -567,53 +574,53 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));  // whole warpgroups
         if (warp < kMmaWarp) {
-        // ---- conversion: codes to fp16, swizzled ----
-        constexpr int kConv = kConvWarps * 32;
-        const int ct = tid - kSoftWarps * 32;
-        const int pieces = hd / 16;                 // 16-byte pieces of a row
-        const int total = KT * pieces;
-        constexpr int L = (KT * PANELS * 4 + kConv - 1) / kConv;  // pieces per thread at most
-        const uint4* kc = reinterpret_cast<const uint4*>(a.c.k + (size_t)kvh * cap * hd);
-        const uint4* vc = reinterpret_cast<const uint4*>(a.c.v + (size_t)kvh * cap * hd);
-        const long long end = (long long)cap * pieces;
-        uint4 kr[L], vr[L];
-        int put[L];  // where a piece goes in a tile
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int p = ct + kConv * i, r = p / pieces;
-            put[i] = p < total ? put_at(KT, r, p - r * pieces) : -1;
-        }
-        auto load = [&](uint4 (&w)[L], const uint4* base, int j) {
-            const long long at = (long long)j * total + ct;
+            // ---- conversion: codes to fp16, swizzled ----
+            constexpr int kConv = kConvWarps * 32;
+            const int ct = tid - kSoftWarps * 32;
+            const int pieces = hd / 16;                 // 16-byte pieces of a row
+            const int total = KT * pieces;
+            constexpr int L = (KT * PANELS * 4 + kConv - 1) / kConv;  // pieces per thread at most
+            const uint4* kc = reinterpret_cast<const uint4*>(a.c.k + (size_t)kvh * cap * hd);
+            const uint4* vc = reinterpret_cast<const uint4*>(a.c.v + (size_t)kvh * cap * hd);
+            const long long end = (long long)cap * pieces;
+            uint4 kr[L], vr[L];
+            int put[L];  // where a piece goes in a tile
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                w[i] = make_uint4(0, 0, 0, 0);
-                if (put[i] >= 0 && at + kConv * i < end) w[i] = base[at + kConv * i];
+                const int p = ct + kConv * i, r = p / pieces;
+                put[i] = p < total ? put_at(KT, r, p - r * pieces) : -1;
             }
-        };
-        auto store = [&](const uint4 (&w)[L], unsigned char* d) {
+            auto load = [&](uint4 (&w)[L], const uint4* base, int j) {
+                const long long at = (long long)j * total + ct;
 #pragma unroll
-            for (int i = 0; i < L; ++i)
-                if (put[i] >= 0) put_codes(d, put[i], w[i]);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-        };
-        if (most) {
-            load(kr, kc, j0);
-            load(vr, vc, j0);
-        }
-        for (int i = 0; i < most; ++i) {
-            const int s = i % ST;
-            const uint32_t ph = (uint32_t)(i / ST) & 1;
-            if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->k_empty[s], ph ^ 1, &bar->dead, a.err))) break;
-            store(kr, ks + s * S::Stage);
-            if (lane == 0) bar_arrive(&bar->k_full[s]);
-            if (i + 1 < most) load(kr, kc, j0 + i + 1);
-            if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->v_empty[s], ph ^ 1, &bar->dead, a.err))) break;
-            store(vr, vs + s * S::Stage);
-            if (lane == 0) bar_arrive(&bar->v_full[s]);
-            if (i + 1 < most) load(vr, vc, j0 + i + 1);
-        }
+                for (int i = 0; i < L; ++i) {
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (put[i] >= 0 && at + kConv * i < end) w[i] = base[at + kConv * i];
+                }
+            };
+            auto store = [&](const uint4 (&w)[L], unsigned char* d) {
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (put[i] >= 0) put_codes(d, put[i], w[i]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            };
+            if (most) {
+                load(kr, kc, j0);
+                load(vr, vc, j0);
+            }
+            for (int i = 0; i < most; ++i) {
+                const int s = i % ST;
+                const uint32_t ph = (uint32_t)(i / ST) & 1;
+                if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->k_empty[s], ph ^ 1, &bar->dead, a.err))) break;
+                store(kr, ks + s * S::Stage);
+                if (lane == 0) bar_arrive(&bar->k_full[s]);
+                if (i + 1 < most) load(kr, kc, j0 + i + 1);
+                if (i >= ST && !__all_sync(0xffffffffu, wait_or(&bar->v_empty[s], ph ^ 1, &bar->dead, a.err))) break;
+                store(vr, vs + s * S::Stage);
+                if (lane == 0) bar_arrive(&bar->v_full[s]);
+                if (i + 1 < most) load(vr, vc, j0 + i + 1);
+            }
         } else if (warp - kMmaWarp < MT && (most || (a.weight && split == 0))) {
             // ---- products: a warp per query tile (a poll takes some 200 clocks while products read shared
             // memory; the other tile's products run meanwhile). The whole warp goes along and one elected lane
