@@ -231,7 +231,8 @@ typedef struct {
 
 /* One tensor of a rotation: n_heads heads of head_dim values per position,
  * positions x_stride (y_stride) values apart. Y may be X (then y_stride is
- * x_stride); otherwise they do not overlap. */
+ * x_stride); otherwise they do not overlap, nor does Y with the X or Y of
+ * another target of the call (heads side by side in one buffer do not). */
 typedef struct {
     const void* X;
     void* Y;

@@ -632,7 +632,7 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     int rc;
     if (p.prompt) {
         a.tile_shift = prompt_tile_shift();
-        a.min_tiles = 8;
+        a.min_tiles = 8;  // (300 tokens of 16 / 8 heads take 21.5 us with 8 and with 1, 21.7 with 32)
         rc = launch_prompt(a, st);
     } else {
         a.tile_shift = 5;

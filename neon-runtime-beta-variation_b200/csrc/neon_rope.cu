@@ -175,6 +175,16 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant
     }
 }
 
+// Whether n rows of x and n of y, each its stride and length in bytes, have no byte in common: rows of one buffer
+// side by side have not.
+bool apart(const void* px, size_t xs, size_t xrow, const void* py, size_t ys, size_t yrow, size_t n) {
+    const char *x = (const char*)px, *y = (const char*)py;
+    if (x + (n - 1) * xs + xrow <= y || y + (n - 1) * ys + yrow <= x) return true;
+    if (xs != ys || n == 1) return false;
+    const size_t d = x < y ? (size_t)(y - x) % xs : (xs - (size_t)(x - y) % xs) % xs;  // y's place in a row of x
+    return d >= xrow && d + yrow <= xs;
+}
+
 using RopeKernel = void (*)(RopeArgs);
 template <typename T>
 RopeKernel rope_kernel_for(bool vec, bool half) {
@@ -216,17 +226,18 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
         if (t.n_heads == 0 || t.n_heads > 65535) return error(NEON_ERR_INVALID, "rope: a target needs 1 to 65535 heads");
         if (t.x_stride < row || t.y_stride < row) return error(NEON_ERR_INVALID, "rope: stride smaller than the heads");
         if (!aligned(t.X, eb) || !aligned(t.Y, eb)) return error(NEON_ERR_INVALID, "rope: buffer not aligned to its type");
-        const char *x = (const char*)t.X, *y = (const char*)t.Y;
-        if (x == y) {
+        if (t.X == t.Y) {
             if (t.x_stride != t.y_stride && n > 1) return error(NEON_ERR_INVALID, "rope: in place, the strides must be equal");
-        } else {
-            const size_t xn = ((n - 1) * t.x_stride + row) * eb, yn = ((n - 1) * t.y_stride + row) * eb;
-            if (x < y + yn && y < x + xn) {
-                // rows of one buffer side by side are fine
-                const size_t d = (size_t)(x < y ? y - x : x - y), s = t.x_stride * eb;
-                if (t.x_stride != t.y_stride || d % s < row * eb || d % s > s - row * eb)
-                    return error(NEON_ERR_INVALID, "rope: X and Y overlap");
-            }
+        } else if (!apart(t.X, t.x_stride * eb, row * eb, t.Y, t.y_stride * eb, row * eb, n)) {
+            return error(NEON_ERR_INVALID, "rope: X and Y overlap");
+        }
+        for (size_t k = 0; k < g; ++k) {
+            const neon_rope_target_t& u = targets[k];
+            const size_t other = u.n_heads * head_dim * eb;
+            if (!apart(t.Y, t.y_stride * eb, row * eb, u.Y, u.y_stride * eb, other, n) ||
+                !apart(t.Y, t.y_stride * eb, row * eb, u.X, u.x_stride * eb, other, n) ||
+                !apart(t.X, t.x_stride * eb, row * eb, u.Y, u.y_stride * eb, other, n))
+                return error(NEON_ERR_INVALID, "rope: a target's Y overlaps another target");
         }
         vec = vec && aligned(t.X, 16) && aligned(t.Y, 16) && (n == 1 || (t.x_stride % V == 0 && t.y_stride % V == 0));
         a.x[g] = t.X;

@@ -55,6 +55,29 @@ def test_rope_arguments(kw, code, word):
     assert rope_call(**kw) == code and word in err()
 
 
+@pytest.mark.parametrize("second", [
+    (P, P, 256, 256, 4),                    # the same rows twice, in place
+    (P * 9, P, 256, 256, 4),                # one output of both
+    (P, P * 9, 256, 256, 2),                # reads what the first writes
+    (P + 4 * 1000, P * 9, 256, 256, 4),     # its last rows
+    (P + 4 * 200, P + 4 * 200, 256, 256, 1),
+    (P - 4 * 64, P - 4 * 64, 256, 256, 2),  # from before the first
+    (P + 4 * 256, P + 4 * 256, 300, 300, 4)])
+def test_rope_targets_are_apart(second):
+    assert rope_call(targets=[(P, P, 256, 256, 4), second]) == INVALID and "another target" in err()
+    assert rope_call(targets=[second, (P * 40, P, 256, 256, 4)]) == INVALID and "another target" in err()
+
+
+@pytest.mark.parametrize("first,second", [
+    ((P, P, 512, 512, 4), (P + 4 * 256, P + 4 * 256, 512, 512, 4)),     # side by side in one buffer
+    ((P + 4 * 448, P + 4 * 448, 512, 512, 1), (P, P, 512, 512, 7)),
+    ((P, P * 9, 256, 256, 4), (P, P * 20, 256, 256, 4)),                # one input read twice
+    ((P, P, 256, 256, 4), (P + 4 * 1024, P + 4 * 1024, 256, 256, 4))])  # one behind the other
+def test_rope_targets_side_by_side(first, second):
+    """Not refused for their places: the call after them is (n_heads 0)."""
+    assert rope_call(targets=[first, second, (P * 50, P * 50, 64, 64, 0)]) == INVALID and "1 to 65535 heads" in err()
+
+
 def test_rope_of_nothing():
     assert rope_call(n=0, pos=None) == 0
 
