@@ -155,7 +155,6 @@ __device__ __forceinline__ float put_queries(const AttnArgs& a, int kvh, int r0,
     const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qs * sizeof(T)) % 16 == 0;
     const float sign = a.scale < 0.f ? -1.f : 1.f, size = fabsf(a.scale);
     const int d = lane % LPR * 8, sub = lane / LPR;
-    const unsigned row_lanes = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << (sub * LPR);
     // token and head of the warp's first row; those of the next 32 by a product (below 2^7 rows: exact)
     const int tok0 = (r0 + row0) / a.group, head0 = r0 + row0 - tok0 * a.group;
     const unsigned magic = 65536u / (unsigned)a.group + 1u;
@@ -180,15 +179,23 @@ __device__ __forceinline__ float put_queries(const AttnArgs& a, int kvh, int r0,
                 for (int e = 0; e < 8; ++e) w[u].t[e] = q[e];
             }
         }
+        float most[U];  // the rows' largest values, each step for all rows: their latencies side by side
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float x[8], mx = 0.f;
+            most[u] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = to_f(w[u].t[e]);
-                mx = fmaxf(mx, fabsf(x[e]));
-            }
-            const unsigned top = __reduce_max_sync(row_lanes, __float_as_uint(mx)) >> 23;
+            for (int e = 0; e < 8; ++e) most[u] = fmaxf(most[u], fabsf(to_f(w[u].t[e])));
+        }
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; ++u) most[u] = fmaxf(most[u], __shfl_xor_sync(0xffffffffu, most[u], o));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = to_f(w[u].t[e]);
+            const unsigned top = __float_as_uint(most[u]) >> 23;
             const int e2 = top >= 255u ? 0 : min(120, 134 - (int)top);
             const float f = pow2(e2) * sign;
             if (d < PANELS * 64) {
