@@ -358,6 +358,68 @@ def test_not_finite_stays_in_its_rows(n):
         assert torch.isnan(o[32:, 2:]).all() and torch.isfinite(o[:32]).all() and torch.isfinite(o[:, :2]).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 40.0, 1e-30])
+def test_shared_passes_of_odd_values(kind, scale):
+    """Sixteen rows a pass: scales of scores, blocks of V of very different sizes and one of zeros, scores that rise
+    along the cache, and a query row that is not a number, which spoils itself and what it sees of the weights."""
+    H, D, heads, past, n = 2, 64, 10, 500, 3
+    k, v = rows(past + n, H, D, 20), rows(past + n, H, D, 21)
+    k *= torch.linspace(0.05, 3.0, past + n)[:, None, None]
+    v[32:64] *= 1e-6
+    v[64:96] *= 1e3
+    v[96:128] = 0
+    c = junk(N.Kv8Cache.empty(H, D, 640))
+    c.append(k.cuda(), v.cuda(), past + n)
+    c.past.fill_(past)
+    kk, vv = torch.empty(past + n, H, D, device="cuda"), torch.empty(past + n, H, D, device="cuda")
+    c.read(0, past + n, kk, vv)
+    q = torch.randn(n, heads, D, generator=torch.Generator().manual_seed(3)).to(getattr(torch, TYPES[kind][1])).cuda()
+    w = torch.zeros(H, 640, device="cuda")
+    o = attend(c, q, kind, weight=w, scale=scale)
+    kn, vn = cpu(kk).transpose(1, 0, 2), cpu(vv).transpose(1, 0, 2)
+    want, ww, big = O.attention(cpu(q), kn, vn, past, scale or D ** -0.5)
+    to, tw = tolerances(kind, want, big, vn, ww)
+    assert (np.abs(cpu(o) - want) <= to).all()
+    assert (np.abs(cpu(w[:, :past + n]) - ww) <= tw + 2.0 ** -23).all()
+    bad = q.clone()
+    bad[1, 2, 7] = float("nan")  # token 1, KV head 0
+    w.zero_()
+    p = attend(c, bad, kind, weight=w, scale=scale)
+    assert torch.isnan(p[1, 2]).all()
+    fine = torch.ones(n, heads, dtype=torch.bool, device="cuda")
+    fine[1, 2] = False
+    assert torch.equal(p[fine], o[fine])
+    assert torch.isnan(w[0, :past + 2]).all() and torch.isfinite(w[0, past + 2:]).all() and torch.isfinite(w[1]).all()
+
+
+def test_prompts_in_graphs_that_share_a_workspace():
+    """Two captured prompts with weights, replayed in turn over one workspace, at lengths other than the captured."""
+    H, D, heads, n = 2, 64, 4, 70
+    c, k, v = filled(H, D, 400, 512, 9, "bf16")
+    q = torch.randn(2, n, heads, D, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    out, weight = torch.empty_like(q), torch.zeros(2, H, 512, device="cuda")
+    ws = torch.empty(c.attention_workspace(heads, n), dtype=torch.uint8, device="cuda")
+    graphs = []
+    c.past.fill_(5)
+    for i in range(2):
+        c.attention(q[i], out[i], n, heads, ws, type=N.GGML_BF16, weight=weight[i])
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            c.attention(q[i], out[i], n, heads, ws, type=N.GGML_BF16, weight=weight[i], stream=torch.cuda.current_stream())
+        graphs.append(g)
+    for past in (330, 0, 129):
+        c.past.fill_(past)
+        weight.zero_()
+        for i in (1, 0):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            w = torch.zeros(H, 512, device="cuda")
+            assert torch.equal(out[i], attend(c, q[i].contiguous(), "bf16", weight=w)) and torch.equal(weight[i], w)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_a_long_share_of_keys(kind):
     """Many key tiles per CTA, scores that rise along the cache (m moves again and again) and values that agree."""
