@@ -17,11 +17,11 @@
 // codes), which six warps do once for all MT tiles. A warp per query tile issues
 // its products; one tile's softmax runs under the other's products.
 //
-// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 360 us in bf16, 2048
-// in fp32 179: 0.76 PFLOP/s of products in bf16. Neither unit is full (tensor
+// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 344 us in bf16, 2048
+// in fp32 172: 0.80 PFLOP/s of products in bf16. Neither unit is full (tensor
 // pipe 36 %, exp2 at 40 % of its rate, issue 50 %): what bounds it is the chain
 // score product, read, softmax, write, output product of a row tile, of which
-// tensor memory holds two, and about a quarter of a CTA's time in its queries'
+// tensor memory holds two, and about a fifth of a CTA's time in its queries'
 // conversion before and the outputs after it. Reading the next tile's scores
 // early, into registers dealt out again for it, took 419 us where this order
 // took 369.
@@ -145,7 +145,9 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
 // 64 values][128 rows][64] fp16, swizzled, row r times 2^e (its largest value near 2^7) and the sign of
 // the scale. Returns each lane's factor |scale| log2(e) 2^-e of row row0 + lane, 0 beyond the last row.
 // A lane has eight values, one 16-byte piece, of one of R rows at a time. (This code runs once per CTA, from
-// a cold instruction cache, and with the output takes a third of a short prompt: little of it, loads first.)
+// a cold instruction cache: little of it, loads first, and one step of the largest values for all rows of a batch.
+// Batches of twice the rows measured 390 us against 344 on a bf16 prompt, of half the rows 348; an fp32 prompt took
+// 190 and 180 against 172.)
 template <int PANELS, int TERMS, typename T>
 __device__ __forceinline__ float put_queries(const AttnArgs& a, int kvh, int r0, int row0, unsigned char* tile) {
     const int hd = (int)a.c.head_dim, rows = a.n * a.group, lane = threadIdx.x & 31;
