@@ -393,6 +393,30 @@ def test_shared_passes_of_odd_values(kind, scale):
     assert torch.isnan(w[0, :past + 2]).all() and torch.isfinite(w[0, past + 2:]).all() and torch.isfinite(w[1]).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompts_on_two_streams(D):
+    """Prompts with weights on two caches at once, short and long ones mixed: each as alone."""
+    H, heads = 2, 8
+    jobs = []
+    for s, (past, n, kind) in enumerate([(500, 300, "f16"), (0, 90, "f32")]):
+        c, _, _ = filled(H, D, past + n, 832, 30 + s, kind)
+        c.past.fill_(past)
+        q = torch.randn(n, heads, D, generator=torch.Generator().manual_seed(s)).to(getattr(torch, TYPES[kind][1])).cuda()
+        w = torch.zeros(H, 832, device="cuda")
+        alone = attend(c, q, kind, weight=w)
+        ws = torch.empty(c.attention_workspace(heads, n), dtype=torch.uint8, device="cuda")
+        jobs.append((c, q, n, kind, alone, w, torch.empty_like(q), torch.zeros_like(w), ws, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, q, n, kind, _, _, o, w, ws, st in jobs:
+            with torch.cuda.stream(st):
+                w.zero_()
+            c.attention(q, o, n, heads, ws, type=TYPES[kind][0], weight=w, stream=st)
+    torch.cuda.synchronize()
+    for _, _, _, _, alone, w, o, got, _, _ in jobs:
+        assert torch.equal(o, alone) and torch.equal(got, w)
+
+
 def test_prompts_in_graphs_that_share_a_workspace():
     """Two captured prompts with weights, replayed in turn over one workspace, at lengths other than the captured."""
     H, D, heads, n = 2, 64, 4, 70
