@@ -694,6 +694,8 @@ int neon_cuda_kv8_attention(const neon_kv8_t* cache, const void* dQ, size_t q_st
     if (workspace_bytes < need)
         return error(NEON_ERR_INVALID, "kv8: workspace below neon_cuda_kv8_attention_workspace() = " + std::to_string(need));
     if (scale == 0.f) scale = 1.f / std::sqrt((float)cache->head_dim);
+    if (!apart(dQ, q_stride * eb, row * eb, dO, o_stride * eb, row * eb, n))
+        return error(NEON_ERR_INVALID, "kv8: Q and O must not overlap");
     OnDevice dev(cache->k);
     if (dev.rc) return dev.rc;
     return kv8_attention(*cache, dQ, q_stride, dO, o_stride, n, n_head, scale, type, d_weight, workspace, dev.device,

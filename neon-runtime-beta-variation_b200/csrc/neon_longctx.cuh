@@ -137,6 +137,16 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, unsigne
 inline size_t type_bytes(int type) { return type == NEON_GGML_F32 ? 4 : type == NEON_GGML_F16 || type == NEON_GGML_BF16 ? 2 : 0; }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// Whether n rows of x and n of y, each its stride and length in bytes, have no byte in common: rows of one buffer
+// side by side have not.
+inline bool apart(const void* px, size_t xs, size_t xrow, const void* py, size_t ys, size_t yrow, size_t n) {
+    const char *x = (const char*)px, *y = (const char*)py;
+    if (x + (n - 1) * xs + xrow <= y || y + (n - 1) * ys + yrow <= x) return true;
+    if (xs != ys || n == 1) return false;
+    const size_t d = x < y ? (size_t)(y - x) % xs : (xs - (size_t)(x - y) % xs) % xs;  // y's place in a row of x
+    return d >= xrow && d + yrow <= xs;
+}
+
 // Runs a scope with the device of a buffer current.
 struct OnDevice {
     int prev = -1, device = -1, rc = NEON_OK;

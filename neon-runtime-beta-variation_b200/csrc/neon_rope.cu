@@ -175,16 +175,6 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant
     }
 }
 
-// Whether n rows of x and n of y, each its stride and length in bytes, have no byte in common: rows of one buffer
-// side by side have not.
-bool apart(const void* px, size_t xs, size_t xrow, const void* py, size_t ys, size_t yrow, size_t n) {
-    const char *x = (const char*)px, *y = (const char*)py;
-    if (x + (n - 1) * xs + xrow <= y || y + (n - 1) * ys + yrow <= x) return true;
-    if (xs != ys || n == 1) return false;
-    const size_t d = x < y ? (size_t)(y - x) % xs : (xs - (size_t)(x - y) % xs) % xs;  // y's place in a row of x
-    return d >= xrow && d + yrow <= xs;
-}
-
 using RopeKernel = void (*)(RopeArgs);
 template <typename T>
 RopeKernel rope_kernel_for(bool vec, bool half) {

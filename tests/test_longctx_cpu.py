@@ -138,6 +138,9 @@ def test_attention_arguments():
     assert f(c, P, 384, P * 2, 384, 4, 6, 0.0, 0, None, None, b.value, None) == INVALID
     assert f(c, P, 384, P, 384, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "same buffer" in err()
     assert f(c, P, 383, P * 2, 384, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "stride" in err()
+    for qs, o, os in ((384, 64, 384), (384, 4 * 384 - 1, 384), (384, -4 * 384 + 1, 384), (800, 384, 700), (800, 383, 800),
+                      (800, 417, 800), (800, -1, 800)):  # o: values from Q's first
+        assert f(c, P * 4, qs, P * 4 + 4 * o, os, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "not overlap" in err()
     assert f(c, P, 384, P * 2, 383, 4, 6, 0.0, 0, None, P, b.value, None) == INVALID and "stride" in err()
     assert f(c, P, 384, P * 2, 384, 4, 5, 0.0, 0, None, P, b.value, None) == INVALID and "n_kv_head" in err()
     assert f(c, P, 384, P * 2, 384, 4, 0, 0.0, 0, None, P, b.value, None) == INVALID
