@@ -28,7 +28,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-constexpr int kMaxSplit = 64;
+constexpr int kMaxSplit = 64;  // (one KV head over 60000 rows takes 25.6 us; with 32 shares 27.8)
 
 // ---------------------------------------------------------------------------
 // Eight or sixteen rows of one KV head over a share of the cache. The MMA's 16
@@ -549,8 +549,13 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     p.prompt = rows > (size_t)kPromptRows;
     p.unit = p.prompt ? prompt_unit((int)hd) : rows > 8 && type != NEON_GGML_F32 ? 16 : 8;
     const size_t units = H * ((rows + p.unit - 1) / p.unit);
-    // shares of the keys: as many as fill the SMs once
-    p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, (size_t)c.capacity / 512}));
+    // shares of the keys: as many as fill the SMs once, and for prompts at least 512 rows each (a share per 128 rows
+    // takes 24.5 us for 300 tokens where this takes 20.1; per 2048 rows, 54 for 40 tokens behind 2000 where this
+    // takes 26). Few rows take a block per warp at least (min_tiles: 512 rows, 256 above head_dim 128); the limit here
+    // only has to leave room for that (one token over 4000 rows of 8 heads x 128 takes 12.6 us; with a limit of one
+    // per 512 rows, seven shares of 18 blocks for 16 warps, 14.3), and is 1 for short caches, which then need no join.
+    const size_t most = p.prompt ? c.capacity / 512 : c.capacity < 1024 ? 1 : c.capacity / 256;
+    p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, most}));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t o = at;
