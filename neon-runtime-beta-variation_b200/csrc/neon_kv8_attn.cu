@@ -36,9 +36,10 @@ constexpr int kMaxSplit = 64;  // (one KV head over 60000 rows takes 25.6 us; wi
 // costs no extra products: a row's score is the sum of its two halves, and its
 // output likewise. Of more than eight rows in a 16-bit type they hold sixteen
 // rows' single terms (q is exact in one, up to values far below the row's
-// largest; p is rounded to 2^-11 of itself, as for prompts): 16 rows over
-// 120000 of 8 heads x 128 take 68 us where two passes of eight took 95, and 32
-// rows 102 where four took 186. Each warp streams its own tiles of 32 rows (a block of the
+// largest), and p's lo terms take a second product: 16 rows over 120000 of 8
+// heads x 128 take 69 us where two passes of eight took 95, and 32 rows 112
+// where four took 186 (with p rounded to one term, 2^-11 of itself: 63 and 100).
+// Each warp streams its own tiles of 32 rows (a block of the
 // cache: K's codes, then V's, a bulk copy each) through its own ring in shared
 // memory, with no barrier between the warps until their results are merged.
 // The order of the summed dimension is free, so each lane reads whole 16-byte
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(RowTile<HD, ROWS>::kThreads, 1) kv8_rows_kerne
                 for (int e = 0; e < 4; ++e) acc[n][e] *= f[ROWS == 8 ? 0 : e >> 1];
         }
         const float vr = vs == 0.f ? 0.f : vs / vref * kPUp;
-        uint32_t pf[2][4];
+        uint32_t pf[2][4], pl[2][ROWS == 16 ? 4 : 1];  // p's terms: of eight rows both in pf, of sixteen hi and lo
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -292,8 +293,8 @@ __global__ void __launch_bounds__(RowTile<HD, ROWS>::kThreads, 1) kv8_rows_kerne
                     const float p0 = ex2(t[h][j][0] - mu[h]), p1 = ex2(t[h][j][1] - mu[h]);
                     l[h] += p0 + p1;
                     const float x0 = on0 ? p0 * vr : 0.f, x1 = on1 ? p1 * vr : 0.f;
-                    if (ROWS == 8) split2(x0, x1, pf[k][2 * hf], pf[k][2 * hf + 1]);
-                    else pf[k][2 * hf + h] = h2_bits(__floats2half2_rn(x0, x1));
+                    if constexpr (ROWS == 8) split2(x0, x1, pf[k][2 * hf], pf[k][2 * hf + 1]);
+                    else split2(x0, x1, pf[k][2 * hf + h], pl[k][2 * hf + h]);
                 }
             }
         }
@@ -334,6 +335,12 @@ __global__ void __launch_bounds__(RowTile<HD, ROWS>::kThreads, 1) kv8_rows_kerne
                 mma16816(acc[4 * i + 1], pf[k], codes_hi(a01), codes_hi(b01));
                 mma16816(acc[4 * i + 2], pf[k], codes_lo(a23), codes_lo(b23));
                 mma16816(acc[4 * i + 3], pf[k], codes_hi(a23), codes_hi(b23));
+                if constexpr (ROWS == 16) {
+                    mma16816(acc[4 * i], pl[k], codes_lo(a01), codes_lo(b01));
+                    mma16816(acc[4 * i + 1], pl[k], codes_hi(a01), codes_hi(b01));
+                    mma16816(acc[4 * i + 2], pl[k], codes_lo(a23), codes_lo(b23));
+                    mma16816(acc[4 * i + 3], pl[k], codes_hi(a23), codes_hi(b23));
+                }
             }
         }
         give(it++);

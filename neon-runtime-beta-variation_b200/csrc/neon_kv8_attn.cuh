@@ -95,8 +95,8 @@ __device__ __forceinline__ Shares shares_of(const AttnArgs& a, int past, int uni
 }
 
 // Query rows of a KV head above which the prompt kernel takes them. Over 20000 rows of 8 heads x 128 the rows kernel
-// takes 32 rows in 41 us (fp32) and 32 us (bf16), the prompt kernel in 59 and 42; over 120000 it is 181 and 102
-// against 250 and 185. At 64 rows the prompt kernel is ahead for fp32 (59 against 71 us over 20000).
+// takes 32 rows in 41 us (fp32) and 32 us (bf16), the prompt kernel in 59 and 47; over 120000 it is 181 and 112
+// against 250 and 199. At 64 rows the prompt kernel is ahead for fp32 (59 against 71 us over 20000).
 constexpr int kPromptRows = 32;
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -8,23 +8,28 @@
 //   S = Q K^T    both operands in shared memory: Q as fp16 (fp32 queries as
 //                hi + lo terms, two products into one sum), K's codes as fp16
 //   P            one thread per row: t = s * (row factor * block scale), lazy
-//                running maximum, p = 2^(t - m), rounded to fp16 (types of 16
-//                bits) or split into hi + lo, written over S in tensor memory
-//   O += P V     P from tensor memory, V's codes as fp16 in shared memory
+//                running maximum, p = 2^(t - m), split into hi + lo, written
+//                over S in tensor memory
+//   O += P V     P from tensor memory (two products into one sum), V's codes
+//                as fp16 in shared memory
 //
 // Codes are exact in fp16, so a tile of codes is half the traffic of a 16-bit
 // cache and costs a conversion (two permutes and a subtraction for four
 // codes), which six warps do once for all MT tiles. A warp per query tile issues
 // its products; one tile's softmax runs under the other's products.
 //
-// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 344 us in bf16, 2048
-// in fp32 172: 0.80 PFLOP/s of products in bf16. Neither unit is full (tensor
-// pipe 36 %, exp2 at 40 % of its rate, issue 50 %): what bounds it is the chain
+// P has two terms in the types of 16 bits too: one, p to 2^-11 of itself, would
+// take 345 us for the bf16 prompt below, but an output far below its values then
+// shows it, and an fp16 output's error is 1.4 times its own rounding's.
+//
+// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 384 us in bf16, 2048
+// in fp32 171: 1.07 PFLOP/s of products in bf16, the second of P counted. No unit
+// is full: what bounds it is the chain
 // score product, read, softmax, write, output product of a row tile, of which
 // tensor memory holds two, and about a fifth of a CTA's time in its queries'
 // conversion before and the outputs after it. Reading the next tile's scores
 // early, into registers dealt out again for it, took 419 us where this order
-// took 369.
+// took 369 (with one term of P).
 //
 // The maximum is lazy: m only moves, and O is only rescaled, when a row's p
 // would sum to more than 2^8 in a tile (the result does not depend on m), so p
@@ -146,8 +151,8 @@ __device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile
 // the scale. Returns each lane's factor |scale| log2(e) 2^-e of row row0 + lane, 0 beyond the last row.
 // A lane has eight values, one 16-byte piece, of one of R rows at a time. (This code runs once per CTA, from
 // a cold instruction cache: little of it, loads first, and one step of the largest values for all rows of a batch.
-// Batches of twice the rows measured 390 us against 344 on a bf16 prompt, of half the rows 348; an fp32 prompt took
-// 190 and 180 against 172.)
+// Batches of twice the rows measured 390 us against 344 on a bf16 prompt with one term of P, of half the rows 348; an
+// fp32 prompt took 190 and 180 against 172.)
 template <int PANELS, int TERMS, typename T>
 __device__ __forceinline__ float put_queries(const AttnArgs& a, int kvh, int r0, int row0, unsigned char* tile) {
     const int hd = (int)a.c.head_dim, rows = a.n * a.group, lane = threadIdx.x & 31;
@@ -463,10 +468,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                             }
                             const __half2 h = __floats2half2_rn(w0, w1);
                             hi[b][e] = h2_bits(h);
+                            const float2 f = __half22float2(h);
+                            const float d0 = w0 - f.x, d1 = w1 - f.y;
+                            lo[b][e] = h2_bits(__floats2half2_rn(d0, d1));
                             if (TERMS == 2) {
-                                const float2 f = __half22float2(h);
-                                const float d0 = w0 - f.x, d1 = w1 - f.y;
-                                lo[b][e] = h2_bits(__floats2half2_rn(d0, d1));
                                 const int s = 2 * b + e / 8;
                                 hs[s] = e % 8 ? add2(hs[s], pair(f.x, f.y)) : pair(f.x, f.y);
                                 ls[s] = e % 8 ? add2(ls[s], pair(d0, d1)) : pair(d0, d1);
@@ -507,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {  // over the block's scores: hi in its first 16 columns, lo in the next
                     tmem_st16(sb + 32 * b, hi[b]);
-                    if (TERMS == 2) tmem_st16(sb + 32 * b + 16, lo[b]);
+                    tmem_st16(sb + 32 * b + 16, lo[b]);
                 }
             };
             for (int i = 0; i < n && alive; ++i) {
@@ -675,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 const uint32_t p = uniform(ts + (t & 1) * KT);
                 if (elected()) {
 #pragma unroll
-                    for (int x = 0; x < TERMS; ++x)
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
                         for (int s = 0; s < KT / 16; ++s)
                             mma_ts(to, p + 32 * (s >> 1) + 16 * x + 8 * (s & 1), operand_of(v + s * 128), id_o, t > 0 || x + s > 0);

@@ -1,0 +1,49 @@
+"""The 8-bit KV cache's attention keeps fp32's bits in every type and at every
+length (neon_cuda.h: computed in fp32, rounded once at the end), against
+float64 over the same codes.
+
+Tolerance, of an output: fp32 outputs as in test_kv8_gpu.py; those of 16 bits
+the same before their rounding, and half a step of their type for it. p is
+held in two fp16 terms (2^-22 of itself) in every type, so nothing else is
+added for the types of 16 bits."""
+import numpy as np
+import pytest
+
+import kv8_oracle as O
+import neon_cuda as N
+from test_kv8_gpu import TYPES, attend, cpu, device, no_device_errors, rows, tolerances  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def once_rounded(kind, want, big, v):
+    to, _ = tolerances("f32", want, big, v, np.zeros(1))
+    return to + (torch.finfo(getattr(torch, TYPES[kind][1])).eps / 2 * (np.abs(want) + to) if kind != "f32" else 0.0)
+
+
+def values(c, n, H, D):
+    k, v = torch.empty(n, H, D, device="cuda"), torch.empty(n, H, D, device="cuda")
+    c.read(0, n, k, v)
+    return cpu(k).transpose(1, 0, 2), cpu(v).transpose(1, 0, 2)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("H,D,heads,past,n", [(2, 64, 8, 60, 1), (2, 64, 24, 60, 1), (1, 128, 16, 90, 2),
+                                              (1, 48, 10, 60, 2), (1, 256, 12, 60, 1), (2, 64, 8, 60, 30),
+                                              (1, 128, 8, 90, 40), (1, 80, 4, 60, 40), (1, 192, 4, 60, 40),
+                                              (1, 256, 4, 60, 40)])
+def test_probabilities_keep_their_bits(kind, H, D, heads, past, n):
+    """Values of one size and either sign: an output far below the values shows how p was rounded, in calls of up
+    to 8 rows, of 9 to 32 and of more."""
+    g = torch.Generator().manual_seed(D + n)
+    k = rows(past + n, H, D, 3)
+    v = torch.where(torch.rand(past + n, H, D, generator=g) < 0.5, 1.0, -1.0)
+    c = N.Kv8Cache.empty(H, D, 192)
+    c.append(k.cuda(), v.cuda(), past + n)
+    c.past.fill_(past)
+    kn, vn = values(c, past + n, H, D)
+    q = (torch.randn(n, heads, D, generator=g) * 0.3).to(getattr(torch, TYPES[kind][1])).cuda()
+    want, _, big = O.attention(cpu(q), kn, vn, past, D ** -0.5)
+    off = np.abs(cpu(attend(c, q, kind)) - want)
+    assert (off <= once_rounded(kind, want, big, vn)).all(), (off / once_rounded(kind, want, big, vn)).max()
