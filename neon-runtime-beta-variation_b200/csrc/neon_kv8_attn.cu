@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
 struct Plan {
     bool prompt;
     int unit, nsplit;
-    size_t stats, part_o, part_ml, scores, qt, qfactor, bytes;  // offsets into the workspace
+    size_t stats, part_o, part_ml, sums, scores, qt, qfactor, bytes;  // offsets into the workspace
 };
 Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     Plan p{};
@@ -572,6 +572,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     p.stats = take(H * rows * 2 * sizeof(float));
     p.part_o = take(p.nsplit > 1 ? H * rows * p.nsplit * hd * sizeof(float) : 0);
     p.part_ml = take(p.nsplit > 1 ? H * rows * p.nsplit * 2 * sizeof(float) : 0);
+    p.sums = take(p.prompt && c.capacity > (size_t)kChainKeys ? units * p.unit * p.nsplit * hd * sizeof(float) : 0);
     p.scores = take(p.prompt ? 0 : H * ((rows + p.unit - 1) / p.unit) * p.unit * c.capacity * sizeof(float));
     const size_t padded = (rows + 255) / 256 * 256;
     p.qfactor = take(p.prompt ? H * padded * sizeof(float) : 0);
@@ -609,7 +610,11 @@ size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
     const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head;
     const size_t unit = rows > (size_t)kPromptRows ? prompt_unit((int)c.head_dim) : 16;
     const size_t padded = (rows + 255) / 256 * 256;
-    return H * rows * 2 * sizeof(float) + 148 * unit * (c.head_dim + 2) * sizeof(float) + H * padded * sizeof(float) +
+    const size_t parts = 148 * unit * (c.head_dim + 2) * sizeof(float);
+    const size_t sums = rows > (size_t)kPromptRows && c.capacity > (size_t)kChainKeys
+                            ? std::max(148 * unit, H * ((rows + unit - 1) / unit * unit)) * c.head_dim * sizeof(float)
+                            : 0;
+    return H * rows * 2 * sizeof(float) + parts + sums + H * padded * sizeof(float) +
            prompt_query_bytes(c, rows, NEON_GGML_F32) +
            H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * c.capacity * sizeof(float) + 10 * 1024;
 }
@@ -637,6 +642,7 @@ int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t
     a.stats = (float*)(base + p.stats);
     a.part_o = (float*)(base + p.part_o);
     a.part_ml = (float*)(base + p.part_ml);
+    a.sums = (float4*)(base + p.sums);
     a.qt = base + p.qt;
     a.qfactor = (float*)(base + p.qfactor);
     a.err = err;

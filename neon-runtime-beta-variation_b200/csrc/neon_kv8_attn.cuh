@@ -70,6 +70,7 @@ struct AttnArgs {
     float* part_o;   // [H][rows][nsplit][hd]: o of a split, not normalised, in units of
     float* part_ml;  // [H][rows][nsplit][2]: 2^m with m, and l
     float* scores;   // few rows, weights kept: [H][rows, to whole units][capacity] scores * log2(e), or null
+    float4* sums;    // prompts: o of the chains of a row that are done, see put_by
     // prompts: query tiles of 128 rows as fp16 (put_queries in neon_kv8_prompt.cu), and the rows' factors
     unsigned char* qt;
     float* qfactor;
@@ -98,6 +99,14 @@ __device__ __forceinline__ Shares shares_of(const AttnArgs& a, int past, int uni
 // takes 32 rows in 41 us (fp32) and 32 us (bf16), the prompt kernel in 59 and 47; over 120000 it is 181 and 112
 // against 250 and 199. At 64 rows the prompt kernel is ahead for fp32 (59 against 71 us over 20000).
 constexpr int kPromptRows = 32;
+
+// Keys whose outputs a prompt's products sum in one go, in fp32 and in types of 16 bits; longer shares are added up in
+// fp32 in the workspace (kv8_prompt_kernel's put_by). The products cut their sums off instead of rounding them, so what
+// came early in a sum fades: one sum over n keys leaves an output 1.4e-9 n off. 600 tokens of 64 / 8 heads x 128 in
+// fp32, error against float64 and time: over 4600 rows 1.1e-6 and 282 us (one sum: 5.0e-6 and 253; sums of 2048 keys:
+// 2.2e-6 and 263; an fp32 product's 1.3e-6), over 16600 rows 1.1e-6 and 1080 us (one sum: 2.1e-5 and 920), over 120600
+// 1.3e-6 and 8.6 ms (1.6e-4 and 7.7). 4096 keys' 5.7e-6 is a fortieth of an fp16 output's rounding.
+constexpr int kChainKeys = 1024, kChainKeys16 = 4096;
 
 constexpr float kLog2e = 1.4426950408889634f;
 

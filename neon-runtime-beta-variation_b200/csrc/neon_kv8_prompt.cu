@@ -22,8 +22,8 @@
 // take 345 us for the bf16 prompt below, but an output far below its values then
 // shows it, and an fp16 output's error is 1.4 times its own rounding's.
 //
-// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 384 us in bf16, 2048
-// in fp32 171: 1.07 PFLOP/s of products in bf16, the second of P counted. No unit
+// 4096 tokens of 64 / 8 heads x 128 from an empty cache take 388 us in bf16, 2048
+// in fp32 179: 1.06 PFLOP/s of products in bf16, the second of P counted. No unit
 // is full: what bounds it is the chain
 // score product, read, softmax, write, output product of a row tile, of which
 // tensor memory holds two, and about a fifth of a CTA's time in its queries'
@@ -291,6 +291,7 @@ template <int PANELS, typename T, int TERMS = sizeof(T) == 4 ? 2 : 1>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
     using S = Shape<PANELS, TERMS>;
     constexpr int MT = S::MT, KT = S::KT, ST = S::ST, NB = KT / 32;
+    constexpr int kChain = (TERMS == 2 ? kChainKeys : kChainKeys16) / KT;  // tiles whose outputs are summed in tensor memory
     extern __shared__ unsigned char raw[];
     unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     unsigned char *qs = smem, *ks = qs + MT * S::QTile, *vs = ks + ST * S::Stage;
@@ -364,7 +365,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // the keys that every row of the warp sees
             const int all = __reduce_min_sync(0xffffffffu, limit);
             float mref = -INFINITY, l = 0.f, vref = 0.f;
-            float lw = 0.f, lz = 0.f;  // the sum of p's terms, and the same as the products sum it (below)
+            float lw = 0.f, lz = 0.f;  // a chain's sum of p's terms, and the same as the products sum it (below)
+            float held = 1.f;          // what the chains that were put by are to be multiplied with
+            // those chains' sums: [32 rows][share][four columns][row][4], a warp's in whole lines
+            float4* sums = a.sums + (((size_t)kvh * units * (4 * MT) + (r0 >> 5) + (warp & 3)) * a.nsplit + split) * (size_t)hd * 8 + lane;
             bool alive = true;
             float nk[NB], nv[NB];  // the scales of the next tile's blocks (a load each: quicker here than shuffles)
             auto scales = [&](int j) {
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 const float f = vtop > 0.f ? fl * (vref / vtop) : fl;
                 // O once the tile before has been added: of the outputs, i - 1 or i have ended here (the scores of
                 // tile i come after output i - 2, output i needs this tile's P), so the parity is clear
-                if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                if (i % kChain && __any_sync(0xffffffffu, f != 1.f)) {
                     alive = __all_sync(0xffffffffu, wait_or(&bar->o_done[m], (uint32_t)(i - 1) & 1, &bar->dead, a.err));
                     tc_after();
 #pragma unroll 1
@@ -415,8 +419,50 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 l *= fl;
                 lw *= f;
                 lz *= f;
+                held *= f;
                 mref = mnew;
                 vref = vtop;
+            };
+            // The products cut each of their sums off towards zero, so that what came early in a long sum fades (see
+            // kChainKeys). So before every kChain-th tile the outputs so far are put by, added up in fp32 in the
+            // workspace, and the products begin a new sum; at the end what was put by is added to the last one.
+            auto put_by = [&](int i, bool end) {
+                float4 by[8];
+                auto fetch = [&](int c) {  // 32 columns of what was put by before
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        by[e] = i > kChain && c + 4 * e < hd ? sums[(c + 4 * e) * 8] : make_float4(0.f, 0.f, 0.f, 0.f);
+                };
+                fetch(0);
+                const float fix = TERMS == 2 && lz != 0.f ? lw / lz : 1.f;
+                if (!end) alive = __all_sync(0xffffffffu, wait_or(&bar->o_done[m], (uint32_t)(i - 1) & 1, &bar->dead, a.err));
+                tc_after();
+#pragma unroll 1
+                for (int c = 0; c < hd; c += 32) {
+                    if (c) fetch(c);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        if (c + 16 * b >= hd) break;
+                        uint32_t o[16];
+                        tmem_ld16(o, ot + c + 16 * b);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float4 x = by[4 * b + e];
+                            const float4 y = make_float4(fmaf(x.x, held, __uint_as_float(o[4 * e]) * fix), fmaf(x.y, held, __uint_as_float(o[4 * e + 1]) * fix),
+                                                         fmaf(x.z, held, __uint_as_float(o[4 * e + 2]) * fix), fmaf(x.w, held, __uint_as_float(o[4 * e + 3]) * fix));
+                            if (!end) sums[(c + 16 * b + 4 * e) * 8] = y;
+                            o[4 * e] = __float_as_uint(y.x);
+                            o[4 * e + 1] = __float_as_uint(y.y);
+                            o[4 * e + 2] = __float_as_uint(y.z);
+                            o[4 * e + 3] = __float_as_uint(y.w);
+                        }
+                        if (end) tmem_st16(ot + c + 16 * b, o);
+                    }
+                }
+                if (end) tmem_wait_st();
+                lw = lz = 0.f;
+                held = 1.f;
             };
             // A tile's P from its S; FULL: no key of the tile is hidden from a row of the warp. The maximum is not
             // taken: p at most 2^8 is all that P needs, and a sum of the row's p at most 2^8 says so. A row whose
@@ -489,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 l += add;
                 if (TERMS == 2) {
-                    // The products cut each of their sums off towards zero (measured: half an ulp per 16 keys and
-                    // term, -2e-6 of an output after 512 keys). lz is cut off the same way, in the same order, and
+                    // What the products cut off of a chain (half an ulp per 16 keys and term, -2e-6 of an output after
+                    // 512 keys) is taken out on average: lz is cut off the same way, in the same order, and
                     // lw / lz takes that out of the output: all of it where the values agree, most where they do not.
                     float all = 0.f;
 #pragma unroll
@@ -533,7 +579,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 ready = false;
                 tc_after();
-                if (moves) move(i, kf, vmax);
+                if (moves || (i && i % kChain == 0)) {
+                    if (i && i % kChain == 0) put_by(i, false);
+                    if (moves) move(i, kf, vmax);
+                }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) vr[b] = vb[b] == 0.f ? 0.f : __fdividef(vb[b], vref) * kPScale;
                 if ((j0 + i + 1) * KT <= all) tile(std::true_type{}, i);
@@ -546,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // ---- the row's output, or its part ----
             if (n && alive) alive = __all_sync(0xffffffffu, wait_or(&bar->o_full[m], 0, &bar->dead, a.err));
             tc_after();
+            if (n > kChain) put_by(n, true);
             const bool whole = sh.whole(), out = on;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale) * (TERMS == 2 && lz != 0.f ? lw / lz : 1.f);
@@ -683,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
                         for (int s = 0; s < KT / 16; ++s)
-                            mma_ts(to, p + 32 * (s >> 1) + 16 * x + 8 * (s & 1), operand_of(v + s * 128), id_o, t > 0 || x + s > 0);
+                            mma_ts(to, p + 32 * (s >> 1) + 16 * x + 8 * (s & 1), operand_of(v + s * 128), id_o, t % kChain || x + s > 0);
                     tc_commit(&bar->o_done[m]);
                     tc_commit(&bar->v_empty[t % ST]);
                     if (t + 1 == n) tc_commit(&bar->o_full[m]);

@@ -47,3 +47,30 @@ def test_probabilities_keep_their_bits(kind, H, D, heads, past, n):
     want, _, big = O.attention(cpu(q), kn, vn, past, D ** -0.5)
     off = np.abs(cpu(attend(c, q, kind)) - want)
     assert (off <= once_rounded(kind, want, big, vn)).all(), (off / once_rounded(kind, want, big, vn)).max()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("D", [64, 144])
+def test_prompt_sums_do_not_fade(kind, D):
+    """A long share of keys per CTA whose first half has values of 1 and whose second half has -1, each of nearly
+    the same weight: a sum in which the early ones have faded is not near zero."""
+    H, heads, n, past = 1, 64, 300 if D == 64 else 150, 40000
+    g = torch.Generator().manual_seed(D)
+    k = rows(past + n, H, D, 5)
+    v = torch.ones(past + n, H, D)
+    v[(past + n) // 2:] = -1.0
+    c = N.Kv8Cache.empty(H, D, (past + n + 31) // 32 * 32)
+    c.append(k.cuda(), v.cuda(), past + n)
+    c.past.fill_(past)
+    q = (torch.randn(n, heads, D, generator=g) * 0.05).to(getattr(torch, TYPES[kind][1])).cuda()
+    out = attend(c, q, kind).double()
+    kk, vv = torch.empty(past + n, H, D, device="cuda"), torch.empty(past + n, H, D, device="cuda")
+    c.read(0, past + n, kk, vv)
+    kk, vv = kk[:, 0].double(), vv[:, 0].double()
+    hidden = torch.ones(n, past + n, dtype=torch.bool, device="cuda").triu(past + 1)
+    for j in range(0, heads, 7):
+        s = (q[:, j].double() @ kk.T) * D ** -0.5
+        want = torch.softmax(s.masked_fill_(hidden, -torch.inf), 1) @ vv
+        big = (q[:, j].double().abs() @ kk.abs().T).amax(1) * D ** -0.5
+        to = once_rounded(kind, want.cpu().numpy(), big.cpu().numpy(), vv.cpu().numpy())
+        assert (np.abs(cpu(out[:, j] - want)) <= to).all(), (np.abs(cpu(out[:, j] - want)) / to).max()
