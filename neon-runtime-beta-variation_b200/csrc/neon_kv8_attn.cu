@@ -544,6 +544,13 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ A
 }
 
 
+// Shares of few rows' keys at least, so that a warp's sums go over 1024 keys at most (see kChainKeys): one token of 96
+// heads x 128 in fp32 over 120000 rows is 9e-7 off and takes 549 us (8.3e-6 and 686 in one share, 7500 keys a warp).
+size_t rows_least_shares(const neon_kv8_t& c) {
+    const size_t keys = (size_t)kChainKeys * (c.head_dim <= 128 ? RowTile<128, 8>::kWarps : RowTile<256, 8>::kWarps);
+    return std::min<size_t>(kMaxSplit, (c.capacity + keys - 1) / keys);
+}
+
 // The plan of a call, from what the host knows of it (not how many rows the cache holds).
 struct Plan {
     bool prompt;
@@ -563,6 +570,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     // per 512 rows, seven shares of 18 blocks for 16 warps, 14.3), and is 1 for short caches, which then need no join.
     const size_t most = p.prompt ? c.capacity / 512 : c.capacity < 1024 ? 1 : c.capacity / 256;
     p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, most}));
+    if (!p.prompt) p.nsplit = (int)std::max<size_t>(p.nsplit, rows_least_shares(c));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t o = at;
@@ -610,7 +618,8 @@ size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
     const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head;
     const size_t unit = rows > (size_t)kPromptRows ? prompt_unit((int)c.head_dim) : 16;
     const size_t padded = (rows + 255) / 256 * 256;
-    const size_t parts = 148 * unit * (c.head_dim + 2) * sizeof(float);
+    const size_t few = H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * rows_least_shares(c);
+    const size_t parts = std::max(148 * unit, few) * (c.head_dim + 2) * sizeof(float);
     const size_t sums = rows > (size_t)kPromptRows && c.capacity > (size_t)kChainKeys
                             ? std::max(148 * unit, H * ((rows + unit - 1) / unit * unit)) * c.head_dim * sizeof(float)
                             : 0;

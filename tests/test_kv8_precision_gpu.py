@@ -74,3 +74,24 @@ def test_prompt_sums_do_not_fade(kind, D):
         big = (q[:, j].double().abs() @ kk.abs().T).amax(1) * D ** -0.5
         to = once_rounded(kind, want.cpu().numpy(), big.cpu().numpy(), vv.cpu().numpy())
         assert (np.abs(cpu(out[:, j] - want)) <= to).all(), (np.abs(cpu(out[:, j] - want)) / to).max()
+
+
+@pytest.mark.parametrize("kind,heads", [("f32", 80), ("f16", 800)])
+@pytest.mark.parametrize("D", [16, 144])
+def test_token_sums_do_not_fade(kind, heads, D):
+    """One token of many KV heads over a long cache: so few shares that a warp would sum 16000 keys in one go. All
+    values are alike, and the output is that value."""
+    H, cap = 80, (1 << 18) if D == 16 else 1 << 17
+    past = cap - 100
+    g = torch.Generator(device="cuda").manual_seed(1)
+    c = N.Kv8Cache.empty(H, D, cap)
+    c.k.copy_(torch.randint(-127, 128, (H, cap, D), generator=g, device="cuda", dtype=torch.int8))
+    c.k_scale.fill_(0.01)
+    c.v.fill_(127)
+    c.v_scale.fill_(1 / 127)
+    c.past.fill_(past)
+    q = (torch.randn(1, heads, D, generator=g, device="cuda") * 0.2).to(getattr(torch, TYPES[kind][1]))
+    out = cpu(attend(c, q, kind))
+    value = np.full(out.shape, np.float64(np.float32(127) * np.float32(1 / 127)))
+    big = cpu(q.double().abs().sum(-1)) * 1.27 * D ** -0.5
+    assert (np.abs(out - value) <= once_rounded(kind, value, big, np.ones(1))).all(), np.abs(out - value).max()
