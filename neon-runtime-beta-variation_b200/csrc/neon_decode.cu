@@ -1488,7 +1488,8 @@ int kv8_layer(neon_model* m, uint32_t li, int seq) {
                                   m->stream);
 }
 
-// A cache in 8 bits of the model's shape in one allocation, `past` apart.
+// A cache in 8 bits of the model's shape in one allocation, `past` apart. Not
+// cleared: kv8_alloc_layer does that.
 int kv8_alloc(neon_model* m, int32_t* past, neon_kv8_t* c) {
     const size_t H = m->n_kv_l, hd = m->cfg.head_dim, cap = m->kv8_cap;
     const size_t codes = H * cap * hd, scales = H * (cap / 32) * sizeof(float), tail = 4 * H * 32 * hd * sizeof(float);
@@ -1496,9 +1497,6 @@ int kv8_alloc(neon_model* m, int32_t* past, neon_kv8_t* c) {
     unsigned char* p = nullptr;
     const size_t bytes = 2 * up(codes) + 2 * up(scales) + up(tail) + up(4 * H * sizeof(int32_t));
     int rc = dev_alloc(m, (void**)&p, bytes);
-    if (rc) return rc;
-    // (rows that set_length goes over before they are written are zeros, as in the fp32 cache)
-    rc = cuda_error_if(cudaMemset(p, 0, bytes), "cudaMemset");
     if (rc) return rc;
     c->n_kv_head = (uint32_t)H;
     c->head_dim = (uint32_t)hd;
@@ -1510,10 +1508,29 @@ int kv8_alloc(neon_model* m, int32_t* past, neon_kv8_t* c) {
     c->tail = (float*)(p + 2 * up(codes) + 2 * up(scales));
     c->tail_block = (int32_t*)(p + 2 * up(codes) + 2 * up(scales) + up(tail));
     c->past = past;
-    return cuda_error_if(cudaMemset(c->tail_block, 0xff, 4 * H * sizeof(int32_t)), "cudaMemset");
+    return NEON_OK;
 }
 
-// The spare cache, made by the first eviction or shift.
+// A layer's cache, at creation: rows that set_length goes over before they are
+// written are zeros, as in the fp32 cache. (create_model waits for the clears:
+// the model's stream does not wait for the legacy one.)
+int kv8_alloc_layer(neon_model* m, neon_kv8_t* c) {
+    int rc = kv8_alloc(m, m->d_pos, c);
+    if (rc) return rc;
+    const size_t codes = (size_t)m->n_kv_l * m->kv8_cap * m->cfg.head_dim, scales = m->n_kv_l * (m->kv8_cap / 32) * sizeof(float);
+    const size_t tail = 4 * (size_t)m->n_kv_l * 32 * m->cfg.head_dim * sizeof(float);
+    DEC_TRY(cudaMemset(c->k, 0, codes));
+    DEC_TRY(cudaMemset(c->v, 0, codes));
+    DEC_TRY(cudaMemset(c->k_scale, 0, scales));
+    DEC_TRY(cudaMemset(c->v_scale, 0, scales));
+    DEC_TRY(cudaMemset(c->tail, 0, tail));
+    DEC_TRY(cudaMemset(c->tail_block, 0xff, 4 * (size_t)m->n_kv_l * sizeof(int32_t)));
+    return NEON_OK;
+}
+
+// The spare cache, made by the first eviction or shift. What is read of it
+// (its first rows and their blocks' scales, its tags) has been written by the
+// kernel before, on the same stream: it needs no clearing.
 int kv8_need_spare(neon_model* m) {
     if (m->kv8_spare.k) return NEON_OK;
     int rc = dev_alloc(m, (void**)&m->kv8_one, sizeof(int));
@@ -1916,7 +1933,7 @@ int create_model(const neon_model_config_t* cfg, neon_comm_t comm, bool kv8, boo
         m->kv8_cap = ((size_t)c.ctx_len + 31) / 32 * 32;
         m->kv8_layers.resize(c.n_layer);
         for (auto& layer : m->kv8_layers)
-            if (!rc) rc = kv8_alloc(m, m->d_pos, &layer);
+            if (!rc) rc = kv8_alloc_layer(m, &layer);
         size_t ws = 0;
         if (!rc) ws = longctx::kv8_attention_workspace(m->kv8_layers[0], std::min(S, m->kv8_cap), m->n_head_l);
         A(&m->kv8_ws, ws);
@@ -1949,6 +1966,8 @@ int create_model(const neon_model_config_t* cfg, neon_comm_t comm, bool kv8, boo
             cudaMemset(m->am_count, 0, sizeof(unsigned int)) != cudaSuccess ||
             (!kv8 && cudaMemset(m->V, 0, kv_bytes) != cudaSuccess))
             rc = error(NEON_ERR_CUDA, "model initialisation copies failed");
+        // m->stream and the uploads' stream do not wait for the legacy stream, which the clears are on
+        if (!rc) rc = cuda_error_if(cudaStreamSynchronize(cudaStreamLegacy), "cudaStreamSynchronize");
     }
     if (!rc && !kv8) rc = build_kv_maps(m);
     if (!rc && !kv8 && c.ctx_len * sizeof(float) > 48 * 1024) {
