@@ -400,7 +400,11 @@ NEON_API int neon_cuda_model_generate(neon_model_t m, const int32_t* prompt, siz
                                       int32_t eos_id, int32_t* out_tokens, size_t* n_out);
 
 /* KV-cache length (KVCache::length), and rewinding it (run_generation's
- * prefix reuse, NEON-3.cpp:690-703). */
+ * prefix reuse, NEON-3.cpp:690-703). A length may also go beyond the rows that
+ * were written: a new model's cache has zeros there, a used one's what it held
+ * last. With the cache in 8 bits, where a step codes whole blocks anew, a
+ * rewind can be undone as long as no step has run since; any other rows that
+ * are gone over become zeros without attention weight. */
 NEON_API int neon_cuda_model_length(neon_model_t m, size_t* length);
 NEON_API int neon_cuda_model_set_length(neon_model_t m, size_t length);
 

@@ -1200,6 +1200,7 @@ struct neon_model {
     // [layer][n_kv_l][kv8_cap] of them; a spare cache for eviction and shifts
     bool kv8 = false;
     size_t kv8_cap = 0;
+    size_t kv8_rows = 0;  // rows from 0 on that are as they were written (set_length may go back and return)
     std::vector<neon_kv8_t> kv8_layers;
     float* kv8_weight = nullptr;
     void* kv8_ws = nullptr;
@@ -2191,6 +2192,7 @@ int neon_cuda_model_forward(neon_model_t m, const int32_t* tokens, size_t n, flo
     int rc = check_ready(m);
     if (rc) return rc;
     ModelDevice md(m->device);
+    m->kv8_rows = m->length;  // an append codes its blocks anew: rows behind it are not kept
     DEC_TRY(cudaEventRecord(m->evf0, m->stream));
     rc = forward_device(m, tokens, n);
     if (!rc) rc = cuda_error_if(cudaEventRecord(m->evf1, m->stream), "cudaEventRecord");
@@ -2198,6 +2200,7 @@ int neon_cuda_model_forward(neon_model_t m, const int32_t* tokens, size_t n, flo
     if (rc) return rc;
     cudaEventElapsedTime(&m->forward_ms, m->evf0, m->evf1);
     m->length += n;
+    m->kv8_rows = m->length;
     if (logits_host)
         DEC_TRY(cudaMemcpy(logits_host, m->world > 1 ? m->logits_full : m->logits, sizeof(float) * m->cfg.n_vocab,
                            cudaMemcpyDeviceToHost));
@@ -2262,6 +2265,7 @@ int neon_cuda_model_generate(neon_model_t m, const int32_t* prompt, size_t n_pro
     }
     *n_out = n;
     m->length += n;  // one forward per emitted token, as run_generation does
+    m->kv8_rows = m->length;
     return NEON_OK;
 }
 
@@ -2274,6 +2278,15 @@ int neon_cuda_model_length(neon_model_t m, size_t* length) {
 int neon_cuda_model_set_length(neon_model_t m, size_t length) {
     if (!m) return error(NEON_ERR_INVALID, "null model");
     if (length > m->cfg.ctx_len) return error(NEON_ERR_INVALID, "length above the KV-cache capacity");
+    if (m->kv8 && length > m->kv8_rows) {
+        ModelDevice md(m->device);
+        for (uint32_t li = 0; li < m->cfg.n_layer; ++li) {
+            float* w = m->kv8_weight ? m->kv8_weight + (size_t)li * m->n_kv_l * m->kv8_cap : nullptr;
+            const int rc = longctx::kv8_clear(m->kv8_layers[li], w, m->kv8_rows, length, m->stream);
+            if (rc) return rc;
+        }
+        m->kv8_rows = length;
+    }
     m->length = length;
     return NEON_OK;
 }
@@ -2302,7 +2315,7 @@ int neon_cuda_model_kv_shift(neon_model_t m, size_t keep, size_t discard) {
             if (!rc) rc = kv8_from_spare(m, li, left);
         }
         if (!rc) rc = cuda_error_if(cudaStreamSynchronize(m->stream), "cudaStreamSynchronize");
-        if (!rc) m->length = left;
+        if (!rc) m->length = m->kv8_rows = left;
         return rc;
     }
     if (!m->shift_scratch) {
@@ -2360,7 +2373,7 @@ int neon_cuda_model_kv_evict(neon_model_t m, size_t keep, size_t sink, size_t re
         if (!rc) rc = kv8_from_spare(m, li, keep);
     }
     if (!rc) rc = sync_and_check(m);
-    if (!rc) m->length = keep;
+    if (!rc) m->length = m->kv8_rows = keep;
     return rc;
 }
 

@@ -625,7 +625,38 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const __grid
     if (tid == 0) dsc[b] = sn;
 }
 
+// Rows from row0 to the end of row1's block as zeros: a CTA per block, head and K or V. The first block keeps its scale
+// where it has earlier rows, and the slot of the tail that holds it those rows; no slot holds one of the others any more.
+__global__ void __launch_bounds__(128) kv8_clear_kernel(const __grid_constant__ neon_kv8_t c, float* w, int row0, int row1) {
+    pdl_wait();
+    pdl_trigger();
+    const int hd = (int)c.head_dim, cap = (int)c.capacity, H = (int)c.n_kv_head, h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+    const int b0 = row0 >> 5, b = b0 + (int)blockIdx.x, r0 = b == b0 ? row0 & 31 : 0;
+    uint4* codes = reinterpret_cast<uint4*>((which ? c.v : c.k) + ((size_t)h * cap + 32 * b) * hd);
+    for (int i = r0 * hd / 16 + tid; i < 2 * hd; i += 128) codes[i] = make_uint4(0, 0, 0, 0);
+    if (r0 == 0 && tid == 0) (which ? c.v_scale : c.k_scale)[(size_t)h * (cap >> 5) + b] = 0.f;
+    if (which == 0 && w && tid < 32 && tid >= r0 && 32 * b + tid < row1) w[(size_t)h * cap + 32 * b + tid] = 0.f;
+    if (blockIdx.x) return;
+    int* tag = c.tail_block + ((size_t)which * H + h) * 2;
+    for (int s = 0; s < 2; ++s) {
+        const int g = tag[s];
+        if (r0 && g == b0) {
+            float4* t = reinterpret_cast<float4*>(c.tail + (((size_t)which * 2 + s) * H + h) * 32 * hd);
+            for (int i = r0 * hd / 4 + tid; i < 8 * hd; i += 128) t[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (g >= b0 && g <= (row1 - 1) >> 5) {
+            __syncthreads();  // every thread has read the tag
+            if (tid == 0) tag[s] = -1;
+        }
+    }
+}
+
 }  // namespace
+
+int kv8_clear(const neon_kv8_t& c, float* w, size_t row0, size_t row1, cudaStream_t st) {
+    if (row0 >= row1) return NEON_OK;
+    const unsigned blocks = (unsigned)((row1 + 31) / 32 - row0 / 32);
+    return launch("kv8_clear_kernel", kv8_clear_kernel, dim3(blocks, c.n_kv_head, 2), 128, 0, st, 1, c, w, (int)row0, (int)row1);
+}
 
 int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, size_t vs, size_t n, int type, int device,
                cudaStream_t st) {

@@ -20,5 +20,8 @@ int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, floa
 // The rows kept[n_kv_head][keep] (ascending, -1 behind the last) of src into dst; weights too unless null.
 int kv8_move(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, const neon_rope_t* rope,
              const int32_t* kept, cudaStream_t st);
+// Rows [row0, row1) as zeros without weight (w unless null), like rows of a new cache; those before them keep their
+// values and their tail, what lies behind them in the last block goes too.
+int kv8_clear(const neon_kv8_t& c, float* w, size_t row0, size_t row1, cudaStream_t st);
 
 }  // namespace longctx

@@ -34,3 +34,79 @@ def test_first_move_of_a_large_cache(how):
         logits = m.forward(tokens)
         close_logits(logits, one.forward(tokens, 100, *rows_of(m, 0, 103))[0])
         m.free()
+
+
+def gone_over(one, m, tokens, past, valid, step):
+    """After set_length(past) on a model with `valid` rows written: they stay, the others are zeros, and so the step runs."""
+    before = rows_of(m, 0, valid)
+    m.set_length(past)
+    k, v = rows_of(m, 0, past)
+    for x, y in zip((k, v), before):
+        assert np.array_equal(x[:valid], y) and not x[valid:].any()
+    logits = m.forward([tokens[step]])
+    k, v = rows_of(m, 0, past + 1)
+    assert not k[max(valid, past // 32 * 32):past].any() and not v[max(valid, past // 32 * 32):past].any()
+    close_logits(logits, one.forward([tokens[step]], past, k, v)[0])
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("steps,to", [(33, 110), (33, 97 + 31), (6, 75), (6, 64 + 6), (1, 159), (0, 90)])
+def test_rows_gone_over_in_a_used_model(steps, to, weights):
+    """A prompt and single steps fill both slots of the tail; then the length jumps inside the block or across some."""
+    one = OneLayer()
+    m = N.Model(one.cfg, one.tensors(), kv8=True, kv_weights=weights)
+    tokens = np.random.default_rng(6).integers(0, one.cfg.n_vocab, 64 + steps + 1)
+    m.forward(tokens[:64])
+    for t in tokens[64:64 + steps]:
+        m.forward([t])
+    gone_over(one, m, tokens, to, 64 + steps, -1)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("back,to", [(70, 96), (70, 75), (64, 100), (3, 159), (95, 97)])
+def test_rows_gone_over_after_a_rewind(back, to, weights):
+    """A rewound run's rows do not come back once a step has coded their block anew, nor do their weights."""
+    one = OneLayer()
+    m = N.Model(one.cfg, one.tensors(), kv8=True, kv_weights=weights)
+    tokens = np.random.default_rng(7).integers(0, one.cfg.n_vocab, 102)
+    m.forward(tokens[:100])
+    m.set_length(back)
+    m.forward([tokens[100]])
+    gone_over(one, m, tokens, to, back + 1, 101)
+    if not weights:
+        return
+    # of the rows between, those gone over have the last step's weight alone: the rest of them is chosen first
+    k, v = rows_of(m, 0, to + 1)
+    gone = to - back - 1
+    if gone > 1:
+        keep = to + 1 - gone
+        m.kv_evict(keep, 0, 1)
+        assert not any((rows_of(m, 0, keep)[1] == 0).all(axis=(1, 2)))
+
+
+def test_a_rewind_undone():
+    """Without a step between, set_length brings the rows back, and their tail: the cache is as if it had not been called."""
+    one = OneLayer()
+    a, b = (N.Model(one.cfg, one.tensors(), kv8=True) for _ in range(2))
+    tokens = np.random.default_rng(8).integers(0, one.cfg.n_vocab, 90)
+    for m in (a, b):
+        m.forward(tokens[:75])
+    a.set_length(10)
+    a.set_length(50)
+    a.set_length(75)
+    for m in (a, b):
+        m.forward(tokens[75:])
+    for x, y in zip(rows_of(a, 0, 90), rows_of(b, 0, 90)):
+        assert np.array_equal(x, y)
+
+
+def test_rows_gone_over_after_an_eviction():
+    one = OneLayer()
+    m = N.Model(one.cfg, one.tensors(), kv8=True, kv_weights=True)
+    tokens = np.random.default_rng(9).integers(0, one.cfg.n_vocab, 121)
+    m.forward(tokens[:120])
+    m.kv_evict(41, 4, 20)
+    gone_over(one, m, tokens, 100, 41, -1)
+    m.set_length(90)
+    m.kv_shift(2, 30)  # 60 rows
+    gone_over(one, m, tokens, 119, 60, -1)
