@@ -48,7 +48,7 @@ struct DeviceState {
     bool ready = false;
     int sms = 0;
     int smem_per_sm = 0;  // shared memory of one SM (bytes)
-    unsigned int* err = nullptr;  // device error word (g_neon_device_err on this device)
+    unsigned int* err = nullptr;  // device error words (g_neon_device_err on this device)
     unsigned int* err_host = nullptr;  // pinned copy of the error word, read back by the host-buffer calls
     std::mutex mu;
     // scratch of multi-position Q4_0 calls (activation quants)
@@ -66,9 +66,10 @@ DeviceState g_dev[kMaxDevices];
 std::mutex g_init_mu;
 }  // namespace
 
-// Device-side error word: bit 0 = a bounded wait in a kernel timed out, bit 1 =
-// rows beyond an 8-bit KV cache's capacity were dropped.
-static __device__ unsigned int g_neon_device_err;
+// Device-side error words: a bounded wait in a kernel timed out (reported by the
+// next call that waits for the device), rows beyond an 8-bit KV cache's capacity
+// were dropped (an operator's caller's affair: reported by neon_cuda_sync alone).
+static __device__ unsigned int g_neon_device_err[2];
 
 namespace {
 
@@ -693,17 +694,20 @@ int launch_dq(const std::vector<const neon_proj_target_t*>& t, int type, size_t 
     return NEON_OK;
 }
 
-// Reads (and clears) the device error word after the stream has drained.
-int check_device_err(int device) {
+// Reads (and clears) the device error word after the stream has drained; with `rows` the one of dropped rows too.
+int check_device_err(int device, bool rows = false) {
     if (device < 0 || device >= kMaxDevices || !g_dev[device].ready) return NEON_OK;
-    unsigned int v = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&v, g_neon_device_err, sizeof(v));
+    unsigned int v[2] = {0, 0};
+    cudaError_t e = cudaMemcpyFromSymbol(v, g_neon_device_err, sizeof(v));
     if (e != cudaSuccess) return cuda_err(e, "cudaMemcpyFromSymbol");
-    if (v) {
-        const unsigned int zero = 0;
+    const unsigned int zero = 0;
+    if (v[0]) {
         cudaMemcpyToSymbol(g_neon_device_err, &zero, sizeof(zero));
-        if (v == 2u) return set_err(NEON_ERR_INVALID, "kv8: rows beyond the cache's capacity were dropped");
         return set_err(NEON_ERR_CUDA, "a device-side wait timed out (shared-memory copy never completed)");
+    }
+    if (rows && v[1]) {
+        cudaMemcpyToSymbol(g_neon_device_err, &zero, sizeof(zero), sizeof(zero));
+        return set_err(NEON_ERR_INVALID, "kv8: rows beyond the cache's capacity were dropped");
     }
     return NEON_OK;
 }
@@ -963,6 +967,7 @@ int device_sms(int device) {
 }
 int check_device_error(int device) { return check_device_err(device); }
 unsigned* device_error_word(int device) { return init_device(device) ? nullptr : g_dev[device].err; }
+unsigned* device_rows_word(int device) { return init_device(device) ? nullptr : g_dev[device].err + 1; }
 }  // namespace neon_internal
 
 extern "C" {
@@ -1429,7 +1434,7 @@ int neon_cuda_sync(void* stream) {
     NEON_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     int device = 0;
     NEON_CUDA_TRY(cudaGetDevice(&device));
-    return check_device_err(device);
+    return check_device_err(device, true);
 }
 
 }  // extern "C"

@@ -175,8 +175,9 @@ int launched(int n);  // count kernels launched outside the matvec path
 bool pdl_enabled();
 int device_sms(int device);
 int check_device_error(int device);
-// The device's error word (neon_cuda_sync reports and clears it): bit 0 = a
-// bounded wait ran out, bit 1 = rows beyond an 8-bit KV cache's capacity were
-// dropped. Null, with the error set, when the device cannot be set up.
+// The device's error words, not zero: a bounded wait ran out; rows beyond an
+// 8-bit KV cache's capacity were dropped (neon_cuda_sync alone reports and
+// clears that one). Null, with the error set, when the device cannot be set up.
 unsigned* device_error_word(int device);
+unsigned* device_rows_word(int device);
 }  // namespace neon_internal

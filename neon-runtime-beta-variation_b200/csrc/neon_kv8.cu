@@ -132,7 +132,7 @@ struct AppendArgs {
     long long ks, vs;
     int n;
     bool vec;
-    unsigned* err;
+    unsigned* dropped;  // the device's word for rows beyond the capacity
 };
 constexpr int kAppThreads = 128;
 
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kAppThreads) kv8_append_kernel(const __grid_co
     const int h = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
     const int past = *a.c.past;
     if (past < 0 || (long long)past + a.n > cap) {
-        if (tid == 0 && h == 0 && which == 0 && blockIdx.x == 0) atomicOr(a.err, kErrRows);
+        if (tid == 0 && h == 0 && which == 0 && blockIdx.x == 0) *a.dropped = 1u;
         if (past < 0 || past >= cap) return;
     }
     const int end = (int)min((long long)past + a.n, (long long)cap);
@@ -660,8 +660,8 @@ int kv8_clear(const neon_kv8_t& c, float* w, size_t row0, size_t row1, cudaStrea
 
 int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, size_t vs, size_t n, int type, int device,
                cudaStream_t st) {
-    unsigned* err = neon_internal::device_error_word(device);
-    if (!err) return NEON_ERR_CUDA;
+    unsigned* dropped = neon_internal::device_rows_word(device);
+    if (!dropped) return NEON_ERR_CUDA;
     const size_t eb = type_bytes(type);
     AppendArgs a{};
     a.c = c;
@@ -671,7 +671,7 @@ int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, siz
     a.vs = (long long)vs;
     a.n = (int)n;
     a.vec = aligned(k, 4 * eb) && aligned(v, 4 * eb) && ks % 4 == 0 && vs % 4 == 0;
-    a.err = err;
+    a.dropped = dropped;
     AppendKernel kern = type == NEON_GGML_F32   ? append_kernel_for<float>((int)c.head_dim)
                         : type == NEON_GGML_F16 ? append_kernel_for<__half>((int)c.head_dim)
                                                 : append_kernel_for<__nv_bfloat16>((int)c.head_dim);

@@ -16,8 +16,7 @@
 
 namespace longctx {
 
-constexpr unsigned kErrWait = 1u;   // device error word: a bounded wait ran out
-constexpr unsigned kErrRows = 2u;   // rows beyond an 8-bit cache's capacity were dropped
+constexpr unsigned kErrWait = 1u;  // device error word: a bounded wait ran out
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

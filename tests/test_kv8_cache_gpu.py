@@ -1,0 +1,71 @@
+"""The 8-bit KV cache next to the library's other calls, and what its append
+leaves alone: rows beyond the capacity."""
+import numpy as np
+import pytest
+
+import kv8_oracle as O
+import neon_cuda as N
+import synth as S
+from test_kv8_gpu import cpu, device, no_device_errors, rows  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def test_dropped_rows_are_no_other_calls_error():
+    """neon_cuda_sync reports them, and nothing else does: not a matvec over host buffers, not a model's step."""
+    tiny = S.ModelConfig(300, 128, 1, 2, 1, 64, 128, ctx_len=64, rope_base=1e4)
+    m = N.Model(tiny, list(S.model_tensors(tiny, seed=3)), kv8=True)
+    w = N.TensorInfo("w", (64, 32), N.GGML_Q4_0, S.q4_0_weights(32, 64, 1))
+    x, y = np.ones(64, np.float32), np.zeros(32, np.float32)
+    N.proj_all_positions(w, x, 64, y, 32, 1)
+    first = m.forward([1, 2])
+    m.set_length(0)
+    c = N.Kv8Cache.empty(1, 64, 32)
+    k = rows(40, 1, 64, 1).cuda()
+    c.past.fill_(20)
+    N.sync()
+    c.append(k, k, 30)
+    torch.cuda.synchronize()
+    again = np.zeros(32, np.float32)
+    N.proj_all_positions(w, x, 64, again, 32, 1)
+    assert np.array_equal(again, y)
+    assert np.array_equal(m.forward([1, 2]), first) and m.length == 2
+    with pytest.raises(RuntimeError, match="capacity"):
+        N.sync()
+    N.sync()
+
+
+def test_rows_beyond_capacity_touch_nothing():
+    """Buffers inside larger ones: the rows before, the other heads' and everything around keep their bytes."""
+    H, D, cap, pad = 2, 64, 64, 4096
+    g = torch.Generator().manual_seed(3)
+
+    def inside(numel, dtype):
+        whole = torch.randint(1, 100, (pad + numel + pad,), generator=g).to(dtype).cuda()
+        return whole, whole[pad:pad + numel]
+
+    sizes = dict(k=(H * cap * D, torch.int8), v=(H * cap * D, torch.int8), k_scale=(H * cap // 32, torch.float32),
+                 v_scale=(H * cap // 32, torch.float32), tail=(4 * H * 32 * D, torch.float32),
+                 tail_block=(4 * H, torch.int32), past=(1, torch.int32))
+    whole, part = zip(*[inside(*s) for s in sizes.values()])
+    b = dict(zip(sizes, part))
+    b["tail_block"].fill_(-1)
+    before = [w.clone() for w in whole]
+    c = N.Kv8Cache(H, D, cap, *b.values())
+    x = rows(80, H, D, 10)
+    b["past"].fill_(40)
+    c.append(x.cuda(), (-x).cuda(), 64)  # rows 40 .. 103 of 64
+    with pytest.raises(RuntimeError, match="capacity"):
+        N.sync()
+    for name, w, was in zip(sizes, whole, before):
+        assert torch.equal(w[:pad], was[:pad]) and torch.equal(w[-pad:], was[-pad:]), name
+    for name, sign in (("k", 1), ("v", -1)):
+        was = dict(zip(sizes, before))[name][pad:-pad].view(H, cap, D)
+        scale = dict(zip(sizes, before))[name + "_scale"][pad:-pad].view(H, 2)
+        now, now_scale = b[name].view(H, cap, D), b[name + "_scale"].view(H, 2)
+        assert torch.equal(now[:, :32], was[:, :32]) and torch.equal(now_scale[:, 0], scale[:, 0])
+        for h in range(H):  # block 1: its earlier rows as their codes say, then the new ones
+            held = was[h, 32:40].float().cpu().numpy() * scale[h, 1].item()
+            cc, ss = O.quantise(np.concatenate([held, sign * x[:24, h].numpy()]))
+            assert np.array_equal(cpu(now[h, 32:]), cc) and now_scale[h, 1].item() == ss[0]
