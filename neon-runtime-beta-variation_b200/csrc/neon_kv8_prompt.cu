@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int blk = min(j * NB + b, (cap >> 5) - 1);  // (past the end: of hidden keys)
-                    nk[b] = __ldg(ksc + blk);
-                    nv[b] = __ldg(vsc + blk);
+                    nk[b] = ksc[blk];  // (not by the read-only path: an append that wrote them may end after this launch began)
+                    nv[b] = vsc[blk];
                 }
             };
             const int n = m == 0 ? nt[0] : nt[MT - 1];

@@ -69,3 +69,27 @@ def test_rows_beyond_capacity_touch_nothing():
             held = was[h, 32:40].float().cpu().numpy() * scale[h, 1].item()
             cc, ss = O.quantise(np.concatenate([held, sign * x[:24, h].numpy()]))
             assert np.array_equal(cpu(now[h, 32:]), cc) and now_scale[h, 1].item() == ss[0]
+
+
+@pytest.mark.parametrize("n,heads", [(200, 4), (1, 4)])
+def test_attention_right_behind_its_append(n, heads):
+    """An attention launched while the append before it still runs reads that append's scales: each step's block
+    scales are others, and the results are those of steps that wait."""
+    H, D, steps = 2, 64, 40
+    k = [(rows(n, H, D, s) * 2.0 ** (s % 9 - 4)).cuda() for s in range(steps)]
+    q = torch.randn(n, heads, D, generator=torch.Generator().manual_seed(1)).cuda()
+    runs = []
+    for wait in (False, True):
+        c = N.Kv8Cache.empty(H, D, 256)
+        ws = torch.empty(c.attention_workspace(heads, n), dtype=torch.uint8, device="cuda")
+        out = torch.empty(steps, n, heads, D, device="cuda")
+        torch.cuda.synchronize()
+        for s in range(steps):
+            c.append(k[s], k[s], n)
+            if wait:
+                torch.cuda.synchronize()
+            c.attention(q, out[s], n, heads, ws)
+            if wait:
+                torch.cuda.synchronize()
+        runs.append(out)
+    assert torch.equal(*runs)
