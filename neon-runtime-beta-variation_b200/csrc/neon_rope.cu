@@ -256,7 +256,7 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
     const long long want = std::min<long long>(std::max<long long>((long long)n * row / (sms * 4), kThreads), 4 * kThreads);
     a.tile = (int)std::min<long long>({std::max<long long>(1, want / row), (long long)kMaxTile, (long long)n});
     a.heads = row <= want ? (int)heads : (int)std::max<long long>(std::min<long long>(want / per, (long long)heads), 1);
-    if (heads > 65535 && a.heads == 1) a.heads = (int)((heads + 65534) / 65535);
+    a.heads = std::max(a.heads, (int)((heads + 65534) / 65535));  // (grid.y is at most 65535)
     const dim3 grid((unsigned)((n + a.tile - 1) / a.tile), (unsigned)((heads + a.heads - 1) / a.heads));
     RopeKernel k = type == NEON_GGML_F32   ? rope_kernel_for<float>(vec, half)
                    : type == NEON_GGML_F16 ? rope_kernel_for<__half>(vec, half)
