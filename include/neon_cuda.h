@@ -302,7 +302,8 @@ NEON_API int neon_cuda_kv8_attention(const neon_kv8_t* cache, const void* dQ, si
 NEON_API int neon_cuda_kv8_attention_workspace(const neon_kv8_t* cache, size_t n, size_t n_head, size_t* bytes);
 
 /* Eviction by accumulated attention weight, from `src` into the separate
- * buffers of `dst` (same heads and head_dim, capacity at least `keep`): when
+ * buffers of `dst` (same heads and head_dim, capacity at least `keep`; nothing
+ * that is written overlaps another buffer of the call): when
  * src holds more than `keep` rows, each KV head keeps its first `sink` rows,
  * its last `recent` rows, and of the rows between them the keep - sink -
  * recent of the largest weight (among equals the lowest row first; a NaN

@@ -761,9 +761,20 @@ int neon_cuda_kv8_evict(const neon_kv8_t* src, const float* d_weight, const neon
         return error(NEON_ERR_INVALID, "kv8: the caches' heads differ");
     if (keep == 0 || keep > dst->capacity) return error(NEON_ERR_INVALID, "kv8: keep must be 1 to the new cache's capacity");
     if (sink > keep || recent > keep - sink) return error(NEON_ERR_INVALID, "kv8: sink + recent above keep");
-    if (src->k == dst->k || src->v == dst->v || src->k_scale == dst->k_scale || src->v_scale == dst->v_scale ||
-        src->past == dst->past || src->tail_block == dst->tail_block || d_weight == d_weight_dst)
-        return error(NEON_ERR_INVALID, "kv8: eviction needs separate buffers");
+    const auto codes = [](const neon_kv8_t* c) { return (size_t)c->n_kv_head * c->capacity * c->head_dim; };
+    const size_t H = src->n_kv_head, from = codes(src), to = codes(dst), tags = H * 4 * sizeof(int32_t);
+    // (the tails are neither read nor written: one may serve both caches, as long as one of them is in use)
+    const Range in[] = {{src->k, from}, {src->v, from}, {src->k_scale, from / src->head_dim / 8}, {src->v_scale, from / src->head_dim / 8},
+                        {src->tail_block, tags}, {src->past, sizeof(int32_t)}, {d_weight, H * src->capacity * sizeof(float)}};
+    const Range out[] = {{dst->k, to}, {dst->v, to}, {dst->k_scale, to / dst->head_dim / 8}, {dst->v_scale, to / dst->head_dim / 8},
+                         {dst->tail_block, tags}, {dst->past, sizeof(int32_t)}, {d_weight_dst, H * dst->capacity * sizeof(float)},
+                         {d_kept, H * keep * sizeof(int32_t)}};
+    for (const Range& o : out) {
+        for (const Range& i : in)
+            if (o.meets(i)) return error(NEON_ERR_INVALID, "kv8: eviction needs separate buffers");
+        for (const Range& p : out)
+            if (&p != &o && o.meets(p)) return error(NEON_ERR_INVALID, "kv8: eviction needs separate buffers");
+    }
     OnDevice dev(src->k);
     if (dev.rc) return dev.rc;
     if (neon_internal::device_sms(dev.device) < 0) return NEON_ERR_CUDA;

@@ -146,6 +146,15 @@ inline bool apart(const void* px, size_t xs, size_t xrow, const void* py, size_t
     return d >= xrow && d + yrow <= xs;
 }
 
+// A buffer that a call reads or writes.
+struct Range {
+    const void* p;
+    size_t bytes;
+    bool meets(const Range& o) const {
+        return bytes && o.bytes && (const char*)p < (const char*)o.p + o.bytes && (const char*)o.p < (const char*)p + bytes;
+    }
+};
+
 // Runs a scope with the device of a buffer current.
 struct OnDevice {
     int prev = -1, device = -1, rc = NEON_OK;
