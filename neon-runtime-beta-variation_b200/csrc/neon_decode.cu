@@ -55,6 +55,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxChunk = 256;      // positions per forward chunk (prefill)
 constexpr int kMaxCtx = 16384;      // attention scores live in shared memory
+constexpr size_t kReadBytes = 16 << 20;  // device buffer of neon_cuda_model_read_kv over an 8-bit cache
 constexpr int kMaxCtxKv8 = 131072;  // with the KV cache in 8 bits (the RoPE table has a row per position)
 
 // neon_cuda_set_attn_rows: the decode attention's cache rows per CTA at
@@ -1208,7 +1209,8 @@ struct neon_model {
     float* kv8_spare_weight = nullptr;
     int32_t* kv8_kept = nullptr;
     int* kv8_one = nullptr;  // the spare cache's length
-    float* kv8_read = nullptr;  // rows read as floats
+    float* kv8_read = nullptr;  // kv8_read_rows rows of K and of V as floats, on their way to the host
+    size_t kv8_read_rows = 0;
     float2* rope_cs = nullptr;          // [ctx][rope_half]
     float *h = nullptr, *xn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *att = nullptr;
     float *gu = nullptr, *act = nullptr, *logits = nullptr;
@@ -1535,7 +1537,7 @@ int kv8_alloc_layer(neon_model* m, neon_kv8_t* c) {
 int kv8_need_spare(neon_model* m) {
     if (m->kv8_spare.k) return NEON_OK;
     int rc = dev_alloc(m, (void**)&m->kv8_one, sizeof(int));
-    if (!rc) rc = dev_alloc(m, (void**)&m->kv8_spare_weight, m->n_kv_l * m->kv8_cap * sizeof(float));
+    if (!rc && m->kv8_weight) rc = dev_alloc(m, (void**)&m->kv8_spare_weight, m->n_kv_l * m->kv8_cap * sizeof(float));
     if (!rc) rc = dev_alloc(m, (void**)&m->kv8_kept, m->n_kv_l * m->kv8_cap * sizeof(int32_t));
     neon_kv8_t c{};
     if (!rc) rc = kv8_alloc(m, m->kv8_one, &c);
@@ -1936,7 +1938,7 @@ int create_model(const neon_model_config_t* cfg, neon_comm_t comm, bool kv8, boo
         for (auto& layer : m->kv8_layers)
             if (!rc) rc = kv8_alloc_layer(m, &layer);
         size_t ws = 0;
-        if (!rc) ws = longctx::kv8_attention_workspace(m->kv8_layers[0], std::min(S, m->kv8_cap), m->n_head_l);
+        if (!rc) ws = longctx::kv8_attention_workspace(m->kv8_layers[0], std::min(S, m->kv8_cap), m->n_head_l, kv8_weights);
         A(&m->kv8_ws, ws);
         if (kv8_weights) A((void**)&m->kv8_weight, sizeof(float) * c.n_layer * m->n_kv_l * m->kv8_cap);
     }
@@ -2384,14 +2386,19 @@ int neon_cuda_model_read_kv(neon_model_t m, int layer, size_t n, float* k_host, 
     if (m->kv8) {
         if (n == 0) return NEON_OK;
         if (!m->kv8_read) {
-            int rc = dev_alloc(m, (void**)&m->kv8_read, 2 * sizeof(float) * (size_t)m->cfg.ctx_len * m->kv_dim);
+            const size_t rows = std::min<size_t>(m->cfg.ctx_len, std::max<size_t>(32, kReadBytes / (2 * sizeof(float) * m->kv_dim)));
+            int rc = dev_alloc(m, (void**)&m->kv8_read, 2 * sizeof(float) * rows * m->kv_dim);
             if (rc) return rc;
+            m->kv8_read_rows = rows;
         }
-        float* v = m->kv8_read + (size_t)m->cfg.ctx_len * m->kv_dim;
-        int rc = neon_cuda_kv8_read(&m->kv8_layers[layer], 0, n, m->kv8_read, v, m->stream);
-        if (rc) return rc;
-        DEC_TRY(cudaMemcpyAsync(k_host, m->kv8_read, sizeof(float) * n * m->kv_dim, cudaMemcpyDeviceToHost, m->stream));
-        DEC_TRY(cudaMemcpyAsync(v_host, v, sizeof(float) * n * m->kv_dim, cudaMemcpyDeviceToHost, m->stream));
+        float* v = m->kv8_read + m->kv8_read_rows * m->kv_dim;
+        for (size_t r = 0; r < n; r += m->kv8_read_rows) {
+            const size_t rows = std::min(n - r, m->kv8_read_rows), bytes = sizeof(float) * rows * m->kv_dim;
+            int rc = neon_cuda_kv8_read(&m->kv8_layers[layer], r, rows, m->kv8_read, v, m->stream);
+            if (rc) return rc;
+            DEC_TRY(cudaMemcpyAsync(k_host + r * m->kv_dim, m->kv8_read, bytes, cudaMemcpyDeviceToHost, m->stream));
+            DEC_TRY(cudaMemcpyAsync(v_host + r * m->kv_dim, v, bytes, cudaMemcpyDeviceToHost, m->stream));
+        }
         return cuda_error_if(cudaStreamSynchronize(m->stream), "cudaStreamSynchronize");
     }
     const size_t off = (size_t)layer * m->cfg.ctx_len * m->kv_dim;

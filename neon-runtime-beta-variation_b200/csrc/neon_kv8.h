@@ -12,7 +12,8 @@ int kv8_check(const neon_kv8_t* c);          // shape
 int kv8_check_buffers(const neon_kv8_t* c);  // shape and pointers
 int kv8_append(const neon_kv8_t& c, const void* k, size_t ks, const void* v, size_t vs, size_t n, int type, int device,
                cudaStream_t st);
-size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head);
+// (a caller that never asks for weights needs no room for the stored scores and queries that they are made from)
+size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head, bool weights);
 int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t os, size_t n, size_t n_head,
                   float scale, int type, float* weight, void* ws, int device, cudaStream_t st);
 int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,

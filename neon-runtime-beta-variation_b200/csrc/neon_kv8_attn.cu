@@ -581,6 +581,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     p.part_o = take(p.nsplit > 1 ? H * rows * p.nsplit * hd * sizeof(float) : 0);
     p.part_ml = take(p.nsplit > 1 ? H * rows * p.nsplit * 2 * sizeof(float) : 0);
     p.sums = take(p.prompt && c.capacity > (size_t)kChainKeys ? units * p.unit * p.nsplit * hd * sizeof(float) : 0);
+    // what only weights need comes last
     p.scores = take(p.prompt ? 0 : H * ((rows + p.unit - 1) / p.unit) * p.unit * c.capacity * sizeof(float));
     const size_t padded = (rows + 255) / 256 * 256;
     p.qfactor = take(p.prompt ? H * padded * sizeof(float) : 0);
@@ -613,7 +614,7 @@ int launch_rows(AttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
+size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head, bool weights) {
     // Fewer tokens may take more shares, but rows * shares is at most 148 units' rows (plan_of).
     const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head;
     const size_t unit = rows > (size_t)kPromptRows ? prompt_unit((int)c.head_dim) : 16;
@@ -623,9 +624,9 @@ size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head) {
     const size_t sums = rows > (size_t)kPromptRows && c.capacity > (size_t)kChainKeys
                             ? std::max(148 * unit, H * ((rows + unit - 1) / unit * unit)) * c.head_dim * sizeof(float)
                             : 0;
-    return H * rows * 2 * sizeof(float) + parts + sums + H * padded * sizeof(float) +
-           prompt_query_bytes(c, rows, NEON_GGML_F32) +
-           H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * c.capacity * sizeof(float) + 10 * 1024;
+    const size_t scores = H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * c.capacity * sizeof(float);
+    return H * rows * 2 * sizeof(float) + parts + sums + 10 * 1024 +
+           (weights ? H * padded * sizeof(float) + prompt_query_bytes(c, rows, NEON_GGML_F32) + scores : 0);
 }
 
 int kv8_attention(const neon_kv8_t& c, const void* q, size_t qs, void* o, size_t os, size_t n, size_t n_head,
@@ -697,7 +698,7 @@ int neon_cuda_kv8_attention_workspace(const neon_kv8_t* cache, size_t n, size_t 
     if (!bytes) return error(NEON_ERR_INVALID, "null bytes");
     int rc = check_heads(cache, n, n_head);
     if (rc) return rc;
-    *bytes = kv8_attention_workspace(*cache, n, n_head);
+    *bytes = kv8_attention_workspace(*cache, n, n_head, true);
     return NEON_OK;
 }
 
@@ -717,7 +718,7 @@ int neon_cuda_kv8_attention(const neon_kv8_t* cache, const void* dQ, size_t q_st
     if (!aligned(dQ, eb) || !aligned(dO, eb) || !aligned(d_weight, 4) || !aligned(workspace, 16))
         return error(NEON_ERR_INVALID, "kv8: buffer not aligned (workspace: 16 bytes)");
     if (!std::isfinite(scale)) return error(NEON_ERR_INVALID, "kv8: scale must be finite");
-    const size_t need = kv8_attention_workspace(*cache, n, n_head);
+    const size_t need = kv8_attention_workspace(*cache, n, n_head, true);
     if (workspace_bytes < need)
         return error(NEON_ERR_INVALID, "kv8: workspace below neon_cuda_kv8_attention_workspace() = " + std::to_string(need));
     if (scale == 0.f) scale = 1.f / std::sqrt((float)cache->head_dim);

@@ -110,3 +110,34 @@ def test_rows_gone_over_after_an_eviction():
     m.set_length(90)
     m.kv_shift(2, 30)  # 60 rows
     gone_over(one, m, tokens, 119, 60, -1)
+
+
+def test_memory_beyond_the_cache():
+    """A model with an 8-bit cache of 131072 rows holds the cache, the RoPE table and a few MB, and no room for the
+    weights that it does not keep; reading rows takes no buffer of the cache's length."""
+    one = OneLayer(ctx=131072, n_embd=128, n_head=8, n_kv=8, hd=128)
+    cache, table = 2 * 8 * 131072 * (128 + 4 / 32), 131072 * 64 * 8
+    torch.cuda.synchronize()
+
+    def used():
+        return torch.cuda.mem_get_info()[1] - torch.cuda.mem_get_info()[0]
+
+    N.Model(one.cfg, one.tensors(), kv8=True).free()  # the library's own set-up
+    start = used()
+    m = N.Model(one.cfg, one.tensors(), kv8=True)
+    tokens = np.random.default_rng(10).integers(0, one.cfg.n_vocab, 9000)
+    m.forward(tokens[:300])
+    assert used() - start <= cache + table + (48 << 20)
+    for t in range(300, 9000, 900):
+        m.forward(tokens[t:t + 900])
+    n = m.length
+    k, v = rows_of(m, 0, n)  # in pieces
+    k1, v1 = rows_of(m, 0, 40)
+    assert np.array_equal(k[:40], k1) and np.array_equal(v[:40], v1) and (np.abs(k).max(axis=(1, 2)) > 0).all()
+    assert used() - start <= cache + table + (72 << 20)
+    m.kv_shift(4, 100)
+    assert used() - start <= 2 * cache + table + (84 << 20)
+    k2, v2 = rows_of(m, 0, n - 100)
+    half = n // 2 // 32 * 32
+    assert np.abs(v2[half:half + 32] - v[half + 100:half + 132]).max() <= np.abs(v[half + 100:half + 132]).max() / 100
+    m.free()
