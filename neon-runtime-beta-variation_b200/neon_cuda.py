@@ -311,19 +311,16 @@ def sync(stream: int = 0) -> None:
 
 def _ptr(a) -> int:
     """Address of a numpy array, a torch tensor or an int."""
-    try:
-        return a.data_ptr()  # a torch tensor, the usual case of a short call
-    except AttributeError:
-        pass
     if a is None:
         return 0
     if isinstance(a, int):
         return a
     if isinstance(a, np.ndarray):
         return a.ctypes.data
-    if hasattr(a, "data_ptr"):
-        return int(a.data_ptr())
-    raise TypeError(f"cannot take the address of {type(a).__name__}")
+    try:
+        return a.data_ptr()
+    except AttributeError:
+        raise TypeError(f"cannot take the address of {type(a).__name__}") from None
 
 
 def _stream(stream) -> int:
