@@ -291,6 +291,12 @@ template <int PANELS, typename T, int TERMS = sizeof(T) == 4 ? 2 : 1>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ AttnArgs a, int tiles128) {
     using S = Shape<PANELS, TERMS>;
     constexpr int MT = S::MT, KT = S::KT, ST = S::ST, NB = KT / 32;
+    // What a tile's products cut off of their sums, as a part of the sum: some 0.4 ulps (an ulp is 0.72 * 2^-23 of a
+    // number in the mean) in each of KT / 16 steps of two terms. Measured over 950 keys: an fp32 output of equal values
+    // is 4.6e-6 short (0.88 ulps a step), one of values from 0.5 to 1.5 3.1e-6; with this added back 2.3e-6 and 8e-7,
+    // and one of values of either sign is 5.7e-7 off where it was 9.7e-7 (0.5 ulps: 1.7e-6, 2e-7 and 7.5e-7).
+    constexpr float kCut = 2 * (KT / 16) * 0.4f * 0.72f / 8388608.f;
+    static_assert(NB == 2, "two blocks a tile");
     constexpr int kChain = (TERMS == 2 ? kChainKeys : kChainKeys16) / KT;  // tiles whose outputs are summed in tensor memory
     extern __shared__ unsigned char raw[];
     unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
@@ -365,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // the keys that every row of the warp sees
             const int all = __reduce_min_sync(0xffffffffu, limit);
             float mref = -INFINITY, l = 0.f, vref = 0.f;
-            float lw = 0.f, lz = 0.f;  // a chain's sum of p's terms, and the same as the products sum it (below)
+            float lw = 0.f, cut = 0.f;  // fp32: a chain's sum of p's terms, and what the products cut off of it
             float held = 1.f;          // what the chains that were put by are to be multiplied with
             // those chains' sums: [32 rows][share][four columns][row][4], a warp's in whole lines
             float4* sums = a.sums + (((size_t)kvh * units * (4 * MT) + (r0 >> 5) + (warp & 3)) * a.nsplit + split) * (size_t)hd * 8 + lane;
@@ -418,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 l *= fl;
                 lw *= f;
-                lz *= f;
+                cut *= f;
                 held *= f;
                 mref = mnew;
                 vref = vtop;
@@ -434,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                         by[e] = i > kChain && c + 4 * e < hd ? sums[(c + 4 * e) * 8] : make_float4(0.f, 0.f, 0.f, 0.f);
                 };
                 fetch(0);
-                const float fix = TERMS == 2 && lz != 0.f ? lw / lz : 1.f;
+                const float fix = TERMS == 2 && lw != 0.f ? 1.f + cut / lw : 1.f;
                 if (!end) alive = __all_sync(0xffffffffu, wait_or(&bar->o_done[m], (uint32_t)(i - 1) & 1, &bar->dead, a.err));
                 tc_after();
 #pragma unroll 1
@@ -461,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     }
                 }
                 if (end) tmem_wait_st();
-                lw = lz = 0.f;
+                lw = cut = 0.f;
                 held = 1.f;
             };
             // A tile's P from its S; FULL: no key of the tile is hidden from a row of the warp. The maximum is not
@@ -477,8 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 const uint32_t sb = st + (i & 1) * KT;
                 constexpr int AT = TERMS == 1 ? NB : 1;  // blocks read at once, as registers allow
                 uint32_t hi[NB][16], lo[NB][16];
-                uint64_t hs[2 * NB], ls[2 * NB];
-                float add;
+                float add, terms = 0.f;
                 for (;;) {
                     const float mu = mref == -INFINITY ? 0.f : mref;
                     const uint64_t mu2 = pair(-mu, -mu);
@@ -506,7 +511,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                                 if (2 * e + 1 >= c) p1 = 0.f;
                             }
                             const uint64_t p = pair(p0, p1);
-                            sum[e & 1] = add2(sum[e & 1], p);
+                            uint64_t& to = sum[TERMS == 2 ? b : e & 1];
+                            to = add2(to, p);
                             unpair(mul2(p, vr2), w0, w1);
                             if (!FULL) {  // (a scale that is not finite may lie behind a row's keys)
                                 if (2 * e >= c) w0 = 0.f;
@@ -517,16 +523,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                             const float2 f = __half22float2(h);
                             const float d0 = w0 - f.x, d1 = w1 - f.y;
                             lo[b][e] = h2_bits(__floats2half2_rn(d0, d1));
-                            if (TERMS == 2) {
-                                const int s = 2 * b + e / 8;
-                                hs[s] = e % 8 ? add2(hs[s], pair(f.x, f.y)) : pair(f.x, f.y);
-                                ls[s] = e % 8 ? add2(ls[s], pair(d0, d1)) : pair(d0, d1);
-                            }
                         }
                     }
-                    float s0, s1;
-                    unpair(add2(sum[0], sum[1]), s0, s1);
-                    add = s0 + s1;
+                    float s0, s1, s2, s3;
+                    unpair(sum[0], s0, s1);
+                    unpair(sum[1], s2, s3);
+                    add = (s0 + s1) + (s2 + s3);
+                    if (TERMS == 2)  // (a block behind the row's keys adds 0, whatever its scale)
+                        terms = (s0 + s1 != 0.f ? (s0 + s1) * vr[0] : 0.f) + (s2 + s3 != 0.f ? (s2 + s3) * vr[NB - 1] : 0.f);
                     const float before = mref;
                     if (!__any_sync(0xffffffffu, add > kMostP)) break;
                     move(i, kf, vmax);
@@ -535,25 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 l += add;
                 if (TERMS == 2) {
-                    // What the products cut off of a chain (half an ulp per 16 keys and term, -2e-6 of an output after
-                    // 512 keys) is taken out on average: lz is cut off the same way, in the same order, and
-                    // lw / lz takes that out of the output: all of it where the values agree, most where they do not.
-                    float all = 0.f;
-#pragma unroll
-                    for (int s = 0; s < 2 * NB; ++s) {
-                        float x0, x1;
-                        unpair(hs[s], x0, x1);
-                        lz = __fadd_rz(lz, x0 + x1);
-                        all += x0 + x1;
-                    }
-#pragma unroll
-                    for (int s = 0; s < 2 * NB; ++s) {
-                        float x0, x1;
-                        unpair(ls[s], x0, x1);
-                        lz = __fadd_rz(lz, x0 + x1);
-                        all += x0 + x1;
-                    }
-                    lw += all;
+                    lw += terms;
+                    cut += kCut * lw;
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {  // over the block's scores: hi in its first 16 columns, lo in the next
@@ -598,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (n > kChain) put_by(n, true);
             const bool whole = sh.whole(), out = on;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale) * (TERMS == 2 && lz != 0.f ? lw / lz : 1.f);
+            const float up = (whole ? inv : 1.f) * vref * (1.f / kPScale) * (TERMS == 2 && lw != 0.f ? 1.f + cut / lw : 1.f);
             const size_t pr = ((size_t)kvh * rows + rr) * a.nsplit + split;
             const long long ob = (long long)(rr / a.group) * a.os + (long long)(kvh * a.group + rr % a.group) * hd;
             float* po = a.part_o + pr * hd;

@@ -95,3 +95,22 @@ def test_token_sums_do_not_fade(kind, heads, D):
     value = np.full(out.shape, np.float64(np.float32(127) * np.float32(1 / 127)))
     big = cpu(q.double().abs().sum(-1)) * 1.27 * D ** -0.5
     assert (np.abs(out - value) <= once_rounded(kind, value, big, np.ones(1))).all(), np.abs(out - value).max()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_sums_are_not_short(D):
+    """fp32 prompts over values that are all alike: the mean of the outputs is the value. The products sum the two terms
+    of 16 keys at a time, and may cut up to an ulp off of the sum so far, which is 0.72 * 2^-23 of it in the mean: of a
+    sum that grows evenly over the 992 keys' 124 steps half as much as 124 such cuts of the whole. 0.4 of that is
+    added back, so that at most 0.6 of it stays, and what is rounded to nearest, 16 tiles' sums at most 2^-24 each."""
+    H, heads, past, n, cap = 2, 8, 892, 100, 992
+    g = torch.Generator().manual_seed(D)
+    k, v = rows(past + n, H, D, 7), torch.ones(past + n, H, D)
+    c = N.Kv8Cache.empty(H, D, cap)
+    c.append(k.cuda(), v.cuda(), past + n)
+    c.past.fill_(past)
+    q = (torch.randn(n, heads, D, generator=g) * 0.2).cuda()
+    out = cpu(attend(c, q, "f32"))
+    value = np.float64(np.float32(127) * np.float32(1 / 127))
+    most = 124 / 2 * 0.72 * 2.0 ** -23
+    assert abs(out.mean() / value - 1) <= 0.6 * most + 2.0 ** -20
