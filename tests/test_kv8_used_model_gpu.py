@@ -141,3 +141,35 @@ def test_memory_beyond_the_cache():
     half = n // 2 // 32 * 32
     assert np.abs(v2[half:half + 32] - v[half + 100:half + 132]).max() <= np.abs(v[half + 100:half + 132]).max() / 100
     m.free()
+
+
+def test_layers_do_not_mix():
+    """Three layers share one spare cache: each keeps rows of its own, twice over."""
+    cfg = S.ModelConfig(300, 128, 3, 4, 2, 64, 128, ctx_len=256, rope_base=1e4)
+    m = N.Model(cfg, list(S.model_tensors(cfg, seed=5)), kv8=True, kv_weights=True)
+    g = np.random.default_rng(11)
+    m.forward(g.permutation(cfg.n_vocab)[:200])  # (rows of the same token are the same in layer 0)
+    for keep, sink, recent in ((120, 4, 30), (61, 2, 20)):
+        n = m.length
+        before = [rows_of(m, li, n) for li in range(3)]
+        m.kv_evict(keep, sink, recent)
+        chosen = []
+        for li in range(3):
+            v = rows_of(m, li, keep)[1]
+            for h in range(cfg.n_kv_head):
+                old = before[li][1][:, h]
+                r = np.array([np.abs(old - x).max(1).argmin() for x in v[:, h]])
+                step = np.repeat([np.abs(v[b:b + 32, h]).max() / 127 for b in range(0, keep, 32)], 32)[:keep]
+                assert (np.abs(old[r] - v[:, h]).max(1) <= step * (0.5 + 2.0 ** -10)).all()  # a row of this layer, coded again
+                assert (np.diff(r) > 0).all() and np.array_equal(r[:sink], np.arange(sink))
+                assert np.array_equal(r[keep - recent:], np.arange(n - recent, n))
+                chosen.append(tuple(r))
+        assert len(set(chosen)) > 1  # by each head's own weights
+        before = [rows_of(m, li, keep) for li in range(3)]
+        m.kv_shift(1, 5)
+        for li in range(3):
+            v = rows_of(m, li, keep - 5)[1]
+            want = np.concatenate([before[li][1][:1], before[li][1][6:]])
+            for h in range(cfg.n_kv_head):
+                assert np.array_equal(v[:, h], O.values(*O.quantise(want[:, h])))
+        m.forward(g.integers(0, cfg.n_vocab, 9))
