@@ -693,7 +693,8 @@ int kv8_move(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float
         g.rotate = 1;
         g.pairs = (int)rope->n_dims / 2;
         g.half = rope->layout == NEON_ROPE_HALF;
-        rope_turns(*rope, &g.turns);
+        const int rc = rope_turns(*rope, &g.turns);
+        if (rc) return rc;
     }
     const int hd = (int)src.head_dim;
     auto kern = hd == 64 ? kv8_gather_kernel<64> : hd == 128 ? kv8_gather_kernel<128> : kv8_gather_kernel<0>;
@@ -703,6 +704,9 @@ int kv8_move(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float
 
 int kv8_evict(const neon_kv8_t& src, const float* w, const neon_kv8_t& dst, float* wd, size_t keep, size_t sink,
               size_t recent, const neon_rope_t* rope, int32_t* kept, cudaStream_t st) {
+    RopeTurns turns;
+    if (rope)  // (nothing is launched for a rotation that is not one)
+        if (const int bad = rope_turns(*rope, &turns)) return bad;
     SelectArgs s{src.past, w, (int)src.capacity, (int)keep, (int)sink, (int)recent, kept};
     const bool one = src.capacity <= kSelThreads * kSelHeld;  // a CTA holds all of a head's weights
     int rc = one ? launch("kv8_select_kernel", kv8_select_kernel<1>, dim3(src.n_kv_head), kSelThreads, 0, st, 1, s)

@@ -213,7 +213,7 @@ struct RopeTurns {
     double f[128];
 };
 int rope_check(const neon_rope_t* r, size_t head_dim);
-void rope_turns(const neon_rope_t& r, RopeTurns* t);
+int rope_turns(const neon_rope_t& r, RopeTurns* t);
 
 // cos and sin of 2 pi * turns * pos: the whole turns drop out in 64 bits (an
 // int32 position times a turn has an error of 2^-53 of its size), the rest is

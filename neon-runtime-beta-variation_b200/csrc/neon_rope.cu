@@ -22,7 +22,7 @@ int rope_check(const neon_rope_t* r, size_t head_dim) {
         return error(NEON_ERR_INVALID, "rope: unknown layout");
     if (!(r->base > 0) || !std::isfinite(r->base) || !(r->scale > 0) || !std::isfinite(r->scale))
         return error(NEON_ERR_INVALID, "rope: base and scale must be positive");
-    if (!std::isfinite(r->magnitude)) return error(NEON_ERR_INVALID, "rope: magnitude must be finite");
+    if (!std::isfinite((float)r->magnitude)) return error(NEON_ERR_INVALID, "rope: magnitude must be finite in fp32");
     if (!(r->yarn >= 0 && r->yarn <= 1)) return error(NEON_ERR_INVALID, "rope: yarn must be from 0 to 1");
     if (r->yarn > 0 && (r->orig_ctx == 0 || !(r->beta_slow > 0) || !(r->beta_fast >= r->beta_slow) ||
                         !std::isfinite(r->beta_fast) || r->base == 1.0))
@@ -34,7 +34,7 @@ int rope_check(const neon_rope_t* r, size_t head_dim) {
     return NEON_OK;
 }
 
-void rope_turns(const neon_rope_t& r, RopeTurns* t) {
+int rope_turns(const neon_rope_t& r, RopeTurns* t) {
     const double pi2 = 6.283185307179586476925286766559;
     const double den = r.freq_dim ? r.freq_dim : r.n_dims;
     double lo = 0, hi = 0;
@@ -55,7 +55,9 @@ void rope_turns(const neon_rope_t& r, RopeTurns* t) {
         if (r.yarn > 0)
             own = r.yarn * (1 - std::min(1.0, std::max(0.0, ((double)i - lo) / std::max(hi - lo, 0.001))));
         t->f[i] = (f / r.scale * (1 - own) + f * own) / pi2;
+        if (!std::isfinite(t->f[i])) return neon_internal::error(NEON_ERR_INVALID, "rope: a frequency beyond the range of doubles");
     }
+    return NEON_OK;
 }
 
 namespace {
@@ -238,6 +240,8 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
     }
     a.head0[kMaxTargets] = (int)heads;
     for (size_t g = n_targets; g < (size_t)kMaxTargets; ++g) a.head0[g] = (int)heads;
+    rc = rope_turns(*rope, &a.turns);
+    if (rc) return rc;
     OnDevice dev(targets[0].Y);
     if (dev.rc) return dev.rc;
     const int sms = neon_internal::device_sms(dev.device);
@@ -248,7 +252,6 @@ extern "C" int neon_cuda_rope(const neon_rope_t* rope, int type, const int32_t* 
     a.pairs = (int)rope->n_dims / 2;
     a.back = backward != 0;
     a.mag = (float)rope->magnitude;
-    rope_turns(*rope, &a.turns);
     // Pieces per CTA: one to four a thread, so that CTAs in their table and CTAs in their heads share the SMs (4099
     // positions of 32 heads: 16 us; always one 28, always four 16; one position of 24 heads: 2.2, always four 2.7).
     const int V1 = vec ? (int)V : half ? 1 : 2;

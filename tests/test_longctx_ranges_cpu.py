@@ -67,3 +67,25 @@ def test_buffers_side_by_side_are_separate(at):
     assert evict(src, dst, w=p, wd=p + H * CAP * 4, kept=p + 2 * H * CAP * 4) != 0 and "separate" not in err()
     one_tail = N._Kv8(H, D, CAP, *[b["s" + n if n == "tail" else "d" + n] for n in SIZES])
     assert evict(src, one_tail, w=p, wd=p + H * CAP * 4, kept=p + 2 * H * CAP * 4) != 0 and "separate" not in err()
+
+
+@pytest.mark.parametrize("kw", [dict(base=1e-300, scale=1e-300), dict(base=1e-308, scale=1e-10), dict(scale=5e-324),
+                                dict(magnitude=1e39)])
+def test_rotations_beyond_the_range_of_numbers(kw):
+    """Finite arguments whose frequencies, or whose magnitude in fp32, are not: refused, where every value came out as
+    not a number."""
+    import struct
+
+    t = struct.pack("5Q", P, 2 * P, 256, 256, 4)
+    r = N.Rope(64, **kw)
+    assert N.load().neon_cuda_rope(r._ref, 0, P, 4, 64, t, 1, 0, None) == INVALID
+    assert "rope: a frequency" in err() or "finite in fp32" in err()
+
+
+@pytest.mark.parametrize("kw", [dict(base=1e300), dict(base=1e-3), dict(scale=1e300), dict(magnitude=3e38)])
+def test_rotations_within_it(kw):
+    import struct
+
+    t = struct.pack("5Q", P, 2 * P, 256, 256, 4)
+    N.load().neon_cuda_rope(N.Rope(64, **kw)._ref, 0, P, 4, 64, t, 1, 0, None)
+    assert "rope" not in err()  # (what it says is that there is no device buffer)
