@@ -196,7 +196,8 @@ NEON_API int neon_cuda_matvec_q4_0_noalloc(neon_tensor_t W, const float* dX, siz
 
 /* The operators of this section take device buffers of F32, F16 or BF16
  * values (`type`, a NEON_GGML_* value; every buffer of one call has it),
- * compute in fp32 and round once at the end. They run on the device that
+ * compute in fp32 (or to as many bits: attention's products take fp32 operands
+ * as two fp16 terms) and round once at the end. They run on the device that
  * their buffers live on, allocate nothing, keep nothing between calls, and
  * may be captured into a CUDA graph (after the first call on a device or
  * neon_cuda_init): lengths and positions are read from device memory, so a
@@ -273,8 +274,8 @@ typedef struct {
  * (dK[t * k_stride + head * head_dim + d]). *past itself is left: the caller
  * moves it on after the step (neon_cuda_kv8_attention reads it too), and may
  * set it back to drop rows, not forward over rows that were not written.
- * Rows from capacity on are dropped and reported by the next neon_cuda_sync
- * on the device. */
+ * Rows from capacity on (n itself is at most the capacity) are dropped and
+ * reported by the next neon_cuda_sync on the device, and by nothing else. */
 NEON_API int neon_cuda_kv8_append(const neon_kv8_t* cache, const void* dK, size_t k_stride, const void* dV,
                                   size_t v_stride, size_t n, int type, void* stream);
 
@@ -294,11 +295,15 @@ NEON_API int neon_cuda_kv8_read(const neon_kv8_t* cache, size_t row0, size_t n, 
  * written for the new rows, which have no weight yet. `workspace`:
  * neon_cuda_kv8_attention_workspace() bytes on the device, 16-byte aligned,
  * not shared by calls that may run at the same time. Sums are taken in a
- * fixed order: the same call gives the same bits. */
+ * fixed order: the same call gives the same bits. What an output is off by is
+ * relative to the largest |v| of the blocks that it attends to: at most 2^-16
+ * of it, and 2^-17 for each unit of its scores' sums of magnitudes, before the
+ * rounding to its type. */
 NEON_API int neon_cuda_kv8_attention(const neon_kv8_t* cache, const void* dQ, size_t q_stride, void* dO,
                                      size_t o_stride, size_t n, size_t n_head, float scale, int type,
                                      float* d_weight, void* workspace, size_t workspace_bytes, void* stream);
-/* Bytes of workspace for calls of up to n tokens (host-only; needs no GPU). */
+/* Bytes of workspace for calls of up to n tokens, with d_weight or without
+ * (host-only; needs no GPU). */
 NEON_API int neon_cuda_kv8_attention_workspace(const neon_kv8_t* cache, size_t n, size_t n_head, size_t* bytes);
 
 /* Eviction by accumulated attention weight, from `src` into the separate

@@ -28,6 +28,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+constexpr size_t kSms = 148;    // of a B200: a constant, as a workspace is sized without a device
 constexpr int kMaxSplit = 64;  // (one KV head over 60000 rows takes 25.6 us; with 32 shares 27.8)
 
 // ---------------------------------------------------------------------------
@@ -117,7 +118,6 @@ template <int HD, bool FULL, int ROWS>
 __global__ void __launch_bounds__(RowTile<HD, ROWS>::kThreads, 1) kv8_rows_kernel(const __grid_constant__ AttnArgs a) {
     using R = RowTile<HD, ROWS>;
     constexpr int RL = ROWS / 8;  // rows of a lane: g, and of 16 g + 8
-    constexpr int KS = HD / 16;   // k-steps of the score product
     constexpr int NT = HD / 8;    // column tiles of the output
     constexpr int W = R::kWarps, S = R::kSlots;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -569,7 +569,7 @@ Plan plan_of(const neon_kv8_t& c, size_t n, size_t n_head, int type) {
     // only has to leave room for that (one token over 4000 rows of 8 heads x 128 takes 12.6 us; with a limit of one
     // per 512 rows, seven shares of 18 blocks for 16 warps, 14.3), and is 1 for short caches, which then need no join.
     const size_t most = p.prompt ? c.capacity / 512 : c.capacity < 1024 ? 1 : c.capacity / 256;
-    p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, 148 / units, most}));
+    p.nsplit = (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMaxSplit, kSms / units, most}));
     if (!p.prompt) p.nsplit = (int)std::max<size_t>(p.nsplit, rows_least_shares(c));
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -615,14 +615,14 @@ int launch_rows(AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 size_t kv8_attention_workspace(const neon_kv8_t& c, size_t n, size_t n_head, bool weights) {
-    // Fewer tokens may take more shares, but rows * shares is at most 148 units' rows (plan_of).
+    // Fewer tokens may take more shares, but rows * shares is at most kSms units' rows, or `few` (plan_of).
     const size_t rows = n * (n_head / c.n_kv_head), H = c.n_kv_head;
     const size_t unit = rows > (size_t)kPromptRows ? prompt_unit((int)c.head_dim) : 16;
     const size_t padded = (rows + 255) / 256 * 256;
     const size_t few = H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * rows_least_shares(c);
-    const size_t parts = std::max(148 * unit, few) * (c.head_dim + 2) * sizeof(float);
+    const size_t parts = std::max(kSms * unit, few) * (c.head_dim + 2) * sizeof(float);
     const size_t sums = rows > (size_t)kPromptRows && c.capacity > (size_t)kChainKeys
-                            ? std::max(148 * unit, H * ((rows + unit - 1) / unit * unit)) * c.head_dim * sizeof(float)
+                            ? std::max(kSms * unit, H * ((rows + unit - 1) / unit * unit)) * c.head_dim * sizeof(float)
                             : 0;
     const size_t scores = H * ((std::min<size_t>(rows, kPromptRows) + 15) / 16 * 16) * c.capacity * sizeof(float);
     return H * rows * 2 * sizeof(float) + parts + sums + 10 * 1024 +

@@ -93,3 +93,32 @@ def test_attention_right_behind_its_append(n, heads):
                 torch.cuda.synchronize()
         runs.append(out)
     assert torch.equal(*runs)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("H,D,heads,cap,n", [(1, 64, 1, 32, 1), (8, 128, 64, 4096, 1), (8, 128, 64, 40000, 4), (1, 256, 9, 70016, 3),
+                                             (160, 16, 160, 20000, 1), (1, 64, 1, 1024, 33), (1, 64, 64, 8192, 300),
+                                             (8, 128, 64, 8192, 40), (2, 192, 4, 9984, 700), (80, 16, 160, 1056, 17),
+                                             (1, 256, 33, 2080, 1)])
+def test_workspace_is_enough(kind, H, D, heads, cap, n):
+    """A workspace of the size that is asked for, anywhere in a larger buffer: nothing before or behind it is touched,
+    and calls of fewer tokens run in it too."""
+    typ, dt = {"f32": (N.GGML_F32, torch.float32), "bf16": (N.GGML_BF16, torch.bfloat16)}[kind]
+    c = N.Kv8Cache.empty(H, D, cap)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for codes, scale in ((c.k, c.k_scale), (c.v, c.v_scale)):
+        codes.copy_(torch.randint(-127, 128, codes.shape, generator=g, device="cuda", dtype=torch.int8))
+        scale.fill_(0.01)
+    size = c.attention_workspace(heads, n)
+    whole = torch.empty(size + 8192, dtype=torch.uint8, device="cuda")
+    q = torch.randn(n, heads, D, generator=g, device="cuda").to(dt)
+    w = torch.zeros(H, cap, device="cuda")
+    for m in {n, max(1, n // 2), min(n, 7), 1}:
+        assert c.attention_workspace(heads, m) <= size
+        for at in (4096, 4096 + 16, 4096 + 1008):
+            whole.fill_(0xA5)
+            o = torch.empty(m, heads, D, dtype=dt, device="cuda")
+            c.past.fill_(cap - m)
+            c.attention(q, o, m, heads, whole[at:], type=typ, weight=w, workspace_bytes=size)
+            assert torch.isfinite(o).all()
+            assert (whole[:at] == 0xA5).all() and (whole[at + size:] == 0xA5).all()
