@@ -1236,7 +1236,10 @@ namespace {
 
 int dev_alloc(neon_model* m, void** p, size_t bytes) {
     cudaError_t e = cudaMalloc(p, bytes ? bytes : 16);
-    if (e != cudaSuccess) return error(NEON_ERR_NOMEM, std::string("cudaMalloc in the decode engine: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // reported here: not by the next launch's check
+        return error(NEON_ERR_NOMEM, std::string("cudaMalloc in the decode engine: ") + cudaGetErrorString(e));
+    }
     m->allocs.push_back(*p);
     return NEON_OK;
 }
@@ -1536,9 +1539,10 @@ int kv8_alloc_layer(neon_model* m, neon_kv8_t* c) {
 // kernel before, on the same stream: it needs no clearing.
 int kv8_need_spare(neon_model* m) {
     if (m->kv8_spare.k) return NEON_OK;
-    int rc = dev_alloc(m, (void**)&m->kv8_one, sizeof(int));
-    if (!rc && m->kv8_weight) rc = dev_alloc(m, (void**)&m->kv8_spare_weight, m->n_kv_l * m->kv8_cap * sizeof(float));
-    if (!rc) rc = dev_alloc(m, (void**)&m->kv8_kept, m->n_kv_l * m->kv8_cap * sizeof(int32_t));
+    // (what an attempt that found too little memory got is there for the next one)
+    int rc = m->kv8_one ? NEON_OK : dev_alloc(m, (void**)&m->kv8_one, sizeof(int));
+    if (!rc && m->kv8_weight && !m->kv8_spare_weight) rc = dev_alloc(m, (void**)&m->kv8_spare_weight, m->n_kv_l * m->kv8_cap * sizeof(float));
+    if (!rc && !m->kv8_kept) rc = dev_alloc(m, (void**)&m->kv8_kept, m->n_kv_l * m->kv8_cap * sizeof(int32_t));
     neon_kv8_t c{};
     if (!rc) rc = kv8_alloc(m, m->kv8_one, &c);
     if (!rc) m->kv8_spare = c;

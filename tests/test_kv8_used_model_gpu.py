@@ -173,3 +173,31 @@ def test_layers_do_not_mix():
             for h in range(cfg.n_kv_head):
                 assert np.array_equal(v[:, h], O.values(*O.quantise(want[:, h])))
         m.forward(g.integers(0, cfg.n_vocab, 9))
+
+
+def test_an_eviction_without_memory_can_be_tried_again():
+    """Too little memory for the spare cache is an error that costs nothing: not the rows, and no memory per attempt."""
+    one = OneLayer(ctx=131072, n_head=8, n_kv=8, hd=128, n_embd=128)
+    m = N.Model(one.cfg, one.tensors(), kv8=True, kv_weights=True)
+    tokens = np.random.default_rng(12).integers(0, one.cfg.n_vocab, 103)
+    m.forward(tokens[:100])
+    before = rows_of(m, 0, 100)
+    torch.cuda.empty_cache()
+    hold = []
+    while torch.cuda.mem_get_info()[0] > 200 << 20:  # the spare cache takes 269 MB
+        hold.append(torch.empty(max(2 << 20, torch.cuda.mem_get_info()[0] - (160 << 20)), dtype=torch.uint8, device="cuda"))
+    used = []
+    for _ in range(4):
+        with pytest.raises(RuntimeError, match="cudaMalloc"):
+            m.kv_evict(50, 4, 46)
+        used.append(torch.cuda.mem_get_info()[0])
+        torch.cuda.synchronize()
+    assert len(set(used)) == 1
+    assert m.length == 100 and all(np.array_equal(a, b) for a, b in zip(rows_of(m, 0, 100), before))
+    m.forward(tokens[100:])  # (nor is it the next step's error)
+    m.set_length(100)
+    before = rows_of(m, 0, 100)  # (the step coded the last block anew)
+    del hold
+    torch.cuda.empty_cache()
+    m.kv_evict(50, 4, 46)
+    check_moved(one, m, before, [np.r_[0:4, 54:100]] * 8, 50)
